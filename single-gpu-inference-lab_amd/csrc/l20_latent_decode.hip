@@ -1,0 +1,639 @@
+// Decode and verification attention over a paged latent cache for MI355X (gfx950).
+//
+// One cache row a token is key (rank + 64 dims) and value (its first rank dims) of every head:
+//   S^T = K Q^T   [tokens x rows],   O^T = V^T P^T   [dims x rows],   rows = (draft row, head).
+//
+//  latent_partial<T, KT, RANK, RB>   16 RB rows of one sequence and a run of its 64-token tiles.  A tile is
+//    staged once in LDS as T (fp8 codes are converted on the way, exactly) and read twice: as the left operand
+//    of K Q^T in 16-byte pieces, and as that of V^T P^T by transposing reads.  The waves split the products
+//    differently: scores by 16-token blocks (and halves of the rows, RB = 4), values by dims, so that each
+//    byte of the value part is read by one wave (two row halves never meet).  Between the two, P goes through
+//    LDS.  Softmax statistics and accumulators are fp32; P is rounded to T for the product (relative error
+//    2^-9 bf16, 2^-12 fp16, as the output's own rounding), its sum is of the unrounded values.
+//    Chunks of 16 bytes are XOR-swizzled by their row so that both kinds of read use all LDS banks.
+//
+//  Work: the 64-token tiles of all sequences in a row, cut into equal runs, one a group of workgroups (one
+//    workgroup for each block of rows).  A sequence inside one run is written out at once; what a run has of a
+//    longer one goes to the workspace (slot 2 g: the sequence began in an earlier run, 2 g + 1: it began here).
+//
+//  latent_merge<T, RANK>   joins those parts.
+
+#include "l20_latent_attention.h"
+
+#include <algorithm>
+
+#include "l20_latent_common.h"
+
+namespace l20la {
+
+constexpr int kTile = 64;
+
+struct DecodeParams {
+  const void *q;
+  int64_t q_sr, q_sh;
+  const uint8_t *cache;
+  int64_t c_block, c_tok;  // bytes from one 16-token block, one token to the next
+  int64_t blocks;          // 16-token blocks of the cache
+  int per_page;            // blocks a page
+  const int32_t *table;
+  int64_t t_sr;
+  int table_blocks;  // blocks a row of the table can name
+  int max_tokens;    // of a sequence: the table's width, or max_seq_len
+  const int32_t *lens;
+  void *out;
+  int64_t o_sr, o_sh;
+  float *lse;
+  int64_t l_sr, l_sh;
+  float *part;     // [slot][row block][row][RANK]
+  float *part_ml;  // [slot][row block][row][2]: maximum (log2 units), sum
+  float c_log2, out_scale;
+  int batch, q_len, heads, rows;  // rows = q_len * heads of a sequence
+  int groups, row_blocks;
+};
+
+__device__ __forceinline__ int seq_tokens(const DecodeParams &p, int b) {
+  return min(max(p.lens[b], 0), p.max_tokens);
+}
+// (a sequence without tokens has one tile, all masked: its rows are written too)
+__device__ __forceinline__ int tiles_of(int tokens) { return max(1, (tokens + kTile - 1) / kTile); }
+
+// Workgroup sum of x over NT threads.
+template <int NT> __device__ __forceinline__ int block_sum(int x, int *s_wave) {
+#pragma unroll
+  for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) total += s_wave[w];
+  return total;
+}
+
+// Four fp8 codes (one dword) -> two dwords of T, exact.  (Whole words: extracting elements of these
+// conversions' results one by one is miscompiled by the ROCm 7.2 LLVM.)
+template <typename T> __device__ __forceinline__ i32x2 fp8x4(int w);
+template <> __device__ __forceinline__ i32x2 fp8x4<__bf16>(int w) {
+  return i32x2{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
+               __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
+}
+template <> __device__ __forceinline__ i32x2 fp8x4<_Float16>(int w) {
+  return i32x2{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
+               __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))};
+}
+
+template <typename T, int KT, int RANK, int RB> struct Partial {
+  static constexpr int kWaves = RB == 4 ? 8 : 4;
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kRows = 16 * RB;
+  static constexpr int kRowGroups = RB == 4 ? 2 : 1;  // of the score product
+  static constexpr int kRowsPerWave = RB / kRowGroups;  // blocks of 16
+  static constexpr int kSlices = (RANK + kRope) / 32;
+  static constexpr int kLatSlices = RANK / 32;
+  static constexpr int kDimBlocks = RANK / 16 / kWaves;  // value dims a wave owns, in blocks of 16
+  static constexpr int kLatRow = RANK * 2, kRopeRow = kRope * 2, kPRow = kTile * 2;  // bytes
+  static constexpr int kLatBytes = kTile * kLatRow, kRopeBytes = kTile * kRopeRow;
+  // 16-byte pieces of the cache that a thread stages
+  static constexpr int kPiece = KT == 0 ? 16 : 8;  // elements
+  static constexpr int kLatPieces = kTile * RANK / kPiece / kThreads;
+  static constexpr int kRopePieces = (kTile * kRope / kPiece + kThreads - 1) / kThreads;
+
+  struct Shared {
+    alignas(16) char lat[kLatBytes];
+    alignas(16) char rope[kRopeBytes];
+    alignas(16) char p[kRows * kPRow];
+    alignas(16) float max4[kRows][4];
+    float sum4[kRows][4];
+    int wave[kWaves];
+    int start[2];
+  };
+
+  // Where chunk c (16 bytes) of a tile row lies.
+  static __device__ __forceinline__ int lat_at(int row, int c) { return row * kLatRow + ((c ^ (row & 15)) << 4); }
+  static __device__ __forceinline__ int rope_at(int row, int c) { return row * kRopeRow + ((c ^ ((row >> 1) & 7)) << 4); }
+  static __device__ __forceinline__ int p_at(int row, int c) { return row * kPRow + ((c ^ ((row >> 1) & 7)) << 4); }
+
+  // The staged pieces of one tile.
+  struct Stage {
+    i32x4 lat[kLatPieces], rope[kRopePieces];
+  };
+  // Blocks: lane k of `pid` holds the cache block (16 tokens) k of a window of 64, -1 for none.
+  static __device__ __forceinline__ int window(const DecodeParams &p, int b, int first_block) {
+    const int blk = first_block + (int)(threadIdx.x & 63);
+    if (blk >= p.table_blocks) return -1;
+    const int page = p.table[b * p.t_sr + blk / p.per_page];
+    const int64_t id = (int64_t)page * p.per_page + blk % p.per_page;
+    return page < 0 || id >= p.blocks ? -1 : (int)id;
+  }
+  // Row `row` (0..63) of the tile whose blocks are lanes 4 k .. 4 k + 3 of pid: its address, or zeros.
+  static __device__ __forceinline__ const uint8_t *row_of(const DecodeParams &p, const int (&blk)[4], int row, int tokens) {
+    const int k = row >> 4;
+    const int id = k == 0 ? blk[0] : k == 1 ? blk[1] : k == 2 ? blk[2] : blk[3];
+    return id < 0 || row >= tokens ? reinterpret_cast<const uint8_t *>(kZeroRow)
+                                   : p.cache + (int64_t)id * p.c_block + (row & 15) * p.c_tok;
+  }
+  static __device__ __forceinline__ void load(const DecodeParams &p, Stage &st, const int (&blk)[4], int tokens) {
+    constexpr int kLatCols = RANK / kPiece, kRopeCols = kRope / kPiece;
+#pragma unroll
+    for (int i = 0; i < kLatPieces; ++i) {
+      const int n = i * kThreads + threadIdx.x, row = n / kLatCols, col = n % kLatCols;
+      st.lat[i] = *reinterpret_cast<const i32x4 *>(row_of(p, blk, row, tokens) + 16 * col);
+    }
+#pragma unroll
+    for (int i = 0; i < kRopePieces; ++i) {
+      const int n = i * kThreads + threadIdx.x, row = n / kRopeCols, col = n % kRopeCols;
+      if (kTile * kRopeCols % kThreads == 0 || n < kTile * kRopeCols)
+        st.rope[i] = *reinterpret_cast<const i32x4 *>(row_of(p, blk, row, tokens) + RANK * (KT == 0 ? 1 : 2) + 16 * col);
+    }
+  }
+  static __device__ __forceinline__ void put(char *base, int at0, int at1, i32x4 w) {
+    if constexpr (KT == 0) {
+      const i32x2 a = fp8x4<T>(w[0]), b = fp8x4<T>(w[1]), c = fp8x4<T>(w[2]), d = fp8x4<T>(w[3]);
+      *reinterpret_cast<i32x4 *>(base + at0) = i32x4{a[0], a[1], b[0], b[1]};
+      *reinterpret_cast<i32x4 *>(base + at1) = i32x4{c[0], c[1], d[0], d[1]};
+    } else {
+      *reinterpret_cast<i32x4 *>(base + at0) = w;
+    }
+  }
+  static __device__ __forceinline__ void store(Shared &s, const Stage &st) {
+    constexpr int kLatCols = RANK / kPiece, kRopeCols = kRope / kPiece;
+    constexpr int kChunks = KT == 0 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < kLatPieces; ++i) {
+      const int n = i * kThreads + threadIdx.x, row = n / kLatCols, col = n % kLatCols;
+      put(s.lat, lat_at(row, kChunks * col), lat_at(row, kChunks * col + 1), st.lat[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRopePieces; ++i) {
+      const int n = i * kThreads + threadIdx.x, row = n / kRopeCols, col = n % kRopeCols;
+      if (kTile * kRopeCols % kThreads == 0 || n < kTile * kRopeCols)
+        put(s.rope, rope_at(row, kChunks * col), rope_at(row, kChunks * col + 1), st.rope[i]);
+    }
+  }
+
+  static __device__ __forceinline__ void run(const DecodeParams &p, Shared &s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n16 = lane & 15, g4 = lane >> 4;
+    const int tok_block = wave & 3, row_group = wave >> 2;
+    // Workgroup (group, row block): the row blocks of a group follow at a distance of 8, on one XCD, whose L2
+    // then serves the tile to all but one of them.
+    const int unit = blockIdx.x >> 3;
+    const int group = (unit / p.row_blocks) * 8 + (blockIdx.x & 7);
+    const int rblk = unit % p.row_blocks;
+
+    // ---- this group's run of tiles ----
+    const int chunk = (p.batch + kThreads - 1) / kThreads;
+    int mine = 0;
+    for (int i = 0; i < chunk; ++i) {
+      const int b = tid * chunk + i;
+      if (b < p.batch) mine += tiles_of(seq_tokens(p, b));
+    }
+    int inc = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(inc, off);
+      if (lane >= off) inc += y;
+    }
+    if (lane == 63) s.wave[wave] = inc;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const int v = s.wave[w];
+      if (w < wave) inc += v;
+      total += v;
+    }
+    const int per = (total + p.groups - 1) / p.groups;
+    const int first = min(group * per, total), last = min(first + per, total);
+    if (first >= last) return;  // the whole workgroup
+    if (inc - mine <= first && first < inc) {
+      int base = inc - mine, b = tid * chunk;
+      for (;; ++b) {
+        const int n = tiles_of(seq_tokens(p, b));
+        if (first < base + n) break;
+        base += n;
+      }
+      s.start[0] = b;
+      s.start[1] = base;
+    }
+    __syncthreads();
+    int b = __builtin_amdgcn_readfirstlane(s.start[0]);
+    int base = __builtin_amdgcn_readfirstlane(s.start[1]);
+
+    // ---- one segment a sequence ----
+    for (int at = first; at < last; ++b) {
+      const int tokens = seq_tokens(p, b), len = p.lens[b], tiles = tiles_of(tokens);
+      const int seg_end = min(last, base + tiles);
+      segment(p, s, b, rblk, group, base, tiles, at, seg_end, first, tokens, len, lane, wave, n16, g4, tok_block,
+              row_group);
+      at = seg_end;
+      base += tiles;
+    }
+  }
+
+  static __device__ __forceinline__ void segment(const DecodeParams &p, Shared &s, int b, int rblk, int group, int base,
+                                                 int tiles, int at, int seg_end, int first, int tokens, int len, int lane,
+                                                 int wave, int n16, int g4, int tok_block, int row_group) {
+    // rows of the score product (two blocks at most) and of the value product (all)
+    i32x4 q[kRowsPerWave][kSlices];
+    int lim[kRowsPerWave];
+#pragma unroll
+    for (int u = 0; u < kRowsPerWave; ++u) {
+      const int r = rblk * kRows + 16 * (row_group * kRowsPerWave + u) + n16;
+      const bool live = r < p.rows;
+      const int i = live ? r / p.heads : 0, h = live ? r - i * p.heads : 0;
+      lim[u] = live ? len - p.q_len + i : -1;
+      const T *src = reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + h * p.q_sh + 8 * g4;
+#pragma unroll
+      for (int k = 0; k < kSlices; ++k) {
+        const i32x4 w = *reinterpret_cast<const i32x4 *>(src + 32 * k);
+        q[u][k] = live ? w : i32x4{0, 0, 0, 0};
+      }
+    }
+    f32x4 acc[RB][kDimBlocks];
+    float m_all[RB];       // running maximum of the lane's row in each block, log2 units
+    float sum[kRowsPerWave];  // of the lane's own tokens
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      m_all[r] = -INFINITY;
+#pragma unroll
+      for (int d = 0; d < kDimBlocks; ++d) acc[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int u = 0; u < kRowsPerWave; ++u) sum[u] = 0.0f;
+
+    // LDS places of the lane's operands
+    int v_lo[kDimBlocks], v_hi[kDimBlocks];
+#pragma unroll
+    for (int d = 0; d < kDimBlocks; ++d) {
+      const int c = 2 * (wave * kDimBlocks + d) + ((n16 >> 1) & 1);
+      v_lo[d] = lat_at(8 * g4 + (n16 >> 2), c) + 8 * (n16 & 1);
+      v_hi[d] = lat_at(8 * g4 + 4 + (n16 >> 2), c) + 8 * (n16 & 1);
+    }
+
+    int win = -1, pid = -1;
+    for (int tile = at; tile < seg_end; ++tile) {
+      const int t0 = (tile - base) * kTile;  // first token
+      if ((t0 >> 10) != win) {
+        win = t0 >> 10;
+        pid = window(p, b, win * 64);
+      }
+      int blk[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) blk[k] = __builtin_amdgcn_readlane(pid, ((t0 >> 4) & 63) + k);
+      Stage st;
+      load(p, st, blk, tokens - t0);
+      __syncthreads();  // the tile before is consumed
+      store(s, st);
+      __syncthreads();
+
+      // ---- S^T = K Q^T: 16 tokens, the wave's rows ----
+      f32x4 sc[kRowsPerWave];
+#pragma unroll
+      for (int u = 0; u < kRowsPerWave; ++u) sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int trow = 16 * tok_block + n16;
+#pragma unroll
+      for (int k = 0; k < kSlices; ++k) {
+        const i32x4 a = k < kLatSlices
+                            ? *reinterpret_cast<const i32x4 *>(s.lat + lat_at(trow, 4 * k + g4))
+                            : *reinterpret_cast<const i32x4 *>(s.rope + rope_at(trow, 4 * (k - kLatSlices) + g4));
+#pragma unroll
+        for (int u = 0; u < kRowsPerWave; ++u) sc[u] = mfma<T>(a, q[u][k], sc[u]);
+      }
+      // ---- scores in log2 units, masked; the block's row maxima ----
+      const int my_blk = tok_block == 0 ? blk[0] : tok_block == 1 ? blk[1] : tok_block == 2 ? blk[2] : blk[3];
+#pragma unroll
+      for (int u = 0; u < kRowsPerWave; ++u) {
+        const int hide = my_blk < 0 ? -1 : min(lim[u], tokens - 1);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = t0 + 16 * tok_block + 4 * g4 + i;
+          sc[u][i] = t <= hide ? sc[u][i] * p.c_log2 : -INFINITY;
+          mx = fmaxf(mx, sc[u][i]);
+        }
+        mx = max_groups(mx);
+        if (g4 == 0) s.max4[16 * (row_group * kRowsPerWave + u) + n16][tok_block] = mx;
+      }
+      __syncthreads();
+      // ---- new maxima, P ----
+      float alpha[RB];
+      float m_use[RB];
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const f32x4 m4 = *reinterpret_cast<const f32x4 *>(s.max4[16 * r + n16]);
+        const float m = fmaxf(m_all[r], fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+        m_use[r] = m == -INFINITY ? 0.0f : m;
+        alpha[r] = exp2f(m_all[r] - m_use[r]);  // 0 before the first visible token
+        m_all[r] = m;
+      }
+#pragma unroll
+      for (int u = 0; u < kRowsPerWave; ++u) {
+        const int rb = row_group * kRowsPerWave + u;
+        float m = m_use[u], al = alpha[u];
+        if constexpr (kRowGroups == 2) {
+          m = row_group ? m_use[kRowsPerWave + u] : m;
+          al = row_group ? alpha[kRowsPerWave + u] : al;
+        }
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = exp2f(sc[u][i] - m);
+        sum[u] = sum[u] * al + ((e[0] + e[1]) + (e[2] + e[3]));
+        *reinterpret_cast<i32x2 *>(s.p + p_at(16 * rb + n16, 2 * tok_block + (g4 >> 1)) + 8 * (g4 & 1)) =
+            i32x2{pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3])};
+      }
+      __syncthreads();
+      // ---- O^T += V^T P^T: the wave's dims, all rows ----
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d) acc[r][d] *= alpha[r];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        i32x4 pb[RB];
+#pragma unroll
+        for (int r = 0; r < RB; ++r) pb[r] = *reinterpret_cast<const i32x4 *>(s.p + p_at(16 * r + n16, 4 * ks + g4));
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d) {
+          const i32x2 lo = read_tr(s.lat + ks * 32 * kLatRow + v_lo[d]);
+          const i32x2 hi = read_tr(s.lat + ks * 32 * kLatRow + v_hi[d]);
+          const i32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+          for (int r = 0; r < RB; ++r) acc[r][d] = mfma<T>(a, pb[r], acc[r][d]);
+        }
+      }
+    }
+
+    // ---- the rows' sums, over lane groups and the waves of a row group ----
+#pragma unroll
+    for (int u = 0; u < kRowsPerWave; ++u) {
+      const float x = sum_groups(sum[u]);
+      if (g4 == 0) s.sum4[16 * (row_group * kRowsPerWave + u) + n16][tok_block] = x;
+    }
+    __syncthreads();
+    const bool whole = at == base && seg_end == base + tiles;
+    const int slot = base < first ? 2 * group : 2 * group + 1;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const int lr = 16 * r + n16;
+      const int row = rblk * kRows + lr;
+      const float l = (s.sum4[lr][0] + s.sum4[lr][1]) + (s.sum4[lr][2] + s.sum4[lr][3]);
+      if (row >= p.rows) continue;
+      if (whole) {
+        const int i = row / p.heads, h = row - i * p.heads;
+        const int64_t orow = (int64_t)b * p.q_len + i;
+        const float inv = l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
+        T *dst = reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + 4 * g4;
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d) {
+          const f32x4 x = acc[r][d] * inv;
+          *reinterpret_cast<i32x2 *>(dst + 16 * (wave * kDimBlocks + d)) =
+              i32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+        }
+        if (p.lse && wave == 0 && g4 == 0)
+          p.lse[orow * p.l_sr + h * p.l_sh] = l == 0.0f ? -INFINITY : (m_all[r] + log2f(l)) * kLn2;
+      } else {
+        const int64_t prow = ((int64_t)slot * p.row_blocks + rblk) * kRows + lr;
+        float *dst = p.part + prow * RANK + 4 * g4;
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d) *reinterpret_cast<f32x4 *>(dst + 16 * (wave * kDimBlocks + d)) = acc[r][d];
+        if (wave == 0 && g4 == 0) *reinterpret_cast<f32x2 *>(p.part_ml + 2 * prow) = f32x2{m_all[r], l};
+      }
+    }
+    __syncthreads();  // the sums are read before the next segment's
+  }
+};
+
+template <typename T, int KT, int RANK, int RB>
+__global__ __launch_bounds__((Partial<T, KT, RANK, RB>::kThreads)) void latent_partial(DecodeParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  Partial<T, KT, RANK, RB>::run(p, *reinterpret_cast<typename Partial<T, KT, RANK, RB>::Shared *>(smem));
+}
+
+// One workgroup of 256 threads a row: RANK / 4 lanes hold four dims each, the others further parts.
+template <typename T, int RANK>
+__global__ __launch_bounds__(256) void latent_merge(DecodeParams p, int block_rows) {
+  constexpr int kCols = RANK / 4, kLanes = 256 / kCols;
+  __shared__ int s_wave[4];
+  __shared__ f32x4 s_acc[kLanes][kCols];
+  __shared__ float s_l[kLanes];
+  const int b = blockIdx.y, row = blockIdx.x;
+  int before = 0, all = 0;
+  for (int i = threadIdx.x; i < p.batch; i += 256) {
+    const int n = tiles_of(seq_tokens(p, i));
+    all += n;
+    before += i < b ? n : 0;
+  }
+  const int total = block_sum<256>(all, s_wave);
+  const int base = block_sum<256>(before, s_wave);
+  const int per = (total + p.groups - 1) / p.groups;
+  const int end = base + tiles_of(seq_tokens(p, b));
+  const int g0 = base / per, g1 = (end - 1) / per;
+  if (g0 == g1) return;  // written already
+  const int rblk = row / block_rows, lr = row - rblk * block_rows;
+  auto prow = [&](int g) {
+    const int slot = base < g * per ? 2 * g : 2 * g + 1;
+    return ((int64_t)slot * p.row_blocks + rblk) * block_rows + lr;
+  };
+  float m = -INFINITY;
+  for (int g = g0; g <= g1; ++g) m = fmaxf(m, p.part_ml[2 * prow(g)]);
+  const float m_use = m == -INFINITY ? 0.0f : m;
+  const int col = threadIdx.x % kCols, part = threadIdx.x / kCols;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.0f;
+  for (int g = g0 + part; g <= g1; g += kLanes) {
+    const int64_t r = prow(g);
+    const f32x2 ml = *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * r);
+    const float w = exp2f(ml[0] - m_use);
+    acc += *reinterpret_cast<const f32x4 *>(p.part + r * RANK + 4 * col) * w;
+    l += ml[1] * w;
+  }
+  s_acc[part][col] = acc;
+  if (col == 0) s_l[part] = l;
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int k = 1; k < kLanes; ++k) {
+    acc += s_acc[k][col];
+    l += s_l[k];
+  }
+  const int i = row / p.heads, h = row - i * p.heads;
+  const int64_t orow = (int64_t)b * p.q_len + i;
+  const f32x4 x = acc * (l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l));
+  *reinterpret_cast<i32x2 *>(reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + 4 * col) =
+      i32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+  if (p.lse && col == 0) p.lse[orow * p.l_sr + h * p.l_sh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+}  // namespace l20la
+
+namespace {
+
+using l20pd_host::set_error;
+
+int device_cus() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+    cus = 256;
+  return cus;
+}
+
+int64_t rows_of(const l20_pd_latent_args &a) { return (int64_t)a.q_len * a.num_heads; }
+// Blocks of 16 rows a workgroup takes: as many as the sequence has, up to four.
+int blocks_of(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+int64_t tiles_bound(const l20_pd_latent_args &a) {
+  return (int64_t)a.batch * std::max<int64_t>(1, ((int64_t)a.max_seq_len + l20la::kTile - 1) / l20la::kTile);
+}
+// Runs of tiles: as many as workgroups fit the chip at once, a multiple of 8 (the XCDs), no more than tiles.
+int groups_of(const l20_pd_latent_args &a, int cus) {
+  const int64_t rows = rows_of(a), rblocks = (rows + 16 * blocks_of(rows) - 1) / (16 * blocks_of(rows));
+  const int64_t fit = std::max<int64_t>(1, cus / rblocks);
+  return (int)((std::min(fit, tiles_bound(a)) + 7) / 8 * 8);
+}
+int64_t workspace_bytes(const l20_pd_latent_args &a, int cus) {
+  if (a.batch <= 0 || tiles_bound(a) <= a.batch) return 0;  // one tile a sequence: nothing to join
+  const int64_t rows = rows_of(a), br = 16 * blocks_of(rows), rblocks = (rows + br - 1) / br;
+  return 2 * groups_of(a, cus) * rblocks * br * (a.rank + 2) * (int64_t)sizeof(float);
+}
+
+int32_t check(const l20_pd_latent_args *a) {
+  if (!a) return set_error(L20_PD_EINVAL, "null argument block");
+  if (a->dtype != L20_PD_BF16 && a->dtype != L20_PD_FP16) return set_error(L20_PD_EINVAL, "query must be bf16 or fp16");
+  const bool fp8 = a->cache_dtype == L20_PD_KV_FP8_E4M3;
+  if (!fp8 && a->cache_dtype != (a->dtype == L20_PD_BF16 ? L20_PD_KV_BF16 : L20_PD_KV_FP16))
+    return set_error(L20_PD_EINVAL, "latent cache must be fp8 e4m3fn or have the query's dtype");
+  if ((a->rank != 256 && a->rank != 512) || a->rope_dim != l20la::kRope)
+    return set_error(L20_PD_EINVAL, "latent attention needs rank 256 or 512 and 64 rotary dims");
+  if (a->page_size < 16 || a->page_size % 16 || a->page_size > 4096)
+    return set_error(L20_PD_EINVAL, "page size must be a multiple of 16 up to 4096");
+  if (a->batch < 0 || a->q_len < 1 || a->num_heads < 1 || a->max_seq_len < 0)
+    return set_error(L20_PD_EINVAL, "batch, q_len, heads and max_seq_len must be positive");
+  if (rows_of(*a) > 65535) return set_error(L20_PD_EINVAL, "at most 65535 query rows (q_len x heads) a sequence");
+  if (a->batch > 65535) return set_error(L20_PD_EINVAL, "at most 65535 sequences");
+  if (tiles_bound(*a) >= ((int64_t)1 << 30)) return set_error(L20_PD_EINVAL, "too many tokens");
+  if (!(a->softmax_scale > 0.0f && isfinite(a->softmax_scale)))
+    return set_error(L20_PD_EINVAL, "softmax_scale must be positive and finite");
+  if (fp8 && !(a->cache_scale > 0.0f && isfinite(a->cache_scale)))
+    return set_error(L20_PD_EINVAL, "cache scale must be positive and finite");
+  if (a->batch == 0) return L20_PD_OK;
+  if (a->num_pages <= 0 || a->table_pages <= 0) return set_error(L20_PD_EINVAL, "latent cache and block table must have pages");
+  if ((int64_t)a->table_pages * a->page_size > INT32_MAX / 2 ||
+      (int64_t)a->batch * ((int64_t)a->table_pages * a->page_size / l20la::kTile + 1) >= ((int64_t)1 << 30))
+    return set_error(L20_PD_EINVAL, "block table names too many tokens");
+  if (a->num_pages * (a->page_size / 16) > INT32_MAX) return set_error(L20_PD_EINVAL, "latent cache has too many pages");
+  if (a->page_size > 16 && a->c_stride_page != a->page_size * a->c_stride_token)
+    return set_error(L20_PD_EINVAL, "tokens of a page above 16 must be contiguous");
+  if (!a->query || !a->cache || !a->block_table || !a->seq_lens || !a->output)
+    return set_error(L20_PD_EINVAL, "null tensor pointer");
+  auto u = [](const void *x) { return (uint64_t)(uintptr_t)x; };
+  if ((u(a->query) | (uint64_t)(2 * a->q_stride_row) | (uint64_t)(2 * a->q_stride_head)) % 16)
+    return set_error(L20_PD_EINVAL, "query rows must be 16-byte aligned");
+  const int64_t es = fp8 ? 1 : 2;
+  if ((u(a->cache) | (uint64_t)(es * a->c_stride_page) | (uint64_t)(es * a->c_stride_token)) % 16)
+    return set_error(L20_PD_EINVAL, "latent cache rows must be 16-byte aligned");
+  if ((u(a->output) | (uint64_t)(2 * a->o_stride_row) | (uint64_t)(2 * a->o_stride_head)) % 8)
+    return set_error(L20_PD_EINVAL, "output rows must be 8-byte aligned");
+  return L20_PD_OK;
+}
+
+template <typename T, int KT, int RANK, int RB> hipError_t launch_partial(const l20la::DecodeParams &p, hipStream_t s) {
+  typedef l20la::Partial<T, KT, RANK, RB> K;
+  const size_t lds = sizeof(typename K::Shared);
+  const void *f = reinterpret_cast<const void *>(&l20la::latent_partial<T, KT, RANK, RB>);
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((l20la::latent_partial<T, KT, RANK, RB>), dim3((unsigned)(p.groups * p.row_blocks)),
+                     dim3(K::kThreads), lds, s, p);
+  return hipGetLastError();
+}
+template <typename T, int KT, int RANK> hipError_t launch_rows(const l20la::DecodeParams &p, hipStream_t s) {
+  switch (blocks_of(p.rows)) {
+    case 1: return launch_partial<T, KT, RANK, 1>(p, s);
+    case 2: return launch_partial<T, KT, RANK, 2>(p, s);
+    default: return launch_partial<T, KT, RANK, 4>(p, s);
+  }
+}
+template <typename T, int RANK> hipError_t launch(const l20la::DecodeParams &p, bool fp8, bool join, hipStream_t s) {
+  const hipError_t e = fp8 ? launch_rows<T, 0, RANK>(p, s) : launch_rows<T, 1, RANK>(p, s);
+  if (e != hipSuccess || !join) return e;
+  hipLaunchKernelGGL((l20la::latent_merge<T, RANK>), dim3((unsigned)p.rows, (unsigned)p.batch), dim3(256), 0, s, p,
+                     16 * blocks_of(p.rows));
+  return hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t l20_pd_paged_latent_check(const l20_pd_latent_args *a) {
+  l20pd_host::clear_error();
+  return check(a);
+}
+
+int64_t l20_pd_paged_latent_workspace(const l20_pd_latent_args *a, int32_t cu_count) {
+  l20pd_host::clear_error();
+  if (!a || a->batch < 0 || a->q_len < 1 || a->num_heads < 1 || a->max_seq_len < 0 || rows_of(*a) > 65535) return 0;
+  return workspace_bytes(*a, cu_count > 0 ? cu_count : device_cus());
+}
+
+int32_t l20_pd_paged_latent(const l20_pd_latent_args *a, void *stream) {
+  l20pd_host::clear_error();
+  const int32_t rc = check(a);
+  if (rc != L20_PD_OK || a->batch == 0) return rc;
+  const int cus = device_cus();
+  const int64_t need = workspace_bytes(*a, cus);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
+    return set_error(L20_PD_EINVAL, "workspace is too small for the request (l20_pd_paged_latent_workspace)");
+  l20la::DecodeParams p{};
+  const bool fp8 = a->cache_dtype == L20_PD_KV_FP8_E4M3;
+  const int64_t es = fp8 ? 1 : 2;
+  p.q = a->query;
+  p.q_sr = a->q_stride_row;
+  p.q_sh = a->q_stride_head;
+  p.cache = static_cast<const uint8_t *>(a->cache);
+  p.c_tok = es * a->c_stride_token;
+  p.c_block = a->page_size == 16 ? es * a->c_stride_page : 16 * p.c_tok;
+  p.per_page = a->page_size / 16;
+  p.blocks = a->num_pages * p.per_page;
+  p.table = a->block_table;
+  p.t_sr = a->bt_stride_row;
+  p.table_blocks = a->table_pages * p.per_page;
+  p.max_tokens = (int)std::min<int64_t>((int64_t)p.table_blocks * 16, a->max_seq_len);
+  p.lens = a->seq_lens;
+  p.out = a->output;
+  p.o_sr = a->o_stride_row;
+  p.o_sh = a->o_stride_head;
+  p.lse = a->lse;
+  p.l_sr = a->lse_stride_row;
+  p.l_sh = a->lse_stride_head;
+  const float cache_scale = fp8 ? a->cache_scale : 1.0f;
+  p.c_log2 = a->softmax_scale * cache_scale * l20la::kLog2e;
+  p.out_scale = cache_scale;
+  p.batch = a->batch;
+  p.q_len = a->q_len;
+  p.heads = a->num_heads;
+  p.rows = (int)rows_of(*a);
+  const int br = 16 * blocks_of(p.rows);
+  p.row_blocks = (p.rows + br - 1) / br;
+  p.groups = groups_of(*a, cus);
+  p.part = static_cast<float *>(a->workspace);
+  p.part_ml = p.part + (int64_t)2 * p.groups * p.row_blocks * br * a->rank;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool join = need > 0;
+  hipError_t e;
+  if (a->dtype == L20_PD_BF16)
+    e = a->rank == 512 ? launch<__bf16, 512>(p, fp8, join, s) : launch<__bf16, 256>(p, fp8, join, s);
+  else
+    e = a->rank == 512 ? launch<_Float16, 512>(p, fp8, join, s) : launch<_Float16, 256>(p, fp8, join, s);
+  if (e != hipSuccess) {
+    char msg[256];
+    snprintf(msg, sizeof(msg), "HIP launch failed: %s", hipGetErrorString(e));
+    return set_error(L20_PD_ELAUNCH, msg);
+  }
+  return L20_PD_OK;
+}
+
+}  // extern "C"

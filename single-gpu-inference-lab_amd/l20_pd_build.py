@@ -3,7 +3,7 @@
 Two shared objects land next to this file:
 
 * ``libl20_paged_decode_hip.so`` -- the HIP kernels and the C ABI declared in
-  ``include/l20_paged_decode.h`` (built by hipcc; no torch dependency).
+  ``include/*.h`` (built by hipcc; no torch dependency).
 * ``l20_paged_decode_ops.so`` -- the ``TORCH_LIBRARY(l20_stack)`` binding,
   linked against the first one with an ``$ORIGIN`` rpath (built by g++
   against the installed torch headers).
@@ -17,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -26,12 +27,16 @@ INCLUDE = ROOT / "include"
 HIP_LIB = HERE / "libl20_paged_decode_hip.so"
 OPS_LIB = HERE / "l20_paged_decode_ops.so"
 ARCH = os.environ.get("L20_PD_ARCH", "gfx950")
-# The decode kernels and the paged KV-cache producer, one shared object.
-HIP_SOURCES = [CSRC / "l20_paged_decode_fp8.hip", CSRC / "l20_kv_write.hip", CSRC / "l20_tree_suffix.hip"]
+OBJECTS = HERE / "_build"
+# The decode kernels, the paged KV-cache producer, latent attention and the block tables, one shared object.
+HIP_SOURCES = [CSRC / f"{name}.hip" for name in (
+    "l20_paged_decode_fp8", "l20_kv_write", "l20_tree_suffix", "l20_latent_decode", "l20_latent_prompt",
+    "l20_latent_write", "l20_block_tables")]
+OPS_SOURCES = [CSRC / "l20_paged_decode_ops.cpp", CSRC / "l20_latent_ops.cpp"]
 
 # Packed-FP32 VALU forms are kept out of every HIP build.
 HIP_FLAGS = [
-    "-O3", "-std=c++17", "-fPIC", "-shared", f"--offload-arch={ARCH}",
+    "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-result",
 ]
@@ -55,9 +60,20 @@ def _run(cmd, verbose: bool) -> None:
         print(out, flush=True)
 
 
+def _object(source: Path) -> Path:
+    return OBJECTS / f"{source.stem}.o"
+
+
 def build_hip_library(verbose: bool = False) -> Path:
+    """Every source to an object (side by side: the decode kernels alone take minutes), then one library."""
+    OBJECTS.mkdir(exist_ok=True)
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        jobs = [pool.submit(_run, [_hipcc(), *HIP_FLAGS, f"-I{INCLUDE}", "-c", src, "-o", _object(src)], verbose)
+                for src in HIP_SOURCES]
+        for job in jobs:
+            job.result()
     tmp = HIP_LIB.with_suffix(".so.tmp")
-    _run([_hipcc(), *HIP_FLAGS, f"-I{INCLUDE}", *HIP_SOURCES, "-o", tmp], verbose)
+    _run([_hipcc(), "-shared", f"--offload-arch={ARCH}", *[_object(src) for src in HIP_SOURCES], "-o", tmp], verbose)
     os.replace(tmp, HIP_LIB)
     return HIP_LIB
 
@@ -73,7 +89,7 @@ def build_torch_ops(verbose: bool = False) -> Path:
     cmd = [
         os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-        *includes, CSRC / "l20_paged_decode_ops.cpp",
+        *includes, *OPS_SOURCES,
         *[f"-L{d}" for d in libdirs], "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
         f"-L{HERE}", "-l:libl20_paged_decode_hip.so",
         "-Wl,-rpath,$ORIGIN", *[f"-Wl,-rpath,{d}" for d in libdirs],

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/l20_paged_decode.h`` and ``include/l20_kv_write.h``.
+"""ctypes binding of the C ABI in ``include/*.h``.
 
 Loads ``libl20_paged_decode_hip.so`` from beside this file and mirrors the
 ``l20_pd_fp8_args`` struct field by field.  ``args_from_tensors`` fills the
@@ -50,6 +50,15 @@ EXPORTED = (
     "l20_pd_tree_suffix_merge",
     "l20_pd_tree_mask_words",
     "l20_pd_tree_prefix_setup",
+    "l20_pd_latent_write_check",
+    "l20_pd_latent_rope_and_cache",
+    "l20_pd_paged_latent_check",
+    "l20_pd_paged_latent_workspace",
+    "l20_pd_paged_latent",
+    "l20_pd_latent_prompt_check",
+    "l20_pd_latent_prompt",
+    "l20_pd_block_tables_check",
+    "l20_pd_block_tables",
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -117,6 +126,67 @@ class L20PdKvWriteArgs(ctypes.Structure):
     ]
 
 
+class L20PdLatentWriteArgs(ctypes.Structure):
+    """Mirror of ``l20_pd_latent_write_args`` (include/l20_latent_attention.h)."""
+
+    _fields_ = [
+        ("query", _vp), ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("query_out", _vp), ("qo_stride_token", _i64), ("qo_stride_head", _i64), ("num_heads", _i32),
+        ("latent", _vp), ("l_stride_token", _i64), ("latent_out", _vp), ("lo_stride_token", _i64),
+        ("key", _vp), ("k_stride_token", _i64), ("key_out", _vp), ("ko_stride_token", _i64),
+        ("dtype", _i32),
+        ("positions", _vp), ("cos_sin_cache", _vp), ("cs_stride_position", _i64), ("max_position", _i64),
+        ("cs_dtype", _i32), ("is_neox", _i32), ("norm_weight", _vp), ("norm_eps", _f32),
+        ("slot_mapping", _vp), ("cache", _vp), ("c_stride_page", _i64), ("c_stride_token", _i64),
+        ("num_pages", _i64), ("page_size", _i32), ("cache_dtype", _i32), ("cache_scale", _f32),
+        ("num_tokens", _i32), ("rank", _i32), ("rope_dim", _i32),
+    ]
+
+
+class L20PdLatentArgs(ctypes.Structure):
+    """Mirror of ``l20_pd_latent_args`` (include/l20_latent_attention.h)."""
+
+    _fields_ = [
+        ("query", _vp), ("q_stride_row", _i64), ("q_stride_head", _i64), ("dtype", _i32),
+        ("cache", _vp), ("c_stride_page", _i64), ("c_stride_token", _i64), ("num_pages", _i64),
+        ("page_size", _i32), ("cache_dtype", _i32), ("cache_scale", _f32),
+        ("block_table", _vp), ("bt_stride_row", _i64), ("table_pages", _i32), ("seq_lens", _vp),
+        ("output", _vp), ("o_stride_row", _i64), ("o_stride_head", _i64),
+        ("lse", _vp), ("lse_stride_row", _i64), ("lse_stride_head", _i64),
+        ("workspace", _vp), ("workspace_bytes", _i64), ("softmax_scale", _f32),
+        ("batch", _i32), ("q_len", _i32), ("num_heads", _i32), ("rank", _i32), ("rope_dim", _i32),
+        ("max_seq_len", _i32),
+    ]
+
+
+class L20PdLatentPromptArgs(ctypes.Structure):
+    """Mirror of ``l20_pd_latent_prompt_args`` (include/l20_latent_attention.h)."""
+
+    _fields_ = [
+        ("query", _vp), ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("key", _vp), ("k_stride_token", _i64), ("k_stride_head", _i64),
+        ("key_rope", _vp), ("kr_stride_token", _i64),
+        ("value", _vp), ("v_stride_token", _i64), ("v_stride_head", _i64), ("dtype", _i32),
+        ("cu_q", _vp), ("cu_k", _vp),
+        ("output", _vp), ("o_stride_token", _i64), ("o_stride_head", _i64),
+        ("lse", _vp), ("lse_stride_token", _i64), ("lse_stride_head", _i64),
+        ("softmax_scale", _f32), ("causal", _i32), ("total_q", _i64), ("total_k", _i64),
+        ("batch", _i32), ("num_heads", _i32), ("max_q_len", _i32), ("head_dim", _i32), ("rope_dim", _i32),
+        ("value_dim", _i32),
+    ]
+
+
+class L20PdBlockTablesArgs(ctypes.Structure):
+    """Mirror of ``l20_pd_block_tables_args`` (include/l20_block_tables.h)."""
+
+    _fields_ = [
+        ("cached_lens", _vp), ("new_lens", _vp), ("block_table", _vp), ("bt_stride_row", _i64),
+        ("table_pages", _i32), ("free_pages", _vp), ("pool", _i32), ("free_count", _vp), ("free_count_out", _vp),
+        ("slots", _vp), ("positions", _vp), ("num_slots", _i32), ("cu_lens", _vp), ("seq_lens", _vp),
+        ("batch", _i32), ("page_size", _i32),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -173,6 +243,16 @@ def load(path: Optional[Path] = None) -> ctypes.CDLL:
     lib.l20_pd_tree_suffix_check.restype = _i32
     lib.l20_pd_tree_suffix_merge.argtypes = [ts_p, _vp]
     lib.l20_pd_tree_suffix_merge.restype = _i32
+    for name, struct in (("latent_write_check", L20PdLatentWriteArgs), ("paged_latent_check", L20PdLatentArgs),
+                         ("latent_prompt_check", L20PdLatentPromptArgs), ("block_tables_check", L20PdBlockTablesArgs)):
+        getattr(lib, "l20_pd_" + name).argtypes = [ctypes.POINTER(struct)]
+        getattr(lib, "l20_pd_" + name).restype = _i32
+    for name, struct in (("latent_rope_and_cache", L20PdLatentWriteArgs), ("paged_latent", L20PdLatentArgs),
+                         ("latent_prompt", L20PdLatentPromptArgs), ("block_tables", L20PdBlockTablesArgs)):
+        getattr(lib, "l20_pd_" + name).argtypes = [ctypes.POINTER(struct), _vp]
+        getattr(lib, "l20_pd_" + name).restype = _i32
+    lib.l20_pd_paged_latent_workspace.argtypes = [ctypes.POINTER(L20PdLatentArgs), _i32]
+    lib.l20_pd_paged_latent_workspace.restype = _i64
     if path is None:
         _lib = lib
     return lib
