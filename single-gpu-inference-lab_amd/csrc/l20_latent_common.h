@@ -21,6 +21,7 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -59,14 +60,52 @@ __device__ __forceinline__ i32x2 read_tr(const char *p) {
                                        (lds_s16x4 *)(__attribute__((address_space(3))) char *)(p)));
 }
 
-__device__ __forceinline__ float max_groups(float x) {  // over the four lane groups of 16
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+// D = A B + C of 32x32x16.  Lane l holds A[l % 32][8 (l / 32) + j], B[8 (l / 32) + j][l % 32] (j = 0..7) and
+// C[8 (i / 4) + 4 (l / 32) + i % 4][l % 32] (i = 0..15).
+template <typename T> __device__ __forceinline__ f32x16 mfma32(i32x4 a, i32x4 b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mfma32<__bf16>(i32x4 a, i32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ float sum_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+template <> __device__ __forceinline__ f32x16 mfma32<_Float16>(i32x4 a, i32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+
+// Reductions by the row swaps of the vector ALU (no LDS round trip): with both operands the same register a
+// swap returns a lane's value and that of the lane 16 (32) away, in one order for both of them.
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+template <int W> __device__ __forceinline__ u32x2 swap_rows(float x) {
+  const unsigned int b = __builtin_bit_cast(unsigned int, x);
+  if constexpr (W == 16) return __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(b, b, false, false));
+  else return __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(b, b, false, false));
+}
+// (by value: hipcc lowers __builtin_bit_cast of an ext_vector element to a load of element 0)
+__device__ __forceinline__ float word_f(unsigned int w) { return __builtin_bit_cast(float, w); }
+template <int W> __device__ __forceinline__ float max_swap(float x) {
+  const u32x2 r = swap_rows<W>(x);
+  return fmaxf(word_f(r[0]), word_f(r[1]));
+}
+template <int W> __device__ __forceinline__ float sum_swap(float x) {
+  const u32x2 r = swap_rows<W>(x);
+  return word_f(r[0]) + word_f(r[1]);
+}
+__device__ __forceinline__ float max_halves(float x) { return max_swap<32>(x); }  // over lanes l and l ^ 32
+__device__ __forceinline__ float sum_halves(float x) { return sum_swap<32>(x); }
+__device__ __forceinline__ float max_groups(float x) { return max_swap<32>(max_swap<16>(x)); }  // the four groups of 16
+__device__ __forceinline__ float sum_groups(float x) { return sum_swap<32>(sum_swap<16>(x)); }
+
+// 16 bytes a lane from global memory to LDS (lane l's land at dst + 16 l), asynchronously: they are there once
+// the wave has waited for its loads.
+__device__ __forceinline__ void load_lds(const void *src, void *dst) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) void *)(const __attribute__((address_space(1))) char *)(src),
+      (__attribute__((address_space(3))) void *)(__attribute__((address_space(3))) char *)(dst), 16, 0, 0);
+}
+// The wave's loads have landed, in LDS too, and so have those of the workgroup's other waves.
+__device__ __forceinline__ void landed_and_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The running maximum of a softmax row moves only when a tile's exceeds it by more than this (log2 units): P is
+// then at most 2^8 where it would be 1, which costs neither type precision (fp16 ends at 2^16).
+constexpr float kRescale = 8.0f;
 
 // 16 bytes of zeros a lane: what rows that take no part are read from (a masked row's values still
 // enter the product with a weight of 0, and 0 x NaN is NaN).

@@ -38,25 +38,25 @@ struct PromptParams {
   int batch, heads, max_q;
 };
 
-constexpr int kDim = 128;       // key dims a head, value dims
-constexpr int kKeys = 64;       // a tile
+constexpr int kDim = 128;  // key dims a head, value dims
+constexpr int kKeys = 64;  // a tile
 constexpr int kWaveRows = 32;
 constexpr int kPromptWaves = 4;
 constexpr int kPromptRows = kWaveRows * kPromptWaves;
+constexpr int kSlices = (kDim + kRope) / 16;  // of the score product
 
-struct PromptShared {
-  alignas(16) char k[kKeys * kDim * 2];
-  alignas(16) char v[kKeys * kDim * 2];
-  alignas(16) char kr[kKeys * kRope * 2];
-};
+constexpr int kWideRow = kDim * 2, kNarrowRow = kRope * 2;  // bytes of a key (or value), of its rotary part
+constexpr int kWideBytes = kKeys * kWideRow, kNarrowBytes = kKeys * kNarrowRow;
+constexpr int kTileBytes = 2 * kWideBytes + kNarrowBytes;
 
-__device__ __forceinline__ int wide_at(int row, int c) { return row * (kDim * 2) + ((c ^ (row & 15)) << 4); }
-__device__ __forceinline__ int narrow_at(int row, int c) { return row * (kRope * 2) + ((c ^ ((row >> 1) & 7)) << 4); }
+// Where chunk c (16 bytes) of a tile row lies.
+__device__ __forceinline__ int wide_at(int row, int c) { return row * kWideRow + ((c ^ (row & 15)) << 4); }
+__device__ __forceinline__ int narrow_at(int row, int c) { return row * kNarrowRow + ((c ^ ((row >> 1) & 7)) << 4); }
 
 template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void latent_prompt(PromptParams p) {
-  __shared__ PromptShared s;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n16 = lane & 15, g4 = lane >> 4;
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // two tiles: keys, values, rotary parts
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n32 = lane & 31, g2 = lane >> 5;
   // (sequence, head) varies fastest, so that a head's keys and values stay with one XCD where the count is a
   // multiple of 8; the last rows, which see the most keys, come first.
   const int bh = blockIdx.x % (p.batch * p.heads);
@@ -67,140 +67,137 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
   const int64_t ks = min(max((int64_t)p.cu_k[b], (int64_t)0), p.total_k);
   const int nq = (int)(min((int64_t)p.cu_q[b + 1], p.total_q) - qs);
   const int nk = max((int)(min((int64_t)p.cu_k[b + 1], p.total_k) - ks), 0);
-  if (q0 >= min(nq, p.max_q)) return;  // the whole workgroup
   const int rows = min(nq, p.max_q);
-  const int shift = p.causal ? nk - nq : nk;  // query i sees keys j <= i + shift (and j < nk)
-  // (without causality every key: i + nk >= nk - 1)
+  if (q0 >= rows) return;  // the whole workgroup
+  // query i sees keys j <= i + shift (and j < nk); without causality every key: i + nk >= nk - 1
+  const int shift = p.causal ? nk - nq : nk;
   const int last_row = min(q0 + kPromptRows, rows) - 1;
   const int seen = min(nk, max(last_row + shift + 1, 0));
   const int tiles = (seen + kKeys - 1) / kKeys;
 
-  i32x4 q[2][6];
-  int lim[2];
+  // ---- staging: a wave's instruction fills four rows of keys (values), or eight of rotary parts ----
+  const char *kb = reinterpret_cast<const char *>(p.k) + 2 * (ks * p.k_st + h * p.k_sh);
+  const char *vb = reinterpret_cast<const char *>(p.v) + 2 * (ks * p.v_st + h * p.v_sh);
+  const char *rb = reinterpret_cast<const char *>(p.kr) + 2 * (ks * p.kr_st);
+  const int64_t k_row = 2 * p.k_st, v_row = 2 * p.v_st, r_row = 2 * p.kr_st;
+  auto stage = [&](int tile) {
+    char *buf = smem + (tile & 1) * kTileBytes;
+    const int j0 = tile * kKeys;
+    // rows past the last key hold that key again: they are masked, and what they hold is as finite as it is
+    const int last = nk - 1 - j0;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int i = q0 + wave * kWaveRows + 16 * u + n16;
-    lim[u] = i < rows ? min(i + shift, nk - 1) : -1;
-    const T *src = reinterpret_cast<const T *>(p.q) + (qs + min(i, rows - 1)) * p.q_st + h * p.q_sh + 8 * g4;
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * wave + 4 * i + (lane >> 4), c = (lane & 15) ^ (row & 15);
+      const int64_t j = j0 + min(row, last);
+      load_lds(kb + j * k_row + 16 * c, buf + (16 * wave + 4 * i) * kWideRow);
+      load_lds(vb + j * v_row + 16 * c, buf + kWideBytes + (16 * wave + 4 * i) * kWideRow);
+    }
 #pragma unroll
-    for (int k = 0; k < 6; ++k) q[u][k] = *reinterpret_cast<const i32x4 *>(src + 32 * k);
+    for (int i = 0; i < 2; ++i) {
+      const int row = 16 * wave + 8 * i + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+      const int64_t j = j0 + min(row, last);
+      load_lds(rb + j * r_row + 16 * c, buf + 2 * kWideBytes + (16 * wave + 8 * i) * kNarrowRow);
+    }
+  };
+  if (tiles > 0) stage(0);
+
+  const int i = q0 + wave * kWaveRows + n32;  // the lane's query row
+  const int lim = i < rows ? min(i + shift, nk - 1) : -1;
+  const int wave_lim = q0 + wave * kWaveRows + shift;  // (its first row's, before the end of the keys)
+  i32x4 q[kSlices];
+  {
+    const T *src = reinterpret_cast<const T *>(p.q) + (qs + min(i, rows - 1)) * p.q_st + h * p.q_sh + 8 * g2;
+#pragma unroll
+    for (int k = 0; k < kSlices; ++k) q[k] = *reinterpret_cast<const i32x4 *>(src + 16 * k);
   }
-  f32x4 acc[2][8];
-  float m[2], sum[2];
+  f32x16 acc[4];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    m[u] = -INFINITY;
-    sum[u] = 0.0f;
+  for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int d = 0; d < 8; ++d) acc[u][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const T *kb = reinterpret_cast<const T *>(p.k) + ks * p.k_st + h * p.k_sh;
-  const T *vb = reinterpret_cast<const T *>(p.v) + ks * p.v_st + h * p.v_sh;
-  const T *rb = reinterpret_cast<const T *>(p.kr) + ks * p.kr_st;
+    for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
+  float m = -INFINITY, sum = 0.0f;  // the row's maximum (log2 units), the sum over the lane's keys
+  // places of the transposing value reads: keys 4 g2 + row, dims 16 (lane / 16 % 2) + 4 (lane % 4)
+  int v_at[2][4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      v_at[u][d] = wide_at(8 * u + 4 * g2 + ((lane & 15) >> 2), 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
 
   for (int tile = 0; tile < tiles; ++tile) {
+    landed_and_barrier();  // this tile is there, and the one before is consumed
+    if (tile + 1 < tiles) stage(tile + 1);
+    const char *buf = smem + (tile & 1) * kTileBytes;
     const int j0 = tile * kKeys;
-    i32x4 kw[4], vw[4], rw[2];
+    // ---- S^T = K Q^T, 32 keys at a time ----
+    f32x16 sc[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = i * 256 + tid, row = n >> 4, c = n & 15;
-      const bool in = j0 + row < nk;
-      kw[i] = *reinterpret_cast<const i32x4 *>((in ? kb + (int64_t)(j0 + row) * p.k_st : reinterpret_cast<const T *>(kZeroRow)) + 8 * c);
-      vw[i] = *reinterpret_cast<const i32x4 *>((in ? vb + (int64_t)(j0 + row) * p.v_st : reinterpret_cast<const T *>(kZeroRow)) + 8 * c);
-    }
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int n = i * 256 + tid, row = n >> 3, c = n & 7;
-      const bool in = j0 + row < nk;
-      rw[i] = *reinterpret_cast<const i32x4 *>((in ? rb + (int64_t)(j0 + row) * p.kr_st : reinterpret_cast<const T *>(kZeroRow)) + 8 * c);
-    }
-    __syncthreads();  // the tile before is consumed
+      for (int e = 0; e < 16; ++e) sc[kb2][e] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = i * 256 + tid, row = n >> 4, c = n & 15;
-      *reinterpret_cast<i32x4 *>(s.k + wide_at(row, c)) = kw[i];
-      *reinterpret_cast<i32x4 *>(s.v + wide_at(row, c)) = vw[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int n = i * 256 + tid, row = n >> 3, c = n & 7;
-      *reinterpret_cast<i32x4 *>(s.kr + narrow_at(row, c)) = rw[i];
-    }
-    __syncthreads();
-    // ---- S^T = K Q^T ----
-    f32x4 sc[2][4];
-#pragma unroll
-    for (int tb = 0; tb < 4; ++tb) {
-      sc[0][tb] = sc[1][tb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < 6; ++k) {
-        const i32x4 a = k < 4 ? *reinterpret_cast<const i32x4 *>(s.k + wide_at(16 * tb + n16, 4 * k + g4))
-                              : *reinterpret_cast<const i32x4 *>(s.kr + narrow_at(16 * tb + n16, 4 * (k - 4) + g4));
-#pragma unroll
-        for (int u = 0; u < 2; ++u) sc[u][tb] = mfma<T>(a, q[u][k], sc[u][tb]);
+      for (int k = 0; k < kSlices; ++k) {
+        const char *at = k < kDim / 16 ? buf + wide_at(32 * kb2 + n32, 2 * k + g2)
+                                       : buf + 2 * kWideBytes + narrow_at(32 * kb2 + n32, 2 * (k - kDim / 16) + g2);
+        sc[kb2] = mfma32<T>(*reinterpret_cast<const i32x4 *>(at), q[k], sc[kb2]);
       }
     }
-    // ---- softmax of the wave's rows ----
-    i32x4 pb[2][2];
+    if (j0 + kKeys - 1 > min(wave_lim, nk - 1)) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float mx = -INFINITY;
+      for (int kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
-      for (int tb = 0; tb < 4; ++tb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = j0 + 16 * tb + 4 * g4 + i;
-          sc[u][tb][i] = j <= lim[u] ? sc[u][tb][i] * p.c_log2 : -INFINITY;
-          mx = fmaxf(mx, sc[u][tb][i]);
-        }
-      mx = fmaxf(m[u], max_groups(mx));
-      const float use = mx == -INFINITY ? 0.0f : mx;
-      const float alpha = exp2f(m[u] - use);
-      m[u] = mx;
-      float add = 0.0f;
-#pragma unroll
-      for (int tb = 0; tb < 4; ++tb) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sc[u][tb][i] = exp2f(sc[u][tb][i] - use);
-          add += sc[u][tb][i];
-        }
-        pb[u][tb >> 1][2 * (tb & 1)] = pack2<T>(sc[u][tb][0], sc[u][tb][1]);
-        pb[u][tb >> 1][2 * (tb & 1) + 1] = pack2<T>(sc[u][tb][2], sc[u][tb][3]);
-      }
-      sum[u] = sum[u] * alpha + add;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) acc[u][d] *= alpha;
+        for (int e = 0; e < 16; ++e)
+          sc[kb2][e] = j0 + 32 * kb2 + 8 * (e >> 2) + 4 * g2 + (e & 3) <= lim ? sc[kb2][e] : -INFINITY;
     }
+    // ---- softmax ----
+    float mx = fmaxf(sc[0][0], sc[1][0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(sc[0][e], sc[1][e]));
+    mx = max_halves(mx) * p.c_log2;
+    if (__any(mx > m + kRescale)) {
+      const float next = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));  // 0 before the first key
+      m = next;
+      sum *= alpha;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) acc[d] *= alpha;
+    }
+    const float use = m == -INFINITY ? 0.0f : m;
+    float add[2] = {0.0f, 0.0f};
+    i32x4 pb[4];  // P^T by 16 keys: slot (g, j) is key 4 g + j (j < 4) or 8 + 4 g + j - 4
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb2][e], p.c_log2, -use));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb2][e + 1], p.c_log2, -use));
+        add[0] += x;
+        add[1] += y;
+        pb[2 * kb2 + (e >> 3)][(e & 7) >> 1] = pack2<T>(x, y);
+      }
+    sum += add[0] + add[1];
     // ---- O^T += V^T P^T ----
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
+    for (int st = 0; st < 4; ++st)
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const int row = 32 * st + 4 * g4 + (n16 >> 2), c = 2 * d + ((n16 >> 1) & 1);
-        const i32x2 lo = read_tr(s.v + wide_at(row, c) + 8 * (n16 & 1));
-        const i32x2 hi = read_tr(s.v + wide_at(row + 16, c) + 8 * (n16 & 1));
-        const i32x4 a = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-        for (int u = 0; u < 2; ++u) acc[u][d] = mfma<T>(a, pb[u][st], acc[u][d]);
+      for (int d = 0; d < 4; ++d) {
+        const char *at = buf + kWideBytes + 16 * st * kWideRow;
+        const i32x2 lo = read_tr(at + v_at[0][d]), hi = read_tr(at + v_at[1][d]);
+        acc[d] = mfma32<T>(i32x4{lo[0], lo[1], hi[0], hi[1]}, pb[st], acc[d]);
       }
   }
 
+  const float l = sum_halves(sum);
+  if (i >= rows) return;
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
+  T *dst = reinterpret_cast<T *>(p.out) + (qs + i) * p.o_st + h * p.o_sh + 4 * g2;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int i = q0 + wave * kWaveRows + 16 * u + n16;
-    const float l = sum_groups(sum[u]);
-    if (i >= rows) continue;
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
-    T *dst = reinterpret_cast<T *>(p.out) + (qs + i) * p.o_st + h * p.o_sh + 4 * g4;
+  for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      const f32x4 x = acc[u][d] * inv;
-      *reinterpret_cast<i32x2 *>(dst + 16 * d) = i32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
-    }
-    if (p.lse && g4 == 0)
-      p.lse[(qs + i) * p.l_st + h * p.l_sh] = l == 0.0f ? -INFINITY : (m[u] + log2f(l)) * kLn2;
-  }
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<i32x2 *>(dst + 32 * d + 2 * e) =
+          i32x2{pack2<T>(acc[d][e] * inv, acc[d][e + 1] * inv), pack2<T>(acc[d][e + 2] * inv, acc[d][e + 3] * inv)};
+  if (p.lse && g2 == 0) p.lse[(qs + i) * p.l_st + h * p.l_sh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 }  // namespace l20la
@@ -281,9 +278,16 @@ int32_t l20_pd_latent_prompt(const l20_pd_latent_prompt_args *a, void *stream) {
   const unsigned blocks = (unsigned)((p.max_q + l20la::kPromptRows - 1) / l20la::kPromptRows);
   const dim3 grid(blocks * (unsigned)(p.batch * p.heads)), block(64 * l20la::kPromptWaves);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (a->dtype == L20_PD_BF16) hipLaunchKernelGGL((l20la::latent_prompt<__bf16>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((l20la::latent_prompt<_Float16>), grid, block, 0, s, p);
-  const hipError_t e = hipGetLastError();
+  const int lds = 2 * l20la::kTileBytes;  // 80 KB: two workgroups a CU
+  const bool bf = a->dtype == L20_PD_BF16;
+  hipError_t e = hipFuncSetAttribute(bf ? reinterpret_cast<const void *>(&l20la::latent_prompt<__bf16>)
+                                        : reinterpret_cast<const void *>(&l20la::latent_prompt<_Float16>),
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e == hipSuccess) {
+    if (bf) hipLaunchKernelGGL((l20la::latent_prompt<__bf16>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((l20la::latent_prompt<_Float16>), grid, block, lds, s, p);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess) {
     char msg[256];
     snprintf(msg, sizeof(msg), "HIP launch failed: %s", hipGetErrorString(e));
