@@ -70,6 +70,13 @@ template <> __device__ __forceinline__ f32x16 mfma32<_Float16>(i32x4 a, i32x4 b,
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// The same of 8-bit elements: lane i's address is row i / 2, columns 8 (i % 2) .. + 7 of a block of 8 rows by 16
+// columns; lane i receives column i of the eight rows.
+__device__ __forceinline__ i32x2 read_tr8(const char *p) {
+  typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(__attribute__((address_space(3))) char *)(p));
+}
+
 // Reductions by the row swaps of the vector ALU (no LDS round trip): with both operands the same register a
 // swap returns a lane's value and that of the lane 16 (32) away, in one order for both of them.
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
@@ -102,6 +109,9 @@ __device__ __forceinline__ void load_lds(const void *src, void *dst) {
 }
 // The wave's loads have landed, in LDS too, and so have those of the workgroup's other waves.
 __device__ __forceinline__ void landed_and_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// LDS writes of the workgroup's waves are there; loads may be in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // The running maximum of a softmax row moves only when a tile's exceeds it by more than this (log2 units): P is
 // then at most 2^8 where it would be 1, which costs neither type precision (fp16 ends at 2^16).

@@ -86,95 +86,99 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   static constexpr int kWaves = RB == 4 ? 8 : 4;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kRows = 16 * RB;
-  static constexpr int kRowGroups = RB == 4 ? 2 : 1;  // of the score product
-  static constexpr int kRowsPerWave = RB / kRowGroups;  // blocks of 16
+  static constexpr int kTokens = KT == 0 || RB == 4 ? 64 : 32;  // of a step: what two LDS buffers hold
+  static constexpr int kSteps = kTile / kTokens;
+  // the score product: a wave takes one block of 16 rows and kBlocks blocks of 16 tokens
+  static constexpr int kTokBlocks = kTokens / 16;
+  static constexpr int kGroups = kWaves / RB < kTokBlocks ? kWaves / RB : kTokBlocks;
+  static constexpr int kBlocks = kTokBlocks / kGroups;
   static constexpr int kSlices = (RANK + kRope) / 32;
-  static constexpr int kLatSlices = RANK / 32;
-  static constexpr int kDimBlocks = RANK / 16 / kWaves;  // value dims a wave owns, in blocks of 16
-  static constexpr int kLatRow = RANK * 2, kRopeRow = kRope * 2, kPRow = kTile * 2;  // bytes
-  static constexpr int kLatBytes = kTile * kLatRow, kRopeBytes = kTile * kRopeRow;
-  // 16-byte pieces of the cache that a thread stages
-  static constexpr int kPiece = KT == 0 ? 16 : 8;  // elements
-  static constexpr int kLatPieces = kTile * RANK / kPiece / kThreads;
-  static constexpr int kRopePieces = (kTile * kRope / kPiece + kThreads - 1) / kThreads;
+  // the value product: a wave takes kDimBlocks blocks of 16 dims, all rows
+  static constexpr int kDimBlocks = RANK / 16 / kWaves;
+  static constexpr int kBytes = KT == 0 ? 1 : 2;  // of a cached element
+  static constexpr int kLatRow = RANK * kBytes, kRopeRow = kRope * kBytes, kPRow = kTokens * 2;
+  static constexpr int kLatBytes = kTokens * kLatRow, kRopeBytes = kTokens * kRopeRow;
 
   struct Shared {
-    alignas(16) char lat[kLatBytes];
-    alignas(16) char rope[kRopeBytes];
+    alignas(16) char lat[2][kLatBytes];
+    alignas(16) char rope[2][kRopeBytes];
     alignas(16) char p[kRows * kPRow];
     alignas(16) float max4[kRows][4];
-    float sum4[kRows][4];
+    alignas(16) float sum4[kRows][4];
     int wave[kWaves];
     int start[2];
+    int rescale[2];
   };
 
-  // Where chunk c (16 bytes) of a tile row lies.
+  // Where chunk c (16 bytes) of a row lies: rows are spread so that 16 of them read at one chunk, and the 4 (8)
+  // of a transposing read, meet all LDS banks.
   static __device__ __forceinline__ int lat_at(int row, int c) { return row * kLatRow + ((c ^ (row & 15)) << 4); }
-  static __device__ __forceinline__ int rope_at(int row, int c) { return row * kRopeRow + ((c ^ ((row >> 1) & 7)) << 4); }
-  static __device__ __forceinline__ int p_at(int row, int c) { return row * kPRow + ((c ^ ((row >> 1) & 7)) << 4); }
+  static __device__ __forceinline__ int rope_swizzle(int row) { return KT == 0 ? (row >> 2) & 3 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int rope_at(int row, int c) { return row * kRopeRow + ((c ^ rope_swizzle(row)) << 4); }
+  static __device__ __forceinline__ int p_at(int row, int c) {
+    return row * kPRow + ((c ^ (kTokens == 64 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
+  }
 
-  // The staged pieces of one tile.
-  struct Stage {
-    i32x4 lat[kLatPieces], rope[kRopePieces];
+  // ---- the stream of steps of a group's run, across its sequences ----
+  struct Fetch {
+    int at, last;             // step of the run, its end
+    int b, end;               // sequence, its last step + 1
+    int t0, tokens;           // first token of the step, of the sequence
+    int window, pid;          // lane k of pid: cache block k of the window's 64 (16 tokens each), -1 for none
   };
-  // Blocks: lane k of `pid` holds the cache block (16 tokens) k of a window of 64, -1 for none.
-  static __device__ __forceinline__ int window(const DecodeParams &p, int b, int first_block) {
+  static __device__ __forceinline__ int blocks_of_window(const DecodeParams &p, int b, int first_block) {
     const int blk = first_block + (int)(threadIdx.x & 63);
     if (blk >= p.table_blocks) return -1;
     const int page = p.table[b * p.t_sr + blk / p.per_page];
     const int64_t id = (int64_t)page * p.per_page + blk % p.per_page;
     return page < 0 || id >= p.blocks ? -1 : (int)id;
   }
-  // Row `row` (0..63) of the tile whose blocks are lanes 4 k .. 4 k + 3 of pid: its address, or zeros.
-  static __device__ __forceinline__ const uint8_t *row_of(const DecodeParams &p, const int (&blk)[4], int row, int tokens) {
-    const int k = row >> 4;
-    const int id = k == 0 ? blk[0] : k == 1 ? blk[1] : k == 2 ? blk[2] : blk[3];
-    return id < 0 || row >= tokens ? reinterpret_cast<const uint8_t *>(kZeroRow)
-                                   : p.cache + (int64_t)id * p.c_block + (row & 15) * p.c_tok;
-  }
-  static __device__ __forceinline__ void load(const DecodeParams &p, Stage &st, const int (&blk)[4], int tokens) {
-    constexpr int kLatCols = RANK / kPiece, kRopeCols = kRope / kPiece;
+  // Start the loads of step f.at into buffer `buf` and move on.  Tokens past the end, or without a page, are
+  // zeros: their scores are masked, but 0 x NaN is NaN in the value product.
+  static __device__ __forceinline__ void stage(const DecodeParams &p, Shared &s, Fetch &f, int buf, int wave, int lane) {
+    if (f.at == f.end) {
+      ++f.b;
+      f.tokens = seq_tokens(p, f.b);
+      f.end += tiles_of(f.tokens) * kSteps;
+      f.t0 = 0;
+      f.window = -1;
+    }
+    if (f.t0 >> 10 != f.window) {
+      f.window = f.t0 >> 10;
+      f.pid = blocks_of_window(p, f.b, f.window * 64);
+    }
+    const int left = f.tokens - f.t0, blk0 = (f.t0 >> 4) & 63;
+    constexpr int kLat = kLatBytes / 1024 / kWaves;  // instructions of a wave
+    constexpr int kChunks = kLatRow / 16;
 #pragma unroll
-    for (int i = 0; i < kLatPieces; ++i) {
-      const int n = i * kThreads + threadIdx.x, row = n / kLatCols, col = n % kLatCols;
-      st.lat[i] = *reinterpret_cast<const i32x4 *>(row_of(p, blk, row, tokens) + 16 * col);
+    for (int i = 0; i < kLat; ++i) {
+      const int at = (wave * kLat + i) * 1024;  // of the buffer
+      const int row = at / kLatRow + lane / kChunks;
+      const int id = __builtin_amdgcn_readlane(f.pid, blk0 + (at / kLatRow >> 4));
+      const int c = (lane % kChunks) ^ (row & 15);
+      const uint8_t *src = p.cache + (int64_t)id * p.c_block + (int64_t)(row & 15) * p.c_tok;
+      src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src;
+      load_lds(src + 16 * c, s.lat[buf] + at);
     }
+    constexpr int kRopeInstr = kRopeBytes / 1024;  // of all waves
 #pragma unroll
-    for (int i = 0; i < kRopePieces; ++i) {
-      const int n = i * kThreads + threadIdx.x, row = n / kRopeCols, col = n % kRopeCols;
-      if (kTile * kRopeCols % kThreads == 0 || n < kTile * kRopeCols)
-        st.rope[i] = *reinterpret_cast<const i32x4 *>(row_of(p, blk, row, tokens) + RANK * (KT == 0 ? 1 : 2) + 16 * col);
+    for (int i = 0; i < (kRopeInstr + kWaves - 1) / kWaves; ++i) {
+      const int n = i * kWaves + wave;
+      if (kRopeInstr % kWaves && n >= kRopeInstr) break;
+      const int at = n * 1024;
+      const int row = at / kRopeRow + lane / (kRopeRow / 16);
+      const int id = __builtin_amdgcn_readlane(f.pid, blk0 + (at / kRopeRow >> 4));
+      const int c = (lane % (kRopeRow / 16)) ^ rope_swizzle(row);
+      const uint8_t *src = p.cache + (int64_t)id * p.c_block + (int64_t)(row & 15) * p.c_tok;
+      src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src + RANK * kBytes;
+      load_lds(src + 16 * c, s.rope[buf] + at);
     }
-  }
-  static __device__ __forceinline__ void put(char *base, int at0, int at1, i32x4 w) {
-    if constexpr (KT == 0) {
-      const i32x2 a = fp8x4<T>(w[0]), b = fp8x4<T>(w[1]), c = fp8x4<T>(w[2]), d = fp8x4<T>(w[3]);
-      *reinterpret_cast<i32x4 *>(base + at0) = i32x4{a[0], a[1], b[0], b[1]};
-      *reinterpret_cast<i32x4 *>(base + at1) = i32x4{c[0], c[1], d[0], d[1]};
-    } else {
-      *reinterpret_cast<i32x4 *>(base + at0) = w;
-    }
-  }
-  static __device__ __forceinline__ void store(Shared &s, const Stage &st) {
-    constexpr int kLatCols = RANK / kPiece, kRopeCols = kRope / kPiece;
-    constexpr int kChunks = KT == 0 ? 2 : 1;
-#pragma unroll
-    for (int i = 0; i < kLatPieces; ++i) {
-      const int n = i * kThreads + threadIdx.x, row = n / kLatCols, col = n % kLatCols;
-      put(s.lat, lat_at(row, kChunks * col), lat_at(row, kChunks * col + 1), st.lat[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kRopePieces; ++i) {
-      const int n = i * kThreads + threadIdx.x, row = n / kRopeCols, col = n % kRopeCols;
-      if (kTile * kRopeCols % kThreads == 0 || n < kTile * kRopeCols)
-        put(s.rope, rope_at(row, kChunks * col), rope_at(row, kChunks * col + 1), st.rope[i]);
-    }
+    ++f.at;
+    f.t0 += kTokens;
   }
 
   static __device__ __forceinline__ void run(const DecodeParams &p, Shared &s) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n16 = lane & 15, g4 = lane >> 4;
-    const int tok_block = wave & 3, row_group = wave >> 2;
     // Workgroup (group, row block): the row blocks of a group follow at a distance of 8, on one XCD, whose L2
     // then serves the tile to all but one of them.
     const int unit = blockIdx.x >> 3;
@@ -195,6 +199,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       if (lane >= off) inc += y;
     }
     if (lane == 63) s.wave[wave] = inc;
+    if (tid < 2) s.rescale[tid] = 0;
     __syncthreads();
     int total = 0;
 #pragma unroll
@@ -220,166 +225,204 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     int b = __builtin_amdgcn_readfirstlane(s.start[0]);
     int base = __builtin_amdgcn_readfirstlane(s.start[1]);
 
+    Fetch f;
+    f.at = first * kSteps;
+    f.last = last * kSteps;
+    f.b = b;
+    f.tokens = seq_tokens(p, b);
+    f.end = (base + tiles_of(f.tokens)) * kSteps;
+    f.t0 = (first - base) * kTile;
+    f.window = -1;
+    f.pid = -1;
+    stage(p, s, f, 0, wave, lane);
+
     // ---- one segment a sequence ----
+    int buf = 0;
     for (int at = first; at < last; ++b) {
-      const int tokens = seq_tokens(p, b), len = p.lens[b], tiles = tiles_of(tokens);
+      const int tokens = seq_tokens(p, b), tiles = tiles_of(tokens);
       const int seg_end = min(last, base + tiles);
-      segment(p, s, b, rblk, group, base, tiles, at, seg_end, first, tokens, len, lane, wave, n16, g4, tok_block,
-              row_group);
+      // (its last step may be all past the end where a step is less than a tile: it is computed, masked)
+      segment(p, s, f, buf, b, rblk, group, base, at, seg_end, seg_end == base + tiles, first, tokens, wave, lane);
       at = seg_end;
       base += tiles;
     }
   }
 
-  static __device__ __forceinline__ void segment(const DecodeParams &p, Shared &s, int b, int rblk, int group, int base,
-                                                 int tiles, int at, int seg_end, int first, int tokens, int len, int lane,
-                                                 int wave, int n16, int g4, int tok_block, int row_group) {
-    // rows of the score product (two blocks at most) and of the value product (all)
-    i32x4 q[kRowsPerWave][kSlices];
-    int lim[kRowsPerWave];
-#pragma unroll
-    for (int u = 0; u < kRowsPerWave; ++u) {
-      const int r = rblk * kRows + 16 * (row_group * kRowsPerWave + u) + n16;
+  static __device__ __forceinline__ void segment(const DecodeParams &p, Shared &s, Fetch &f, int &buf, int b, int rblk,
+                                                 int group, int base, int at, int seg_end, bool ends, int first,
+                                                 int tokens, int wave, int lane) {
+    const int n16 = lane & 15, g4 = lane >> 4;
+    const int own = wave % RB, tg = wave / RB;  // block of rows, group of tokens of the score product
+    const bool scores = tg < kGroups;
+    const int len = p.lens[b];
+    i32x4 q[kSlices];
+    int lim;
+    {
+      const int r = rblk * kRows + 16 * own + n16;
       const bool live = r < p.rows;
       const int i = live ? r / p.heads : 0, h = live ? r - i * p.heads : 0;
-      lim[u] = live ? len - p.q_len + i : -1;
-      const T *src = reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + h * p.q_sh + 8 * g4;
+      lim = live ? min(len - p.q_len + i, tokens - 1) : -1;
+      // the order of the dims in the product is free: over an fp8 cache a lane's are 16 in a row of each 64, so
+      // that one 16-byte read gives two slices
+      const T *src = reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + h * p.q_sh;
 #pragma unroll
       for (int k = 0; k < kSlices; ++k) {
-        const i32x4 w = *reinterpret_cast<const i32x4 *>(src + 32 * k);
-        q[u][k] = live ? w : i32x4{0, 0, 0, 0};
+        const int d = KT == 0 ? 64 * (k >> 1) + 16 * g4 + 8 * (k & 1) : 32 * k + 8 * g4;
+        const i32x4 w = *reinterpret_cast<const i32x4 *>(src + d);
+        q[k] = live ? w : i32x4{0, 0, 0, 0};
       }
     }
     f32x4 acc[RB][kDimBlocks];
-    float m_all[RB];       // running maximum of the lane's row in each block, log2 units
-    float sum[kRowsPerWave];  // of the lane's own tokens
+    float m_all[RB];  // the maximum that P of the lane's row in each block refers to, log2 units
+    float m_own = -INFINITY, sum = 0.0f;  // of the wave's own block, its tokens
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       m_all[r] = -INFINITY;
 #pragma unroll
       for (int d = 0; d < kDimBlocks; ++d) acc[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-#pragma unroll
-    for (int u = 0; u < kRowsPerWave; ++u) sum[u] = 0.0f;
+    // LDS places of the lane's operands at token block 0 and dim 0; the others differ by an XOR of the chunk
+    int k_at = lat_at(16 * (scores ? tg * kBlocks : 0) + n16, g4);
+    int r_at = rope_at(16 * (scores ? tg * kBlocks : 0) + n16, g4);
+    int v_at = KT == 0 ? lat_at(8 * g4 + (n16 >> 1), wave * kDimBlocks) + 8 * (n16 & 1)
+                       : lat_at(8 * g4 + (n16 >> 2), 2 * wave * kDimBlocks + ((n16 >> 1) & 1)) + 8 * (n16 & 1);
 
-    // LDS places of the lane's operands
-    int v_lo[kDimBlocks], v_hi[kDimBlocks];
+    int t0 = (at - base) * kTile;
+    for (int step = at * kSteps; step < seg_end * kSteps; ++step, t0 += kTokens, buf ^= 1) {
+      const int blk0 = (t0 >> 4) & 63;
+      int bad = 0;  // token blocks without a page (f is still at this step)
 #pragma unroll
-    for (int d = 0; d < kDimBlocks; ++d) {
-      const int c = 2 * (wave * kDimBlocks + d) + ((n16 >> 1) & 1);
-      v_lo[d] = lat_at(8 * g4 + (n16 >> 2), c) + 8 * (n16 & 1);
-      v_hi[d] = lat_at(8 * g4 + 4 + (n16 >> 2), c) + 8 * (n16 & 1);
-    }
+      for (int k = 0; k < kTokBlocks; ++k) bad |= __builtin_amdgcn_readlane(f.pid, blk0 + k) < 0 ? 1 << k : 0;
+      const bool whole = t0 + kTokens <= min(tokens, len - p.q_len + 1) && !bad;
+      landed_and_barrier();  // this step is there, and the one before is consumed
+      if (wave == 0) s.rescale[buf ^ 1] = 0;
+      if (f.at < f.last) stage(p, s, f, buf ^ 1, wave, lane);
+      const char *lat = s.lat[buf], *rope = s.rope[buf];
+      asm volatile("" : "+v"(k_at), "+v"(r_at), "+v"(v_at));  // (not loop invariant: hoisted, they take 30 registers)
 
-    int win = -1, pid = -1;
-    for (int tile = at; tile < seg_end; ++tile) {
-      const int t0 = (tile - base) * kTile;  // first token
-      if ((t0 >> 10) != win) {
-        win = t0 >> 10;
-        pid = window(p, b, win * 64);
-      }
-      int blk[4];
+      // ---- S^T = K Q^T ----
+      f32x4 sc[kBlocks];
+      float mx = -INFINITY;
+      if (scores) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) blk[k] = __builtin_amdgcn_readlane(pid, ((t0 >> 4) & 63) + k);
-      Stage st;
-      load(p, st, blk, tokens - t0);
-      __syncthreads();  // the tile before is consumed
-      store(s, st);
-      __syncthreads();
-
-      // ---- S^T = K Q^T: 16 tokens, the wave's rows ----
-      f32x4 sc[kRowsPerWave];
+        for (int u = 0; u < kBlocks; ++u) {
+          const char *ku = lat + u * 16 * kLatRow, *ru = rope + u * 16 * kRopeRow;
+          f32x4 part[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+          if constexpr (KT == 0) {
 #pragma unroll
-      for (int u = 0; u < kRowsPerWave; ++u) sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int trow = 16 * tok_block + n16;
+            for (int k = 0; k < kSlices; k += 2) {
+              const char *src = 32 * k < RANK ? ku + (k_at ^ ((k / 2 & 3) << 6)) + (k / 2 >> 2) * 256 : ru + r_at;
+              const i32x4 w = *reinterpret_cast<const i32x4 *>(src);
+              const i32x2 c0 = fp8x4<T>(w[0]), c1 = fp8x4<T>(w[1]), c2 = fp8x4<T>(w[2]), c3 = fp8x4<T>(w[3]);
+              part[0] = mfma<T>(i32x4{c0[0], c0[1], c1[0], c1[1]}, q[k], part[0]);
+              part[1] = mfma<T>(i32x4{c2[0], c2[1], c3[0], c3[1]}, q[k + 1], part[1]);
+            }
+          } else {
 #pragma unroll
-      for (int k = 0; k < kSlices; ++k) {
-        const i32x4 a = k < kLatSlices
-                            ? *reinterpret_cast<const i32x4 *>(s.lat + lat_at(trow, 4 * k + g4))
-                            : *reinterpret_cast<const i32x4 *>(s.rope + rope_at(trow, 4 * (k - kLatSlices) + g4));
-#pragma unroll
-        for (int u = 0; u < kRowsPerWave; ++u) sc[u] = mfma<T>(a, q[u][k], sc[u]);
-      }
-      // ---- scores in log2 units, masked; the block's row maxima ----
-      const int my_blk = tok_block == 0 ? blk[0] : tok_block == 1 ? blk[1] : tok_block == 2 ? blk[2] : blk[3];
-#pragma unroll
-      for (int u = 0; u < kRowsPerWave; ++u) {
-        const int hide = my_blk < 0 ? -1 : min(lim[u], tokens - 1);
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = t0 + 16 * tok_block + 4 * g4 + i;
-          sc[u][i] = t <= hide ? sc[u][i] * p.c_log2 : -INFINITY;
-          mx = fmaxf(mx, sc[u][i]);
+            for (int k = 0; k < kSlices; ++k) {
+              const char *src = 32 * k < RANK ? ku + (k_at ^ ((k & 3) << 6)) + (k >> 2) * 256
+                                              : ru + (r_at ^ ((k - RANK / 32) << 6));
+              part[k & 1] = mfma<T>(*reinterpret_cast<const i32x4 *>(src), q[k], part[k & 1]);
+            }
+          }
+          sc[u] = part[0] + part[1];
         }
-        mx = max_groups(mx);
-        if (g4 == 0) s.max4[16 * (row_group * kRowsPerWave + u) + n16][tok_block] = mx;
-      }
-      __syncthreads();
-      // ---- new maxima, P ----
-      float alpha[RB];
-      float m_use[RB];
+        if (!whole) {
 #pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const f32x4 m4 = *reinterpret_cast<const f32x4 *>(s.max4[16 * r + n16]);
-        const float m = fmaxf(m_all[r], fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-        m_use[r] = m == -INFINITY ? 0.0f : m;
-        alpha[r] = exp2f(m_all[r] - m_use[r]);  // 0 before the first visible token
-        m_all[r] = m;
-      }
+          for (int u = 0; u < kBlocks; ++u) {
+            const int tb = tg * kBlocks + u;
+            const int hide = bad >> tb & 1 ? -1 : lim;
 #pragma unroll
-      for (int u = 0; u < kRowsPerWave; ++u) {
-        const int rb = row_group * kRowsPerWave + u;
-        float m = m_use[u], al = alpha[u];
-        if constexpr (kRowGroups == 2) {
-          m = row_group ? m_use[kRowsPerWave + u] : m;
-          al = row_group ? alpha[kRowsPerWave + u] : al;
+            for (int i = 0; i < 4; ++i) sc[u][i] = t0 + 16 * tb + 4 * g4 + i <= hide ? sc[u][i] : -INFINITY;
+          }
         }
-        float e[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = exp2f(sc[u][i] - m);
-        sum[u] = sum[u] * al + ((e[0] + e[1]) + (e[2] + e[3]));
-        *reinterpret_cast<i32x2 *>(s.p + p_at(16 * rb + n16, 2 * tok_block + (g4 >> 1)) + 8 * (g4 & 1)) =
-            i32x2{pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3])};
+        for (int u = 0; u < kBlocks; ++u) mx = fmaxf(mx, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
+        mx = max_groups(mx) * p.c_log2;
       }
-      __syncthreads();
+      // ---- P from the maximum so far; where a row exceeds that by much, all waves go back and move it ----
+      float add = 0.0f;
+      auto weights = [&]() {
+        const float use = m_own == -INFINITY ? 0.0f : m_own;
+        add = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kBlocks; ++u) {
+          const int tb = tg * kBlocks + u;
+          float e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], p.c_log2, -use));
+          add += (e[0] + e[1]) + (e[2] + e[3]);
+          *reinterpret_cast<i32x2 *>(s.p + p_at(16 * own + n16, 2 * tb + (g4 >> 1)) + 8 * (g4 & 1)) =
+              i32x2{pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3])};
+        }
+      };
+      if (scores) {
+        weights();
+        if (__any(mx > m_own + kRescale) && lane == 0) s.rescale[buf] = 1;
+      }
+      lds_barrier();
+      if (__builtin_amdgcn_readfirstlane(s.rescale[buf])) {  // the same for all waves
+        if (g4 == 0) s.max4[16 * own + n16][tg] = mx;
+        lds_barrier();
+        float alpha_own = 1.0f;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          const f32x4 m4 = *reinterpret_cast<const f32x4 *>(s.max4[16 * r + n16]);
+          float m = fmaxf(m4[0], m4[1]);
+          if constexpr (kWaves / RB == 4) m = fmaxf(m, fmaxf(m4[2], m4[3]));
+          m = fmaxf(m_all[r], m);
+          const float alpha = __builtin_amdgcn_exp2f(m_all[r] - (m == -INFINITY ? 0.0f : m));  // 0 before the first token
+          m_all[r] = m;
+#pragma unroll
+          for (int d = 0; d < kDimBlocks; ++d) acc[r][d] *= alpha;
+          m_own = r == own ? m : m_own;
+          alpha_own = r == own ? alpha : alpha_own;
+        }
+        sum *= alpha_own;
+        if (scores) weights();
+        lds_barrier();
+      }
+      sum += add;
       // ---- O^T += V^T P^T: the wave's dims, all rows ----
 #pragma unroll
-      for (int r = 0; r < RB; ++r)
-#pragma unroll
-        for (int d = 0; d < kDimBlocks; ++d) acc[r][d] *= alpha[r];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
+      for (int ks = 0; ks < kTokens / 32; ++ks) {
         i32x4 pb[RB];
 #pragma unroll
         for (int r = 0; r < RB; ++r) pb[r] = *reinterpret_cast<const i32x4 *>(s.p + p_at(16 * r + n16, 4 * ks + g4));
 #pragma unroll
         for (int d = 0; d < kDimBlocks; ++d) {
-          const i32x2 lo = read_tr(s.lat + ks * 32 * kLatRow + v_lo[d]);
-          const i32x2 hi = read_tr(s.lat + ks * 32 * kLatRow + v_hi[d]);
-          const i32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+          i32x4 a;
+          if constexpr (KT == 0) {
+            const i32x2 w = read_tr8(lat + ks * 32 * kLatRow + (v_at ^ (d << 4)));
+            const i32x2 lo = fp8x4<T>(w[0]), hi = fp8x4<T>(w[1]);
+            a = i32x4{lo[0], lo[1], hi[0], hi[1]};
+          } else {
+            // (four rows on, the swizzle differs in chunk bit 2)
+            const i32x2 lo = read_tr(lat + ks * 32 * kLatRow + (v_at ^ (d << 5)));
+            const i32x2 hi = read_tr(lat + (ks * 32 + 4) * kLatRow + (v_at ^ (d << 5) ^ 64));
+            a = i32x4{lo[0], lo[1], hi[0], hi[1]};
+          }
 #pragma unroll
           for (int r = 0; r < RB; ++r) acc[r][d] = mfma<T>(a, pb[r], acc[r][d]);
         }
       }
     }
 
-    // ---- the rows' sums, over lane groups and the waves of a row group ----
-#pragma unroll
-    for (int u = 0; u < kRowsPerWave; ++u) {
-      const float x = sum_groups(sum[u]);
-      if (g4 == 0) s.sum4[16 * (row_group * kRowsPerWave + u) + n16][tok_block] = x;
-    }
-    __syncthreads();
-    const bool whole = at == base && seg_end == base + tiles;
+    // ---- the rows' sums, over lane groups and token groups ----
+    sum = sum_groups(sum);
+    if (g4 == 0) s.sum4[16 * own + n16][tg] = sum;
+    lds_barrier();
+    const bool all = at == base && ends;
     const int slot = base < first ? 2 * group : 2 * group + 1;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const int lr = 16 * r + n16;
       const int row = rblk * kRows + lr;
-      const float l = (s.sum4[lr][0] + s.sum4[lr][1]) + (s.sum4[lr][2] + s.sum4[lr][3]);
+      const f32x4 l4 = *reinterpret_cast<const f32x4 *>(s.sum4[lr]);
+      float l = l4[0] + l4[1];
+      if constexpr (kWaves / RB == 4) l += l4[2] + l4[3];
       if (row >= p.rows) continue;
-      if (whole) {
+      if (all) {
         const int i = row / p.heads, h = row - i * p.heads;
         const int64_t orow = (int64_t)b * p.q_len + i;
         const float inv = l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
@@ -400,12 +443,11 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         if (wave == 0 && g4 == 0) *reinterpret_cast<f32x2 *>(p.part_ml + 2 * prow) = f32x2{m_all[r], l};
       }
     }
-    __syncthreads();  // the sums are read before the next segment's
   }
 };
 
 template <typename T, int KT, int RANK, int RB>
-__global__ __launch_bounds__((Partial<T, KT, RANK, RB>::kThreads)) void latent_partial(DecodeParams p) {
+__global__ __launch_bounds__((Partial<T, KT, RANK, RB>::kThreads), 2) void latent_partial(DecodeParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Partial<T, KT, RANK, RB>::run(p, *reinterpret_cast<typename Partial<T, KT, RANK, RB>::Shared *>(smem));
 }
@@ -488,7 +530,7 @@ int64_t tiles_bound(const l20_pd_latent_args &a) {
 // Runs of tiles: as many as workgroups fit the chip at once, a multiple of 8 (the XCDs), no more than tiles.
 int groups_of(const l20_pd_latent_args &a, int cus) {
   const int64_t rows = rows_of(a), rblocks = (rows + 16 * blocks_of(rows) - 1) / (16 * blocks_of(rows));
-  const int64_t fit = std::max<int64_t>(1, cus / rblocks);
+  const int64_t fit = std::max<int64_t>(1, cus * (rows <= 32 ? 2 : 1) / rblocks);
   return (int)((std::min(fit, tiles_bound(a)) + 7) / 8 * 8);
 }
 int64_t workspace_bytes(const l20_pd_latent_args &a, int cus) {
