@@ -98,7 +98,7 @@ int32_t l20_pd_latent_rope_and_cache(const l20_pd_latent_write_args *args, void 
  * page outside [0, num_pages), or beyond max_seq_len, are masked for every row.  The tokens of one sequence are read in tiles:
  * a value that is not finite in a token some rows of the sequence see may reach its other rows.
  *
- * The work (64-token tiles of all sequences) is split evenly over the CUs; what a workgroup has of a
+ * The work (tiles of tokens of all sequences) is split evenly over the CUs; what a workgroup has of a
  * sequence that others share goes to `workspace` (l20_pd_paged_latent_workspace bytes, 16-byte aligned)
  * and a second kernel joins the parts.  The workspace's contents before and after do not matter; calls
  * that may overlap each need their own.  max_seq_len sizes the grid and the workspace.
@@ -129,7 +129,7 @@ typedef struct l20_pd_latent_args {
 
 int32_t l20_pd_paged_latent_check(const l20_pd_latent_args *args);
 /* Workspace bytes of a call on a device of cu_count compute units (0: the current device's); reads only
- * batch, q_len, num_heads, rank and max_seq_len.  0 where no workspace is needed. */
+ * batch, q_len, num_heads, rank, cache_dtype and max_seq_len.  0 where no workspace is needed. */
 int64_t l20_pd_paged_latent_workspace(const l20_pd_latent_args *args, int32_t cu_count);
 int32_t l20_pd_paged_latent(const l20_pd_latent_args *args, void *stream);
 

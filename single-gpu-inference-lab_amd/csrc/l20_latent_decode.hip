@@ -26,7 +26,8 @@
 
 namespace l20la {
 
-constexpr int kTile = 64;
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
 
 struct DecodeParams {
   const void *q;
@@ -46,30 +47,16 @@ struct DecodeParams {
   int64_t l_sr, l_sh;
   float *part;     // [slot][row block][row][RANK]
   float *part_ml;  // [slot][row block][row][2]: maximum (log2 units), sum
+  i32x2 *runs;     // [batch]: the first and the last run that hold a part of the sequence
   float c_log2, out_scale;
   int batch, q_len, heads, rows;  // rows = q_len * heads of a sequence
   int groups, row_blocks;
+  int split;  // 0: one run a sequence
 };
 
 __device__ __forceinline__ int seq_tokens(const DecodeParams &p, int b) {
   return min(max(p.lens[b], 0), p.max_tokens);
 }
-// (a sequence without tokens has one tile, all masked: its rows are written too)
-__device__ __forceinline__ int tiles_of(int tokens) { return max(1, (tokens + kTile - 1) / kTile); }
-
-// Workgroup sum of x over NT threads.
-template <int NT> __device__ __forceinline__ int block_sum(int x, int *s_wave) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = x;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) total += s_wave[w];
-  return total;
-}
-
 // Four fp8 codes (one dword) -> two dwords of T, exact.  (Whole words: extracting elements of these
 // conversions' results one by one is miscompiled by the ROCm 7.2 LLVM.)
 template <typename T> __device__ __forceinline__ i32x2 fp8x4(int w);
@@ -83,11 +70,8 @@ template <> __device__ __forceinline__ i32x2 fp8x4<_Float16>(int w) {
 }
 
 template <typename T, int KT, int RANK, int RB> struct Partial {
-  static constexpr int kWaves = RB == 4 ? 8 : 4;
-  static constexpr int kThreads = 64 * kWaves;
   static constexpr int kRows = 16 * RB;
-  static constexpr int kTokens = KT == 0 || RB == 4 ? 64 : 32;  // of a step: what two LDS buffers hold
-  static constexpr int kSteps = kTile / kTokens;
+  static constexpr int kTokens = KT == 0 && RB < 4 ? 128 : 64;  // of a tile: two of them fill the LDS
   // the score product: a wave takes one block of 16 rows and kBlocks blocks of 16 tokens
   static constexpr int kTokBlocks = kTokens / 16;
   static constexpr int kGroups = kWaves / RB < kTokBlocks ? kWaves / RB : kTokBlocks;
@@ -103,8 +87,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     alignas(16) char lat[2][kLatBytes];
     alignas(16) char rope[2][kRopeBytes];
     alignas(16) char p[kRows * kPRow];
-    alignas(16) float max4[kRows][4];
-    alignas(16) float sum4[kRows][4];
+    alignas(16) float max[kRows][kGroups];
+    alignas(16) float sum[kRows][kGroups];
     int wave[kWaves];
     int start[2];
     int rescale[2];
@@ -116,15 +100,18 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   static __device__ __forceinline__ int rope_swizzle(int row) { return KT == 0 ? (row >> 2) & 3 : (row >> 1) & 7; }
   static __device__ __forceinline__ int rope_at(int row, int c) { return row * kRopeRow + ((c ^ rope_swizzle(row)) << 4); }
   static __device__ __forceinline__ int p_at(int row, int c) {
-    return row * kPRow + ((c ^ (kTokens == 64 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
+    return row * kPRow + ((c ^ (kTokens == 64 ? (row >> 1) & 7 : row & 15)) << 4);
   }
 
-  // ---- the stream of steps of a group's run, across its sequences ----
+  // (a sequence without tokens has one tile, all masked: its rows are written too)
+  static __device__ __forceinline__ int tiles_of(int tokens) { return max(1, (tokens + kTokens - 1) / kTokens); }
+
+  // ---- the stream of tiles of a group's run, across its sequences ----
   struct Fetch {
-    int at, last;             // step of the run, its end
-    int b, end;               // sequence, its last step + 1
-    int t0, tokens;           // first token of the step, of the sequence
-    int window, pid;          // lane k of pid: cache block k of the window's 64 (16 tokens each), -1 for none
+    int at, last;     // tile of the run, its end
+    int b, end;       // sequence, its last tile + 1
+    int t0, tokens;   // first token of the tile, tokens of the sequence
+    int window, pid;  // lane k of pid: cache block k of the window's 64 (16 tokens each), -1 for none
   };
   static __device__ __forceinline__ int blocks_of_window(const DecodeParams &p, int b, int first_block) {
     const int blk = first_block + (int)(threadIdx.x & 63);
@@ -133,13 +120,13 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     const int64_t id = (int64_t)page * p.per_page + blk % p.per_page;
     return page < 0 || id >= p.blocks ? -1 : (int)id;
   }
-  // Start the loads of step f.at into buffer `buf` and move on.  Tokens past the end, or without a page, are
+  // Start the loads of tile f.at into buffer `buf` and move on.  Tokens past the end, or without a page, are
   // zeros: their scores are masked, but 0 x NaN is NaN in the value product.
   static __device__ __forceinline__ void stage(const DecodeParams &p, Shared &s, Fetch &f, int buf, int wave, int lane) {
     if (f.at == f.end) {
       ++f.b;
       f.tokens = seq_tokens(p, f.b);
-      f.end += tiles_of(f.tokens) * kSteps;
+      f.end += tiles_of(f.tokens);
       f.t0 = 0;
       f.window = -1;
     }
@@ -186,52 +173,59 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     const int rblk = unit % p.row_blocks;
 
     // ---- this group's run of tiles ----
-    const int chunk = (p.batch + kThreads - 1) / kThreads;
-    int mine = 0;
-    for (int i = 0; i < chunk; ++i) {
-      const int b = tid * chunk + i;
-      if (b < p.batch) mine += tiles_of(seq_tokens(p, b));
-    }
-    int inc = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int y = __shfl_up(inc, off);
-      if (lane >= off) inc += y;
-    }
-    if (lane == 63) s.wave[wave] = inc;
+    int b = group, base = 0, first = 0, last = 0, per = 1;
     if (tid < 2) s.rescale[tid] = 0;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const int v = s.wave[w];
-      if (w < wave) inc += v;
-      total += v;
-    }
-    const int per = (total + p.groups - 1) / p.groups;
-    const int first = min(group * per, total), last = min(first + per, total);
-    if (first >= last) return;  // the whole workgroup
-    if (inc - mine <= first && first < inc) {
-      int base = inc - mine, b = tid * chunk;
-      for (;; ++b) {
-        const int n = tiles_of(seq_tokens(p, b));
-        if (first < base + n) break;
-        base += n;
+    if (!p.split) {
+      if (b >= p.batch) return;  // the whole workgroup
+      last = tiles_of(seq_tokens(p, b));
+    } else {
+      const int chunk = (p.batch + kThreads - 1) / kThreads;
+      int mine = 0;
+      for (int i = 0; i < chunk; ++i) {
+        const int n = tid * chunk + i;
+        if (n < p.batch) mine += tiles_of(seq_tokens(p, n));
       }
-      s.start[0] = b;
-      s.start[1] = base;
+      int inc = mine;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(inc, off);
+        if (lane >= off) inc += y;
+      }
+      if (lane == 63) s.wave[wave] = inc;
+      __syncthreads();
+      int total = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const int v = s.wave[w];
+        if (w < wave) inc += v;
+        total += v;
+      }
+      per = (total + p.groups - 1) / p.groups;
+      first = min(group * per, total);
+      last = min(first + per, total);
+      if (first >= last) return;  // the whole workgroup
+      if (inc - mine <= first && first < inc) {
+        int at = inc - mine, n = tid * chunk;
+        for (;; ++n) {
+          const int tiles = tiles_of(seq_tokens(p, n));
+          if (first < at + tiles) break;
+          at += tiles;
+        }
+        s.start[0] = n;
+        s.start[1] = at;
+      }
+      __syncthreads();
+      b = __builtin_amdgcn_readfirstlane(s.start[0]);
+      base = __builtin_amdgcn_readfirstlane(s.start[1]);
     }
-    __syncthreads();
-    int b = __builtin_amdgcn_readfirstlane(s.start[0]);
-    int base = __builtin_amdgcn_readfirstlane(s.start[1]);
 
     Fetch f;
-    f.at = first * kSteps;
-    f.last = last * kSteps;
+    f.at = first;
+    f.last = last;
     f.b = b;
     f.tokens = seq_tokens(p, b);
-    f.end = (base + tiles_of(f.tokens)) * kSteps;
-    f.t0 = (first - base) * kTile;
+    f.end = base + tiles_of(f.tokens);
+    f.t0 = (first - base) * kTokens;
     f.window = -1;
     f.pid = -1;
     stage(p, s, f, 0, wave, lane);
@@ -241,7 +235,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     for (int at = first; at < last; ++b) {
       const int tokens = seq_tokens(p, b), tiles = tiles_of(tokens);
       const int seg_end = min(last, base + tiles);
-      // (its last step may be all past the end where a step is less than a tile: it is computed, masked)
+      if (p.split && at == base && rblk == 0 && tid == 0) p.runs[b] = i32x2{group, (base + tiles - 1) / per};
       segment(p, s, f, buf, b, rblk, group, base, at, seg_end, seg_end == base + tiles, first, tokens, wave, lane);
       at = seg_end;
       base += tiles;
@@ -287,14 +281,14 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     int v_at = KT == 0 ? lat_at(8 * g4 + (n16 >> 1), wave * kDimBlocks) + 8 * (n16 & 1)
                        : lat_at(8 * g4 + (n16 >> 2), 2 * wave * kDimBlocks + ((n16 >> 1) & 1)) + 8 * (n16 & 1);
 
-    int t0 = (at - base) * kTile;
-    for (int step = at * kSteps; step < seg_end * kSteps; ++step, t0 += kTokens, buf ^= 1) {
+    int t0 = (at - base) * kTokens;
+    for (int tile = at; tile < seg_end; ++tile, t0 += kTokens, buf ^= 1) {
       const int blk0 = (t0 >> 4) & 63;
-      int bad = 0;  // token blocks without a page (f is still at this step)
+      int bad = 0;  // token blocks without a page (f is still at this tile)
 #pragma unroll
       for (int k = 0; k < kTokBlocks; ++k) bad |= __builtin_amdgcn_readlane(f.pid, blk0 + k) < 0 ? 1 << k : 0;
       const bool whole = t0 + kTokens <= min(tokens, len - p.q_len + 1) && !bad;
-      landed_and_barrier();  // this step is there, and the one before is consumed
+      landed_and_barrier();  // this tile is there, and the one before is consumed
       if (wave == 0) s.rescale[buf ^ 1] = 0;
       if (f.at < f.last) stage(p, s, f, buf ^ 1, wave, lane);
       const char *lat = s.lat[buf], *rope = s.rope[buf];
@@ -362,15 +356,14 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       }
       lds_barrier();
       if (__builtin_amdgcn_readfirstlane(s.rescale[buf])) {  // the same for all waves
-        if (g4 == 0) s.max4[16 * own + n16][tg] = mx;
+        if (scores && g4 == 0) s.max[16 * own + n16][tg] = mx;
         lds_barrier();
         float alpha_own = 1.0f;
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
-          const f32x4 m4 = *reinterpret_cast<const f32x4 *>(s.max4[16 * r + n16]);
-          float m = fmaxf(m4[0], m4[1]);
-          if constexpr (kWaves / RB == 4) m = fmaxf(m, fmaxf(m4[2], m4[3]));
-          m = fmaxf(m_all[r], m);
+          float m = m_all[r];
+#pragma unroll
+          for (int k = 0; k < kGroups; ++k) m = fmaxf(m, s.max[16 * r + n16][k]);
           const float alpha = __builtin_amdgcn_exp2f(m_all[r] - (m == -INFINITY ? 0.0f : m));  // 0 before the first token
           m_all[r] = m;
 #pragma unroll
@@ -410,7 +403,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
 
     // ---- the rows' sums, over lane groups and token groups ----
     sum = sum_groups(sum);
-    if (g4 == 0) s.sum4[16 * own + n16][tg] = sum;
+    if (scores && g4 == 0) s.sum[16 * own + n16][tg] = sum;
     lds_barrier();
     const bool all = at == base && ends;
     const int slot = base < first ? 2 * group : 2 * group + 1;
@@ -418,9 +411,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     for (int r = 0; r < RB; ++r) {
       const int lr = 16 * r + n16;
       const int row = rblk * kRows + lr;
-      const f32x4 l4 = *reinterpret_cast<const f32x4 *>(s.sum4[lr]);
-      float l = l4[0] + l4[1];
-      if constexpr (kWaves / RB == 4) l += l4[2] + l4[3];
+      float l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) l += s.sum[lr][k];
       if (row >= p.rows) continue;
       if (all) {
         const int i = row / p.heads, h = row - i * p.heads;
@@ -446,48 +439,43 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   }
 };
 
-template <typename T, int KT, int RANK, int RB>
-__global__ __launch_bounds__((Partial<T, KT, RANK, RB>::kThreads), 2) void latent_partial(DecodeParams p) {
+template <typename T, int KT, int RANK, int RB> __global__ __launch_bounds__(kThreads, 2) void latent_partial(DecodeParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Partial<T, KT, RANK, RB>::run(p, *reinterpret_cast<typename Partial<T, KT, RANK, RB>::Shared *>(smem));
 }
 
-// One workgroup of 256 threads a row: RANK / 4 lanes hold four dims each, the others further parts.
+// One workgroup a row: RANK / 4 lanes hold four dims each, the others take further parts.  Bound by its chain of
+// loads (runs, maxima, parts); no scan of the lengths, the partial kernel has left each sequence's runs.
 template <typename T, int RANK>
-__global__ __launch_bounds__(256) void latent_merge(DecodeParams p, int block_rows) {
-  constexpr int kCols = RANK / 4, kLanes = 256 / kCols;
-  __shared__ int s_wave[4];
-  __shared__ f32x4 s_acc[kLanes][kCols];
-  __shared__ float s_l[kLanes];
+__global__ __launch_bounds__(kThreads) void latent_merge(DecodeParams p, int block_rows) {
+  constexpr int kCols = RANK / 4, kParts = kThreads / kCols;
+  __shared__ f32x4 s_acc[kParts][kCols];
+  __shared__ float s_l[kParts];
   const int b = blockIdx.y, row = blockIdx.x;
-  int before = 0, all = 0;
-  for (int i = threadIdx.x; i < p.batch; i += 256) {
-    const int n = tiles_of(seq_tokens(p, i));
-    all += n;
-    before += i < b ? n : 0;
-  }
-  const int total = block_sum<256>(all, s_wave);
-  const int base = block_sum<256>(before, s_wave);
-  const int per = (total + p.groups - 1) / p.groups;
-  const int end = base + tiles_of(seq_tokens(p, b));
-  const int g0 = base / per, g1 = (end - 1) / per;
+  const i32x2 runs = p.runs[b];
+  const int g0 = runs[0], g1 = runs[1];
   if (g0 == g1) return;  // written already
   const int rblk = row / block_rows, lr = row - rblk * block_rows;
   auto prow = [&](int g) {
-    const int slot = base < g * per ? 2 * g : 2 * g + 1;
+    const int slot = g == g0 ? 2 * g + 1 : 2 * g;
     return ((int64_t)slot * p.row_blocks + rblk) * block_rows + lr;
   };
   float m = -INFINITY;
-  for (int g = g0; g <= g1; ++g) m = fmaxf(m, p.part_ml[2 * prow(g)]);
+  for (int g = g0 + (threadIdx.x & 63); g <= g1; g += 64) m = fmaxf(m, p.part_ml[2 * prow(g)]);
+  m = max_groups(m);
+#pragma unroll
+  for (int off = 8; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
   const float m_use = m == -INFINITY ? 0.0f : m;
   const int col = threadIdx.x % kCols, part = threadIdx.x / kCols;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float l = 0.0f;
-  for (int g = g0 + part; g <= g1; g += kLanes) {
+#pragma unroll 4
+  for (int g = g0 + part; g <= g1; g += kParts) {
     const int64_t r = prow(g);
     const f32x2 ml = *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * r);
-    const float w = exp2f(ml[0] - m_use);
-    acc += *reinterpret_cast<const f32x4 *>(p.part + r * RANK + 4 * col) * w;
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(p.part + r * RANK + 4 * col);
+    const float w = __builtin_amdgcn_exp2f(ml[0] - m_use);
+    acc += x * w;
     l += ml[1] * w;
   }
   s_acc[part][col] = acc;
@@ -495,7 +483,7 @@ __global__ __launch_bounds__(256) void latent_merge(DecodeParams p, int block_ro
   __syncthreads();
   if (part) return;
 #pragma unroll
-  for (int k = 1; k < kLanes; ++k) {
+  for (int k = 1; k < kParts; ++k) {
     acc += s_acc[k][col];
     l += s_l[k];
   }
@@ -522,21 +510,35 @@ int device_cus() {
 }
 
 int64_t rows_of(const l20_pd_latent_args &a) { return (int64_t)a.q_len * a.num_heads; }
-// Blocks of 16 rows a workgroup takes: as many as the sequence has, up to four.
-int blocks_of(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-int64_t tiles_bound(const l20_pd_latent_args &a) {
-  return (int64_t)a.batch * std::max<int64_t>(1, ((int64_t)a.max_seq_len + l20la::kTile - 1) / l20la::kTile);
-}
-// Runs of tiles: as many as workgroups fit the chip at once, a multiple of 8 (the XCDs), no more than tiles.
-int groups_of(const l20_pd_latent_args &a, int cus) {
-  const int64_t rows = rows_of(a), rblocks = (rows + 16 * blocks_of(rows) - 1) / (16 * blocks_of(rows));
-  const int64_t fit = std::max<int64_t>(1, cus * (rows <= 32 ? 2 : 1) / rblocks);
-  return (int)((std::min(fit, tiles_bound(a)) + 7) / 8 * 8);
-}
-int64_t workspace_bytes(const l20_pd_latent_args &a, int cus) {
-  if (a.batch <= 0 || tiles_bound(a) <= a.batch) return 0;  // one tile a sequence: nothing to join
-  const int64_t rows = rows_of(a), br = 16 * blocks_of(rows), rblocks = (rows + br - 1) / br;
-  return 2 * groups_of(a, cus) * rblocks * br * (a.rank + 2) * (int64_t)sizeof(float);
+
+// How a call is cut: blocks of 16 rows a workgroup takes (as many as the sequence has, up to four), tokens of a
+// tile, runs of tiles.
+struct Plan {
+  int row_blocks16, row_blocks, tile, groups;
+  bool split;
+  int64_t workspace;
+};
+constexpr int kWholeTiles = 1;  // sequences of up to this many tiles are not split
+
+Plan plan_of(const l20_pd_latent_args &a, int cus) {
+  Plan n{};
+  const int64_t rows = rows_of(a);
+  n.row_blocks16 = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t block = 16 * n.row_blocks16;
+  n.row_blocks = (int)((rows + block - 1) / block);
+  n.tile = a.cache_dtype == L20_PD_KV_FP8_E4M3 && n.row_blocks16 < 4 ? 128 : 64;
+  const int64_t tiles = std::max<int64_t>(1, ((int64_t)a.max_seq_len + n.tile - 1) / n.tile);
+  n.split = tiles > kWholeTiles;
+  if (!n.split) {
+    n.groups = (a.batch + 7) / 8 * 8;
+    return n;
+  }
+  // As many runs as workgroups fit the chip at once, a multiple of 8 (the XCDs), no more than tiles.
+  const int64_t fit = std::max<int64_t>(1, cus / n.row_blocks);
+  n.groups = (int)((std::min<int64_t>(fit, a.batch * tiles) + 7) / 8 * 8);
+  n.workspace = 2 * (int64_t)n.groups * n.row_blocks * block * (a.rank + 2) * (int64_t)sizeof(float) +
+                (int64_t)a.batch * (int64_t)sizeof(int32_t) * 2;
+  return n;
 }
 
 int32_t check(const l20_pd_latent_args *a) {
@@ -553,7 +555,6 @@ int32_t check(const l20_pd_latent_args *a) {
     return set_error(L20_PD_EINVAL, "batch, q_len, heads and max_seq_len must be positive");
   if (rows_of(*a) > 65535) return set_error(L20_PD_EINVAL, "at most 65535 query rows (q_len x heads) a sequence");
   if (a->batch > 65535) return set_error(L20_PD_EINVAL, "at most 65535 sequences");
-  if (tiles_bound(*a) >= ((int64_t)1 << 30)) return set_error(L20_PD_EINVAL, "too many tokens");
   if (!(a->softmax_scale > 0.0f && isfinite(a->softmax_scale)))
     return set_error(L20_PD_EINVAL, "softmax_scale must be positive and finite");
   if (fp8 && !(a->cache_scale > 0.0f && isfinite(a->cache_scale)))
@@ -561,7 +562,7 @@ int32_t check(const l20_pd_latent_args *a) {
   if (a->batch == 0) return L20_PD_OK;
   if (a->num_pages <= 0 || a->table_pages <= 0) return set_error(L20_PD_EINVAL, "latent cache and block table must have pages");
   if ((int64_t)a->table_pages * a->page_size > INT32_MAX / 2 ||
-      (int64_t)a->batch * ((int64_t)a->table_pages * a->page_size / l20la::kTile + 1) >= ((int64_t)1 << 30))
+      (int64_t)a->batch * ((int64_t)a->table_pages * a->page_size / 64 + 1) >= ((int64_t)1 << 30))
     return set_error(L20_PD_EINVAL, "block table names too many tokens");
   if (a->num_pages * (a->page_size / 16) > INT32_MAX) return set_error(L20_PD_EINVAL, "latent cache has too many pages");
   if (a->page_size > 16 && a->c_stride_page != a->page_size * a->c_stride_token)
@@ -580,29 +581,28 @@ int32_t check(const l20_pd_latent_args *a) {
 }
 
 template <typename T, int KT, int RANK, int RB> hipError_t launch_partial(const l20la::DecodeParams &p, hipStream_t s) {
-  typedef l20la::Partial<T, KT, RANK, RB> K;
-  const size_t lds = sizeof(typename K::Shared);
-  const void *f = reinterpret_cast<const void *>(&l20la::latent_partial<T, KT, RANK, RB>);
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-  }
+  const size_t lds = sizeof(typename l20la::Partial<T, KT, RANK, RB>::Shared);
+  static_assert(sizeof(typename l20la::Partial<T, KT, RANK, RB>::Shared) <= 160 * 1024, "more than the LDS of a CU");
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&l20la::latent_partial<T, KT, RANK, RB>),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL((l20la::latent_partial<T, KT, RANK, RB>), dim3((unsigned)(p.groups * p.row_blocks)),
-                     dim3(K::kThreads), lds, s, p);
+                     dim3(l20la::kThreads), lds, s, p);
   return hipGetLastError();
 }
-template <typename T, int KT, int RANK> hipError_t launch_rows(const l20la::DecodeParams &p, hipStream_t s) {
-  switch (blocks_of(p.rows)) {
+template <typename T, int KT, int RANK> hipError_t launch_rows(const l20la::DecodeParams &p, int blocks, hipStream_t s) {
+  switch (blocks) {
     case 1: return launch_partial<T, KT, RANK, 1>(p, s);
     case 2: return launch_partial<T, KT, RANK, 2>(p, s);
     default: return launch_partial<T, KT, RANK, 4>(p, s);
   }
 }
-template <typename T, int RANK> hipError_t launch(const l20la::DecodeParams &p, bool fp8, bool join, hipStream_t s) {
-  const hipError_t e = fp8 ? launch_rows<T, 0, RANK>(p, s) : launch_rows<T, 1, RANK>(p, s);
-  if (e != hipSuccess || !join) return e;
-  hipLaunchKernelGGL((l20la::latent_merge<T, RANK>), dim3((unsigned)p.rows, (unsigned)p.batch), dim3(256), 0, s, p,
-                     16 * blocks_of(p.rows));
+template <typename T, int RANK>
+hipError_t launch(const l20la::DecodeParams &p, bool fp8, int blocks, hipStream_t s) {
+  const hipError_t e = fp8 ? launch_rows<T, 0, RANK>(p, blocks, s) : launch_rows<T, 1, RANK>(p, blocks, s);
+  if (e != hipSuccess || !p.split) return e;
+  hipLaunchKernelGGL((l20la::latent_merge<T, RANK>), dim3((unsigned)p.rows, (unsigned)p.batch), dim3(l20la::kThreads), 0,
+                     s, p, 16 * blocks);
   return hipGetLastError();
 }
 
@@ -618,7 +618,7 @@ int32_t l20_pd_paged_latent_check(const l20_pd_latent_args *a) {
 int64_t l20_pd_paged_latent_workspace(const l20_pd_latent_args *a, int32_t cu_count) {
   l20pd_host::clear_error();
   if (!a || a->batch < 0 || a->q_len < 1 || a->num_heads < 1 || a->max_seq_len < 0 || rows_of(*a) > 65535) return 0;
-  return workspace_bytes(*a, cu_count > 0 ? cu_count : device_cus());
+  return plan_of(*a, cu_count > 0 ? cu_count : device_cus()).workspace;
 }
 
 int32_t l20_pd_paged_latent(const l20_pd_latent_args *a, void *stream) {
@@ -626,8 +626,8 @@ int32_t l20_pd_paged_latent(const l20_pd_latent_args *a, void *stream) {
   const int32_t rc = check(a);
   if (rc != L20_PD_OK || a->batch == 0) return rc;
   const int cus = device_cus();
-  const int64_t need = workspace_bytes(*a, cus);
-  if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
+  const Plan plan = plan_of(*a, cus);
+  if (plan.workspace > 0 && (!a->workspace || a->workspace_bytes < plan.workspace || (uintptr_t)a->workspace % 16))
     return set_error(L20_PD_EINVAL, "workspace is too small for the request (l20_pd_paged_latent_workspace)");
   l20la::DecodeParams p{};
   const bool fp8 = a->cache_dtype == L20_PD_KV_FP8_E4M3;
@@ -658,18 +658,20 @@ int32_t l20_pd_paged_latent(const l20_pd_latent_args *a, void *stream) {
   p.q_len = a->q_len;
   p.heads = a->num_heads;
   p.rows = (int)rows_of(*a);
-  const int br = 16 * blocks_of(p.rows);
-  p.row_blocks = (p.rows + br - 1) / br;
-  p.groups = groups_of(*a, cus);
+  p.row_blocks = plan.row_blocks;
+  p.groups = plan.groups;
+  p.split = plan.split;
   p.part = static_cast<float *>(a->workspace);
-  p.part_ml = p.part + (int64_t)2 * p.groups * p.row_blocks * br * a->rank;
+  const int64_t part_rows = (int64_t)2 * p.groups * p.row_blocks * 16 * plan.row_blocks16;
+  p.part_ml = p.part + part_rows * a->rank;
+  p.runs = reinterpret_cast<l20la::i32x2 *>(p.part_ml + part_rows * 2);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const bool join = need > 0;
   hipError_t e;
   if (a->dtype == L20_PD_BF16)
-    e = a->rank == 512 ? launch<__bf16, 512>(p, fp8, join, s) : launch<__bf16, 256>(p, fp8, join, s);
+    e = a->rank == 512 ? launch<__bf16, 512>(p, fp8, plan.row_blocks16, s) : launch<__bf16, 256>(p, fp8, plan.row_blocks16, s);
   else
-    e = a->rank == 512 ? launch<_Float16, 512>(p, fp8, join, s) : launch<_Float16, 256>(p, fp8, join, s);
+    e = a->rank == 512 ? launch<_Float16, 512>(p, fp8, plan.row_blocks16, s)
+                       : launch<_Float16, 256>(p, fp8, plan.row_blocks16, s);
   if (e != hipSuccess) {
     char msg[256];
     snprintf(msg, sizeof(msg), "HIP launch failed: %s", hipGetErrorString(e));

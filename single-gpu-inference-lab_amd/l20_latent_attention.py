@@ -99,7 +99,7 @@ def allocate_l20_paged_latent_workspace(
 
     a = l20_pd_cabi.L20PdLatentArgs()
     a.batch, a.q_len, a.num_heads = query.shape[0] // q_len, q_len, query.shape[1]
-    a.rank, a.max_seq_len = kv_rank, int(max_seq_len)
+    a.rank, a.max_seq_len, a.cache_dtype = kv_rank, int(max_seq_len), l20_pd_cabi._kv_code(latent_cache)
     size = int(l20_pd_cabi.load().l20_pd_paged_latent_workspace(l20_pd_cabi.ctypes.byref(a), gpu_cus(latent_cache.device)))
     return torch.empty(size, dtype=torch.uint8, device=latent_cache.device)
 
