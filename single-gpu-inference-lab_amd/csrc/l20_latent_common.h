@@ -101,15 +101,17 @@ __device__ __forceinline__ float max_groups(float x) { return max_swap<32>(max_s
 __device__ __forceinline__ float sum_groups(float x) { return sum_swap<32>(sum_swap<16>(x)); }
 
 // 16 bytes a lane from global memory to LDS (lane l's land at dst + 16 l), asynchronously: they are there once
-// the wave has waited for its loads.
+// the wave has waited for its loads (landed_and_barrier).  Not the builtin: with a builtin's load in flight the
+// compiler waits for all loads before every transposing read, which ends the prefetch; a load into LDS has no
+// result registers that could be taken for written.
 __device__ __forceinline__ void load_lds(const void *src, void *dst) {
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) void *)(const __attribute__((address_space(1))) char *)(src),
-      (__attribute__((address_space(3))) void *)(__attribute__((address_space(3))) char *)(dst), 16, 0, 0);
+  const int at = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)dst);  // (an LDS address' low half)
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(at) : "memory");
 }
-// The wave's loads have landed, in LDS too, and so have those of the workgroup's other waves.
-__device__ __forceinline__ void landed_and_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
+// All but the wave's last N loads have landed, in LDS too, and so for the workgroup's other waves.
+template <int N> __device__ __forceinline__ void landed_and_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 // LDS writes of the workgroup's waves are there; loads may be in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 

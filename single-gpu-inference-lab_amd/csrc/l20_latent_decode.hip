@@ -21,6 +21,7 @@
 #include "l20_latent_attention.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "l20_latent_common.h"
 
@@ -36,6 +37,7 @@ struct DecodeParams {
   int64_t c_block, c_tok;  // bytes from one 16-token block, one token to the next
   int64_t blocks;          // 16-token blocks of the cache
   int per_page;            // blocks a page
+  uint64_t page_magic;     // n * page_magic >> 38 = n / per_page
   const int32_t *table;
   int64_t t_sr;
   int table_blocks;  // blocks a row of the table can name
@@ -54,9 +56,13 @@ struct DecodeParams {
   int split;  // 0: one run a sequence
 };
 
-__device__ __forceinline__ int seq_tokens(const DecodeParams &p, int b) {
-  return min(max(p.lens[b], 0), p.max_tokens);
+__device__ __forceinline__ int seq_tokens(const DecodeParams &p, int b) { return min(max(p.lens[b], 0), p.max_tokens); }
+// The length of a wave-uniform sequence, by a scalar load: the wait for a vector load would be one for the tiles
+// in flight too.
+__device__ __forceinline__ int uniform_len(const DecodeParams &p, int b) {
+  return ((const __attribute__((address_space(4))) int *)(uintptr_t)(p.lens))[b];
 }
+__device__ __forceinline__ int uniform_tokens(const DecodeParams &p, int b) { return min(max(uniform_len(p, b), 0), p.max_tokens); }
 // Four fp8 codes (one dword) -> two dwords of T, exact.  (Whole words: extracting elements of these
 // conversions' results one by one is miscompiled by the ROCm 7.2 LLVM.)
 template <typename T> __device__ __forceinline__ i32x2 fp8x4(int w);
@@ -71,7 +77,7 @@ template <> __device__ __forceinline__ i32x2 fp8x4<_Float16>(int w) {
 
 template <typename T, int KT, int RANK, int RB> struct Partial {
   static constexpr int kRows = 16 * RB;
-  static constexpr int kTokens = KT == 0 && RB < 4 ? 128 : 64;  // of a tile: two of them fill the LDS
+  static constexpr int kTokens = KT == 0 ? 64 : 32;  // of a tile
   // the score product: a wave takes one block of 16 rows and kBlocks blocks of 16 tokens
   static constexpr int kTokBlocks = kTokens / 16;
   static constexpr int kGroups = kWaves / RB < kTokBlocks ? kWaves / RB : kTokBlocks;
@@ -84,14 +90,14 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   static constexpr int kLatBytes = kTokens * kLatRow, kRopeBytes = kTokens * kRopeRow;
 
   struct Shared {
-    alignas(16) char lat[2][kLatBytes];
-    alignas(16) char rope[2][kRopeBytes];
-    alignas(16) char p[kRows * kPRow];
+    alignas(16) char lat[4][kLatBytes];  // tiles n - 1 (its value product), n (its scores), n + 1 and n + 2 (loading)
+    alignas(16) char rope[3][kRopeBytes];
+    alignas(16) char p[2][kRows * kPRow];
     alignas(16) float max[kRows][kGroups];
     alignas(16) float sum[kRows][kGroups];
     int wave[kWaves];
     int start[2];
-    int rescale[2];
+    int rescale[3];
   };
 
   // Where chunk c (16 bytes) of a row lies: rows are spread so that 16 of them read at one chunk, and the 4 (8)
@@ -100,7 +106,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   static __device__ __forceinline__ int rope_swizzle(int row) { return KT == 0 ? (row >> 2) & 3 : (row >> 1) & 7; }
   static __device__ __forceinline__ int rope_at(int row, int c) { return row * kRopeRow + ((c ^ rope_swizzle(row)) << 4); }
   static __device__ __forceinline__ int p_at(int row, int c) {
-    return row * kPRow + ((c ^ (kTokens == 64 ? (row >> 1) & 7 : row & 15)) << 4);
+    return row * kPRow + ((c ^ (kTokens == 64 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
   }
 
   // (a sequence without tokens has one tile, all masked: its rows are written too)
@@ -112,20 +118,27 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     int b, end;       // sequence, its last tile + 1
     int t0, tokens;   // first token of the tile, tokens of the sequence
     int window, pid;  // lane k of pid: cache block k of the window's 64 (16 tokens each), -1 for none
+    int lat, rope;    // LDS buffers
+    uint32_t bad;     // bits 4 n .. of buffer n: blocks of its tile without a page
   };
   static __device__ __forceinline__ int blocks_of_window(const DecodeParams &p, int b, int first_block) {
     const int blk = first_block + (int)(threadIdx.x & 63);
     if (blk >= p.table_blocks) return -1;
-    const int page = p.table[b * p.t_sr + blk / p.per_page];
-    const int64_t id = (int64_t)page * p.per_page + blk % p.per_page;
+    const int col = p.per_page == 1 ? blk : (int)((uint64_t)blk * p.page_magic >> 38);
+    const int page = p.table[b * p.t_sr + col];
+    const int64_t id = (int64_t)page * p.per_page + (blk - col * p.per_page);
     return page < 0 || id >= p.blocks ? -1 : (int)id;
   }
-  // Start the loads of tile f.at into buffer `buf` and move on.  Tokens past the end, or without a page, are
-  // zeros: their scores are masked, but 0 x NaN is NaN in the value product.
-  static __device__ __forceinline__ void stage(const DecodeParams &p, Shared &s, Fetch &f, int buf, int wave, int lane) {
+  // Start the loads of f's tile into its buffers and move on.  Tokens past the end, or without a page, are zeros:
+  // their scores are masked, but 0 x NaN is NaN in the value product.  The page ids come by one vector load every
+  // 1024 tokens (which waits for the tiles in flight).
+  static constexpr int kLatLoads = kLatBytes / 1024 / kWaves;  // a wave's instructions of 1 KB
+  static constexpr int kRopeLoads = (kRopeBytes / 1024 + kWaves - 1) / kWaves;
+  static constexpr int kLoads = kLatLoads + kRopeLoads;
+  static __device__ __forceinline__ void stage(const DecodeParams &p, Shared &s, Fetch &f, int wave, int lane) {
     if (f.at == f.end) {
       ++f.b;
-      f.tokens = seq_tokens(p, f.b);
+      f.tokens = uniform_tokens(p, f.b);
       f.end += tiles_of(f.tokens);
       f.t0 = 0;
       f.window = -1;
@@ -134,34 +147,38 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       f.window = f.t0 >> 10;
       f.pid = blocks_of_window(p, f.b, f.window * 64);
     }
-    const int left = f.tokens - f.t0, blk0 = (f.t0 >> 4) & 63;
-    constexpr int kLat = kLatBytes / 1024 / kWaves;  // instructions of a wave
+    const int blk0 = (f.t0 >> 4) & 63;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int k = 0; k < kTokBlocks; ++k) bad |= __builtin_amdgcn_readlane(f.pid, blk0 + k) < 0 ? 1u << k : 0u;
+    f.bad = (f.bad & ~(15u << 4 * f.lat)) | bad << 4 * f.lat;
+    const int left = f.tokens - f.t0;
     constexpr int kChunks = kLatRow / 16;
 #pragma unroll
-    for (int i = 0; i < kLat; ++i) {
-      const int at = (wave * kLat + i) * 1024;  // of the buffer
+    for (int i = 0; i < kLatLoads; ++i) {
+      const int at = (wave * kLatLoads + i) * 1024;  // of the buffer
       const int row = at / kLatRow + lane / kChunks;
       const int id = __builtin_amdgcn_readlane(f.pid, blk0 + (at / kLatRow >> 4));
       const int c = (lane % kChunks) ^ (row & 15);
       const uint8_t *src = p.cache + (int64_t)id * p.c_block + (int64_t)(row & 15) * p.c_tok;
       src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src;
-      load_lds(src + 16 * c, s.lat[buf] + at);
+      load_lds(src + 16 * c, s.lat[f.lat] + at);
     }
-    constexpr int kRopeInstr = kRopeBytes / 1024;  // of all waves
 #pragma unroll
-    for (int i = 0; i < (kRopeInstr + kWaves - 1) / kWaves; ++i) {
-      const int n = i * kWaves + wave;
-      if (kRopeInstr % kWaves && n >= kRopeInstr) break;
-      const int at = n * 1024;
+    for (int i = 0; i < kRopeLoads; ++i) {
+      // (where there are fewer instructions than waves some are made twice: every wave counts the same loads)
+      const int at = (i * kWaves + wave) % (kRopeBytes / 1024) * 1024;
       const int row = at / kRopeRow + lane / (kRopeRow / 16);
       const int id = __builtin_amdgcn_readlane(f.pid, blk0 + (at / kRopeRow >> 4));
       const int c = (lane % (kRopeRow / 16)) ^ rope_swizzle(row);
       const uint8_t *src = p.cache + (int64_t)id * p.c_block + (int64_t)(row & 15) * p.c_tok;
       src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src + RANK * kBytes;
-      load_lds(src + 16 * c, s.rope[buf] + at);
+      load_lds(src + 16 * c, s.rope[f.rope] + at);
     }
     ++f.at;
     f.t0 += kTokens;
+    f.lat = (f.lat + 1) & 3;
+    f.rope = f.rope == 2 ? 0 : f.rope + 1;
   }
 
   static __device__ __forceinline__ void run(const DecodeParams &p, Shared &s) {
@@ -174,10 +191,10 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
 
     // ---- this group's run of tiles ----
     int b = group, base = 0, first = 0, last = 0, per = 1;
-    if (tid < 2) s.rescale[tid] = 0;
+    if (tid < 3) s.rescale[tid] = 0;
     if (!p.split) {
       if (b >= p.batch) return;  // the whole workgroup
-      last = tiles_of(seq_tokens(p, b));
+      last = tiles_of(uniform_tokens(p, b));
     } else {
       const int chunk = (p.batch + kThreads - 1) / kThreads;
       int mine = 0;
@@ -223,37 +240,43 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     f.at = first;
     f.last = last;
     f.b = b;
-    f.tokens = seq_tokens(p, b);
+    f.tokens = uniform_tokens(p, b);
     f.end = base + tiles_of(f.tokens);
     f.t0 = (first - base) * kTokens;
-    f.window = -1;
-    f.pid = -1;
-    stage(p, s, f, 0, wave, lane);
+    f.window = f.pid = -1;
+    f.lat = f.rope = 0;
+    f.bad = 0;
 
     // ---- one segment a sequence ----
-    int buf = 0;
-    for (int at = first; at < last; ++b) {
-      const int tokens = seq_tokens(p, b), tiles = tiles_of(tokens);
+    Place at{first, 0, 0};
+    while (at.tile < last) {
+      const int tokens = f.at == first ? f.tokens : uniform_tokens(p, b), tiles = tiles_of(tokens);
       const int seg_end = min(last, base + tiles);
-      if (p.split && at == base && rblk == 0 && tid == 0) p.runs[b] = i32x2{group, (base + tiles - 1) / per};
-      segment(p, s, f, buf, b, rblk, group, base, at, seg_end, seg_end == base + tiles, first, tokens, wave, lane);
-      at = seg_end;
+      if (p.split && at.tile == base && rblk == 0 && tid == 0) p.runs[b] = i32x2{group, (base + tiles - 1) / per};
+      segment(p, s, f, at, b, rblk, group, base, seg_end, seg_end == base + tiles, first, tokens, wave, lane);
       base += tiles;
+      ++b;
     }
   }
 
-  static __device__ __forceinline__ void segment(const DecodeParams &p, Shared &s, Fetch &f, int &buf, int b, int rblk,
-                                                 int group, int base, int at, int seg_end, bool ends, int first,
-                                                 int tokens, int wave, int lane) {
+  // A tile of the run and its LDS buffers.
+  struct Place {
+    int tile, lat, rope;
+  };
+
+  static __device__ __forceinline__ void segment(const DecodeParams &p, Shared &s, Fetch &f, Place &at, int b, int rblk,
+                                                 int group, int base, int seg_end, bool ends, int first, int tokens,
+                                                 int wave, int lane) {
     const int n16 = lane & 15, g4 = lane >> 4;
     const int own = wave % RB, tg = wave / RB;  // block of rows, group of tokens of the score product
-    const bool scores = tg < kGroups;
-    const int len = p.lens[b];
+    const bool scores = kWaves / RB == kGroups || tg < kGroups;
+    const int len = uniform_len(p, b);
     i32x4 q[kSlices];
     int lim;
+    bool live;
     {
       const int r = rblk * kRows + 16 * own + n16;
-      const bool live = r < p.rows;
+      live = r < p.rows;
       const int i = live ? r / p.heads : 0, h = live ? r - i * p.heads : 0;
       lim = live ? min(len - p.q_len + i, tokens - 1) : -1;
       // the order of the dims in the product is free: over an fp8 cache a lane's are 16 in a row of each 64, so
@@ -262,10 +285,16 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
 #pragma unroll
       for (int k = 0; k < kSlices; ++k) {
         const int d = KT == 0 ? 64 * (k >> 1) + 16 * g4 + 8 * (k & 1) : 32 * k + 8 * g4;
-        const i32x4 w = *reinterpret_cast<const i32x4 *>(src + d);
-        q[k] = live ? w : i32x4{0, 0, 0, 0};
+        q[k] = *reinterpret_cast<const i32x4 *>(src + d);
       }
     }
+    if (at.tile == first) {  // (behind the query's loads, which come back in order)
+      stage(p, s, f, wave, lane);
+      if (f.at < f.last) stage(p, s, f, wave, lane);
+    }
+#pragma unroll
+    for (int k = 0; k < kSlices; ++k) q[k] = live ? q[k] : i32x4{0, 0, 0, 0};
+
     f32x4 acc[RB][kDimBlocks];
     float m_all[RB];  // the maximum that P of the lane's row in each block refers to, log2 units
     float m_own = -INFINITY, sum = 0.0f;  // of the wave's own block, its tokens
@@ -281,81 +310,29 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     int v_at = KT == 0 ? lat_at(8 * g4 + (n16 >> 1), wave * kDimBlocks) + 8 * (n16 & 1)
                        : lat_at(8 * g4 + (n16 >> 2), 2 * wave * kDimBlocks + ((n16 >> 1) & 1)) + 8 * (n16 & 1);
 
-    int t0 = (at - base) * kTokens;
-    for (int tile = at; tile < seg_end; ++tile, t0 += kTokens, buf ^= 1) {
-      const int blk0 = (t0 >> 4) & 63;
-      int bad = 0;  // token blocks without a page (f is still at this tile)
-#pragma unroll
-      for (int k = 0; k < kTokBlocks; ++k) bad |= __builtin_amdgcn_readlane(f.pid, blk0 + k) < 0 ? 1 << k : 0;
-      const bool whole = t0 + kTokens <= min(tokens, len - p.q_len + 1) && !bad;
-      landed_and_barrier();  // this tile is there, and the one before is consumed
-      if (wave == 0) s.rescale[buf ^ 1] = 0;
-      if (f.at < f.last) stage(p, s, f, buf ^ 1, wave, lane);
-      const char *lat = s.lat[buf], *rope = s.rope[buf];
-      asm volatile("" : "+v"(k_at), "+v"(r_at), "+v"(v_at));  // (not loop invariant: hoisted, they take 30 registers)
+    // What a tile leaves for the next iteration, which takes its value product.
+    f32x4 sc[kBlocks];
+    float mx = -INFINITY, add = 0.0f;
 
-      // ---- S^T = K Q^T ----
-      f32x4 sc[kBlocks];
-      float mx = -INFINITY;
-      if (scores) {
+    // P of the tile from m_own, and its sum over the lane's tokens.
+    auto weights = [&](char *pbuf) {
+      const float use = m_own == -INFINITY ? 0.0f : m_own;
+      add = 0.0f;
 #pragma unroll
-        for (int u = 0; u < kBlocks; ++u) {
-          const char *ku = lat + u * 16 * kLatRow, *ru = rope + u * 16 * kRopeRow;
-          f32x4 part[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-          if constexpr (KT == 0) {
+      for (int u = 0; u < kBlocks; ++u) {
+        const int tb = tg * kBlocks + u;
+        float e[4];
 #pragma unroll
-            for (int k = 0; k < kSlices; k += 2) {
-              const char *src = 32 * k < RANK ? ku + (k_at ^ ((k / 2 & 3) << 6)) + (k / 2 >> 2) * 256 : ru + r_at;
-              const i32x4 w = *reinterpret_cast<const i32x4 *>(src);
-              const i32x2 c0 = fp8x4<T>(w[0]), c1 = fp8x4<T>(w[1]), c2 = fp8x4<T>(w[2]), c3 = fp8x4<T>(w[3]);
-              part[0] = mfma<T>(i32x4{c0[0], c0[1], c1[0], c1[1]}, q[k], part[0]);
-              part[1] = mfma<T>(i32x4{c2[0], c2[1], c3[0], c3[1]}, q[k + 1], part[1]);
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < kSlices; ++k) {
-              const char *src = 32 * k < RANK ? ku + (k_at ^ ((k & 3) << 6)) + (k >> 2) * 256
-                                              : ru + (r_at ^ ((k - RANK / 32) << 6));
-              part[k & 1] = mfma<T>(*reinterpret_cast<const i32x4 *>(src), q[k], part[k & 1]);
-            }
-          }
-          sc[u] = part[0] + part[1];
-        }
-        if (!whole) {
-#pragma unroll
-          for (int u = 0; u < kBlocks; ++u) {
-            const int tb = tg * kBlocks + u;
-            const int hide = bad >> tb & 1 ? -1 : lim;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[u][i] = t0 + 16 * tb + 4 * g4 + i <= hide ? sc[u][i] : -INFINITY;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < kBlocks; ++u) mx = fmaxf(mx, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
-        mx = max_groups(mx) * p.c_log2;
+        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], p.c_log2, -use));
+        add += (e[0] + e[1]) + (e[2] + e[3]);
+        *reinterpret_cast<i32x2 *>(pbuf + p_at(16 * own + n16, 2 * tb + (g4 >> 1)) + 8 * (g4 & 1)) =
+            i32x2{pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3])};
       }
-      // ---- P from the maximum so far; where a row exceeds that by much, all waves go back and move it ----
-      float add = 0.0f;
-      auto weights = [&]() {
-        const float use = m_own == -INFINITY ? 0.0f : m_own;
-        add = 0.0f;
-#pragma unroll
-        for (int u = 0; u < kBlocks; ++u) {
-          const int tb = tg * kBlocks + u;
-          float e[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], p.c_log2, -use));
-          add += (e[0] + e[1]) + (e[2] + e[3]);
-          *reinterpret_cast<i32x2 *>(s.p + p_at(16 * own + n16, 2 * tb + (g4 >> 1)) + 8 * (g4 & 1)) =
-              i32x2{pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3])};
-        }
-      };
-      if (scores) {
-        weights();
-        if (__any(mx > m_own + kRescale) && lane == 0) s.rescale[buf] = 1;
-      }
-      lds_barrier();
-      if (__builtin_amdgcn_readfirstlane(s.rescale[buf])) {  // the same for all waves
+    };
+    // A finished tile's P is in LDS, from the maximum so far.  Where a row exceeded that by much, all waves move
+    // the maxima and P is written again.
+    auto settle = [&](int tile) {
+      if (__builtin_amdgcn_readfirstlane(s.rescale[tile % 3])) {  // the same for all waves
         if (scores && g4 == 0) s.max[16 * own + n16][tg] = mx;
         lds_barrier();
         float alpha_own = 1.0f;
@@ -372,40 +349,158 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
           alpha_own = r == own ? alpha : alpha_own;
         }
         sum *= alpha_own;
-        if (scores) weights();
+        if (scores) weights(s.p[tile & 1]);
         lds_barrier();
       }
       sum += add;
-      // ---- O^T += V^T P^T: the wave's dims, all rows ----
+    };
+    // Part n of a tile's O^T += V^T P^T (the wave's dims, all rows): 32 tokens, 16 dims.
+    constexpr int kParts = kTokens / 32 * kDimBlocks;
+    i32x4 pb[RB];
+    auto read_p = [&](const char *pbuf, int ks) {
 #pragma unroll
-      for (int ks = 0; ks < kTokens / 32; ++ks) {
-        i32x4 pb[RB];
+      for (int r = 0; r < RB; ++r) pb[r] = *reinterpret_cast<const i32x4 *>(pbuf + p_at(16 * r + n16, 4 * ks + g4));
+    };
+    auto read_v = [&](const char *lat, int n) -> i32x4 {
+      const int ks = n / kDimBlocks, d = n % kDimBlocks;
+      if constexpr (KT == 0) {
+        const i32x2 w = read_tr8(lat + ks * 32 * kLatRow + (v_at ^ (d << 4)));
+        return i32x4{w[0], w[1], 0, 0};
+      } else {
+        // (four rows on, the swizzle differs in chunk bit 2)
+        const i32x2 lo = read_tr(lat + ks * 32 * kLatRow + (v_at ^ (d << 5)));
+        const i32x2 hi = read_tr(lat + (ks * 32 + 4) * kLatRow + (v_at ^ (d << 5) ^ 64));
+        return i32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    };
+    auto values = [&](i32x4 w, int n) {
+      const int d = n % kDimBlocks;
+      if constexpr (KT == 0) {
+        const i32x2 lo = fp8x4<T>(w[0]), hi = fp8x4<T>(w[1]);
+        w = i32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
 #pragma unroll
-        for (int r = 0; r < RB; ++r) pb[r] = *reinterpret_cast<const i32x4 *>(s.p + p_at(16 * r + n16, 4 * ks + g4));
+      for (int r = 0; r < RB; ++r) acc[r][d] = mfma<T>(w, pb[r], acc[r][d]);
+    };
+    auto all_values = [&](const char *lat, const char *pbuf) {
 #pragma unroll
-        for (int d = 0; d < kDimBlocks; ++d) {
-          i32x4 a;
-          if constexpr (KT == 0) {
-            const i32x2 w = read_tr8(lat + ks * 32 * kLatRow + (v_at ^ (d << 4)));
-            const i32x2 lo = fp8x4<T>(w[0]), hi = fp8x4<T>(w[1]);
-            a = i32x4{lo[0], lo[1], hi[0], hi[1]};
-          } else {
-            // (four rows on, the swizzle differs in chunk bit 2)
-            const i32x2 lo = read_tr(lat + ks * 32 * kLatRow + (v_at ^ (d << 5)));
-            const i32x2 hi = read_tr(lat + (ks * 32 + 4) * kLatRow + (v_at ^ (d << 5) ^ 64));
-            a = i32x4{lo[0], lo[1], hi[0], hi[1]};
-          }
+      for (int n = 0; n < kParts; ++n) {
+        if (n % kDimBlocks == 0) read_p(pbuf, n / kDimBlocks);
+        values(read_v(lat, n), n);
+      }
+    };
+    // Step n of the score product: two slices, the wave's token blocks.
+    constexpr int kReads = KT == 0 ? 1 : 2;  // of 16 bytes
+    struct Keys {
+      i32x4 w[kBlocks][kReads];
+    };
+    auto read_k = [&](const char *lat, const char *rope, int n, Keys &key) {
 #pragma unroll
-          for (int r = 0; r < RB; ++r) acc[r][d] = mfma<T>(a, pb[r], acc[r][d]);
+      for (int u = 0; u < kBlocks; ++u) {
+        const char *ku = lat + u * 16 * kLatRow, *ru = rope + u * 16 * kRopeRow;
+#pragma unroll
+        for (int e = 0; e < kReads; ++e) {
+          const int c = kReads * n + e;  // chunk / 4
+          const char *src = 64 * n < RANK ? ku + (k_at ^ ((c & 3) << 6)) + (c >> 2) * 256
+                                          : ru + (r_at ^ ((c - kReads * RANK / 64) << 6));
+          key.w[u][e] = *reinterpret_cast<const i32x4 *>(src);
         }
       }
-    }
+    };
+    auto score_step = [&](const Keys &key, int n, f32x4 (&part)[kBlocks][2]) {
+#pragma unroll
+      for (int u = 0; u < kBlocks; ++u) {
+        if constexpr (KT == 0) {
+          const i32x4 w = key.w[u][0];
+          const i32x2 c0 = fp8x4<T>(w[0]), c1 = fp8x4<T>(w[1]), c2 = fp8x4<T>(w[2]), c3 = fp8x4<T>(w[3]);
+          part[u][0] = mfma<T>(i32x4{c0[0], c0[1], c1[0], c1[1]}, q[2 * n], part[u][0]);
+          part[u][1] = mfma<T>(i32x4{c2[0], c2[1], c3[0], c3[1]}, q[2 * n + 1], part[u][1]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kReads; ++e) part[u][e] = mfma<T>(key.w[u][e], q[2 * n + e], part[u][e]);
+        }
+      }
+    };
+    // One iteration: the scores of tile `at` and, with PV, the value product of the tile before -- two independent
+    // streams of LDS reads and matrix products, interleaved.
+    int t0 = (at.tile - base) * kTokens;
+    auto iteration = [&](auto with_values) {
+      constexpr bool PV = decltype(with_values)::value;
+      const uint32_t bad = f.bad >> 4 * at.lat & 15;  // token blocks without a page
+      const bool whole = t0 + kTokens <= min(tokens, len - p.q_len + 1) && !bad;
+      // this tile has landed, its predecessor's P is written, the one before that is consumed
+      if (f.at - at.tile >= 2) landed_and_barrier<kLoads>();
+      else landed_and_barrier<0>();
+      if (f.at < f.last) stage(p, s, f, wave, lane);
+      if (wave == 0) s.rescale[(at.tile + 1) % 3] = 0;
+      if constexpr (PV) settle(at.tile - 1);
+      const char *lat = s.lat[at.lat], *rope = s.rope[at.rope];
+      const char *old = s.lat[(at.lat + 3) & 3], *oldp = s.p[(at.tile + 1) & 1];
+      asm volatile("" : "+v"(k_at), "+v"(r_at), "+v"(v_at));  // (not loop invariant: hoisted, they take 30 registers)
+      if (scores) {
+        // The operands of a step are read while the step before is computed; the barriers keep the compiler from
+        // reading further ahead, which costs more registers than there are.
+        f32x4 part[kBlocks][2];
+#pragma unroll
+        for (int u = 0; u < kBlocks; ++u) part[u][0] = part[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int kKeySteps = kSlices / 2, kSteps = PV && kParts > kKeySteps ? kParts : kKeySteps;
+        Keys key;
+        i32x4 val;
+        read_k(lat, rope, 0, key);
+        if constexpr (PV) {
+          read_p(oldp, 0);
+          val = read_v(old, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < kSteps; ++n) {
+          const Keys k_now = key;
+          const i32x4 v_now = val;
+          if (n + 1 < kKeySteps) read_k(lat, rope, n + 1, key);
+          if constexpr (PV)
+            if (n + 1 < kParts) val = read_v(old, n + 1);
+          if (n < kKeySteps) score_step(k_now, n, part);
+          if constexpr (PV) {
+            if (n < kParts) values(v_now, n);
+            if (n + 1 < kParts && (n + 1) % kDimBlocks == 0) read_p(oldp, (n + 1) / kDimBlocks);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int u = 0; u < kBlocks; ++u) sc[u] = part[u][0] + part[u][1];
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < kBlocks; ++u) {
+            const int tb = tg * kBlocks + u;
+            const int hide = bad >> tb & 1 ? -1 : lim;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[u][i] = t0 + 16 * tb + 4 * g4 + i <= hide ? sc[u][i] : -INFINITY;
+          }
+        }
+        mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kBlocks; ++u) mx = fmaxf(mx, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
+        mx = max_groups(mx) * p.c_log2;
+        weights(s.p[at.tile & 1]);
+        if (__any(mx > m_own + kRescale) && lane == 0) s.rescale[at.tile % 3] = 1;
+      } else if constexpr (PV) {
+        all_values(old, oldp);
+      }
+      ++at.tile;
+      at.lat = (at.lat + 1) & 3;
+      at.rope = at.rope == 2 ? 0 : at.rope + 1;
+      t0 += kTokens;
+    };
+    iteration(std::false_type{});
+    while (at.tile < seg_end) iteration(std::true_type{});
+    lds_barrier();
+    settle(at.tile - 1);
+    all_values(s.lat[(at.lat + 3) & 3], s.p[(at.tile + 1) & 1]);
 
     // ---- the rows' sums, over lane groups and token groups ----
     sum = sum_groups(sum);
     if (scores && g4 == 0) s.sum[16 * own + n16][tg] = sum;
     lds_barrier();
-    const bool all = at == base && ends;
+    const bool all = first <= base && ends;
     const int slot = base < first ? 2 * group : 2 * group + 1;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
@@ -526,7 +621,7 @@ Plan plan_of(const l20_pd_latent_args &a, int cus) {
   n.row_blocks16 = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const int64_t block = 16 * n.row_blocks16;
   n.row_blocks = (int)((rows + block - 1) / block);
-  n.tile = a.cache_dtype == L20_PD_KV_FP8_E4M3 && n.row_blocks16 < 4 ? 128 : 64;
+  n.tile = a.cache_dtype == L20_PD_KV_FP8_E4M3 ? 64 : 32;
   const int64_t tiles = std::max<int64_t>(1, ((int64_t)a.max_seq_len + n.tile - 1) / n.tile);
   n.split = tiles > kWholeTiles;
   if (!n.split) {
@@ -639,6 +734,8 @@ int32_t l20_pd_paged_latent(const l20_pd_latent_args *a, void *stream) {
   p.c_tok = es * a->c_stride_token;
   p.c_block = a->page_size == 16 ? es * a->c_stride_page : 16 * p.c_tok;
   p.per_page = a->page_size / 16;
+  // (exact: block numbers are below 2^27, the rounding of the magic below per_page <= 2^8)
+  p.page_magic = (((uint64_t)1 << 38) + p.per_page - 1) / p.per_page;
   p.blocks = a->num_pages * p.per_page;
   p.table = a->block_table;
   p.t_sr = a->bt_stride_row;

@@ -125,7 +125,7 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
       v_at[u][d] = wide_at(8 * u + 4 * g2 + ((lane & 15) >> 2), 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
 
   for (int tile = 0; tile < tiles; ++tile) {
-    landed_and_barrier();  // this tile is there, and the one before is consumed
+    landed_and_barrier<0>();  // this tile is there, and the one before is consumed
     if (tile + 1 < tiles) stage(tile + 1);
     const char *buf = smem + (tile & 1) * kTileBytes;
     const int j0 = tile * kKeys;
