@@ -63,6 +63,12 @@ __device__ __forceinline__ int uniform_len(const DecodeParams &p, int b) {
   return ((const __attribute__((address_space(4))) int *)(uintptr_t)(p.lens))[b];
 }
 __device__ __forceinline__ int uniform_tokens(const DecodeParams &p, int b) { return min(max(uniform_len(p, b), 0), p.max_tokens); }
+// a b / c, rounded down (operands not negative).
+__device__ __forceinline__ uint32_t scaled(uint32_t a, uint32_t b, uint32_t c) {
+  const uint64_t n = (uint64_t)a * b;
+  return n >> 32 ? (uint32_t)(n / c) : (uint32_t)n / c;
+}
+
 // Four fp8 codes (one dword) -> two dwords of T, exact.  (Whole words: extracting elements of these
 // conversions' results one by one is miscompiled by the ROCm 7.2 LLVM.)
 template <typename T> __device__ __forceinline__ i32x2 fp8x4(int w);
@@ -96,7 +102,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     alignas(16) float max[kRows][kGroups];
     alignas(16) float sum[kRows][kGroups];
     int wave[kWaves];
-    int start[2];
+    int start[3];
     int rescale[3];
   };
 
@@ -109,14 +115,18 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     return row * kPRow + ((c ^ (kTokens == 64 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
   }
 
+  // What a run spends on one sequence more, in tiles (its query, its output, the stream's pause).
+  static constexpr int kSwitch = 4;
   // (a sequence without tokens has one tile, all masked: its rows are written too)
   static __device__ __forceinline__ int tiles_of(int tokens) { return max(1, (tokens + kTokens - 1) / kTokens); }
 
   // ---- the stream of tiles of a group's run, across its sequences ----
   struct Fetch {
-    int at, last;     // tile of the run, its end
-    int b, end;       // sequence, its last tile + 1
-    int t0, tokens;   // first token of the tile, tokens of the sequence
+    int n;            // tiles staged so far
+    bool more;        // there is another one:
+    int b, tile, end;  // sequence, tile of it, the run's last of it + 1
+    int base, last;   // cost at which the sequence begins, at which the run ends
+    int tokens;       // of the sequence
     int window, pid;  // lane k of pid: cache block k of the window's 64 (16 tokens each), -1 for none
     int lat, rope;    // LDS buffers
     uint32_t bad;     // bits 4 n .. of buffer n: blocks of its tile without a page
@@ -136,23 +146,17 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   static constexpr int kRopeLoads = (kRopeBytes / 1024 + kWaves - 1) / kWaves;
   static constexpr int kLoads = kLatLoads + kRopeLoads;
   static __device__ __forceinline__ void stage(const DecodeParams &p, Shared &s, Fetch &f, int wave, int lane) {
-    if (f.at == f.end) {
-      ++f.b;
-      f.tokens = uniform_tokens(p, f.b);
-      f.end += tiles_of(f.tokens);
-      f.t0 = 0;
-      f.window = -1;
-    }
-    if (f.t0 >> 10 != f.window) {
-      f.window = f.t0 >> 10;
+    const int t0 = f.tile * kTokens;
+    if (t0 >> 10 != f.window) {
+      f.window = t0 >> 10;
       f.pid = blocks_of_window(p, f.b, f.window * 64);
     }
-    const int blk0 = (f.t0 >> 4) & 63;
+    const int blk0 = (t0 >> 4) & 63;
     uint32_t bad = 0;
 #pragma unroll
     for (int k = 0; k < kTokBlocks; ++k) bad |= __builtin_amdgcn_readlane(f.pid, blk0 + k) < 0 ? 1u << k : 0u;
     f.bad = (f.bad & ~(15u << 4 * f.lat)) | bad << 4 * f.lat;
-    const int left = f.tokens - f.t0;
+    const int left = f.tokens - t0;
     constexpr int kChunks = kLatRow / 16;
 #pragma unroll
     for (int i = 0; i < kLatLoads; ++i) {
@@ -175,10 +179,18 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src + RANK * kBytes;
       load_lds(src + 16 * c, s.rope[f.rope] + at);
     }
-    ++f.at;
-    f.t0 += kTokens;
+    ++f.n;
     f.lat = (f.lat + 1) & 3;
     f.rope = f.rope == 2 ? 0 : f.rope + 1;
+    if (++f.tile < f.end) return;
+    f.base += kSwitch + tiles_of(f.tokens);
+    f.more = f.base + kSwitch < f.last;
+    if (!f.more) return;
+    ++f.b;
+    f.tokens = uniform_tokens(p, f.b);
+    f.tile = 0;
+    f.end = min(tiles_of(f.tokens), f.last - f.base - kSwitch);
+    f.window = -1;
   }
 
   static __device__ __forceinline__ void run(const DecodeParams &p, Shared &s) {
@@ -189,18 +201,21 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     const int group = (unit / p.row_blocks) * 8 + (blockIdx.x & 7);
     const int rblk = unit % p.row_blocks;
 
-    // ---- this group's run of tiles ----
-    int b = group, base = 0, first = 0, last = 0, per = 1;
+    // ---- this group's run ----
+    int b = group, base = 0, first = 0, last = 0, total = 0, tokens = 0;
     if (tid < 3) s.rescale[tid] = 0;
     if (!p.split) {
       if (b >= p.batch) return;  // the whole workgroup
-      last = tiles_of(uniform_tokens(p, b));
+      tokens = uniform_tokens(p, b);
+      last = kSwitch + tiles_of(tokens);
     } else {
       const int chunk = (p.batch + kThreads - 1) / kThreads;
-      int mine = 0;
+      int mine = 0, mine_tokens = 0;
       for (int i = 0; i < chunk; ++i) {
         const int n = tid * chunk + i;
-        if (n < p.batch) mine += tiles_of(seq_tokens(p, n));
+        if (n >= p.batch) break;
+        mine_tokens = seq_tokens(p, n);
+        mine += kSwitch + tiles_of(mine_tokens);
       }
       int inc = mine;
 #pragma unroll
@@ -210,63 +225,71 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       }
       if (lane == 63) s.wave[wave] = inc;
       __syncthreads();
-      int total = 0;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const int v = s.wave[w];
         if (w < wave) inc += v;
         total += v;
       }
-      per = (total + p.groups - 1) / p.groups;
-      first = min(group * per, total);
-      last = min(first + per, total);
+      // run g is cost floor(g total / groups) .. floor((g + 1) total / groups)
+      first = (int)scaled(group, total, p.groups);
+      last = (int)scaled(group + 1, total, p.groups);
       if (first >= last) return;  // the whole workgroup
       if (inc - mine <= first && first < inc) {
         int at = inc - mine, n = tid * chunk;
-        for (;; ++n) {
-          const int tiles = tiles_of(seq_tokens(p, n));
-          if (first < at + tiles) break;
-          at += tiles;
+        for (; chunk > 1; ++n) {
+          mine_tokens = seq_tokens(p, n);
+          if (first < at + kSwitch + tiles_of(mine_tokens)) break;
+          at += kSwitch + tiles_of(mine_tokens);
         }
         s.start[0] = n;
         s.start[1] = at;
+        s.start[2] = mine_tokens;
       }
       __syncthreads();
       b = __builtin_amdgcn_readfirstlane(s.start[0]);
       base = __builtin_amdgcn_readfirstlane(s.start[1]);
+      tokens = __builtin_amdgcn_readfirstlane(s.start[2]);
     }
+    if (base + kSwitch >= last) return;  // (the run ends before the sequence's first tile)
 
     Fetch f;
-    f.at = first;
-    f.last = last;
+    f.n = 0;
+    f.more = true;
     f.b = b;
-    f.tokens = uniform_tokens(p, b);
-    f.end = base + tiles_of(f.tokens);
-    f.t0 = (first - base) * kTokens;
-    f.window = f.pid = -1;
+    f.base = base;
+    f.last = last;
+    f.tokens = tokens;
+    f.tile = max(first - base - kSwitch, 0);
+    f.end = min(tiles_of(tokens), last - base - kSwitch);
+    f.window = f.tile * kTokens >> 10;
+    f.pid = blocks_of_window(p, b, f.window * 64);
     f.lat = f.rope = 0;
     f.bad = 0;
 
     // ---- one segment a sequence ----
-    Place at{first, 0, 0};
-    while (at.tile < last) {
-      const int tokens = f.at == first ? f.tokens : uniform_tokens(p, b), tiles = tiles_of(tokens);
-      const int seg_end = min(last, base + tiles);
-      if (p.split && at.tile == base && rblk == 0 && tid == 0) p.runs[b] = i32x2{group, (base + tiles - 1) / per};
-      segment(p, s, f, at, b, rblk, group, base, seg_end, seg_end == base + tiles, first, tokens, wave, lane);
-      base += tiles;
-      ++b;
+    Place at{0, 0, 0};
+    int lo = f.tile;
+    for (;;) {
+      const int tiles = tiles_of(tokens), hi = min(tiles, last - base - kSwitch);
+      // (the run of cost x: the last g with floor(g total / groups) <= x)
+      if (p.split && lo == 0 && rblk == 0 && tid == 0)
+        p.runs[b] = i32x2{group, (int)(((uint64_t)(base + kSwitch + tiles) * p.groups - 1) / (uint32_t)total)};
+      segment(p, s, f, at, b, rblk, group, lo, hi, tiles, tokens, wave, lane);
+      base += kSwitch + tiles;
+      if (base + kSwitch >= last) return;
+      lo = 0;
+      tokens = uniform_tokens(p, ++b);
     }
   }
 
-  // A tile of the run and its LDS buffers.
+  // A tile of the run (its number) and its LDS buffers.
   struct Place {
-    int tile, lat, rope;
+    int n, lat, rope;
   };
 
   static __device__ __forceinline__ void segment(const DecodeParams &p, Shared &s, Fetch &f, Place &at, int b, int rblk,
-                                                 int group, int base, int seg_end, bool ends, int first, int tokens,
-                                                 int wave, int lane) {
+                                                 int group, int lo, int hi, int tiles, int tokens, int wave, int lane) {
     const int n16 = lane & 15, g4 = lane >> 4;
     const int own = wave % RB, tg = wave / RB;  // block of rows, group of tokens of the score product
     const bool scores = kWaves / RB == kGroups || tg < kGroups;
@@ -288,9 +311,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         q[k] = *reinterpret_cast<const i32x4 *>(src + d);
       }
     }
-    if (at.tile == first) {  // (behind the query's loads, which come back in order)
+    if (f.n == 0) {  // (behind the query's loads, which come back in order)
       stage(p, s, f, wave, lane);
-      if (f.at < f.last) stage(p, s, f, wave, lane);
+      if (f.more) stage(p, s, f, wave, lane);
     }
 #pragma unroll
     for (int k = 0; k < kSlices; ++k) q[k] = live ? q[k] : i32x4{0, 0, 0, 0};
@@ -331,8 +354,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     };
     // A finished tile's P is in LDS, from the maximum so far.  Where a row exceeded that by much, all waves move
     // the maxima and P is written again.
-    auto settle = [&](int tile) {
-      if (__builtin_amdgcn_readfirstlane(s.rescale[tile % 3])) {  // the same for all waves
+    auto settle = [&](int n) {
+      if (__builtin_amdgcn_readfirstlane(s.rescale[n % 3])) {  // the same for all waves
         if (scores && g4 == 0) s.max[16 * own + n16][tg] = mx;
         lds_barrier();
         float alpha_own = 1.0f;
@@ -349,7 +372,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
           alpha_own = r == own ? alpha : alpha_own;
         }
         sum *= alpha_own;
-        if (scores) weights(s.p[tile & 1]);
+        if (scores) weights(s.p[n & 1]);
         lds_barrier();
       }
       sum += add;
@@ -423,19 +446,19 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     };
     // One iteration: the scores of tile `at` and, with PV, the value product of the tile before -- two independent
     // streams of LDS reads and matrix products, interleaved.
-    int t0 = (at.tile - base) * kTokens;
+    int t0 = lo * kTokens;
     auto iteration = [&](auto with_values) {
       constexpr bool PV = decltype(with_values)::value;
       const uint32_t bad = f.bad >> 4 * at.lat & 15;  // token blocks without a page
       const bool whole = t0 + kTokens <= min(tokens, len - p.q_len + 1) && !bad;
       // this tile has landed, its predecessor's P is written, the one before that is consumed
-      if (f.at - at.tile >= 2) landed_and_barrier<kLoads>();
+      if (f.n - at.n >= 2) landed_and_barrier<kLoads>();
       else landed_and_barrier<0>();
-      if (f.at < f.last) stage(p, s, f, wave, lane);
-      if (wave == 0) s.rescale[(at.tile + 1) % 3] = 0;
-      if constexpr (PV) settle(at.tile - 1);
+      if (f.more) stage(p, s, f, wave, lane);
+      if (wave == 0) s.rescale[(at.n + 1) % 3] = 0;
+      if constexpr (PV) settle(at.n - 1);
       const char *lat = s.lat[at.lat], *rope = s.rope[at.rope];
-      const char *old = s.lat[(at.lat + 3) & 3], *oldp = s.p[(at.tile + 1) & 1];
+      const char *old = s.lat[(at.lat + 3) & 3], *oldp = s.p[(at.n + 1) & 1];
       asm volatile("" : "+v"(k_at), "+v"(r_at), "+v"(v_at));  // (not loop invariant: hoisted, they take 30 registers)
       if (scores) {
         // The operands of a step are read while the step before is computed; the barriers keep the compiler from
@@ -480,28 +503,28 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
 #pragma unroll
         for (int u = 0; u < kBlocks; ++u) mx = fmaxf(mx, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
         mx = max_groups(mx) * p.c_log2;
-        weights(s.p[at.tile & 1]);
-        if (__any(mx > m_own + kRescale) && lane == 0) s.rescale[at.tile % 3] = 1;
+        weights(s.p[at.n & 1]);
+        if (__any(mx > m_own + kRescale) && lane == 0) s.rescale[at.n % 3] = 1;
       } else if constexpr (PV) {
         all_values(old, oldp);
       }
-      ++at.tile;
+      ++at.n;
       at.lat = (at.lat + 1) & 3;
       at.rope = at.rope == 2 ? 0 : at.rope + 1;
       t0 += kTokens;
     };
     iteration(std::false_type{});
-    while (at.tile < seg_end) iteration(std::true_type{});
+    for (int n = hi - lo; n > 1; --n) iteration(std::true_type{});
     lds_barrier();
-    settle(at.tile - 1);
-    all_values(s.lat[(at.lat + 3) & 3], s.p[(at.tile + 1) & 1]);
+    settle(at.n - 1);
+    all_values(s.lat[(at.lat + 3) & 3], s.p[(at.n + 1) & 1]);
 
     // ---- the rows' sums, over lane groups and token groups ----
     sum = sum_groups(sum);
     if (scores && g4 == 0) s.sum[16 * own + n16][tg] = sum;
     lds_barrier();
-    const bool all = first <= base && ends;
-    const int slot = base < first ? 2 * group : 2 * group + 1;
+    const bool all = lo == 0 && hi == tiles;
+    const int slot = lo > 0 ? 2 * group : 2 * group + 1;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const int lr = 16 * r + n16;
@@ -539,55 +562,85 @@ template <typename T, int KT, int RANK, int RB> __global__ __launch_bounds__(kTh
   Partial<T, KT, RANK, RB>::run(p, *reinterpret_cast<typename Partial<T, KT, RANK, RB>::Shared *>(smem));
 }
 
-// One workgroup a row: RANK / 4 lanes hold four dims each, the others take further parts.  Bound by its chain of
-// loads (runs, maxima, parts); no scan of the lengths, the partial kernel has left each sequence's runs.
-template <typename T, int RANK>
+// A row's output from the parts of its runs.  Bound by a chain of loads (runs, maxima, parts), so a call's rows
+// are on the chip at once: with few runs a sequence a wave takes a whole row (WIDE = false, 8 rows a workgroup);
+// with many a workgroup takes 128 dims of one row, and its 16 half waves every 16th run each (32 x 4096 tokens of
+// 128 heads, four runs a sequence: 12.5 us with a workgroup a row; 2 x 131072 tokens, 128 runs: 8.0).
+template <typename T, int RANK, bool WIDE>
 __global__ __launch_bounds__(kThreads) void latent_merge(DecodeParams p, int block_rows) {
-  constexpr int kCols = RANK / 4, kParts = kThreads / kCols;
-  __shared__ f32x4 s_acc[kParts][kCols];
-  __shared__ float s_l[kParts];
-  const int b = blockIdx.y, row = blockIdx.x;
-  const i32x2 runs = p.runs[b];
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = WIDE ? blockIdx.x : blockIdx.x * kWaves + wave;
+  const i32x2 runs = ((const __attribute__((address_space(4))) i32x2 *)(uintptr_t)(p.runs))[b];
   const int g0 = runs[0], g1 = runs[1];
-  if (g0 == g1) return;  // written already
+  if (g0 == g1 || row >= p.rows) return;  // written already; (whole waves, and without WIDE there is no barrier)
   const int rblk = row / block_rows, lr = row - rblk * block_rows;
   auto prow = [&](int g) {
     const int slot = g == g0 ? 2 * g + 1 : 2 * g;
     return ((int64_t)slot * p.row_blocks + rblk) * block_rows + lr;
   };
+  constexpr int kVecs = WIDE ? 1 : RANK / 256;  // of four dims a lane
+  constexpr int kStep = WIDE ? kThreads / 32 : 1, kAhead = 8;
+  const int part = WIDE ? threadIdx.x >> 5 : 0;
+  const int d0 = WIDE ? blockIdx.z * 128 + 4 * (lane & 31) : 4 * lane;  // the others follow at 256
+  // the first parts are on their way with the maxima
+  f32x4 x[kAhead][kVecs];
+  f32x2 ml[kAhead];
+  auto load = [&](int g) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t r = prow(min(g + k * kStep, g1));
+      ml[k] = *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * r);
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) x[k][v] = *reinterpret_cast<const f32x4 *>(p.part + r * RANK + d0 + 256 * v);
+    }
+  };
+  load(g0 + part);
   float m = -INFINITY;
-  for (int g = g0 + (threadIdx.x & 63); g <= g1; g += 64) m = fmaxf(m, p.part_ml[2 * prow(g)]);
+  for (int g = g0 + lane; g <= g1; g += 64) m = fmaxf(m, p.part_ml[2 * prow(g)]);
   m = max_groups(m);
 #pragma unroll
   for (int off = 8; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
   const float m_use = m == -INFINITY ? 0.0f : m;
-  const int col = threadIdx.x % kCols, part = threadIdx.x / kCols;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.0f;
-#pragma unroll 4
-  for (int g = g0 + part; g <= g1; g += kParts) {
-    const int64_t r = prow(g);
-    const f32x2 ml = *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * r);
-    const f32x4 x = *reinterpret_cast<const f32x4 *>(p.part + r * RANK + 4 * col);
-    const float w = __builtin_amdgcn_exp2f(ml[0] - m_use);
-    acc += x * w;
-    l += ml[1] * w;
-  }
-  s_acc[part][col] = acc;
-  if (col == 0) s_l[part] = l;
-  __syncthreads();
-  if (part) return;
+  f32x4 acc[kVecs];
 #pragma unroll
-  for (int k = 1; k < kParts; ++k) {
-    acc += s_acc[k][col];
-    l += s_l[k];
+  for (int v = 0; v < kVecs; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float l = 0.0f;
+  for (int g = g0 + part;;) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (g + k * kStep > g1) continue;
+      const float w = __builtin_amdgcn_exp2f(ml[k][0] - m_use);
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) acc[v] += x[k][v] * w;
+      l += ml[k][1] * w;
+    }
+    g += kAhead * kStep;
+    if (g > g1) break;
+    load(g);
+  }
+  if constexpr (WIDE) {
+    __shared__ f32x4 s_acc[kThreads];
+    __shared__ float s_l[kThreads / 32];
+    s_acc[threadIdx.x] = acc[0];
+    if ((lane & 31) == 0) s_l[part] = l;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int k = 1; k < kThreads / 32; ++k) {
+      acc[0] += s_acc[32 * k + lane];
+      l += s_l[k];
+    }
   }
   const int i = row / p.heads, h = row - i * p.heads;
   const int64_t orow = (int64_t)b * p.q_len + i;
-  const f32x4 x = acc * (l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l));
-  *reinterpret_cast<i32x2 *>(reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + 4 * col) =
-      i32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
-  if (p.lse && col == 0) p.lse[orow * p.l_sr + h * p.l_sh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+  const float inv = l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    const f32x4 x = acc[v] * inv;
+    *reinterpret_cast<i32x2 *>(reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + d0 + 256 * v) =
+        i32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+  }
+  if (p.lse && d0 == 0) p.lse[orow * p.l_sr + h * p.l_sh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 }  // namespace l20la
@@ -696,8 +749,13 @@ template <typename T, int RANK>
 hipError_t launch(const l20la::DecodeParams &p, bool fp8, int blocks, hipStream_t s) {
   const hipError_t e = fp8 ? launch_rows<T, 0, RANK>(p, blocks, s) : launch_rows<T, 1, RANK>(p, blocks, s);
   if (e != hipSuccess || !p.split) return e;
-  hipLaunchKernelGGL((l20la::latent_merge<T, RANK>), dim3((unsigned)p.rows, (unsigned)p.batch), dim3(l20la::kThreads), 0,
-                     s, p, 16 * blocks);
+  if (p.groups > 8 * p.batch)
+    hipLaunchKernelGGL((l20la::latent_merge<T, RANK, true>), dim3((unsigned)p.rows, (unsigned)p.batch, RANK / 128),
+                       dim3(l20la::kThreads), 0, s, p, 16 * blocks);
+  else
+    hipLaunchKernelGGL((l20la::latent_merge<T, RANK, false>),
+                       dim3((unsigned)((p.rows + l20la::kWaves - 1) / l20la::kWaves), (unsigned)p.batch),
+                       dim3(l20la::kThreads), 0, s, p, 16 * blocks);
   return hipGetLastError();
 }
 
