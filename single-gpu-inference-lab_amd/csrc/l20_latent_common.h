@@ -104,10 +104,15 @@ __device__ __forceinline__ float sum_groups(float x) { return sum_swap<32>(sum_s
 // the wave has waited for its loads (landed_and_barrier).  Not the builtin: with a builtin's load in flight the
 // compiler waits for all loads before every transposing read, which ends the prefetch; a load into LDS has no
 // result registers that could be taken for written.
-__device__ __forceinline__ void load_lds(const void *src, void *dst) {
-  const int at = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)dst);  // (an LDS address' low half)
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(at) : "memory");
+__device__ __forceinline__ void load_lds(const void *src, uint32_t dst) {  // dst: wave-uniform
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(dst) : "memory");
 }
+__device__ __forceinline__ void load_lds(const void *base, uint32_t off, uint32_t dst) {  // base, dst: wave-uniform
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(dst) : "memory");
+}
+// The LDS address of a pointer into shared memory (the low half of a generic one).
+__device__ __forceinline__ uint32_t lds_address(const void *p) { return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)p); }
+
 // All but the wave's last N loads have landed, in LDS too, and so for the workgroup's other waves.
 template <int N> __device__ __forceinline__ void landed_and_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");

@@ -157,27 +157,41 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     for (int k = 0; k < kTokBlocks; ++k) bad |= __builtin_amdgcn_readlane(f.pid, blk0 + k) < 0 ? 1u << k : 0u;
     f.bad = (f.bad & ~(15u << 4 * f.lat)) | bad << 4 * f.lat;
     const int left = f.tokens - t0;
-    constexpr int kChunks = kLatRow / 16;
+    const uint32_t lat = lds_address(s.lat[f.lat]) + wave * kLatLoads * 1024, rope = lds_address(s.rope[f.rope]);
+    // a wave's latent rows are some consecutive ones of a block; (where there are fewer instructions for the rotary
+    // parts than waves some are made twice: every wave counts the same loads)
+    constexpr int kWaveRows = kTokens / kWaves, kLoadRows = 1024 / kLatRow, kChunks = kLatRow / 16;
+    constexpr int kRopeRows = 1024 / kRopeRow, kRopeChunks = kRopeRow / 16;
+    static_assert(kRopeLoads == 1 && kWaveRows == kLatLoads * kLoadRows, "a wave's share of a tile");
+    const int row0 = wave * kWaveRows, rope0 = wave % (kRopeBytes / 1024) * kRopeRows;
+    const int id = __builtin_amdgcn_readlane(f.pid, blk0 + (row0 >> 4));
+    const int rope_id = __builtin_amdgcn_readlane(f.pid, blk0 + (rope0 >> 4));
+    if (left >= kTokens && !bad) {
+      // one scalar base and a lane's offset: the swizzle of load i is an XOR of the lane's chunk
+      const uint32_t c_tok = (uint32_t)p.c_tok;
+      const int lrow = lane / kChunks;
+      const uint32_t row_off = lrow * c_tok, chunk = ((lane % kChunks) ^ lrow) << 4;
+      const uint8_t *src = p.cache + (int64_t)id * p.c_block + (uint32_t)(row0 & 15) * c_tok;
 #pragma unroll
-    for (int i = 0; i < kLatLoads; ++i) {
-      const int at = (wave * kLatLoads + i) * 1024;  // of the buffer
-      const int row = at / kLatRow + lane / kChunks;
-      const int id = __builtin_amdgcn_readlane(f.pid, blk0 + (at / kLatRow >> 4));
-      const int c = (lane % kChunks) ^ (row & 15);
-      const uint8_t *src = p.cache + (int64_t)id * p.c_block + (int64_t)(row & 15) * p.c_tok;
-      src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src;
-      load_lds(src + 16 * c, s.lat[f.lat] + at);
-    }
+      for (int i = 0; i < kLatLoads; ++i) {
+        const uint32_t swizzle = ((row0 & 15) + i * kLoadRows) << 4;
+        load_lds(src + i * kLoadRows * c_tok, (chunk ^ swizzle) + row_off, lat + i * 1024);
+      }
+      const int rrow = (rope0 & 15) + lane / kRopeChunks;
+      load_lds(p.cache + (int64_t)rope_id * p.c_block + RANK * kBytes,
+               rrow * c_tok + (((lane % kRopeChunks) ^ rope_swizzle(rrow)) << 4), rope + rope0 * kRopeRow);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kRopeLoads; ++i) {
-      // (where there are fewer instructions than waves some are made twice: every wave counts the same loads)
-      const int at = (i * kWaves + wave) % (kRopeBytes / 1024) * 1024;
-      const int row = at / kRopeRow + lane / (kRopeRow / 16);
-      const int id = __builtin_amdgcn_readlane(f.pid, blk0 + (at / kRopeRow >> 4));
-      const int c = (lane % (kRopeRow / 16)) ^ rope_swizzle(row);
-      const uint8_t *src = p.cache + (int64_t)id * p.c_block + (int64_t)(row & 15) * p.c_tok;
-      src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src + RANK * kBytes;
-      load_lds(src + 16 * c, s.rope[f.rope] + at);
+      for (int i = 0; i < kLatLoads; ++i) {
+        const int row = row0 + i * kLoadRows + lane / kChunks, c = (lane % kChunks) ^ (row & 15);
+        const uint8_t *src = p.cache + (int64_t)id * p.c_block + (int64_t)(row & 15) * p.c_tok;
+        src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src;
+        load_lds(src + 16 * c, lat + i * 1024);
+      }
+      const int row = rope0 + lane / kRopeChunks, c = (lane % kRopeChunks) ^ rope_swizzle(row);
+      const uint8_t *src = p.cache + (int64_t)rope_id * p.c_block + (int64_t)(row & 15) * p.c_tok;
+      src = rope_id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src + RANK * kBytes;
+      load_lds(src + 16 * c, rope + rope0 * kRopeRow);
     }
     ++f.n;
     f.lat = (f.lat + 1) & 3;
@@ -202,7 +216,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     const int rblk = unit % p.row_blocks;
 
     // ---- this group's run ----
-    int b = group, base = 0, first = 0, last = 0, total = 0, tokens = 0;
+    int b = group, base = 0, first = 0, last = 0, total = 0, runs = 1, tokens = 0;
     if (tid < 3) s.rescale[tid] = 0;
     if (!p.split) {
       if (b >= p.batch) return;  // the whole workgroup
@@ -231,10 +245,11 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         if (w < wave) inc += v;
         total += v;
       }
-      // run g is cost floor(g total / groups) .. floor((g + 1) total / groups)
-      first = (int)scaled(group, total, p.groups);
-      last = (int)scaled(group + 1, total, p.groups);
-      if (first >= last) return;  // the whole workgroup
+      // run g is cost floor(g total / runs) .. floor((g + 1) total / runs); none is empty
+      runs = min(p.groups, total);
+      if (group >= runs) return;  // the whole workgroup
+      first = (int)scaled(group, total, runs);
+      last = (int)scaled(group + 1, total, runs);
       if (inc - mine <= first && first < inc) {
         int at = inc - mine, n = tid * chunk;
         for (; chunk > 1; ++n) {
@@ -272,9 +287,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     int lo = f.tile;
     for (;;) {
       const int tiles = tiles_of(tokens), hi = min(tiles, last - base - kSwitch);
-      // (the run of cost x: the last g with floor(g total / groups) <= x)
+      // (the run of cost x: the last g with floor(g total / runs) <= x)
       if (p.split && lo == 0 && rblk == 0 && tid == 0)
-        p.runs[b] = i32x2{group, (int)(((uint64_t)(base + kSwitch + tiles) * p.groups - 1) / (uint32_t)total)};
+        p.runs[b] = i32x2{group, (int)(((uint64_t)(base + kSwitch + tiles) * runs - 1) / (uint32_t)total)};
       segment(p, s, f, at, b, rblk, group, lo, hi, tiles, tokens, wave, lane);
       base += kSwitch + tiles;
       if (base + kSwitch >= last) return;
@@ -354,8 +369,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     };
     // A finished tile's P is in LDS, from the maximum so far.  Where a row exceeded that by much, all waves move
     // the maxima and P is written again.
-    auto settle = [&](int n) {
-      if (__builtin_amdgcn_readfirstlane(s.rescale[n % 3])) {  // the same for all waves
+    auto settle = [&](int n, int move) {
+      if (__builtin_amdgcn_readfirstlane(move)) {  // the same for all waves
         if (scores && g4 == 0) s.max[16 * own + n16][tg] = mx;
         lds_barrier();
         float alpha_own = 1.0f;
@@ -454,9 +469,10 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       // this tile has landed, its predecessor's P is written, the one before that is consumed
       if (f.n - at.n >= 2) landed_and_barrier<kLoads>();
       else landed_and_barrier<0>();
+      const int move = PV ? s.rescale[(at.n + 2) % 3] : 0;  // (read early: its latency passes while the loads start)
       if (f.more) stage(p, s, f, wave, lane);
       if (wave == 0) s.rescale[(at.n + 1) % 3] = 0;
-      if constexpr (PV) settle(at.n - 1);
+      if constexpr (PV) settle(at.n - 1, move);
       const char *lat = s.lat[at.lat], *rope = s.rope[at.rope];
       const char *old = s.lat[(at.lat + 3) & 3], *oldp = s.p[(at.n + 1) & 1];
       asm volatile("" : "+v"(k_at), "+v"(r_at), "+v"(v_at));  // (not loop invariant: hoisted, they take 30 registers)
@@ -516,7 +532,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     iteration(std::false_type{});
     for (int n = hi - lo; n > 1; --n) iteration(std::true_type{});
     lds_barrier();
-    settle(at.n - 1);
+    settle(at.n - 1, s.rescale[(at.n + 2) % 3]);
     all_values(s.lat[(at.lat + 3) & 3], s.p[(at.n + 1) & 1]);
 
     // ---- the rows' sums, over lane groups and token groups ----
@@ -717,6 +733,7 @@ int32_t check(const l20_pd_latent_args *a) {
     return set_error(L20_PD_EINVAL, "tokens of a page above 16 must be contiguous");
   if (!a->query || !a->cache || !a->block_table || !a->seq_lens || !a->output)
     return set_error(L20_PD_EINVAL, "null tensor pointer");
+  if (a->c_stride_token < 0 || a->c_stride_token >= (1 << 26)) return set_error(L20_PD_EINVAL, "latent cache token stride out of range");
   auto u = [](const void *x) { return (uint64_t)(uintptr_t)x; };
   if ((u(a->query) | (uint64_t)(2 * a->q_stride_row) | (uint64_t)(2 * a->q_stride_head)) % 16)
     return set_error(L20_PD_EINVAL, "query rows must be 16-byte aligned");

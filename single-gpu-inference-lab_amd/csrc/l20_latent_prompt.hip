@@ -79,24 +79,25 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
   const char *kb = reinterpret_cast<const char *>(p.k) + 2 * (ks * p.k_st + h * p.k_sh);
   const char *vb = reinterpret_cast<const char *>(p.v) + 2 * (ks * p.v_st + h * p.v_sh);
   const char *rb = reinterpret_cast<const char *>(p.kr) + 2 * (ks * p.kr_st);
-  const int64_t k_row = 2 * p.k_st, v_row = 2 * p.v_st, r_row = 2 * p.kr_st;
+  // (a tile's rows are within 32 bits of its first, checked on the host)
+  const uint32_t k_row = 2 * (uint32_t)p.k_st, v_row = 2 * (uint32_t)p.v_st, r_row = 2 * (uint32_t)p.kr_st;
+  const uint32_t lds = lds_address(smem);
   auto stage = [&](int tile) {
-    char *buf = smem + (tile & 1) * kTileBytes;
+    const uint32_t buf = lds + (tile & 1) * kTileBytes;
     const int j0 = tile * kKeys;
+    const char *kt = kb + (int64_t)j0 * (2 * p.k_st), *vt = vb + (int64_t)j0 * (2 * p.v_st), *rt = rb + (int64_t)j0 * (2 * p.kr_st);
     // rows past the last key hold that key again: they are masked, and what they hold is as finite as it is
     const int last = nk - 1 - j0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 16 * wave + 4 * i + (lane >> 4), c = (lane & 15) ^ (row & 15);
-      const int64_t j = j0 + min(row, last);
-      load_lds(kb + j * k_row + 16 * c, buf + (16 * wave + 4 * i) * kWideRow);
-      load_lds(vb + j * v_row + 16 * c, buf + kWideBytes + (16 * wave + 4 * i) * kWideRow);
+      const int row = 16 * wave + 4 * i + (lane >> 4), c = (lane & 15) ^ (row & 15), r = min(row, last);
+      load_lds(kt, r * k_row + 16 * c, buf + (16 * wave + 4 * i) * kWideRow);
+      load_lds(vt, r * v_row + 16 * c, buf + kWideBytes + (16 * wave + 4 * i) * kWideRow);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = 16 * wave + 8 * i + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
-      const int64_t j = j0 + min(row, last);
-      load_lds(rb + j * r_row + 16 * c, buf + 2 * kWideBytes + (16 * wave + 8 * i) * kNarrowRow);
+      load_lds(rt, min(row, last) * r_row + 16 * c, buf + 2 * kWideBytes + (16 * wave + 8 * i) * kNarrowRow);
     }
   };
   if (tiles > 0) stage(0);
@@ -224,6 +225,8 @@ int32_t check(const l20_pd_latent_prompt_args *a) {
   if (a->batch == 0 || a->total_q == 0 || a->max_q_len == 0) return L20_PD_OK;
   if (!a->query || !a->output || !a->cu_q || !a->cu_k || (a->total_k > 0 && (!a->key || !a->key_rope || !a->value)))
     return set_error(L20_PD_EINVAL, "null tensor pointer");
+  for (const int64_t stride : {a->k_stride_token, a->v_stride_token, a->kr_stride_token})
+    if (stride < 0 || stride >= (1 << 24)) return set_error(L20_PD_EINVAL, "key and value token strides out of range");
   auto u = [](const void *x) { return (uint64_t)(uintptr_t)x; };
   const uint64_t in = u(a->query) | u(a->key) | u(a->key_rope) | u(a->value) | (uint64_t)(2 * a->q_stride_token) |
                       (uint64_t)(2 * a->q_stride_head) | (uint64_t)(2 * a->k_stride_token) |
