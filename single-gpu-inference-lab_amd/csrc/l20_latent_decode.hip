@@ -47,7 +47,7 @@ struct DecodeParams {
   int64_t o_sr, o_sh;
   float *lse;
   int64_t l_sr, l_sh;
-  float *part;     // [slot][row block][row][RANK]
+  float *part;     // [slot][row block][16 rows][16 dims][lane][4], as the accumulators lie
   float *part_ml;  // [slot][row block][row][2]: maximum (log2 units), sum
   i32x2 *runs;     // [batch]: the first and the last run that hold a part of the sequence
   float c_log2, out_scale;
@@ -146,6 +146,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   static constexpr int kRopeLoads = (kRopeBytes / 1024 + kWaves - 1) / kWaves;
   static constexpr int kLoads = kLatLoads + kRopeLoads;
   static __device__ __forceinline__ void stage(const DecodeParams &p, Shared &s, Fetch &f, int wave, int lane) {
+    asm volatile("" : "+v"(lane));  // (what follows from it is not kept in registers over the tiles)
     const int t0 = f.tile * kTokens;
     if (t0 >> 10 != f.window) {
       f.window = t0 >> 10;
@@ -267,6 +268,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       tokens = __builtin_amdgcn_readfirstlane(s.start[2]);
     }
     if (base + kSwitch >= last) return;  // (the run ends before the sequence's first tile)
+    load_query(p, s, b, rblk, wave, lane);
 
     Fetch f;
     f.n = 0;
@@ -298,6 +300,26 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     }
   }
 
+  // The query rows of sequence b into LDS, in the buffers of the tiles that come later: whole rows, a load touches
+  // few lines of 128 bytes.  (As operands straight from memory a load touches 16, and the waves that share rows
+  // load them again: 2 to 5 us before the first tile.)
+  static __device__ __forceinline__ void load_query(const DecodeParams &p, Shared &s, int b, int rblk, int wave, int lane) {
+    constexpr int kRow = RANK * 2, kLoadsQ = kRows * kRow / 1024 / kWaves, kRopeQ = kRows * kRope * 2 / 1024;
+    static_assert(sizeof(s.lat[0]) * 2 >= kRows * kRow && sizeof(s.p) >= kRows * kRope * 2, "the buffers hold the rows");
+    auto row_of = [&](int row) {
+      const int r = min(rblk * kRows + row, p.rows - 1), i = r / p.heads;
+      return reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + (r - i * p.heads) * p.q_sh;
+    };
+    const uint32_t lat = lds_address(s.lat[2]), rope = lds_address(s.p[0]);
+#pragma unroll
+    for (int i = 0; i < kLoadsQ; ++i) {
+      const int at = (wave * kLoadsQ + i) * 1024, row = at / kRow + lane / (kRow / 16);
+      load_lds(row_of(row) + 8 * ((lane % (kRow / 16)) ^ (row & 15)), lat + at);
+    }
+    const int n = wave % kRopeQ, row = 8 * n + lane / 8;
+    load_lds(row_of(row) + RANK + 8 * ((lane & 7) ^ ((row >> 1) & 7)), rope + n * 1024);
+  }
+
   // A tile of the run (its number) and its LDS buffers.
   struct Place {
     int n, lat, rope;
@@ -311,27 +333,30 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     const int len = uniform_len(p, b);
     i32x4 q[kSlices];
     int lim;
-    bool live;
     {
-      const int r = rblk * kRows + 16 * own + n16;
-      live = r < p.rows;
-      const int i = live ? r / p.heads : 0, h = live ? r - i * p.heads : 0;
-      lim = live ? min(len - p.q_len + i, tokens - 1) : -1;
+      // (rows past the last repeat it: they are not stored)
+      const int r = min(rblk * kRows + 16 * own + n16, p.rows - 1), i = r / p.heads;
+      lim = min(len - p.q_len + i, tokens - 1);
       // the order of the dims in the product is free: over an fp8 cache a lane's are 16 in a row of each 64, so
       // that one 16-byte read gives two slices
-      const T *src = reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + h * p.q_sh;
+      if (f.n == 0) {
+        landed_and_barrier<0>();  // the query of the run's first sequence is in LDS
+        stage(p, s, f, wave, lane);
+        if (f.more) stage(p, s, f, wave, lane);
 #pragma unroll
-      for (int k = 0; k < kSlices; ++k) {
-        const int d = KT == 0 ? 64 * (k >> 1) + 16 * g4 + 8 * (k & 1) : 32 * k + 8 * g4;
-        q[k] = *reinterpret_cast<const i32x4 *>(src + d);
+        for (int k = 0; k < kSlices; ++k) {
+          const int c = KT == 0 ? 8 * (k >> 1) + 2 * g4 + (k & 1) : 4 * k + g4, row = 16 * own + n16;
+          q[k] = *reinterpret_cast<const i32x4 *>(
+              32 * k < RANK ? s.lat[2] + row * (2 * RANK) + ((c ^ (row & 15)) << 4)
+                            : s.p[0] + row * (2 * kRope) + (((c - RANK / 8) ^ ((row >> 1) & 7)) << 4));
+        }
+      } else if (scores) {
+        const T *src = reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + (r - i * p.heads) * p.q_sh;
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k)
+          q[k] = *reinterpret_cast<const i32x4 *>(src + (KT == 0 ? 64 * (k >> 1) + 16 * g4 + 8 * (k & 1) : 32 * k + 8 * g4));
       }
     }
-    if (f.n == 0) {  // (behind the query's loads, which come back in order)
-      stage(p, s, f, wave, lane);
-      if (f.more) stage(p, s, f, wave, lane);
-    }
-#pragma unroll
-    for (int k = 0; k < kSlices; ++k) q[k] = live ? q[k] : i32x4{0, 0, 0, 0};
 
     f32x4 acc[RB][kDimBlocks];
     float m_all[RB];  // the maximum that P of the lane's row in each block refers to, log2 units
@@ -540,7 +565,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     if (scores && g4 == 0) s.sum[16 * own + n16][tg] = sum;
     lds_barrier();
     const bool all = lo == 0 && hi == tiles;
-    const int slot = lo > 0 ? 2 * group : 2 * group + 1;
+    const int64_t part = (int64_t)(lo > 0 ? 2 * group : 2 * group + 1) * p.row_blocks + rblk;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const int lr = 16 * r + n16;
@@ -548,27 +573,26 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       float l = 0.0f;
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) l += s.sum[lr][k];
-      if (row >= p.rows) continue;
-      if (all) {
-        const int i = row / p.heads, h = row - i * p.heads;
-        const int64_t orow = (int64_t)b * p.q_len + i;
-        const float inv = l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
-        T *dst = reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + 4 * g4;
+      if (!all) {
+        // as the accumulators lie: block of 16 rows, block of 16 dims, lane
+        f32x4 *dst = reinterpret_cast<f32x4 *>(p.part) + ((part * RB + r) * (RANK / 16) + wave * kDimBlocks) * 64 + lane;
 #pragma unroll
-        for (int d = 0; d < kDimBlocks; ++d) {
-          const f32x4 x = acc[r][d] * inv;
-          *reinterpret_cast<i32x2 *>(dst + 16 * (wave * kDimBlocks + d)) =
-              i32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
-        }
-        if (p.lse && wave == 0 && g4 == 0)
-          p.lse[orow * p.l_sr + h * p.l_sh] = l == 0.0f ? -INFINITY : (m_all[r] + log2f(l)) * kLn2;
-      } else {
-        const int64_t prow = ((int64_t)slot * p.row_blocks + rblk) * kRows + lr;
-        float *dst = p.part + prow * RANK + 4 * g4;
-#pragma unroll
-        for (int d = 0; d < kDimBlocks; ++d) *reinterpret_cast<f32x4 *>(dst + 16 * (wave * kDimBlocks + d)) = acc[r][d];
-        if (wave == 0 && g4 == 0) *reinterpret_cast<f32x2 *>(p.part_ml + 2 * prow) = f32x2{m_all[r], l};
+        for (int d = 0; d < kDimBlocks; ++d) dst[64 * d] = acc[r][d];
+        if (wave == 0 && g4 == 0) *reinterpret_cast<f32x2 *>(p.part_ml + 2 * (part * kRows + lr)) = f32x2{m_all[r], l};
+        continue;
       }
+      if (row >= p.rows) continue;
+      const int i = row / p.heads, h = row - i * p.heads;
+      const int64_t orow = (int64_t)b * p.q_len + i;
+      const float inv = l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
+      T *dst = reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + 4 * g4;
+#pragma unroll
+      for (int d = 0; d < kDimBlocks; ++d) {
+        const f32x4 x = acc[r][d] * inv;
+        *reinterpret_cast<i32x2 *>(dst + 16 * (wave * kDimBlocks + d)) = i32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+      }
+      if (p.lse && wave == 0 && g4 == 0)
+        p.lse[orow * p.l_sr + h * p.l_sh] = l == 0.0f ? -INFINITY : (m_all[r] + log2f(l)) * kLn2;
     }
   }
 };
@@ -578,85 +602,97 @@ template <typename T, int KT, int RANK, int RB> __global__ __launch_bounds__(kTh
   Partial<T, KT, RANK, RB>::run(p, *reinterpret_cast<typename Partial<T, KT, RANK, RB>::Shared *>(smem));
 }
 
-// A row's output from the parts of its runs.  Bound by a chain of loads (runs, maxima, parts), so a call's rows
-// are on the chip at once: with few runs a sequence a wave takes a whole row (WIDE = false, 8 rows a workgroup);
-// with many a workgroup takes 128 dims of one row, and its 16 half waves every 16th run each (32 x 4096 tokens of
-// 128 heads, four runs a sequence: 12.5 us with a workgroup a row; 2 x 131072 tokens, 128 runs: 8.0).
+// Outputs of sequences that several runs share, from their parts, which lie as the accumulators did: a lane holds
+// row lane % 16 of a block of 16, dims 4 (lane / 16) .. + 3 of a block of 16.  Bound by a chain of loads (runs,
+// maxima and parts), so a call's rows are on the chip at once: with few runs a sequence a wave takes all runs of one
+// row block and RANK / 8 dims; with many (WIDE) a workgroup takes 16 dims, its waves every eighth run.
 template <typename T, int RANK, bool WIDE>
 __global__ __launch_bounds__(kThreads) void latent_merge(DecodeParams p, int block_rows) {
-  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = WIDE ? blockIdx.x : blockIdx.x * kWaves + wave;
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n16 = lane & 15, g4 = lane >> 4;
   const i32x2 runs = ((const __attribute__((address_space(4))) i32x2 *)(uintptr_t)(p.runs))[b];
   const int g0 = runs[0], g1 = runs[1];
-  if (g0 == g1 || row >= p.rows) return;  // written already; (whole waves, and without WIDE there is no barrier)
-  const int rblk = row / block_rows, lr = row - rblk * block_rows;
-  auto prow = [&](int g) {
-    const int slot = g == g0 ? 2 * g + 1 : 2 * g;
-    return ((int64_t)slot * p.row_blocks + rblk) * block_rows + lr;
+  if (g0 == g1) return;  // written already; the whole workgroup
+  constexpr int kBlocks = WIDE ? 1 : RANK / 16 / kWaves;  // of 16 dims
+  constexpr int kStep = WIDE ? kWaves : 1, kAhead = 8;
+  const int row16 = blockIdx.x;  // block of 16 rows of the sequence
+  const int per = block_rows / 16, rblk = row16 / per, r = row16 - rblk * per;
+  const int dim0 = WIDE ? blockIdx.z : wave * kBlocks, first = WIDE ? g0 + wave : g0;
+  auto part_of = [&](int g) { return (int64_t)(g == g0 ? 2 * g + 1 : 2 * g) * p.row_blocks + rblk; };
+  auto ml_of = [&](int g) {
+    return *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * (part_of(g) * block_rows + 16 * r + n16));
   };
-  constexpr int kVecs = WIDE ? 1 : RANK / 256;  // of four dims a lane
-  constexpr int kStep = WIDE ? kThreads / 32 : 1, kAhead = 8;
-  const int part = WIDE ? threadIdx.x >> 5 : 0;
-  const int d0 = WIDE ? blockIdx.z * 128 + 4 * (lane & 31) : 4 * lane;  // the others follow at 256
-  // the first parts are on their way with the maxima
-  f32x4 x[kAhead][kVecs];
+  f32x4 x[kAhead][kBlocks];
   f32x2 ml[kAhead];
   auto load = [&](int g) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int64_t r = prow(min(g + k * kStep, g1));
-      ml[k] = *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * r);
+      const int gk = min(g + k * kStep, g1);
+      ml[k] = ml_of(gk);
+      const f32x4 *src = reinterpret_cast<const f32x4 *>(p.part) + ((part_of(gk) * per + r) * (RANK / 16) + dim0) * 64 + lane;
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) x[k][v] = *reinterpret_cast<const f32x4 *>(p.part + r * RANK + d0 + 256 * v);
+      for (int d = 0; d < kBlocks; ++d) x[k][d] = src[64 * d];
     }
   };
-  load(g0 + part);
-  float m = -INFINITY;
-  for (int g = g0 + lane; g <= g1; g += 64) m = fmaxf(m, p.part_ml[2 * prow(g)]);
-  m = max_groups(m);
+  f32x4 acc[kBlocks];
 #pragma unroll
-  for (int off = 8; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-  const float m_use = m == -INFINITY ? 0.0f : m;
-  f32x4 acc[kVecs];
+  for (int d = 0; d < kBlocks; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.0f;
+  // (of what m refers to; a row that no part has seen keeps -inf)
+  auto rescale = [&](float next) {
+    const float a = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));
+    m = next;
+    l *= a;
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float l = 0.0f;
-  for (int g = g0 + part;;) {
+    for (int d = 0; d < kBlocks; ++d) acc[d] *= a;
+  };
+  auto weight = [&](float x) { return __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.0f : m)); };
+  for (int g = first; g <= g1; g += kAhead * kStep) {
+    load(g);
+    float next = m;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) next = fmaxf(next, ml[k][0]);  // (past the last run: that one again)
+    rescale(next);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (g + k * kStep > g1) continue;
-      const float w = __builtin_amdgcn_exp2f(ml[k][0] - m_use);
+      const float w = weight(ml[k][0]);
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) acc[v] += x[k][v] * w;
+      for (int d = 0; d < kBlocks; ++d) acc[d] += x[k][d] * w;
       l += ml[k][1] * w;
     }
-    g += kAhead * kStep;
-    if (g > g1) break;
-    load(g);
   }
   if constexpr (WIDE) {
-    __shared__ f32x4 s_acc[kThreads];
-    __shared__ float s_l[kThreads / 32];
-    s_acc[threadIdx.x] = acc[0];
-    if ((lane & 31) == 0) s_l[part] = l;
+    __shared__ f32x4 s_acc[kWaves][64];
+    __shared__ f32x2 s_ml[kWaves][64];
+    s_acc[wave][lane] = acc[0];
+    s_ml[wave][lane] = f32x2{m, l};
     __syncthreads();
-    if (part) return;
+    if (wave) return;
+    float next = m;
 #pragma unroll
-    for (int k = 1; k < kThreads / 32; ++k) {
-      acc[0] += s_acc[32 * k + lane];
-      l += s_l[k];
+    for (int k = 1; k < kWaves; ++k) next = fmaxf(next, s_ml[k][lane][0]);
+    rescale(next);
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) {
+      const f32x2 o = s_ml[k][lane];
+      const float w = weight(o[0]);
+      acc[0] += s_acc[k][lane] * w;
+      l += o[1] * w;
     }
   }
+  const int row = 16 * row16 + n16;
+  if (row >= p.rows) return;
   const int i = row / p.heads, h = row - i * p.heads;
   const int64_t orow = (int64_t)b * p.q_len + i;
   const float inv = l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
+  T *dst = reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + 4 * g4;
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    const f32x4 x = acc[v] * inv;
-    *reinterpret_cast<i32x2 *>(reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + d0 + 256 * v) =
-        i32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+  for (int d = 0; d < kBlocks; ++d) {
+    const f32x4 y = acc[d] * inv;
+    *reinterpret_cast<i32x2 *>(dst + 16 * (dim0 + d)) = i32x2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
   }
-  if (p.lse && d0 == 0) p.lse[orow * p.l_sr + h * p.l_sh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (p.lse && dim0 == 0 && g4 == 0) p.lse[orow * p.l_sr + h * p.l_sh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 }  // namespace l20la
@@ -766,13 +802,13 @@ template <typename T, int RANK>
 hipError_t launch(const l20la::DecodeParams &p, bool fp8, int blocks, hipStream_t s) {
   const hipError_t e = fp8 ? launch_rows<T, 0, RANK>(p, blocks, s) : launch_rows<T, 1, RANK>(p, blocks, s);
   if (e != hipSuccess || !p.split) return e;
+  const unsigned row16s = (unsigned)((p.rows + 15) / 16);
   if (p.groups > 8 * p.batch)
-    hipLaunchKernelGGL((l20la::latent_merge<T, RANK, true>), dim3((unsigned)p.rows, (unsigned)p.batch, RANK / 128),
+    hipLaunchKernelGGL((l20la::latent_merge<T, RANK, true>), dim3(row16s, (unsigned)p.batch, RANK / 16),
                        dim3(l20la::kThreads), 0, s, p, 16 * blocks);
   else
-    hipLaunchKernelGGL((l20la::latent_merge<T, RANK, false>),
-                       dim3((unsigned)((p.rows + l20la::kWaves - 1) / l20la::kWaves), (unsigned)p.batch),
-                       dim3(l20la::kThreads), 0, s, p, 16 * blocks);
+    hipLaunchKernelGGL((l20la::latent_merge<T, RANK, false>), dim3(row16s, (unsigned)p.batch), dim3(l20la::kThreads), 0, s,
+                       p, 16 * blocks);
   return hipGetLastError();
 }
 
