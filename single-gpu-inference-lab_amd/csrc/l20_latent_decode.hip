@@ -327,6 +327,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
 
   static __device__ __forceinline__ void segment(const DecodeParams &p, Shared &s, Fetch &f, Place &at, int b, int rblk,
                                                  int group, int lo, int hi, int tiles, int tokens, int wave, int lane) {
+    // (what follows from the lane is computed for each sequence: hoisted out of the loop over them it takes 60
+    // registers more than there are)
+    asm volatile("" : "+v"(lane));
     const int n16 = lane & 15, g4 = lane >> 4;
     const int own = wave % RB, tg = wave / RB;  // block of rows, group of tokens of the score product
     const bool scores = kWaves / RB == kGroups || tg < kGroups;
