@@ -106,9 +106,10 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     int rescale[3];
   };
 
-  // Where chunk c (16 bytes) of a row lies: rows are spread so that 16 of them read at one chunk, and the 4 (8)
-  // of a transposing read, meet all LDS banks.
-  static __device__ __forceinline__ int lat_at(int row, int c) { return row * kLatRow + ((c ^ (row & 15)) << 4); }
+  // Where chunk c (16 bytes) of a row lies: rows are spread so that 16 of them read at one chunk, and the 4 rows of
+  // 32 bytes (8 of 16, fp8) of a transposing read, meet all LDS banks.
+  static __device__ __forceinline__ int spread(int row) { return KT == 0 ? row & 15 : spread_row(row); }
+  static __device__ __forceinline__ int lat_at(int row, int c) { return row * kLatRow + ((c ^ spread(row)) << 4); }
   static __device__ __forceinline__ int rope_swizzle(int row) { return KT == 0 ? (row >> 2) & 3 : (row >> 1) & 7; }
   static __device__ __forceinline__ int rope_at(int row, int c) { return row * kRopeRow + ((c ^ rope_swizzle(row)) << 4); }
   static __device__ __forceinline__ int p_at(int row, int c) {
@@ -171,11 +172,11 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       // one scalar base and a lane's offset: the swizzle of load i is an XOR of the lane's chunk
       const uint32_t c_tok = (uint32_t)p.c_tok;
       const int lrow = lane / kChunks;
-      const uint32_t row_off = lrow * c_tok, chunk = ((lane % kChunks) ^ lrow) << 4;
+      const uint32_t row_off = lrow * c_tok, chunk = ((lane % kChunks) ^ spread(lrow)) << 4;
       const uint8_t *src = p.cache + (int64_t)id * p.c_block + (uint32_t)(row0 & 15) * c_tok;
 #pragma unroll
       for (int i = 0; i < kLatLoads; ++i) {
-        const uint32_t swizzle = ((row0 & 15) + i * kLoadRows) << 4;
+        const uint32_t swizzle = spread((row0 & 15) + i * kLoadRows) << 4;
         load_lds(src + i * kLoadRows * c_tok, (chunk ^ swizzle) + row_off, lat + i * 1024);
       }
       const int rrow = (rope0 & 15) + lane / kRopeChunks;
@@ -184,7 +185,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     } else {
 #pragma unroll
       for (int i = 0; i < kLatLoads; ++i) {
-        const int row = row0 + i * kLoadRows + lane / kChunks, c = (lane % kChunks) ^ (row & 15);
+        const int row = row0 + i * kLoadRows + lane / kChunks, c = (lane % kChunks) ^ spread(row);
         const uint8_t *src = p.cache + (int64_t)id * p.c_block + (int64_t)(row & 15) * p.c_tok;
         src = id < 0 || row >= left ? reinterpret_cast<const uint8_t *>(kZeroRow) : src;
         load_lds(src + 16 * c, lat + i * 1024);
@@ -433,9 +434,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         const i32x2 w = read_tr8(lat + ks * 32 * kLatRow + (v_at ^ (d << 4)));
         return i32x4{w[0], w[1], 0, 0};
       } else {
-        // (four rows on, the swizzle differs in chunk bit 2)
+        // (four rows on, the swizzle differs in chunk bit 3)
         const i32x2 lo = read_tr(lat + ks * 32 * kLatRow + (v_at ^ (d << 5)));
-        const i32x2 hi = read_tr(lat + (ks * 32 + 4) * kLatRow + (v_at ^ (d << 5) ^ 64));
+        const i32x2 hi = read_tr(lat + (ks * 32 + 4) * kLatRow + (v_at ^ (d << 5) ^ 128));
         return i32x4{lo[0], lo[1], hi[0], hi[1]};
       }
     };

@@ -50,7 +50,7 @@ constexpr int kWideBytes = kKeys * kWideRow, kNarrowBytes = kKeys * kNarrowRow;
 constexpr int kTileBytes = 2 * kWideBytes + kNarrowBytes;
 
 // Where chunk c (16 bytes) of a tile row lies.
-__device__ __forceinline__ int wide_at(int row, int c) { return row * kWideRow + ((c ^ (row & 15)) << 4); }
+__device__ __forceinline__ int wide_at(int row, int c) { return row * kWideRow + ((c ^ spread_row(row)) << 4); }
 __device__ __forceinline__ int narrow_at(int row, int c) { return row * kNarrowRow + ((c ^ ((row >> 1) & 7)) << 4); }
 
 template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void latent_prompt(PromptParams p) {
@@ -90,7 +90,7 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
     const int last = nk - 1 - j0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 16 * wave + 4 * i + (lane >> 4), c = (lane & 15) ^ (row & 15), r = min(row, last);
+      const int row = 16 * wave + 4 * i + (lane >> 4), c = (lane & 15) ^ spread_row(row), r = min(row, last);
       load_lds(kt, r * k_row + 16 * c, buf + (16 * wave + 4 * i) * kWideRow);
       load_lds(vt, r * v_row + 16 * c, buf + kWideBytes + (16 * wave + 4 * i) * kWideRow);
     }
