@@ -105,6 +105,13 @@ __device__ __forceinline__ float sum_halves(float x) { return sum_swap<32>(x); }
 __device__ __forceinline__ float max_groups(float x) { return max_swap<32>(max_swap<16>(x)); }  // the four groups of 16
 __device__ __forceinline__ float sum_groups(float x) { return sum_swap<32>(sum_swap<16>(x)); }
 
+// The largest of three (fmaxf quiets each operand first, one instruction more a value).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
 // 16 bytes a lane from global memory to LDS (lane l's land at dst + 16 l), asynchronously: they are there once
 // the wave has waited for its loads (landed_and_barrier).  Not the builtin: with a builtin's load in flight the
 // compiler waits for all loads before every transposing read, which ends the prefetch; a load into LDS has no

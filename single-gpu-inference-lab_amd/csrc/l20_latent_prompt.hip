@@ -13,6 +13,7 @@
 #include "l20_latent_attention.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "l20_latent_common.h"
 
@@ -86,17 +87,36 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
     const uint32_t buf = lds + (tile & 1) * kTileBytes;
     const int j0 = tile * kKeys;
     const char *kt = kb + (int64_t)j0 * (2 * p.k_st), *vt = vb + (int64_t)j0 * (2 * p.v_st), *rt = rb + (int64_t)j0 * (2 * p.kr_st);
-    // rows past the last key hold that key again: they are masked, and what they hold is as finite as it is
     const int last = nk - 1 - j0;
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (the offsets are not kept in registers over the tiles)
+    if (last >= kKeys - 1) {
+      // one scalar base and a lane's offset; the swizzle of load i is an XOR of the lane's chunk
+      const uint32_t wide = ((ln & 15) ^ spread_row(ln >> 4)) << 4, wrow = ln >> 4;
+      const char *kt4 = kt + 16 * wave * (2 * p.k_st), *vt4 = vt + 16 * wave * (2 * p.v_st), *rt8 = rt + 16 * wave * (2 * p.kr_st);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t c = wide ^ (spread_row(4 * i) << 4), to = buf + (16 * wave + 4 * i) * kWideRow;
+        load_lds(kt4 + 4 * i * k_row, c + wrow * k_row, to);
+        load_lds(vt4 + 4 * i * v_row, c + wrow * v_row, to + kWideBytes);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t row = ln >> 3, c = ((ln & 7) ^ ((row >> 1) + 4 * i)) << 4;
+        load_lds(rt8 + 8 * i * r_row, c + row * r_row, buf + 2 * kWideBytes + (16 * wave + 8 * i) * kNarrowRow);
+      }
+      return;
+    }
+    // rows past the last key hold that key again: they are masked, and what they hold is as finite as it is
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 16 * wave + 4 * i + (lane >> 4), c = (lane & 15) ^ spread_row(row), r = min(row, last);
+      const int row = 16 * wave + 4 * i + (ln >> 4), c = (ln & 15) ^ spread_row(row), r = min(row, last);
       load_lds(kt, r * k_row + 16 * c, buf + (16 * wave + 4 * i) * kWideRow);
       load_lds(vt, r * v_row + 16 * c, buf + kWideBytes + (16 * wave + 4 * i) * kWideRow);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = 16 * wave + 8 * i + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+      const int row = 16 * wave + 8 * i + (ln >> 3), c = (ln & 7) ^ ((row >> 1) & 7);
       load_lds(rt, min(row, last) * r_row + 16 * c, buf + 2 * kWideBytes + (16 * wave + 8 * i) * kNarrowRow);
     }
   };
@@ -125,24 +145,43 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
     for (int d = 0; d < 4; ++d)
       v_at[u][d] = wide_at(8 * u + 4 * g2 + ((lane & 15) >> 2), 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
 
-  for (int tile = 0; tile < tiles; ++tile) {
+#pragma unroll
+  for (int k = 0; k < kSlices; ++k) asm volatile("" : "+v"(q[k]));  // (here: or its waits are waits for the tiles, each time)
+  // One tile; its buffer is a constant, so that the reads' places are immediates.
+  auto step = [&](int tile, auto which) {
     landed_and_barrier<0>();  // this tile is there, and the one before is consumed
     if (tile + 1 < tiles) stage(tile + 1);
-    const char *buf = smem + (tile & 1) * kTileBytes;
+    const char *buf = smem + decltype(which)::value * kTileBytes;
     const int j0 = tile * kKeys;
-    // ---- S^T = K Q^T, 32 keys at a time ----
+    // ---- S^T = K Q^T, 32 keys a product.  The operands of a step are read three steps ahead (left to itself the
+    // compiler reads each where it is used and waits for it).
+    auto read_key = [&](int n) -> i32x4 {
+      const int kb2 = n & 1, k = n >> 1;
+      const char *at = k < kDim / 16 ? buf + wide_at(32 * kb2 + n32, 2 * k + g2)
+                                     : buf + 2 * kWideBytes + narrow_at(32 * kb2 + n32, 2 * (k - kDim / 16) + g2);
+      return *reinterpret_cast<const i32x4 *>(at);
+    };
+    auto read_value = [&](int n) -> i32x4 {
+      const char *at = buf + kWideBytes + 16 * (n >> 2) * kWideRow;
+      const i32x2 lo = read_tr(at + v_at[0][n & 3]), hi = read_tr(at + v_at[1][n & 3]);
+      return i32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    constexpr int kAhead = 3;
+    i32x4 ring[kAhead + 1];
     f32x16 sc[2];
 #pragma unroll
-    for (int kb2 = 0; kb2 < 2; ++kb2) {
+    for (int e = 0; e < 16; ++e) sc[0][e] = sc[1][e] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[kb2][e] = 0.0f;
+    for (int n = 0; n < kAhead; ++n) ring[n] = read_key(n);
 #pragma unroll
-      for (int k = 0; k < kSlices; ++k) {
-        const char *at = k < kDim / 16 ? buf + wide_at(32 * kb2 + n32, 2 * k + g2)
-                                       : buf + 2 * kWideBytes + narrow_at(32 * kb2 + n32, 2 * (k - kDim / 16) + g2);
-        sc[kb2] = mfma32<T>(*reinterpret_cast<const i32x4 *>(at), q[k], sc[kb2]);
-      }
+    for (int n = 0; n < 2 * kSlices; ++n) {
+      if (n + kAhead < 2 * kSlices) ring[(n + kAhead) & 3] = read_key(n + kAhead);
+      sc[n & 1] = mfma32<T>(ring[n & 3], q[n >> 1], sc[n & 1]);
+      __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) ring[n] = read_value(n);
+    __builtin_amdgcn_sched_barrier(0);
     if (j0 + kKeys - 1 > min(wave_lim, nk - 1)) {
 #pragma unroll
       for (int kb2 = 0; kb2 < 2; ++kb2)
@@ -151,9 +190,9 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
           sc[kb2][e] = j0 + 32 * kb2 + 8 * (e >> 2) + 4 * g2 + (e & 3) <= lim ? sc[kb2][e] : -INFINITY;
     }
     // ---- softmax ----
-    float mx = fmaxf(sc[0][0], sc[1][0]);
+    float mx = -INFINITY;
 #pragma unroll
-    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(sc[0][e], sc[1][e]));
+    for (int e = 0; e < 16; ++e) mx = max3(mx, sc[0][e], sc[1][e]);
     mx = max_halves(mx) * p.c_log2;
     if (__any(mx > m + kRescale)) {
       const float next = fmaxf(m, mx);
@@ -179,13 +218,15 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
     sum += add[0] + add[1];
     // ---- O^T += V^T P^T ----
 #pragma unroll
-    for (int st = 0; st < 4; ++st)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const char *at = buf + kWideBytes + 16 * st * kWideRow;
-        const i32x2 lo = read_tr(at + v_at[0][d]), hi = read_tr(at + v_at[1][d]);
-        acc[d] = mfma32<T>(i32x4{lo[0], lo[1], hi[0], hi[1]}, pb[st], acc[d]);
-      }
+    for (int n = 0; n < 16; ++n) {
+      if (n + kAhead < 16) ring[(n + kAhead) & 3] = read_value(n + kAhead);
+      acc[n & 3] = mfma32<T>(ring[n & 3], pb[n >> 2], acc[n & 3]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  for (int tile = 0; tile < tiles; tile += 2) {
+    step(tile, std::integral_constant<int, 0>{});
+    if (tile + 1 < tiles) step(tile + 1, std::integral_constant<int, 1>{});
   }
 
   const float l = sum_halves(sum);
