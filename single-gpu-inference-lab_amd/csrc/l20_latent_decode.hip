@@ -359,6 +359,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
 #pragma unroll
         for (int k = 0; k < kSlices; ++k)
           q[k] = *reinterpret_cast<const i32x4 *>(src + (KT == 0 ? 64 * (k >> 1) + 16 * g4 + 8 * (k & 1) : 32 * k + 8 * g4));
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) asm volatile("" : "+v"(q[k]));  // (waited for here, not behind the next tile)
       }
     }
 
@@ -546,7 +548,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         }
         mx = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kBlocks; ++u) mx = fmaxf(mx, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
+        for (int u = 0; u < kBlocks; ++u) mx = max3(max3(mx, sc[u][0], sc[u][1]), sc[u][2], sc[u][3]);
         mx = max_groups(mx) * p.c_log2;
         weights(s.p[at.n & 1]);
         if (__any(mx > m_own + kRescale) && lane == 0) s.rescale[at.n % 3] = 1;
@@ -631,7 +633,9 @@ __global__ __launch_bounds__(kThreads) void latent_merge(DecodeParams p, int blo
   auto load = [&](int g) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int gk = min(g + k * kStep, g1);
+      const int gk = g + k * kStep;
+      ml[k] = f32x2{-INFINITY, 0.0f};
+      if (gk > g1) continue;  // (uniform)
       ml[k] = ml_of(gk);
       const f32x4 *src = reinterpret_cast<const f32x4 *>(p.part) + ((part_of(gk) * per + r) * (RANK / 16) + dim0) * 64 + lane;
 #pragma unroll
@@ -655,7 +659,7 @@ __global__ __launch_bounds__(kThreads) void latent_merge(DecodeParams p, int blo
     load(g);
     float next = m;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) next = fmaxf(next, ml[k][0]);  // (past the last run: that one again)
+    for (int k = 0; k < kAhead; ++k) next = fmaxf(next, ml[k][0]);
     rescale(next);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
