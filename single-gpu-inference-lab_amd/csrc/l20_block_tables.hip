@@ -216,16 +216,16 @@ using l20pd_host::set_error;
 
 int32_t check(const l20_pd_block_tables_args *a) {
   if (!a) return set_error(L20_PD_EINVAL, "null argument block");
-  if (a->batch < 1 || a->batch > L20_PD_MAX_REQUESTS)
-    return set_error(L20_PD_EINVAL, "block tables: 1 to 8192 requests");
+  if (a->batch < 0 || a->batch > L20_PD_MAX_REQUESTS)
+    return set_error(L20_PD_EINVAL, "block tables: at most 8192 requests");
   if (a->page_size < 16 || a->page_size % 16 || a->page_size > 4096)
     return set_error(L20_PD_EINVAL, "page size must be a multiple of 16 up to 4096");
-  if (a->table_pages < 1 || a->pool < 1 || a->num_slots < 0)
+  if ((a->batch > 0 && a->table_pages < 1) || a->pool < 1 || a->num_slots < 0)
     return set_error(L20_PD_EINVAL, "block table and page pool must not be empty");
-  if (!a->cached_lens || !a->new_lens || !a->block_table || !a->free_pages || !a->free_count || !a->free_count_out ||
-      !a->cu_lens || !a->seq_lens || (a->num_slots > 0 && (!a->slots || !a->positions)))
+  if ((a->batch > 0 && (!a->cached_lens || !a->new_lens || !a->block_table || !a->seq_lens)) || !a->free_pages ||
+      !a->free_count || !a->free_count_out || !a->cu_lens || (a->num_slots > 0 && (!a->slots || !a->positions)))
     return set_error(L20_PD_EINVAL, "null tensor pointer");
-  if (a->seq_lens == a->cached_lens || a->seq_lens == a->new_lens)
+  if (a->batch > 0 && (a->seq_lens == a->cached_lens || a->seq_lens == a->new_lens))
     return set_error(L20_PD_EINVAL, "seq_lens must not be cached_lens or new_lens");
   return L20_PD_OK;
 }
@@ -271,11 +271,9 @@ int32_t l20_pd_block_tables(const l20_pd_block_tables_args *a, void *stream) {
   p.inline_tokens = a->num_slots <= l20bt::kTokensInline;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t lds = (size_t)(4 * (a->batch + 1)) * sizeof(int);  // at most 128 KB
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&l20bt::bt_requests),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return set_error(L20_PD_ELAUNCH, hipGetErrorString(e));
-  }
+  static l20la::LdsLimit limit;
+  const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20bt::bt_requests), 4 * (L20_PD_MAX_REQUESTS + 1) * (int)sizeof(int));
+  if (e != hipSuccess) return set_error(L20_PD_ELAUNCH, hipGetErrorString(e));
   hipLaunchKernelGGL(l20bt::bt_requests, dim3(1), dim3(l20bt::kThreads), lds, s, p);
   int32_t r = launched();
   if (r != L20_PD_OK || p.inline_tokens) return r;

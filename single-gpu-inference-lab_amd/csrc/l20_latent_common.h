@@ -5,6 +5,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
+
 #include <math.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -105,6 +107,17 @@ __device__ __forceinline__ float sum_halves(float x) { return sum_swap<32>(x); }
 __device__ __forceinline__ float max_groups(float x) { return max_swap<32>(max_swap<16>(x)); }  // the four groups of 16
 __device__ __forceinline__ float sum_groups(float x) { return sum_swap<32>(sum_swap<16>(x)); }
 
+// Lane n's value (n: wave-uniform).
+__device__ __forceinline__ float lane_f(float x, int n) {
+  return word_f((unsigned int)__builtin_amdgcn_readlane(__builtin_bit_cast(int, x), n));
+}
+// Two products of the pairs of Ts in two words, added to x one after the other.
+template <typename T> __device__ __forceinline__ float dot2(int a, int b, float x) {
+  typedef T pair __attribute__((ext_vector_type(2)));
+  const pair u = __builtin_bit_cast(pair, a), v = __builtin_bit_cast(pair, b);
+  return __builtin_fmaf((float)u[1], (float)v[1], __builtin_fmaf((float)u[0], (float)v[0], x));
+}
+
 // The largest of three (fmaxf quiets each operand first, one instruction more a value).
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -135,6 +148,21 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // The running maximum of a softmax row moves only when a tile's exceeds it by more than this (log2 units): P is
 // then at most 2^8 where it would be 1, which costs neither type precision (fp16 ends at 2^16).
 constexpr float kRescale = 8.0f;
+
+// A kernel's limit of dynamic LDS, raised once a device (each raise costs a launch a good part of a microsecond).
+struct LdsLimit {
+  std::atomic<uint64_t> devices{0};
+  hipError_t raise(const void *kernel, int bytes) {
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
+    if (devices.load(std::memory_order_acquire) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) devices.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 
 // 16 bytes of zeros a lane: what rows that take no part are read from (a masked row's values still
 // enter the product with a weight of 0, and 0 x NaN is NaN).

@@ -133,7 +133,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     uint32_t bad;     // bits 4 n .. of buffer n: blocks of its tile without a page
   };
   static __device__ __forceinline__ int blocks_of_window(const DecodeParams &p, int b, int first_block) {
-    const int blk = first_block + (int)(threadIdx.x & 63);
+    return block_of(p, b, first_block + (int)(threadIdx.x & 63));
+  }
+  static __device__ __forceinline__ int block_of(const DecodeParams &p, int b, int blk) {
     if (blk >= p.table_blocks) return -1;
     const int col = p.per_page == 1 ? blk : (int)((uint64_t)blk * p.page_magic >> 38);
     const int page = p.table[b * p.t_sr + col];
@@ -319,6 +321,44 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     }
     const int n = wave % kRopeQ, row = 8 * n + lane / 8;
     load_lds(row_of(row) + RANK + 8 * ((lane & 7) ^ ((row >> 1) & 7)), rope + n * 1024);
+  }
+
+  // The wave's dims (one a lane) of row (i, h)'s sum of weighted values over tokens first .. last, given its maximum
+  // (log2 units): 64 tokens at a time, scores by a lane each.
+  static __device__ float exact_row(const DecodeParams &p, int b, int i, int h, int first, int last, int wave, float m) {
+    const int lane = threadIdx.x & 63;
+    const T *q = reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + h * p.q_sh;
+    const float use = m == -INFINITY ? 0.0f : m;
+    const int dim = wave * (16 * kDimBlocks) + lane % (16 * kDimBlocks);
+    float out = 0.0f;
+    for (int t0 = first; t0 <= last; t0 += 64) {
+      const int t = min(t0 + lane, last), id = block_of(p, b, t >> 4);
+      const uint8_t *key = p.cache + (int64_t)max(id, 0) * p.c_block + (int64_t)(t & 15) * p.c_tok;
+      float s = 0.0f;
+      for (int c = 0; c < RANK + kRope; c += 8) {
+        const i32x4 qw = *reinterpret_cast<const i32x4 *>(q + c);
+        i32x4 kw;
+        if constexpr (KT == 0) {
+          const i32x2 w = *reinterpret_cast<const i32x2 *>(key + c), lo = fp8x4<T>(w[0]), hi = fp8x4<T>(w[1]);
+          kw = i32x4{lo[0], lo[1], hi[0], hi[1]};
+        } else {
+          kw = *reinterpret_cast<const i32x4 *>(key + 2 * c);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = dot2<T>(kw[e], qw[e], s);
+      }
+      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c_log2, -use));
+      for (int n = 0; n < min(64, last + 1 - t0); ++n) {
+        const int block = __builtin_amdgcn_readlane(id, n);
+        if (block < 0) continue;
+        const uint8_t *src = p.cache + (int64_t)block * p.c_block + (int64_t)((t0 + n) & 15) * p.c_tok + dim * kBytes;
+        float v;
+        if constexpr (KT == 0) v = __builtin_amdgcn_cvt_f32_fp8(*src, 0);
+        else v = (float)*reinterpret_cast<const T *>(src);
+        out += lane_f(w, n) * v;
+      }
+    }
+    return out;
   }
 
   // A tile of the run (its number) and its LDS buffers.
@@ -515,7 +555,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         for (int u = 0; u < kBlocks; ++u) part[u][0] = part[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
         constexpr int kKeySteps = kSlices / 2, kSteps = PV && kParts > kKeySteps ? kParts : kKeySteps;
         Keys key;
-        i32x4 val;
+        i32x4 val{};
         read_k(lat, rope, 0, key);
         if constexpr (PV) {
           read_p(oldp, 0);
@@ -570,6 +610,34 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     sum = sum_groups(sum);
     if (scores && g4 == 0) s.sum[16 * own + n16][tg] = sum;
     lds_barrier();
+    // A token that a draft row does not see enters its value product with a weight of 0, and 0 x NaN is NaN: rows
+    // that are not finite though their sum is are computed again, from the run's tokens that they see alone.
+    if (p.q_len > 1 && hi * kTokens > len - p.q_len + 1) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        float l = 0.0f, odd = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) l += s.sum[16 * r + n16][k];
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd = __builtin_fmaf(acc[r][d][e], 0.0f, odd);
+        uint64_t again = __ballot(odd != odd && l == l);
+        again |= again >> 32;
+        for (uint32_t left = (uint32_t)(again | again >> 16) & 0xffff; left; left &= left - 1) {
+          const int n = __builtin_ctz(left), row = min(rblk * kRows + 16 * r + n, p.rows - 1), i = row / p.heads;
+          const float x = exact_row(p, b, i, row - i * p.heads, lo * kTokens, min(min(hi * kTokens, tokens) - 1, len - p.q_len + i),
+                                    wave, lane_f(m_all[r], n));
+#pragma unroll
+          for (int d = 0; d < kDimBlocks; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = __shfl(x, 16 * d + 4 * g4 + e);
+              acc[r][d][e] = n16 == n ? y : acc[r][d][e];
+            }
+        }
+      }
+    }
     const bool all = lo == 0 && hi == tiles;
     const int64_t part = (int64_t)(lo > 0 ? 2 * group : 2 * group + 1) * p.row_blocks + rblk;
 #pragma unroll
@@ -710,10 +778,12 @@ namespace {
 using l20pd_host::set_error;
 
 int device_cus() {
+  static std::atomic<int> known[64];  // by device
   int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
-    cus = 256;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  if (dev < 64 && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+  if (dev < 64) known[dev].store(cus, std::memory_order_relaxed);
   return cus;
 }
 
@@ -769,8 +839,9 @@ int32_t check(const l20_pd_latent_args *a) {
     return set_error(L20_PD_EINVAL, "cache scale must be positive and finite");
   if (a->batch == 0) return L20_PD_OK;
   if (a->num_pages <= 0 || a->table_pages <= 0) return set_error(L20_PD_EINVAL, "latent cache and block table must have pages");
+  // (the costs of all sequences, at most tokens / 32 + 1 tiles and a switch each, are added up in 31 bits)
   if ((int64_t)a->table_pages * a->page_size > INT32_MAX / 2 ||
-      (int64_t)a->batch * ((int64_t)a->table_pages * a->page_size / 64 + 1) >= ((int64_t)1 << 30))
+      (int64_t)a->batch * ((int64_t)a->table_pages * a->page_size / 32 + 8) > INT32_MAX)
     return set_error(L20_PD_EINVAL, "block table names too many tokens");
   if (a->num_pages * (a->page_size / 16) > INT32_MAX) return set_error(L20_PD_EINVAL, "latent cache has too many pages");
   if (a->page_size > 16 && a->c_stride_page != a->page_size * a->c_stride_token)
@@ -792,8 +863,8 @@ int32_t check(const l20_pd_latent_args *a) {
 template <typename T, int KT, int RANK, int RB> hipError_t launch_partial(const l20la::DecodeParams &p, hipStream_t s) {
   const size_t lds = sizeof(typename l20la::Partial<T, KT, RANK, RB>::Shared);
   static_assert(sizeof(typename l20la::Partial<T, KT, RANK, RB>::Shared) <= 160 * 1024, "more than the LDS of a CU");
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&l20la::latent_partial<T, KT, RANK, RB>),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  static l20la::LdsLimit limit;
+  const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20la::latent_partial<T, KT, RANK, RB>), (int)lds);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((l20la::latent_partial<T, KT, RANK, RB>), dim3((unsigned)(p.groups * p.row_blocks)),
                      dim3(l20la::kThreads), lds, s, p);

@@ -60,7 +60,7 @@ void latent_rope_and_cache(const std::optional<at::Tensor> &query, const at::Ten
   TORCH_CHECK(key_rope.dim() == 2 && key_rope.size(0) == tokens && key_rope_out.sizes() == key_rope.sizes(),
               "expected key_rope and key_rope_out [tokens, rope]");
   TORCH_CHECK(latent_cache.dim() == 3 && latent_cache.size(2) == rank + key_rope.size(1),
-              "latent cache must be [pages, page, rank + rope]");
+              "latent cache must be [pages, page, rank + 64] with rank 256 or 512");
   TORCH_CHECK(positions.scalar_type() == at::kLong && positions.dim() == 1 && positions.is_contiguous() &&
                   positions.size(0) == tokens && slot_mapping.scalar_type() == at::kLong && slot_mapping.dim() == 1 &&
                   slot_mapping.is_contiguous() && slot_mapping.size(0) == tokens,
@@ -284,7 +284,6 @@ void build_block_tables(const at::Tensor &cached_lens, const at::Tensor &new_len
   for (const at::Tensor *t : {&cached_lens, &new_lens, &free_pages, &free_count, &free_count_out, &slot_mapping, &positions,
                               &cu_lens, &seq_lens})
     check_device(*t, block_table);
-  if (batch == 0 && slot_mapping.size(0) == 0) return;
   l20_pd_block_tables_args a{};
   a.cached_lens = cached_lens.data_ptr<int32_t>();
   a.new_lens = new_lens.data_ptr<int32_t>();

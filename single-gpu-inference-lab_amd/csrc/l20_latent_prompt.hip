@@ -54,6 +54,34 @@ constexpr int kTileBytes = 2 * kWideBytes + kNarrowBytes;
 __device__ __forceinline__ int wide_at(int row, int c) { return row * kWideRow + ((c ^ spread_row(row)) << 4); }
 __device__ __forceinline__ int narrow_at(int row, int c) { return row * kNarrowRow + ((c ^ ((row >> 1) & 7)) << 4); }
 
+// The output of one row by a wave, from keys 0 .. lim of its sequence, given its maximum (log2 units) and 1 / sum:
+// 64 keys at a time, scores by a lane each, then two dims a lane.
+template <typename T>
+__device__ void exact_row(const PromptParams &p, int h, int64_t row, int64_t ks, int lim, float m, float inv) {
+  const int lane = threadIdx.x & 63;
+  const T *q = reinterpret_cast<const T *>(p.q) + row * p.q_st + h * p.q_sh;
+  const float use = m == -INFINITY ? 0.0f : m;
+  float out[2] = {0.0f, 0.0f};
+  for (int j0 = 0; j0 <= lim; j0 += 64) {
+    const int64_t j = ks + min(j0 + lane, lim);
+    const T *k = reinterpret_cast<const T *>(p.k) + j * p.k_st + h * p.k_sh, *kr = reinterpret_cast<const T *>(p.kr) + j * p.kr_st;
+    float s = 0.0f;
+    for (int c = 0; c < kDim + kRope; c += 8) {
+      const i32x4 kw = *reinterpret_cast<const i32x4 *>(c < kDim ? k + c : kr + (c - kDim)), qw = *reinterpret_cast<const i32x4 *>(q + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = dot2<T>(kw[e], qw[e], s);
+    }
+    const float w = j0 + lane <= lim ? __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c_log2, -use)) : 0.0f;
+    for (int n = 0; n < min(64, lim + 1 - j0); ++n) {
+      const float wn = lane_f(w, n);
+      const T *v = reinterpret_cast<const T *>(p.v) + (ks + j0 + n) * p.v_st + h * p.v_sh + 2 * lane;
+      out[0] += wn * (float)v[0];
+      out[1] += wn * (float)v[1];
+    }
+  }
+  *reinterpret_cast<int *>(reinterpret_cast<T *>(p.out) + row * p.o_st + h * p.o_sh + 2 * lane) = pack2<T>(out[0] * inv, out[1] * inv);
+}
+
 template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void latent_prompt(PromptParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];  // two tiles: keys, values, rotary parts
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -230,9 +258,23 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
   }
 
   const float l = sum_halves(sum);
-  if (i >= rows) return;
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
+  // A key that a row does not see enters its value product with a weight of 0, and 0 x NaN is NaN: rows that are
+  // not finite though their sum is are computed again, from the keys they see alone.
+  float odd = 0.0f;
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) odd = __builtin_fmaf(acc[d][e], 0.0f, odd);
+  const uint64_t odd_lanes = __ballot(p.causal && i < rows && odd != odd && l == l);
+  const uint32_t again = (uint32_t)(odd_lanes | odd_lanes >> 32);
+  for (uint32_t left = again; left; left &= left - 1) {
+    const int r = __builtin_ctz(left), row = q0 + wave * kWaveRows + r;
+    exact_row<T>(p, h, qs + row, ks, __builtin_amdgcn_readlane(lim, r), lane_f(m, r), lane_f(inv, r));
+  }
+  if (i >= rows) return;
   T *dst = reinterpret_cast<T *>(p.out) + (qs + i) * p.o_st + h * p.o_sh + 4 * g2;
+  if (!(again >> n32 & 1))
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -259,7 +301,7 @@ int32_t check(const l20_pd_latent_prompt_args *a) {
   if (a->total_q > INT32_MAX - 4096 || a->total_k > INT32_MAX - 4096 || a->max_q_len > INT32_MAX - 4096)
     return set_error(L20_PD_EINVAL, "too many tokens");
   const int64_t blocks = ((int64_t)a->max_q_len + l20la::kPromptRows - 1) / l20la::kPromptRows;
-  if ((int64_t)a->batch * a->num_heads > INT32_MAX / std::max<int64_t>(1, blocks))
+  if ((int64_t)a->batch * a->num_heads * 256 > (int64_t)UINT32_MAX / std::max<int64_t>(1, blocks))  // (the threads of a grid)
     return set_error(L20_PD_EINVAL, "too many (sequence, head, row block) units");
   if (!(a->softmax_scale > 0.0f && isfinite(a->softmax_scale)))
     return set_error(L20_PD_EINVAL, "softmax_scale must be positive and finite");
@@ -324,9 +366,9 @@ int32_t l20_pd_latent_prompt(const l20_pd_latent_prompt_args *a, void *stream) {
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int lds = 2 * l20la::kTileBytes;  // 80 KB: two workgroups a CU
   const bool bf = a->dtype == L20_PD_BF16;
-  hipError_t e = hipFuncSetAttribute(bf ? reinterpret_cast<const void *>(&l20la::latent_prompt<__bf16>)
-                                        : reinterpret_cast<const void *>(&l20la::latent_prompt<_Float16>),
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  static l20la::LdsLimit limit[2];
+  hipError_t e = limit[bf].raise(bf ? reinterpret_cast<const void *>(&l20la::latent_prompt<__bf16>)
+                                    : reinterpret_cast<const void *>(&l20la::latent_prompt<_Float16>), lds);
   if (e == hipSuccess) {
     if (bf) hipLaunchKernelGGL((l20la::latent_prompt<__bf16>), grid, block, lds, s, p);
     else hipLaunchKernelGGL((l20la::latent_prompt<_Float16>), grid, block, lds, s, p);

@@ -166,6 +166,16 @@ __device__ __forceinline__ void rope_rows(const WriteParams &p) {
   if (is_key) store_cache<T, CT>(p, slot, RANK + e0, out);
 }
 
+// x^-1/2 to within a rounding: one Newton step on the instruction's result r, r + r (1 - x r r) / 2, with the
+// residual exact enough (x r in two parts).
+__device__ __forceinline__ float inverse_root(float x) {
+  if (!(x > 0x1p-100f && x < INFINITY)) return 1.0f / sqrtf(x);
+  const float r = __builtin_amdgcn_rsqf(x);
+  const float h = x * r, low = __builtin_fmaf(x, r, -h);
+  const float residual = __builtin_fmaf(-low, r, __builtin_fmaf(-h, r, 1.0f));
+  return __builtin_fmaf(0.5f * r, residual, r);
+}
+
 template <typename T, int CT, int RANK> __device__ __forceinline__ void latent_rows(const WriteParams &p) {
 #pragma clang fp contract(off)
   constexpr int kLanes = RANK / 8;  // a token
@@ -184,9 +194,9 @@ template <typename T, int CT, int RANK> __device__ __forceinline__ void latent_r
     for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
 #pragma unroll
     for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-    const float inv = 1.0f / sqrtf(sum * (1.0f / RANK) + p.eps);
+    const float inv = inverse_root(sum * (1.0f / RANK) + p.eps);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
+    for (int i = 0; i < 8; ++i) x[i] = (x[i] * g[i]) * inv;  // (the product of two Ts is exact in fp32)
     out = pack8<T>(x);
   }
   if (p.weight || p.lo != p.l)  // (in place and without a norm nothing changes)
@@ -232,6 +242,9 @@ int32_t check(const l20_pd_latent_write_args *a) {
       !a->cos_sin_cache || !a->slot_mapping || !a->cache)
     return set_error(L20_PD_EINVAL, "null tensor pointer");
   if ((int64_t)a->num_tokens * ((int64_t)(a->query ? a->num_heads : 0) + 1) >= ((int64_t)1 << 31))
+    return set_error(L20_PD_EINVAL, "too many query rows");
+  // (a grid holds fewer than 2^32 threads: eight lanes a rotary row, rank / 8 a latent)
+  if (8 * (uint64_t)a->num_tokens * ((a->query ? a->num_heads : 0) + 1 + 8) >= ((uint64_t)1 << 32) - 1024)
     return set_error(L20_PD_EINVAL, "too many query rows");
   auto u = [](const void *x) { return (uint64_t)(uintptr_t)x; };
   uint64_t rows = u(a->latent) | u(a->latent_out) | u(a->key) | u(a->key_out) | u(a->norm_weight) |

@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 import l20_paged_decode  # noqa: F401  (loads the ops library)
-from l20_paged_split_kv import is_mi355x
+from l20_paged_split_kv import _gpu_facts
 
 MAX_REQUESTS = 8192
 
@@ -44,7 +44,7 @@ def l20_build_block_tables(
     Outputs: ``slot_mapping`` and ``positions`` int64 [tokens] in packed order (rows past the last token: slot -1,
     position 0), ``cu_seqlens`` int32 [requests + 1], ``seq_lens`` int32 [requests] (0 where finished; not the same
     tensor as ``cached_lens``)."""
-    if not is_mi355x(block_table.device):
+    if not (block_table.is_cuda and _gpu_facts(block_table.device)[0]):
         raise RuntimeError("l20_build_block_tables requires an MI355X (gfx950) GPU")
     if cached_lens.ndim != 1 or not 0 <= cached_lens.shape[0] <= MAX_REQUESTS:
         raise RuntimeError(f"cached_lens must be [requests] with at most {MAX_REQUESTS} requests")

@@ -22,15 +22,15 @@ from typing import Optional
 import torch
 
 import l20_paged_decode  # noqa: F401  (loads the ops library)
-from l20_paged_split_kv import gpu_cus, is_mi355x
+from l20_paged_split_kv import _gpu_facts, gpu_cus
 
 ROPE_DIM = 64
 RANKS = (256, 512)
 HEAD_DIM = 128  # key and value dims of a head in the expanded form
 
 
-def _need_gpu(name: str, device: torch.device) -> None:
-    if not is_mi355x(device):
+def _need_gpu(name: str, tensor: torch.Tensor) -> None:
+    if not (tensor.is_cuda and _gpu_facts(tensor.device)[0]):
         raise RuntimeError(f"{name} requires an MI355X (gfx950) GPU")
 
 
@@ -65,18 +65,10 @@ def l20_latent_rope_and_cache(
     ``query_out`` that is the last 64 dims of the absorbed query saves the copy there.  ``slot_mapping`` below 0
     or beyond the cache: the token is not stored.  An fp8 cache stores ``clamp(x / cache_scale)`` of the rounded
     results."""
-    _need_gpu("l20_latent_rope_and_cache", latent.device)
-    dtype = latent.dtype
-    if dtype not in (torch.float16, torch.bfloat16):
+    _need_gpu("l20_latent_rope_and_cache", latent)
+    # (shapes and strides are checked by the op: a second time here they would take as long as the kernel)
+    if latent.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("l20_latent_rope_and_cache supports FP16 and BF16")
-    if latent.ndim != 2 or key_rope.ndim != 2 or key_rope.shape != (latent.shape[0], ROPE_DIM):
-        raise RuntimeError("expected latent [tokens, rank] and key_rope [tokens, 64]")
-    if query_rope is not None and (query_rope.ndim != 3 or query_rope.shape[0] != latent.shape[0]
-                                   or query_rope.shape[2] != ROPE_DIM):
-        raise RuntimeError("expected query_rope [tokens, heads, 64]")
-    _cache_ok(latent_cache, dtype, latent.shape[1])
-    if positions.numel() != latent.shape[0] or slot_mapping.numel() != latent.shape[0]:
-        raise RuntimeError("positions and slot_mapping must match token count")
     if query_rope is None and query_out is not None:
         raise RuntimeError("query_out needs query_rope")
     torch.ops.l20_stack.latent_rope_and_cache(
@@ -127,7 +119,7 @@ def l20_paged_latent_attention(
     ``kv_rank``, set it).  ``max_seq_len`` bounds the lengths (default: what the block table can name) and sizes
     grid and workspace; tokens beyond it, the table, or on a page outside the cache are masked.  With ``output``
     and ``workspace`` given nothing is allocated and the call can be captured in a graph."""
-    _need_gpu("l20_paged_latent_attention", query.device)
+    _need_gpu("l20_paged_latent_attention", query)
     if query.ndim != 3 or query.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("expected an FP16 or BF16 query [batch * q_len, heads, kv_rank + 64]")
     _cache_ok(latent_cache, query.dtype, kv_rank)
@@ -170,7 +162,7 @@ def l20_latent_prompt_attention(
     keys up to i + (keys - n), so that a chunk whose first tokens are cached already passes all keys.  A row that
     sees none gives zeros (``lse``: -inf); rows outside the ranges, or beyond ``max_seqlen_q``, keep what they
     held.  ``softmax_scale`` defaults to 192^-0.5."""
-    _need_gpu("l20_latent_prompt_attention", query.device)
+    _need_gpu("l20_latent_prompt_attention", query)
     if query.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("l20_latent_prompt_attention supports FP16 and BF16")
     if query.ndim != 3 or query.shape[2] != HEAD_DIM + ROPE_DIM:

@@ -149,6 +149,17 @@ def test_replayed_step_by_step():
         cached, table, free, left = want["seq_lens"], want["table"], want["free"], want["left"]
 
 
+def test_no_requests():
+    import l20_block_tables as bt
+
+    none, left, cu = t32([]), t32([0]), t32([9])
+    slots, positions = torch.full((5,), 7, device="cuda"), torch.full((5,), 7, device="cuda")
+    bt.l20_build_block_tables(none, none, t32([]).reshape(0, 4), t32([3, 1, 2]), t32([2]), slots, positions, cu, none, 16,
+                              free_count_out=left)
+    torch.cuda.synchronize()
+    assert int(left) == 2 and cu.tolist() == [0] and slots.tolist() == [-1] * 5 and positions.tolist() == [0] * 5
+
+
 def test_refusals():
     import l20_block_tables as bt
 

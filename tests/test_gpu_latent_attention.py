@@ -144,6 +144,27 @@ def test_decode_nan_in_one_sequence_stays_there():
     assert torch.equal(out[0], clean[0]) and torch.equal(out[2], clean[2])
 
 
+@pytest.mark.parametrize("fp8", [True, False], ids=["e4m3", "model"])
+@pytest.mark.parametrize("heads", [5, 16, 40])
+@pytest.mark.parametrize("rank", [512, 256])
+def test_decode_nan_of_a_draft_reaches_only_the_rows_that_see_it(fp8, heads, rank):
+    """The last, and the second last, token of two sequences hold NaN; the rows before them are as without."""
+    q_len = 3
+    c = make_decode([70, 2, 129, 900, 64], heads, q_len=q_len, rank=rank, fp8=fp8, seed=31, poison=False)
+    clean, clean_lse = run_decode(c)
+    kept = c["cache"].clone()
+    for b, t in ((0, 69), (2, 127), (3, 899), (4, 63)):
+        c["cache"][c["table"][b, t // 16].long(), t % 16] = float("nan")
+    out, lse = run_decode(c)
+    c["cache"] = kept
+    seen = torch.zeros(5, q_len, dtype=torch.bool, device="cuda")
+    seen[[0, 2, 2, 3, 4], [2, 1, 2, 2, 2]] = True
+    seen = seen.flatten()
+    assert bool(torch.isnan(out[seen]).all()) and bool(torch.isnan(lse[seen]).all())
+    out[seen], lse[seen] = clean[seen], clean_lse[seen]
+    check_decode(c, out, lse)
+
+
 def test_decode_workspace_is_reused_and_calls_repeat_bitwise():
     import l20_latent_attention as la
 
@@ -250,6 +271,21 @@ def test_prompt_against_float64(spec, dtype, causal):
     c = make_prompt(lens, keys, heads, dtype, seed=sum(lens) + heads)
     out, lse = run_prompt(c, causal)
     R.check_prompt(out, lse, c["query"], c["key"], c["key_rope"], c["value"], c["cu_q"], c["cu_k"], SCALE, causal)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_prompt_nan_of_a_later_key_reaches_only_the_rows_that_see_it(dtype):
+    c = make_prompt([200, 90], [200, 210], 3, dtype, seed=25)
+    clean, clean_lse = run_prompt(c)
+    value, key = c["value"].clone(), c["key"].clone()
+    c["value"][137, 1, 9] = float("inf")   # seen by rows 137 .. 199 of the first sequence
+    c["key"][200 + 150, 2] = float("nan")  # by rows 30 .. 89 of the second
+    c["value"][200 + 150, 2] = float("nan")
+    out, lse = run_prompt(c)
+    assert bool(torch.isinf(out[137:200, 1, 9]).all()) and bool(torch.isnan(out[230:, 2]).all())
+    out[137:200, 1, 9] = clean[137:200, 1, 9]
+    out[230:, 2], lse[230:, 2] = clean[230:, 2], clean_lse[230:, 2]
+    R.check_prompt(out, lse, c["query"], key, c["key_rope"], value, c["cu_q"], c["cu_k"], SCALE)
 
 
 def test_prompt_leaves_other_rows_alone():
