@@ -95,8 +95,8 @@ int32_t l20_pd_latent_rope_and_cache(const l20_pd_latent_write_args *args, void 
  * Row b*q_len+i sees tokens 0 .. seq_lens[b]-q_len+i:
  *   s_t = softmax_scale q . row_t,  out = sum_t softmax(s)_t row_t[0 .. rank)
  * A row that sees nothing gives zeros and an LSE of -inf.  Tokens beyond the table's width, or on a
- * page outside [0, num_pages), or beyond max_seq_len, are masked for every row.  The tokens of one sequence are read in tiles:
- * a value that is not finite in a token some rows of the sequence see may reach its other rows.
+ * page outside [0, num_pages), or beyond max_seq_len, are masked for every row.  A value that is not finite
+ * reaches only the rows that see its token.
  *
  * The work (tiles of tokens of all sequences) is split evenly over the CUs; what a workgroup has of a
  * sequence that others share goes to `workspace` (l20_pd_paged_latent_workspace bytes, 16-byte aligned)
@@ -145,6 +145,10 @@ int32_t l20_pd_paged_latent(const l20_pd_latent_args *args, void *stream);
  * s_ij = softmax_scale (q_i[0..128) . key_j + q_i[128..192) . key_rope_j); with causal != 0 query i of
  * n sees keys j <= i + (keys - n).  A row that sees nothing gives zeros and an LSE of -inf.  Query rows
  * outside cu_q's ranges, or beyond max_q_len of their sequence, keep what they held.
+ *
+ * Calls of few (row block, head) units and many keys split the keys over the CUs as l20_pd_paged_latent
+ * does, with `workspace` (l20_pd_latent_prompt_workspace bytes, 16-byte aligned, one for each of the calls
+ * that may overlap); with workspace = NULL they do not.
  */
 typedef struct l20_pd_latent_prompt_args {
   const void *query;
@@ -165,9 +169,14 @@ typedef struct l20_pd_latent_prompt_args {
   int32_t causal;
   int64_t total_q, total_k;
   int32_t batch, num_heads, max_q_len, head_dim, rope_dim, value_dim;
+  void *workspace;
+  int64_t workspace_bytes;
 } l20_pd_latent_prompt_args;
 
 int32_t l20_pd_latent_prompt_check(const l20_pd_latent_prompt_args *args);
+/* Workspace bytes of a call on a device of cu_count compute units (0: the current device's); reads only
+ * total_q, total_k, batch, num_heads and max_q_len.  0 where the keys are not split. */
+int64_t l20_pd_latent_prompt_workspace(const l20_pd_latent_prompt_args *args, int32_t cu_count);
 int32_t l20_pd_latent_prompt(const l20_pd_latent_prompt_args *args, void *stream);
 
 #ifdef __cplusplus

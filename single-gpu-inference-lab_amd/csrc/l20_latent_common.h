@@ -164,6 +164,17 @@ struct LdsLimit {
   }
 };
 
+// The compute units of the current device.
+inline int device_cus() {
+  static std::atomic<int> known[64];  // by device
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  if (dev < 64 && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+  if (dev < 64) known[dev].store(cus, std::memory_order_relaxed);
+  return cus;
+}
+
 // 16 bytes of zeros a lane: what rows that take no part are read from (a masked row's values still
 // enter the product with a weight of 0, and 0 x NaN is NaN).
 __device__ const i32x4 kZeroRow[128] = {};

@@ -777,16 +777,6 @@ namespace {
 
 using l20pd_host::set_error;
 
-int device_cus() {
-  static std::atomic<int> known[64];  // by device
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return 256;
-  if (dev < 64 && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
-  if (dev < 64) known[dev].store(cus, std::memory_order_relaxed);
-  return cus;
-}
-
 int64_t rows_of(const l20_pd_latent_args &a) { return (int64_t)a.q_len * a.num_heads; }
 
 // How a call is cut: blocks of 16 rows a workgroup takes (as many as the sequence has, up to four), tokens of a
@@ -903,14 +893,14 @@ int32_t l20_pd_paged_latent_check(const l20_pd_latent_args *a) {
 int64_t l20_pd_paged_latent_workspace(const l20_pd_latent_args *a, int32_t cu_count) {
   l20pd_host::clear_error();
   if (!a || a->batch < 0 || a->q_len < 1 || a->num_heads < 1 || a->max_seq_len < 0 || rows_of(*a) > 65535) return 0;
-  return plan_of(*a, cu_count > 0 ? cu_count : device_cus()).workspace;
+  return plan_of(*a, cu_count > 0 ? cu_count : l20la::device_cus()).workspace;
 }
 
 int32_t l20_pd_paged_latent(const l20_pd_latent_args *a, void *stream) {
   l20pd_host::clear_error();
   const int32_t rc = check(a);
   if (rc != L20_PD_OK || a->batch == 0) return rc;
-  const int cus = device_cus();
+  const int cus = l20la::device_cus();
   const Plan plan = plan_of(*a, cus);
   if (plan.workspace > 0 && (!a->workspace || a->workspace_bytes < plan.workspace || (uintptr_t)a->workspace % 16))
     return set_error(L20_PD_EINVAL, "workspace is too small for the request (l20_pd_paged_latent_workspace)");

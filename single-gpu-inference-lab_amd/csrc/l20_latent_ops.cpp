@@ -198,7 +198,8 @@ at::Tensor paged_latent(const at::Tensor &query, const at::Tensor &latent_cache,
 
 at::Tensor latent_prompt(const at::Tensor &query, const at::Tensor &key, const at::Tensor &key_rope, const at::Tensor &value,
                          const at::Tensor &cu_seqlens_q, const at::Tensor &cu_seqlens_k, int64_t max_seqlen_q,
-                         const at::Tensor &output, double softmax_scale, bool causal, const std::optional<at::Tensor> &lse) {
+                         const at::Tensor &output, double softmax_scale, bool causal, const std::optional<at::Tensor> &lse,
+                         const std::optional<at::Tensor> &workspace) {
   TORCH_CHECK(query.is_cuda(), "query must be CUDA");
   TORCH_CHECK(query.dim() == 3 && key.dim() == 3 && value.dim() == 3 && key_rope.dim() == 2 && output.dim() == 3,
               "expected query, key, value and output [tokens, heads, dims] and key_rope [tokens, rope]");
@@ -226,6 +227,12 @@ at::Tensor latent_prompt(const at::Tensor &query, const at::Tensor &key, const a
     a.lse = lse->data_ptr<float>();
     a.lse_stride_token = lse->stride(0);
     a.lse_stride_head = lse->stride(1);
+  }
+  if (workspace.has_value() && workspace->defined() && workspace->nbytes() > 0) {
+    TORCH_CHECK(workspace->is_contiguous(), "workspace must be contiguous");
+    check_device(*workspace, query);
+    a.workspace = workspace->data_ptr();
+    a.workspace_bytes = (int64_t)workspace->nbytes();
   }
   a.query = query.data_ptr();
   a.q_stride_token = query.stride(0);
@@ -320,7 +327,7 @@ TORCH_LIBRARY_FRAGMENT(l20_stack, m) {
   m.def(
       "latent_prompt_attention_out(Tensor query, Tensor key, Tensor key_rope, Tensor value, "
       "Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, Tensor(a!) output, float softmax_scale, "
-      "bool causal=True, Tensor(b!)? lse=None) -> Tensor(a!)");
+      "bool causal=True, Tensor(b!)? lse=None, Tensor(c!)? workspace=None) -> Tensor(a!)");
   m.def(
       "build_block_tables(Tensor cached_lens, Tensor new_lens, Tensor(a!) block_table, Tensor(b!) free_pages, "
       "Tensor free_count, Tensor(c!) slot_mapping, Tensor(d!) positions, Tensor(e!) cu_seqlens, "

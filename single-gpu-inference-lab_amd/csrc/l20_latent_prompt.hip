@@ -37,6 +37,11 @@ struct PromptParams {
   int causal;
   int64_t total_q, total_k;
   int batch, heads, max_q;
+  // what follows is for calls whose keys are split
+  float *part;     // [slot][wave][dims / 8][lane][4], as the accumulators lie
+  float *part_ml;  // [slot][row][2]: maximum (log2 units), sum
+  i32x2 *runs;     // [batch][head][row block]: the first and the last run that hold a part of it
+  int groups;
 };
 
 constexpr int kDim = 128;  // key dims a head, value dims
@@ -54,16 +59,48 @@ constexpr int kTileBytes = 2 * kWideBytes + kNarrowBytes;
 __device__ __forceinline__ int wide_at(int row, int c) { return row * kWideRow + ((c ^ spread_row(row)) << 4); }
 __device__ __forceinline__ int narrow_at(int row, int c) { return row * kNarrowRow + ((c ^ ((row >> 1) & 7)) << 4); }
 
-// The output of one row by a wave, from keys 0 .. lim of its sequence, given its maximum (log2 units) and 1 / sum:
-// 64 keys at a time, scores by a lane each, then two dims a lane.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
+// A sequence of the batch: its rows and keys, clipped to the tensors, and what a row sees.
+struct Seq {
+  int64_t qs, ks;
+  int rows, nk, shift;  // row i sees keys j <= i + shift (and j < nk); without causality every key: i + nk >= nk - 1
+  __device__ __forceinline__ Seq(const PromptParams &p, int b) {
+    // (constant memory: scalar loads where b is uniform)
+    typedef const __attribute__((address_space(4))) int32_t constant;
+    constant *cu_q = (constant *)(uintptr_t)p.cu_q, *cu_k = (constant *)(uintptr_t)p.cu_k;
+    qs = min(max((int64_t)cu_q[b], (int64_t)0), p.total_q);
+    ks = min(max((int64_t)cu_k[b], (int64_t)0), p.total_k);
+    const int nq = (int)(min((int64_t)cu_q[b + 1], p.total_q) - qs);
+    nk = max((int)(min((int64_t)cu_k[b + 1], p.total_k) - ks), 0);
+    rows = max(min(nq, p.max_q), 0);
+    shift = p.causal ? nk - nq : nk;
+  }
+  // In scalar registers, whatever the compiler has made of its uniformity.
+  __device__ __forceinline__ void to_scalars() {
+    qs = uniform(qs), ks = uniform(ks);
+    rows = uniform(rows), nk = uniform(nk), shift = uniform(shift);
+  }
+  __device__ __forceinline__ int blocks() const { return (rows + kPromptRows - 1) / kPromptRows; }
+  // tiles of keys that a block's last row sees
+  __device__ __forceinline__ int tiles(int block) const {
+    return (min(max(min((block + 1) * kPromptRows, rows) + shift, 0), nk) + kKeys - 1) / kKeys;
+  }
+};
+
+// The sum of one row's weighted values by a wave, over keys first .. last of its sequence, given its maximum (log2
+// units): 64 keys at a time, scores by a lane each, then dims 2 lane and 2 lane + 1.
 template <typename T>
-__device__ void exact_row(const PromptParams &p, int h, int64_t row, int64_t ks, int lim, float m, float inv) {
+__device__ f32x2 exact_row(const PromptParams &p, int h, int64_t row, int64_t ks, int first, int last, float m) {
   const int lane = threadIdx.x & 63;
   const T *q = reinterpret_cast<const T *>(p.q) + row * p.q_st + h * p.q_sh;
   const float use = m == -INFINITY ? 0.0f : m;
-  float out[2] = {0.0f, 0.0f};
-  for (int j0 = 0; j0 <= lim; j0 += 64) {
-    const int64_t j = ks + min(j0 + lane, lim);
+  f32x2 out = {0.0f, 0.0f};
+  for (int j0 = first; j0 <= last; j0 += 64) {
+    const int64_t j = ks + min(j0 + lane, last);
     const T *k = reinterpret_cast<const T *>(p.k) + j * p.k_st + h * p.k_sh, *kr = reinterpret_cast<const T *>(p.kr) + j * p.kr_st;
     float s = 0.0f;
     for (int c = 0; c < kDim + kRope; c += 8) {
@@ -71,48 +108,52 @@ __device__ void exact_row(const PromptParams &p, int h, int64_t row, int64_t ks,
 #pragma unroll
       for (int e = 0; e < 4; ++e) s = dot2<T>(kw[e], qw[e], s);
     }
-    const float w = j0 + lane <= lim ? __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c_log2, -use)) : 0.0f;
-    for (int n = 0; n < min(64, lim + 1 - j0); ++n) {
+    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c_log2, -use));
+    for (int n = 0; n < min(64, last + 1 - j0); ++n) {
       const float wn = lane_f(w, n);
       const T *v = reinterpret_cast<const T *>(p.v) + (ks + j0 + n) * p.v_st + h * p.v_sh + 2 * lane;
       out[0] += wn * (float)v[0];
       out[1] += wn * (float)v[1];
     }
   }
-  *reinterpret_cast<int *>(reinterpret_cast<T *>(p.out) + row * p.o_st + h * p.o_sh + 2 * lane) = pack2<T>(out[0] * inv, out[1] * inv);
+  return out;
 }
 
-template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void latent_prompt(PromptParams p) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];  // two tiles: keys, values, rotary parts
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// A lane's share of a row: dims 32 d + 8 k + 4 g2 .. + 3 in x[k].
+template <typename T>
+__device__ __forceinline__ void store_dims(const PromptParams &p, int64_t row, int h, int g2, int d, const f32x4 (&x)[4], float l) {
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
+  T *dst = reinterpret_cast<T *>(p.out) + row * p.o_st + h * p.o_sh + 4 * g2 + 32 * d;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<i32x2 *>(dst + 8 * k) =
+        i32x2{pack2<T>(x[k][0] * inv, x[k][1] * inv), pack2<T>(x[k][2] * inv, x[k][3] * inv)};
+}
+__device__ __forceinline__ void store_lse(const PromptParams &p, int64_t row, int h, int g2, float m, float l) {
+  if (p.lse && g2 == 0) p.lse[row * p.l_st + h * p.l_sh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Tiles lo .. hi - 1 of the keys for rows q0 .. of (sequence, head): to the output (slot < 0), or as a part to the
+// workspace.
+template <typename T>
+__device__ __forceinline__ void block_of_rows(const PromptParams &p, char *smem, const Seq &seq, int h, int q0, int lo, int hi,
+                                              int64_t slot) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (what follows from it is computed for each block: hoisted out of their loop it spills)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, g2 = lane >> 5;
-  // (sequence, head) varies fastest, so that a head's keys and values stay with one XCD where the count is a
-  // multiple of 8; the last rows, which see the most keys, come first.
-  const int bh = blockIdx.x % (p.batch * p.heads);
-  const int b = bh / p.heads, h = bh % p.heads;
-  const int blocks = (p.max_q + kPromptRows - 1) / kPromptRows;
-  const int q0 = (blocks - 1 - (int)(blockIdx.x / (p.batch * p.heads))) * kPromptRows;
-  const int64_t qs = min(max((int64_t)p.cu_q[b], (int64_t)0), p.total_q);
-  const int64_t ks = min(max((int64_t)p.cu_k[b], (int64_t)0), p.total_k);
-  const int nq = (int)(min((int64_t)p.cu_q[b + 1], p.total_q) - qs);
-  const int nk = max((int)(min((int64_t)p.cu_k[b + 1], p.total_k) - ks), 0);
-  const int rows = min(nq, p.max_q);
-  if (q0 >= rows) return;  // the whole workgroup
-  // query i sees keys j <= i + shift (and j < nk); without causality every key: i + nk >= nk - 1
-  const int shift = p.causal ? nk - nq : nk;
-  const int last_row = min(q0 + kPromptRows, rows) - 1;
-  const int seen = min(nk, max(last_row + shift + 1, 0));
-  const int tiles = (seen + kKeys - 1) / kKeys;
+  const int64_t qs = seq.qs, ks = seq.ks;
+  const int nk = seq.nk, rows = seq.rows, shift = seq.shift;
 
   // ---- staging: a wave's instruction fills four rows of keys (values), or eight of rotary parts ----
-  const char *kb = reinterpret_cast<const char *>(p.k) + 2 * (ks * p.k_st + h * p.k_sh);
-  const char *vb = reinterpret_cast<const char *>(p.v) + 2 * (ks * p.v_st + h * p.v_sh);
-  const char *rb = reinterpret_cast<const char *>(p.kr) + 2 * (ks * p.kr_st);
+  const char *kb = reinterpret_cast<const char *>(p.k) + uniform(2 * (ks * p.k_st + h * p.k_sh));
+  const char *vb = reinterpret_cast<const char *>(p.v) + uniform(2 * (ks * p.v_st + h * p.v_sh));
+  const char *rb = reinterpret_cast<const char *>(p.kr) + uniform(2 * (ks * p.kr_st));
   // (a tile's rows are within 32 bits of its first, checked on the host)
   const uint32_t k_row = 2 * (uint32_t)p.k_st, v_row = 2 * (uint32_t)p.v_st, r_row = 2 * (uint32_t)p.kr_st;
   const uint32_t lds = lds_address(smem);
   auto stage = [&](int tile) {
-    const uint32_t buf = lds + (tile & 1) * kTileBytes;
+    const uint32_t buf = lds + ((tile - lo) & 1) * kTileBytes;
     const int j0 = tile * kKeys;
     const char *kt = kb + (int64_t)j0 * (2 * p.k_st), *vt = vb + (int64_t)j0 * (2 * p.v_st), *rt = rb + (int64_t)j0 * (2 * p.kr_st);
     const int last = nk - 1 - j0;
@@ -148,11 +189,13 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
       load_lds(rt, min(row, last) * r_row + 16 * c, buf + 2 * kWideBytes + (16 * wave + 8 * i) * kNarrowRow);
     }
   };
-  if (tiles > 0) stage(0);
+  if (lo < hi) stage(lo);
 
   const int i = q0 + wave * kWaveRows + n32;  // the lane's query row
   const int lim = i < rows ? min(i + shift, nk - 1) : -1;
-  const int wave_lim = q0 + wave * kWaveRows + shift;  // (its first row's, before the end of the keys)
+  const int wave_row = q0 + wave * kWaveRows;
+  const int wave_lim = wave_row + shift;  // (its first row's, before the end of the keys)
+  const int wave_end = wave_row < rows ? min(wave_row + kWaveRows, rows) - 1 + shift : -1;  // (its last row's)
   i32x4 q[kSlices];
   {
     const T *src = reinterpret_cast<const T *>(p.q) + (qs + min(i, rows - 1)) * p.q_st + h * p.q_sh + 8 * g2;
@@ -178,7 +221,8 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
   // One tile; its buffer is a constant, so that the reads' places are immediates.
   auto step = [&](int tile, auto which) {
     landed_and_barrier<0>();  // this tile is there, and the one before is consumed
-    if (tile + 1 < tiles) stage(tile + 1);
+    if (tile + 1 < hi) stage(tile + 1);
+    if (tile * kKeys > wave_end) return;  // none of the wave's rows sees any of it
     const char *buf = smem + decltype(which)::value * kTileBytes;
     const int j0 = tile * kKeys;
     // ---- S^T = K Q^T, 32 keys a product.  The operands of a step are read three steps ahead (left to itself the
@@ -252,13 +296,12 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  for (int tile = 0; tile < tiles; tile += 2) {
+  for (int tile = lo; tile < hi; tile += 2) {
     step(tile, std::integral_constant<int, 0>{});
-    if (tile + 1 < tiles) step(tile + 1, std::integral_constant<int, 1>{});
+    if (tile + 1 < hi) step(tile + 1, std::integral_constant<int, 1>{});
   }
 
   const float l = sum_halves(sum);
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
   // A key that a row does not see enters its value product with a weight of 0, and 0 x NaN is NaN: rows that are
   // not finite though their sum is are computed again, from the keys they see alone.
   float odd = 0.0f;
@@ -267,21 +310,185 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
 #pragma unroll
     for (int e = 0; e < 16; ++e) odd = __builtin_fmaf(acc[d][e], 0.0f, odd);
   const uint64_t odd_lanes = __ballot(p.causal && i < rows && odd != odd && l == l);
-  const uint32_t again = (uint32_t)(odd_lanes | odd_lanes >> 32);
-  for (uint32_t left = again; left; left &= left - 1) {
-    const int r = __builtin_ctz(left), row = q0 + wave * kWaveRows + r;
-    exact_row<T>(p, h, qs + row, ks, __builtin_amdgcn_readlane(lim, r), lane_f(m, r), lane_f(inv, r));
+  for (uint32_t left = (uint32_t)(odd_lanes | odd_lanes >> 32); left; left &= left - 1) {
+    const int r = __builtin_ctz(left);
+    const f32x2 x = exact_row<T>(p, h, qs + q0 + wave * kWaveRows + r, ks, lo * kKeys,
+                                 min(hi * kKeys - 1, __builtin_amdgcn_readlane(lim, r)), lane_f(m, r));
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float y = __shfl(x[e & 1], (32 * d + 8 * (e >> 2) + 4 * g2 + (e & 3)) >> 1);
+        acc[d][e] = n32 == r ? y : acc[d][e];
+      }
   }
-  if (i >= rows) return;
-  T *dst = reinterpret_cast<T *>(p.out) + (qs + i) * p.o_st + h * p.o_sh + 4 * g2;
-  if (!(again >> n32 & 1))
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
+  for (int d = 0; d < 4; ++d) {
+    f32x4 x[4];
 #pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      *reinterpret_cast<i32x2 *>(dst + 32 * d + 2 * e) =
-          i32x2{pack2<T>(acc[d][e] * inv, acc[d][e + 1] * inv), pack2<T>(acc[d][e + 2] * inv, acc[d][e + 3] * inv)};
-  if (p.lse && g2 == 0) p.lse[(qs + i) * p.l_st + h * p.l_sh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    for (int k = 0; k < 4; ++k) x[k] = f32x4{acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]};
+    if (slot >= 0) {
+      f32x4 *dst = reinterpret_cast<f32x4 *>(p.part) + ((slot * kPromptWaves + wave) * 16 + 4 * d) * 64 + lane;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) dst[64 * k] = x[k];
+    } else if (i < rows) {
+      store_dims<T>(p, qs + i, h, g2, d, x, l);
+    }
+  }
+  if (slot < 0 && i < rows) store_lse(p, qs + i, h, g2, m, l);
+  if (slot >= 0 && g2 == 0)
+    *reinterpret_cast<f32x2 *>(p.part_ml + 2 * (slot * kPromptRows + wave * kWaveRows + n32)) = f32x2{m, l};
+}
+
+template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void latent_prompt(PromptParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // two tiles: keys, values, rotary parts
+  // (sequence, head) varies fastest, so that a head's keys and values stay with one XCD where the count is a
+  // multiple of 8; the last rows, which see the most keys, come first.
+  const int bh = blockIdx.x % (p.batch * p.heads);
+  const int b = bh / p.heads, h = bh % p.heads;
+  const int blocks = (p.max_q + kPromptRows - 1) / kPromptRows;
+  const int block = blocks - 1 - (int)(blockIdx.x / (p.batch * p.heads));
+  const Seq seq(p, b);
+  if (block * kPromptRows >= seq.rows) return;  // the whole workgroup
+  block_of_rows<T>(p, smem, seq, h, block * kPromptRows, 0, seq.tiles(block), -1);
+}
+
+// ---- the keys split over runs ----
+// What a run spends on one block of rows more, in tiles (its query, its output, the pipeline's start), and the tiles
+// a run has at the least.
+constexpr int kPromptSwitch = 2, kRunTiles = 4;
+
+// The tiles and switches of one head of a sequence, and of one block of rows.
+__device__ __forceinline__ int block_cost(const Seq &q, int block) { return kPromptSwitch + max(1, q.tiles(block)); }
+__device__ __forceinline__ int64_t head_cost(const PromptParams &p, const Seq &q) {
+  const int n = q.blocks();
+  if (n == 0) return 0;
+  if (!p.causal) return (int64_t)n * block_cost(q, 0);
+  // the full blocks: block k has 2 (k + 1) + c tiles, and where that is below 1 it counts as 1
+  static_assert(kPromptRows == 2 * kKeys, "tiles a block adds");
+  const int c = (q.shift + kKeys - 1) >> 6, k1 = min(max(((2 - c) >> 1) - 1, 0), n - 1);
+  const int64_t full = n - 1 - k1;
+  return (int64_t)n * kPromptSwitch + k1 + full * c + full * (k1 + n) + max(1, q.tiles(n - 1));
+}
+
+template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void latent_prompt_runs(PromptParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int kPromptThreads = 64 * kPromptWaves;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // neighbouring runs, which share keys and values, on one XCD
+  const int group = (int)(blockIdx.x & 7) * (p.groups >> 3) + (int)(blockIdx.x >> 3);
+  int64_t *const s_wave = reinterpret_cast<int64_t *>(smem), *const s_start = s_wave + kPromptWaves;
+  const int chunk = (p.batch + kPromptThreads - 1) / kPromptThreads;
+  int64_t mine = 0;
+  for (int k = 0; k < chunk; ++k)
+    if (tid * chunk + k < p.batch) mine += p.heads * head_cost(p, Seq(p, tid * chunk + k));
+  int64_t inc = mine, total = 0;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t y = __shfl_up(inc, off);
+    if (lane >= off) inc += y;
+  }
+  if (lane == 63) s_wave[wave] = inc;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPromptWaves; ++w) {
+    if (w < wave) inc += s_wave[w];
+    total += s_wave[w];
+  }
+  total = uniform(total);
+  // run g is cost g total / runs .. (g + 1) total / runs, rounded down; none is empty
+  const int64_t runs = min((int64_t)p.groups, max(total / kRunTiles, (int64_t)1));
+  if (group >= runs || total == 0) return;  // the whole workgroup
+  const int64_t first = group * total / runs, last = (group + 1) * total / runs;
+  if (inc - mine <= first && first < inc) {
+    int64_t at = inc - mine;
+    int n = tid * chunk;
+    for (; chunk > 1; ++n) {
+      const int64_t cost = p.heads * head_cost(p, Seq(p, n));
+      if (first < at + cost) break;
+      at += cost;
+    }
+    s_start[0] = n;
+    s_start[1] = at;
+  }
+  __syncthreads();
+  int b = __builtin_amdgcn_readfirstlane((int)s_start[0]);
+  int64_t at = uniform(s_start[1]);  // the cost at which (sequence, head, block) begins
+  Seq seq(p, b);
+  const int64_t per_head = head_cost(p, seq);
+  int h = (int)((first - at) / per_head), block = 0;
+  at += h * per_head;
+  while (first >= at + block_cost(seq, block)) at += block_cost(seq, block++);
+  int lo = (int)max(first - at - kPromptSwitch, (int64_t)0);
+  while (at + kPromptSwitch < last) {  // (or the run ends before the block's first tile)
+    seq.to_scalars(), lo = uniform(lo), block = uniform(block), h = uniform(h), at = uniform(at);
+    const int tiles = seq.tiles(block), cost = block_cost(seq, block);
+    const int hi = uniform((int)min((int64_t)tiles, last - at - kPromptSwitch));
+    if (lo == 0 && tid == 0)
+      p.runs[((int64_t)b * p.heads + h) * ((p.max_q + kPromptRows - 1) / kPromptRows) + block] =
+          i32x2{group, (int)(((at + cost) * runs - 1) / total)};
+    lds_barrier();  // (what the buffers hold is consumed)
+    block_of_rows<T>(p, smem, seq, h, block * kPromptRows, lo, hi, lo == 0 && hi == tiles ? -1 : lo > 0 ? 2 * group : 2 * group + 1);
+    lo = 0;
+    at += cost;
+    if (++block < seq.blocks()) continue;
+    block = 0;
+    if (++h < p.heads) continue;
+    h = 0;
+    do {
+      if (++b == p.batch) return;
+      seq = Seq(p, b);
+    } while (seq.rows == 0);
+  }
+}
+
+// Outputs of blocks of rows that several runs share, from their parts, which lie as the accumulators did: a workgroup
+// takes 32 dims of a block, with the loads of two parts in flight.
+template <typename T> __global__ __launch_bounds__(64 * kPromptWaves) void latent_prompt_merge(PromptParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n32 = lane & 31, g2 = lane >> 5;
+  const int block = blockIdx.x, b = blockIdx.y / p.heads, h = blockIdx.y % p.heads, d = blockIdx.z;
+  const Seq seq(p, b);
+  if (block * kPromptRows >= seq.rows) return;  // the whole workgroup
+  const i32x2 runs = ((const __attribute__((address_space(4))) i32x2 *)(uintptr_t)(p.runs))[(int64_t)blockIdx.y * gridDim.x + block];
+  const int g0 = runs[0], g1 = runs[1];
+  if (g0 == g1) return;  // written already
+  f32x4 acc[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.0f;
+  for (int g = g0; g <= g1; g += 2) {
+    f32x4 x[2][4];
+    f32x2 ml[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      ml[u] = f32x2{-INFINITY, 0.0f};
+      if (g + u > g1) continue;  // (uniform)
+      const int64_t slot = g + u == g0 ? 2 * (g + u) + 1 : 2 * (g + u);
+      ml[u] = *reinterpret_cast<const f32x2 *>(p.part_ml + 2 * (slot * kPromptRows + wave * kWaveRows + n32));
+      const f32x4 *src = reinterpret_cast<const f32x4 *>(p.part) + ((slot * kPromptWaves + wave) * 16 + 4 * d) * 64 + lane;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[u][k] = src[64 * k];
+    }
+    const float next = fmaxf(m, fmaxf(ml[0][0], ml[1][0])), use = next == -INFINITY ? 0.0f : next;
+    const float a = __builtin_amdgcn_exp2f(m - use);
+    m = next;
+    l *= a;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] *= a;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (g + u > g1) continue;
+      const float w = __builtin_amdgcn_exp2f(ml[u][0] - use);
+      l += ml[u][1] * w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += x[u][k] * w;
+    }
+  }
+  const int i = block * kPromptRows + wave * kWaveRows + n32;
+  if (i < seq.rows) {
+    store_dims<T>(p, seq.qs + i, h, g2, d, acc, l);
+    if (d == 0) store_lse(p, seq.qs + i, h, g2, m, l);
+  }
 }
 
 }  // namespace l20la
@@ -289,6 +496,13 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
 namespace {
 
 using l20pd_host::set_error;
+
+// The keys are split where the longest block of rows takes more than kSplitRatio times what a workgroup's even share
+// of all tiles is (by the mean lengths, which the host knows), and sequences have kSplitTiles tiles or more.  Measured
+// (bf16, whole -> split): 300 queries on 5000 keys, 28 heads 107 -> 52 us, 8 heads 106 -> 33; 4 x 64 on 8064, 16 heads
+// 168 -> 61; 4096 tokens, 8 heads 95 -> 69, 16 heads (ratio 1.9) 109 -> 112, 32 heads (1.0) 181 -> 205; of few tiles
+// 1000 tokens, 16 heads (16 tiles) 26 -> 30, 2048 tokens, 16 heads (32 tiles) 48 -> 48.
+constexpr int kSplitRatio = 2, kSplitTiles = 24;
 
 int32_t check(const l20_pd_latent_prompt_args *a) {
   if (!a) return set_error(L20_PD_EINVAL, "null argument block");
@@ -321,9 +535,56 @@ int32_t check(const l20_pd_latent_prompt_args *a) {
   return L20_PD_OK;
 }
 
+template <typename T> hipError_t launch(const l20la::PromptParams &p, int blocks, hipStream_t s) {
+  const int lds = 2 * l20la::kTileBytes;  // 80 KB: two workgroups a CU
+  const dim3 block(64 * l20la::kPromptWaves);
+  if (!p.groups) {
+    static l20la::LdsLimit limit;
+    const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20la::latent_prompt<T>), lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(l20la::latent_prompt<T>, dim3((unsigned)blocks * (unsigned)(p.batch * p.heads)), block, lds, s, p);
+    return hipGetLastError();
+  }
+  static l20la::LdsLimit limit;
+  hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20la::latent_prompt_runs<T>), lds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(l20la::latent_prompt_runs<T>, dim3((unsigned)p.groups), block, lds, s, p);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(l20la::latent_prompt_merge<T>, dim3((unsigned)blocks, (unsigned)(p.batch * p.heads), l20la::kDim / 32), block,
+                     0, s, p);
+  return hipGetLastError();
+}
+
+struct PromptPlan {
+  int blocks, groups;  // groups = 0: the keys are not split
+  int64_t part_rows, workspace;
+};
+
+PromptPlan plan_of(const l20_pd_latent_prompt_args &a, int cus) {
+  PromptPlan n{};
+  const int64_t max_q = std::min<int64_t>(a.max_q_len, a.total_q);
+  n.blocks = (int)((max_q + l20la::kPromptRows - 1) / l20la::kPromptRows);
+  const int64_t units = (int64_t)a.batch * a.num_heads * n.blocks, slots = 2 * cus;  // two workgroups a CU
+  const int64_t queries = std::min((a.total_q + a.batch - 1) / a.batch, max_q), keys = a.total_k / a.batch;
+  const int64_t blocks = (int64_t)a.batch * a.num_heads * ((queries + l20la::kPromptRows - 1) / l20la::kPromptRows);
+  const int64_t longest = (keys + max_q - queries) / l20la::kKeys, mean = std::max<int64_t>(keys - queries / 2, 0) / l20la::kKeys;
+  if (keys < kSplitTiles * l20la::kKeys || kSplitRatio * blocks * mean > slots * longest) return n;
+  n.groups = (int)((slots + 7) / 8 * 8);
+  n.part_rows = (int64_t)2 * n.groups * l20la::kPromptRows;
+  n.workspace = n.part_rows * (l20la::kDim + 2) * (int64_t)sizeof(float) + units * (int64_t)sizeof(l20la::i32x2);
+  return n;
+}
+
 }  // namespace
 
 extern "C" {
+
+int64_t l20_pd_latent_prompt_workspace(const l20_pd_latent_prompt_args *a, int32_t cu_count) {
+  l20pd_host::clear_error();
+  if (!a || a->batch < 1 || a->num_heads < 1 || a->max_q_len < 1 || a->total_q < 1 || a->total_k < 0) return 0;
+  return plan_of(*a, cu_count > 0 ? cu_count : l20la::device_cus()).workspace;
+}
 
 int32_t l20_pd_latent_prompt_check(const l20_pd_latent_prompt_args *a) {
   l20pd_host::clear_error();
@@ -361,19 +622,16 @@ int32_t l20_pd_latent_prompt(const l20_pd_latent_prompt_args *a, void *stream) {
   p.batch = a->batch;
   p.heads = a->num_heads;
   p.max_q = (int)std::min<int64_t>(a->max_q_len, a->total_q);
-  const unsigned blocks = (unsigned)((p.max_q + l20la::kPromptRows - 1) / l20la::kPromptRows);
-  const dim3 grid(blocks * (unsigned)(p.batch * p.heads)), block(64 * l20la::kPromptWaves);
+  PromptPlan plan = plan_of(*a, l20la::device_cus());
+  if (!a->workspace) plan.groups = 0;
+  if (plan.groups && (a->workspace_bytes < plan.workspace || (uintptr_t)a->workspace % 16))
+    return set_error(L20_PD_EINVAL, "workspace is too small for the request (l20_pd_latent_prompt_workspace)");
+  p.groups = plan.groups;
+  p.part = static_cast<float *>(a->workspace);
+  p.part_ml = p.part + plan.part_rows * l20la::kDim;
+  p.runs = reinterpret_cast<l20la::i32x2 *>(p.part_ml + plan.part_rows * 2);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int lds = 2 * l20la::kTileBytes;  // 80 KB: two workgroups a CU
-  const bool bf = a->dtype == L20_PD_BF16;
-  static l20la::LdsLimit limit[2];
-  hipError_t e = limit[bf].raise(bf ? reinterpret_cast<const void *>(&l20la::latent_prompt<__bf16>)
-                                    : reinterpret_cast<const void *>(&l20la::latent_prompt<_Float16>), lds);
-  if (e == hipSuccess) {
-    if (bf) hipLaunchKernelGGL((l20la::latent_prompt<__bf16>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((l20la::latent_prompt<_Float16>), grid, block, lds, s, p);
-    e = hipGetLastError();
-  }
+  const hipError_t e = a->dtype == L20_PD_BF16 ? launch<__bf16>(p, plan.blocks, s) : launch<_Float16>(p, plan.blocks, s);
   if (e != hipSuccess) {
     char msg[256];
     snprintf(msg, sizeof(msg), "HIP launch failed: %s", hipGetErrorString(e));

@@ -140,6 +140,23 @@ def l20_paged_latent_attention(
                                                           int(q_len), lse)
 
 
+def allocate_l20_latent_prompt_workspace(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    batch: int,
+    max_seqlen_q: int,
+) -> torch.Tensor:
+    """The workspace of ``l20_latent_prompt_attention`` for these shapes (uint8; empty where the keys are not split).
+    Calls that may overlap each need their own; its contents do not matter."""
+    import l20_pd_cabi
+
+    a = l20_pd_cabi.L20PdLatentPromptArgs()
+    a.total_q, a.num_heads, a.total_k = query.shape[0], query.shape[1], key.shape[0]
+    a.batch, a.max_q_len = batch, int(max_seqlen_q)
+    size = int(l20_pd_cabi.load().l20_pd_latent_prompt_workspace(l20_pd_cabi.ctypes.byref(a), gpu_cus(query.device)))
+    return torch.empty(size, dtype=torch.uint8, device=query.device)
+
+
 def l20_latent_prompt_attention(
     query: torch.Tensor,
     key: torch.Tensor,
@@ -152,6 +169,7 @@ def l20_latent_prompt_attention(
     softmax_scale: Optional[float] = None,
     causal: bool = True,
     output: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
     lse: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Attention of packed prompts: ``query`` [tokens, heads, 192] (its last 64 dims rotated), ``key`` and
@@ -161,7 +179,8 @@ def l20_latent_prompt_attention(
     Sequence b has the query rows and the keys of its ``cu_seqlens`` ranges; with ``causal`` query i of n sees
     keys up to i + (keys - n), so that a chunk whose first tokens are cached already passes all keys.  A row that
     sees none gives zeros (``lse``: -inf); rows outside the ranges, or beyond ``max_seqlen_q``, keep what they
-    held.  ``softmax_scale`` defaults to 192^-0.5."""
+    held.  ``softmax_scale`` defaults to 192^-0.5.  Calls of few rows and many keys split the keys, with a
+    ``workspace`` (default: allocated)."""
     _need_gpu("l20_latent_prompt_attention", query)
     if query.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("l20_latent_prompt_attention supports FP16 and BF16")
@@ -173,9 +192,11 @@ def l20_latent_prompt_attention(
         output = query.new_empty(*query.shape[:2], HEAD_DIM)
     if softmax_scale is None:
         softmax_scale = (HEAD_DIM + ROPE_DIM) ** -0.5
+    if workspace is None and cu_seqlens_q.ndim == 1 and cu_seqlens_q.shape[0] > 1:
+        workspace = allocate_l20_latent_prompt_workspace(query, key, cu_seqlens_q.shape[0] - 1, max_seqlen_q)
     return torch.ops.l20_stack.latent_prompt_attention_out(query, key, key_rope, value, cu_seqlens_q, cu_seqlens_k,
                                                            int(max_seqlen_q), output, float(softmax_scale), bool(causal),
-                                                           lse)
+                                                           lse, workspace)
 
 
 def _register_fake() -> None:
@@ -192,7 +213,7 @@ def _register_fake() -> None:
 
     @torch.library.register_fake("l20_stack::latent_prompt_attention_out")
     def _latent_prompt_attention_fake(query, key, key_rope, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, output,
-                                      softmax_scale, causal=True, lse=None):
+                                      softmax_scale, causal=True, lse=None, workspace=None):
         return output
 
 

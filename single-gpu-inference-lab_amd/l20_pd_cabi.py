@@ -56,6 +56,7 @@ EXPORTED = (
     "l20_pd_paged_latent_workspace",
     "l20_pd_paged_latent",
     "l20_pd_latent_prompt_check",
+    "l20_pd_latent_prompt_workspace",
     "l20_pd_latent_prompt",
     "l20_pd_block_tables_check",
     "l20_pd_block_tables",
@@ -172,7 +173,7 @@ class L20PdLatentPromptArgs(ctypes.Structure):
         ("lse", _vp), ("lse_stride_token", _i64), ("lse_stride_head", _i64),
         ("softmax_scale", _f32), ("causal", _i32), ("total_q", _i64), ("total_k", _i64),
         ("batch", _i32), ("num_heads", _i32), ("max_q_len", _i32), ("head_dim", _i32), ("rope_dim", _i32),
-        ("value_dim", _i32),
+        ("value_dim", _i32), ("workspace", _vp), ("workspace_bytes", _i64),
     ]
 
 
@@ -253,6 +254,8 @@ def load(path: Optional[Path] = None) -> ctypes.CDLL:
         getattr(lib, "l20_pd_" + name).restype = _i32
     lib.l20_pd_paged_latent_workspace.argtypes = [ctypes.POINTER(L20PdLatentArgs), _i32]
     lib.l20_pd_paged_latent_workspace.restype = _i64
+    lib.l20_pd_latent_prompt_workspace.argtypes = [ctypes.POINTER(L20PdLatentPromptArgs), _i32]
+    lib.l20_pd_latent_prompt_workspace.restype = _i64
     if path is None:
         _lib = lib
     return lib

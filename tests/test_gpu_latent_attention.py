@@ -260,10 +260,15 @@ PROMPT = [
     ([5, 130], [700, 333], 4),            # chunks behind cached tokens
     ([40, 1, 3], [10, 0, 200], 2),        # fewer keys than queries: rows that see nothing
     ([700], [700], 1),
+    # (from here on the keys are split over runs)
+    ([1, 300, 0, 129], [4000, 1900, 50, 1029], 3),
+    ([1700, 1], [1600, 3000], 2),         # blocks of rows that see nothing
+    ([260], [4000], 1),
+    ([200, 100] + [3] * 9, [9000, 8000, 100, 50, 1, 64, 65, 128, 30, 0, 90], 8),  # runs of several blocks
 ]
 
 
-@pytest.mark.parametrize("spec", PROMPT, ids=[f"q{'_'.join(map(str, s[0]))}_k{'_'.join(map(str, s[1]))}_h{s[2]}" for s in PROMPT])
+@pytest.mark.parametrize("spec", PROMPT, ids=[f"q{'_'.join(map(str, s[0][:4]))}_k{'_'.join(map(str, s[1][:4]))}_h{s[2]}" for s in PROMPT])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
 def test_prompt_against_float64(spec, dtype, causal):
@@ -286,6 +291,52 @@ def test_prompt_nan_of_a_later_key_reaches_only_the_rows_that_see_it(dtype):
     out[137:200, 1, 9] = clean[137:200, 1, 9]
     out[230:, 2], lse[230:, 2] = clean[230:, 2], clean_lse[230:, 2]
     R.check_prompt(out, lse, c["query"], key, c["key_rope"], value, c["cu_q"], c["cu_k"], SCALE)
+
+
+def test_prompt_split_with_a_used_workspace_on_another_stream_and_in_a_graph():
+    """Any contents of the workspace; replays with other lengths; NaN keys that some rows of a split block do not see."""
+    import l20_latent_attention as la
+
+    c = make_prompt([200, 90], [1800, 1490], 3, seed=26)
+    ws = la.allocate_l20_latent_prompt_workspace(c["query"], c["key"], 2, c["max_q"])
+    assert ws.numel() > 0
+    ws.fill_(255)
+    clean, clean_lse = run_prompt(c, workspace=ws)
+    R.check_prompt(clean, clean_lse, c["query"], c["key"], c["key_rope"], c["value"], c["cu_q"], c["cu_k"], SCALE)
+    whole, _ = run_prompt(c, workspace=torch.empty(0, dtype=torch.uint8, device="cuda"))
+    assert float((whole.float() - clean.float()).abs().max()) < 0.02
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again, again_lse = run_prompt(c, workspace=ws)
+    side.synchronize()
+    assert torch.equal(again, clean) and torch.equal(again_lse, clean_lse)
+    with pytest.raises(RuntimeError, match="workspace is too small"):
+        run_prompt(c, workspace=ws[:1024])
+    out, lse = torch.empty_like(clean), torch.empty_like(clean_lse)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        la.l20_latent_prompt_attention(c["query"], c["key"], c["key_rope"], c["value"], c["cu_q"], c["cu_k"], c["max_q"],
+                                       output=out, lse=lse, workspace=ws)
+    for k in range(4):
+        c["cu_q"].copy_(torch.tensor([0, 200 - 30 * k, 290 - 40 * k], dtype=torch.int32))
+        c["cu_k"].copy_(torch.tensor([0, 1800 - 400 * k, 3290 - 450 * k], dtype=torch.int32))
+        out.fill_(3)
+        lse.fill_(5)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager, eager_lse = run_prompt(c, output=torch.full_like(out, 3))
+        assert torch.equal(out, eager) and torch.equal(lse, eager_lse)
+    c["cu_q"].copy_(torch.tensor([0, 200, 290], dtype=torch.int32))
+    c["cu_k"].copy_(torch.tensor([0, 1800, 3290], dtype=torch.int32))
+    c["key"][1600 + 137, 1] = float("nan")
+    c["value"][1600 + 137, 1] = float("nan")
+    got, got_lse = run_prompt(c, workspace=ws)
+    assert bool(torch.isnan(got[137:200, 1]).all())
+    keep = torch.ones(290, 3, dtype=torch.bool, device="cuda")
+    keep[137:200, 1] = False
+    assert float((got.float() - clean.float()).abs()[keep].max()) < 0.02
+    assert float((got_lse - clean_lse).abs()[keep].max()) < 1e-4
 
 
 def test_prompt_leaves_other_rows_alone():
