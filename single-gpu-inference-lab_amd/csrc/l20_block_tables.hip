@@ -5,10 +5,12 @@
 //    the first).  The offsets lie in LDS, and freed pages, fresh pages and (small batches) tokens are each
 //    spread over all threads: a thread finds its request by binary search, so one long prompt is as quick as
 //    many short ones.  Freed pages are on the stack before any is taken from it: one call does both.
-//  bt_tokens     slots and positions of larger batches, a grid of workgroups that hold cu_lens in LDS.
+//  bt_tokens     slots and positions of larger batches, a token a thread, cu_lens in LDS.
 //
-// The work is a few bytes a token: what a call costs is its launches and the chain of dependent loads and
-// barriers in the first (lengths, two scans, stack, table).
+// The work is a few bytes a token: what a call costs is its launches (two 3 us apart) and the chain of dependent
+// loads and barriers in the first: lengths, two scans, then the stack and the table at once.  256 requests of one
+// token take 6.3 us, 48 requests with 20 000 new tokens 10.5 (the empty launch of such a workgroup: 2 to 3); a
+// workgroup of 256 threads instead took 7.9, tokens that wait for the table to be written 7.2.
 
 #include "l20_block_tables.h"
 
@@ -20,7 +22,8 @@ namespace l20bt {
 
 constexpr int kThreads = 1024;
 constexpr int kPerThread = L20_PD_MAX_REQUESTS / kThreads;
-// Tokens that bt_requests places itself; more go to bt_tokens in a second launch.
+// Tokens that bt_requests places itself; more go to bt_tokens in a second launch.  Measured, 256 requests, one launch
+// against two: 2048 tokens 7.4 and 8.7 us, 4096 tokens 11.3 and 11.2, 8192 tokens 15.6 and 11.4.
 constexpr int kTokensInline = 4096;
 
 struct Params {
@@ -36,29 +39,39 @@ struct Params {
   int tokens;
   int32_t *cu, *seq_lens;
   int batch, page;
+  uint64_t magic;  // (n / 16) * magic >> 38 = n / page
   int inline_tokens;
 };
 
-// Inclusive scan of one value a thread over the workgroup; `total` is the sum.
-__device__ __forceinline__ int64_t scan(int64_t x, int64_t *s_wave, int64_t &total) {
+// n / page, for n through 2^31 + 4095 (a division takes a good hundred instructions at 64 bits, some thirty at 32).
+__device__ __forceinline__ uint32_t div_page(const Params &p, uint32_t n) { return (uint32_t)((uint64_t)(n >> 4) * p.magic >> 38); }
+// The pages of n tokens.
+__device__ __forceinline__ int pages_of(const Params &p, int n) { return (int)div_page(p, (uint32_t)n + (uint32_t)p.page - 1); }
+
+// Inclusive scans of N values a thread over the workgroup; `total` are the sums.
+template <int N> __device__ __forceinline__ void scan(int64_t (&x)[N], int64_t (*s_wave)[kThreads / 64], int64_t (&total)[N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(x, off);
-    if (lane >= off) x += y;
-  }
-  __syncthreads();  // s_wave may still be read from the scan before
-  if (lane == 63) s_wave[wave] = x;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
+  for (int off = 1; off < 64; off <<= 1)
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    const int64_t v = s_wave[w];
-    before += w < wave ? v : 0;
-    total += v;
+    for (int n = 0; n < N; ++n) {
+      const int64_t y = __shfl_up(x[n], off);
+      if (lane >= off) x[n] += y;
+    }
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (lane == 63) s_wave[n][wave] = x[n];
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    total[n] = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+      const int64_t v = s_wave[n][w];
+      x[n] += w < wave ? v : 0;
+      total[n] += v;
+    }
   }
-  return x + before;
 }
 
 // The request whose range [at[b], at[b + 1]) holds x (at[0] = 0 <= x < at[n]).
@@ -74,31 +87,20 @@ __device__ __forceinline__ int find(const int *at, int n, int x) {
 
 __device__ __forceinline__ int clamp32(int64_t x) { return (int)(x < INT32_MAX ? x : INT32_MAX); }
 
-__device__ __forceinline__ void place(const Params &p, int t, int start, int cached, bool served, int b) {
-  const int64_t pos = (int64_t)cached + (t - start);
-  int64_t slot = -1;
-  if (served) {  // its pages are inside the table's width
-    const int64_t row = pos / p.page;
-    const int page = p.table[b * p.t_sr + row];
-    if (page >= 0) slot = (int64_t)page * p.page + (pos - row * p.page);
-  }
-  p.slots[t] = slot;
-  p.positions[t] = pos;
-}
-
 __global__ __launch_bounds__(kThreads) void bt_requests(Params p) {
   extern __shared__ int s_mem[];
-  __shared__ int64_t s_wave[kThreads / 64];
+  __shared__ int64_t s_wave[3][kThreads / 64];
   __shared__ int s_taken;
   int *const s_cu = s_mem;                // [batch + 1] token offsets
   int *const s_back = s_cu + p.batch + 1;  // [batch + 1] freed pages
   int *const s_need = s_back + p.batch + 1;
   int *const s_len = s_need + p.batch + 1;  // cached tokens, -1 - cached where not served
   const int tid = threadIdx.x;
+  if (tid == 0) s_taken = 0;
   const int per = (p.batch + kThreads - 1) / kThreads;
   const int count = min(max(*p.count, 0), p.pool);
   int cached[kPerThread], fresh[kPerThread];
-  int64_t tokens = 0, back = 0, total;
+  int64_t tokens = 0, back = 0;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     const int b = tid * per + i;
@@ -107,15 +109,15 @@ __global__ __launch_bounds__(kThreads) void bt_requests(Params p) {
       cached[i] = max(p.cached[b], 0);
       fresh[i] = p.fresh[b];
       tokens += max(fresh[i], 0);
-      if (fresh[i] < 0) back += min((int)(((int64_t)cached[i] + p.page - 1) / p.page), p.width);
+      if (fresh[i] < 0) back += min(pages_of(p, cached[i]), p.width);
     }
   }
-  int64_t token_end = scan(tokens, s_wave, total);
-  const int64_t all_tokens = total;
-  int64_t back_end = scan(back, s_wave, total);
-  const int64_t have = min((int64_t)count + total, (int64_t)p.pool);
+  int64_t ends[2] = {tokens, back}, totals[2];
+  scan<2>(ends, s_wave, totals);
+  const int64_t all_tokens = totals[0];
+  const int64_t have = min((int64_t)count + totals[1], (int64_t)p.pool);
   // offsets, and what each request wants
-  int64_t at = token_end - tokens, bk = back_end - back, need = 0;
+  int64_t at = ends[0] - tokens, bk = ends[1] - back, need = 0;
   int want[kPerThread];
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
@@ -126,24 +128,21 @@ __global__ __launch_bounds__(kThreads) void bt_requests(Params p) {
       s_back[b] = clamp32(bk);
       const int n = max(fresh[i], 0);
       at += n;
-      const int64_t held = ((int64_t)cached[i] + p.page - 1) / p.page;
-      const int64_t all = ((int64_t)cached[i] + n + p.page - 1) / p.page;
-      if (fresh[i] < 0) bk += min(held, (int64_t)p.width);
-      else if (all <= p.width && at <= p.tokens && (int64_t)cached[i] + n <= INT32_MAX) want[i] = (int)(all - held);
+      const int held = pages_of(p, cached[i]), all = pages_of(p, (int)min((int64_t)cached[i] + n, (int64_t)INT32_MAX));
+      if (fresh[i] < 0) bk += min(held, p.width);
+      else if (all <= p.width && at <= p.tokens && (int64_t)cached[i] + n <= INT32_MAX) want[i] = all - held;
       need += max(want[i], 0);
     }
   }
-  int64_t need_total;
-  const int64_t need_end = scan(need, s_wave, need_total);
+  int64_t need_end[1] = {need}, need_total[1];
+  scan<1>(need_end, s_wave + 2, need_total);
   if (tid == 0) {
-    s_taken = 0;
     s_cu[p.batch] = clamp32(all_tokens);
-    s_back[p.batch] = clamp32(total);
-    s_need[p.batch] = clamp32(need_total);
+    s_back[p.batch] = clamp32(totals[1]);
+    s_need[p.batch] = clamp32(need_total[0]);
     p.cu[p.batch] = (int)min(all_tokens, (int64_t)p.tokens);
   }
-  __syncthreads();
-  int64_t taken = need_end - need;
+  int64_t taken = need_end[0] - need;
   int most = 0;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
@@ -160,32 +159,40 @@ __global__ __launch_bounds__(kThreads) void bt_requests(Params p) {
     }
   }
   if (most) atomicMax(&s_taken, most);  // (a maximum has no order)
+  __syncthreads();
   // freed pages onto the stack
   const int freed = s_back[p.batch];
   for (int64_t k = tid; k < freed && count + k < p.pool; k += kThreads) {
     const int b = find(s_back, p.batch, (int)k);
     p.stack[count + k] = p.table[b * p.t_sr + ((int)k - s_back[b])];
   }
-  __syncthreads();
-  // fresh pages from its top
+  if (freed) __syncthreads();
+  // fresh pages from its top; where both are few one half of the workgroup does them and the other the tokens, at the
+  // same time (256 requests of one token 6.8 -> 6.3 us)
   const int used = s_taken;
-  for (int64_t k = tid; k < used; k += kThreads) {
+  const bool halves = p.inline_tokens && max(used, p.tokens) <= kThreads / 2;
+  for (int64_t k = halves && tid >= kThreads / 2 ? used : tid; k < used; k += kThreads) {
     const int b = find(s_need, p.batch, (int)k);
-    const int64_t held = ((int64_t)s_len[b] + p.page - 1) / p.page;  // served: s_len is the cached length
+    const int64_t held = pages_of(p, s_len[b]);  // served: s_len is the cached length
     p.table[b * p.t_sr + held + (k - s_need[b])] = p.stack[have - 1 - k];
   }
   if (tid == 0) *p.count_out = (int)have - used;
   if (!p.inline_tokens) return;
-  __syncthreads();
-  for (int64_t t = tid; t < p.tokens; t += kThreads) {
-    if (t >= all_tokens) {
-      p.slots[t] = -1;
-      p.positions[t] = 0;
-      continue;
+  // (a token's page is one that the request held, or comes from the stack as above: no wait for the table)
+  for (int64_t t = !halves ? tid : tid >= kThreads / 2 ? tid - kThreads / 2 : p.tokens; t < p.tokens; t += kThreads) {
+    int64_t slot = -1, pos = 0;
+    if (t < all_tokens) {
+      const int b = find(s_cu, p.batch, (int)t), len = s_len[b];
+      const int64_t cached = len >= 0 ? len : -1 - len;
+      pos = cached + (t - s_cu[b]);
+      if (len >= 0) {
+        const int64_t row = div_page(p, (uint32_t)pos), held = pages_of(p, len);
+        const int page = row < held ? p.table[b * p.t_sr + row] : p.stack[have - 1 - (s_need[b] + row - held)];
+        if (page >= 0) slot = (int64_t)page * p.page + (pos - row * p.page);
+      }
     }
-    const int b = find(s_cu, p.batch, (int)t);
-    const int len = s_len[b];
-    place(p, (int)t, s_cu[b], len >= 0 ? len : -1 - len, len >= 0, b);
+    p.slots[t] = slot;
+    p.positions[t] = pos;
   }
 }
 
@@ -196,15 +203,18 @@ __global__ __launch_bounds__(256) void bt_tokens(Params p, int per_block) {
   const int64_t first = (int64_t)blockIdx.x * per_block;
   const int64_t end = min(first + per_block, (int64_t)p.tokens);
   for (int64_t t = first + threadIdx.x; t < end; t += 256) {
-    if (t >= s_cu[p.batch]) {
-      p.slots[t] = -1;
-      p.positions[t] = 0;
-      continue;
+    int64_t slot = -1, pos = 0;
+    if (t < s_cu[p.batch]) {
+      const int b = find(s_cu, p.batch, (int)t);
+      const int cached = max(p.cached[b], 0);
+      pos = (int64_t)cached + (t - s_cu[b]);
+      const int64_t row = div_page(p, (uint32_t)pos);
+      // (a request with tokens is served if and only if its length has grown; its pages are in the table)
+      const int page = p.seq_lens[b] != cached ? p.table[b * p.t_sr + row] : -1;
+      if (page >= 0) slot = (int64_t)page * p.page + (pos - row * p.page);
     }
-    const int b = find(s_cu, p.batch, (int)t);
-    const int cached = max(p.cached[b], 0);
-    // (a request with tokens is served if and only if its length has grown)
-    place(p, (int)t, s_cu[b], cached, p.seq_lens[b] != cached, b);
+    p.slots[t] = slot;
+    p.positions[t] = pos;
   }
 }
 
@@ -268,6 +278,8 @@ int32_t l20_pd_block_tables(const l20_pd_block_tables_args *a, void *stream) {
   p.seq_lens = a->seq_lens;
   p.batch = a->batch;
   p.page = a->page_size;
+  // (exact: n / 16 is at most 2^27 + 255, the rounding of the magic below page / 16 <= 2^8)
+  p.magic = (((uint64_t)1 << 38) + p.page / 16 - 1) / (uint64_t)(p.page / 16);
   p.inline_tokens = a->num_slots <= l20bt::kTokensInline;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t lds = (size_t)(4 * (a->batch + 1)) * sizeof(int);  // at most 128 KB
@@ -277,7 +289,7 @@ int32_t l20_pd_block_tables(const l20_pd_block_tables_args *a, void *stream) {
   hipLaunchKernelGGL(l20bt::bt_requests, dim3(1), dim3(l20bt::kThreads), lds, s, p);
   int32_t r = launched();
   if (r != L20_PD_OK || p.inline_tokens) return r;
-  const int per_block = 1024;
+  const int per_block = 256;
   hipLaunchKernelGGL(l20bt::bt_tokens, dim3((unsigned)(((int64_t)p.tokens + per_block - 1) / per_block)), dim3(256),
                      (size_t)(a->batch + 1) * sizeof(int), s, p, per_block);
   return launched();

@@ -17,6 +17,7 @@ The reference has no latent attention, so these names have no counterpart there.
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -39,6 +40,26 @@ def _cache_ok(cache: torch.Tensor, dtype: torch.dtype, rank: int) -> None:
         raise RuntimeError("latent cache must be [pages, page, rank + 64] with rank 256 or 512")
     if cache.dtype not in (torch.float8_e4m3fn, dtype):
         raise RuntimeError("latent cache must be torch.float8_e4m3fn or the model dtype")
+
+
+# (sizes from shapes alone; the calls into the library take longer than a small kernel)
+@lru_cache(maxsize=4096)
+def _paged_bytes(batch: int, q_len: int, heads: int, rank: int, max_seq_len: int, cache_dtype: torch.dtype, cus: int) -> int:
+    import l20_pd_cabi
+
+    a = l20_pd_cabi.L20PdLatentArgs()
+    a.batch, a.q_len, a.num_heads, a.rank, a.max_seq_len = batch, q_len, heads, rank, max_seq_len
+    a.cache_dtype = l20_pd_cabi._kv_code(torch.empty(0, dtype=cache_dtype))
+    return int(l20_pd_cabi.load().l20_pd_paged_latent_workspace(l20_pd_cabi.ctypes.byref(a), cus))
+
+
+@lru_cache(maxsize=4096)
+def _prompt_bytes(total_q: int, heads: int, total_k: int, batch: int, max_q: int, cus: int) -> int:
+    import l20_pd_cabi
+
+    a = l20_pd_cabi.L20PdLatentPromptArgs()
+    a.total_q, a.num_heads, a.total_k, a.batch, a.max_q_len = total_q, heads, total_k, batch, max_q
+    return int(l20_pd_cabi.load().l20_pd_latent_prompt_workspace(l20_pd_cabi.ctypes.byref(a), cus))
 
 
 def l20_latent_rope_and_cache(
@@ -87,12 +108,8 @@ def allocate_l20_paged_latent_workspace(
 ) -> torch.Tensor:
     """The workspace of ``l20_paged_latent_attention`` for this query shape and ``max_seq_len`` (uint8; empty
     where none is needed).  Calls that may overlap each need their own; its contents do not matter."""
-    import l20_pd_cabi
-
-    a = l20_pd_cabi.L20PdLatentArgs()
-    a.batch, a.q_len, a.num_heads = query.shape[0] // q_len, q_len, query.shape[1]
-    a.rank, a.max_seq_len, a.cache_dtype = kv_rank, int(max_seq_len), l20_pd_cabi._kv_code(latent_cache)
-    size = int(l20_pd_cabi.load().l20_pd_paged_latent_workspace(l20_pd_cabi.ctypes.byref(a), gpu_cus(latent_cache.device)))
+    size = _paged_bytes(query.shape[0] // q_len, q_len, query.shape[1], kv_rank, int(max_seq_len), latent_cache.dtype,
+                        gpu_cus(latent_cache.device))
     return torch.empty(size, dtype=torch.uint8, device=latent_cache.device)
 
 
@@ -148,12 +165,7 @@ def allocate_l20_latent_prompt_workspace(
 ) -> torch.Tensor:
     """The workspace of ``l20_latent_prompt_attention`` for these shapes (uint8; empty where the keys are not split).
     Calls that may overlap each need their own; its contents do not matter."""
-    import l20_pd_cabi
-
-    a = l20_pd_cabi.L20PdLatentPromptArgs()
-    a.total_q, a.num_heads, a.total_k = query.shape[0], query.shape[1], key.shape[0]
-    a.batch, a.max_q_len = batch, int(max_seqlen_q)
-    size = int(l20_pd_cabi.load().l20_pd_latent_prompt_workspace(l20_pd_cabi.ctypes.byref(a), gpu_cus(query.device)))
+    size = _prompt_bytes(query.shape[0], query.shape[1], key.shape[0], batch, int(max_seqlen_q), gpu_cus(query.device))
     return torch.empty(size, dtype=torch.uint8, device=query.device)
 
 
@@ -193,7 +205,9 @@ def l20_latent_prompt_attention(
     if softmax_scale is None:
         softmax_scale = (HEAD_DIM + ROPE_DIM) ** -0.5
     if workspace is None and cu_seqlens_q.ndim == 1 and cu_seqlens_q.shape[0] > 1:
-        workspace = allocate_l20_latent_prompt_workspace(query, key, cu_seqlens_q.shape[0] - 1, max_seqlen_q)
+        size = _prompt_bytes(query.shape[0], query.shape[1], key.shape[0], cu_seqlens_q.shape[0] - 1, int(max_seqlen_q),
+                             gpu_cus(query.device))
+        workspace = torch.empty(size, dtype=torch.uint8, device=query.device) if size else None
     return torch.ops.l20_stack.latent_prompt_attention_out(query, key, key_rope, value, cu_seqlens_q, cu_seqlens_k,
                                                            int(max_seqlen_q), output, float(softmax_scale), bool(causal),
                                                            lse, workspace)
