@@ -107,6 +107,12 @@ __device__ __forceinline__ float sum_halves(float x) { return sum_swap<32>(x); }
 __device__ __forceinline__ float max_groups(float x) { return max_swap<32>(max_swap<16>(x)); }  // the four groups of 16
 __device__ __forceinline__ float sum_groups(float x) { return sum_swap<32>(sum_swap<16>(x)); }
 
+// The lane's number, made anew: where registers are short it is not kept.
+__device__ __forceinline__ int lane_id() {
+  int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
 // Lane n's value (n: wave-uniform).
 __device__ __forceinline__ float lane_f(float x, int n) {
   return word_f((unsigned int)__builtin_amdgcn_readlane(__builtin_bit_cast(int, x), n));

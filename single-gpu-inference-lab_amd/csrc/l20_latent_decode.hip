@@ -133,7 +133,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     uint32_t bad;     // bits 4 n .. of buffer n: blocks of its tile without a page
   };
   static __device__ __forceinline__ int blocks_of_window(const DecodeParams &p, int b, int first_block) {
-    return block_of(p, b, first_block + (int)(threadIdx.x & 63));
+    return block_of(p, b, first_block + lane_id());
   }
   static __device__ __forceinline__ int block_of(const DecodeParams &p, int b, int blk) {
     if (blk >= p.table_blocks) return -1;
@@ -148,8 +148,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   static constexpr int kLatLoads = kLatBytes / 1024 / kWaves;  // a wave's instructions of 1 KB
   static constexpr int kRopeLoads = (kRopeBytes / 1024 + kWaves - 1) / kWaves;
   static constexpr int kLoads = kLatLoads + kRopeLoads;
-  static __device__ __forceinline__ void stage(const DecodeParams &p, Shared &s, Fetch &f, int wave, int lane) {
-    asm volatile("" : "+v"(lane));  // (what follows from it is not kept in registers over the tiles)
+  static __device__ __forceinline__ void stage(const DecodeParams &p, Shared &s, Fetch &f, int wave) {
+    const int lane = lane_id();  // (what follows from it is not kept in registers over the tiles)
     const int t0 = f.tile * kTokens;
     if (t0 >> 10 != f.window) {
       f.window = t0 >> 10;
@@ -293,9 +293,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     for (;;) {
       const int tiles = tiles_of(tokens), hi = min(tiles, last - base - kSwitch);
       // (the run of cost x: the last g with floor(g total / runs) <= x)
-      if (p.split && lo == 0 && rblk == 0 && tid == 0)
+      if (p.split && lo == 0 && rblk == 0 && wave == 0 && lane_id() == 0)
         p.runs[b] = i32x2{group, (int)(((uint64_t)(base + kSwitch + tiles) * runs - 1) / (uint32_t)total)};
-      segment(p, s, f, at, b, rblk, group, lo, hi, tiles, tokens, wave, lane);
+      segment(p, s, f, at, b, rblk, group, lo, hi, tiles, tokens, wave);
       base += kSwitch + tiles;
       if (base + kSwitch >= last) return;
       lo = 0;
@@ -326,7 +326,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   // The wave's dims (one a lane) of row (i, h)'s sum of weighted values over tokens first .. last, given its maximum
   // (log2 units): 64 tokens at a time, scores by a lane each.
   static __device__ float exact_row(const DecodeParams &p, int b, int i, int h, int first, int last, int wave, float m) {
-    const int lane = threadIdx.x & 63;
+    const int lane = lane_id();
     const T *q = reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + h * p.q_sh;
     const float use = m == -INFINITY ? 0.0f : m;
     const int dim = wave * (16 * kDimBlocks) + lane % (16 * kDimBlocks);
@@ -367,10 +367,10 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
   };
 
   static __device__ __forceinline__ void segment(const DecodeParams &p, Shared &s, Fetch &f, Place &at, int b, int rblk,
-                                                 int group, int lo, int hi, int tiles, int tokens, int wave, int lane) {
+                                                 int group, int lo, int hi, int tiles, int tokens, int wave) {
     // (what follows from the lane is computed for each sequence: hoisted out of the loop over them it takes 60
     // registers more than there are)
-    asm volatile("" : "+v"(lane));
+    const int lane = lane_id();
     const int n16 = lane & 15, g4 = lane >> 4;
     const int own = wave % RB, tg = wave / RB;  // block of rows, group of tokens of the score product
     const bool scores = kWaves / RB == kGroups || tg < kGroups;
@@ -385,8 +385,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       // that one 16-byte read gives two slices
       if (f.n == 0) {
         landed_and_barrier<0>();  // the query of the run's first sequence is in LDS
-        stage(p, s, f, wave, lane);
-        if (f.more) stage(p, s, f, wave, lane);
+        stage(p, s, f, wave);
+        if (f.more) stage(p, s, f, wave);
 #pragma unroll
         for (int k = 0; k < kSlices; ++k) {
           const int c = KT == 0 ? 8 * (k >> 1) + 2 * g4 + (k & 1) : 4 * k + g4, row = 16 * own + n16;
@@ -541,7 +541,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
       if (f.n - at.n >= 2) landed_and_barrier<kLoads>();
       else landed_and_barrier<0>();
       const int move = PV ? s.rescale[(at.n + 2) % 3] : 0;  // (read early: its latency passes while the loads start)
-      if (f.more) stage(p, s, f, wave, lane);
+      if (f.more) stage(p, s, f, wave);
       if (wave == 0) s.rescale[(at.n + 1) % 3] = 0;
       if constexpr (PV) settle(at.n - 1, move);
       const char *lat = s.lat[at.lat], *rope = s.rope[at.rope];
@@ -786,7 +786,11 @@ struct Plan {
   bool split;
   int64_t workspace;
 };
-constexpr int kWholeTiles = 1;  // sequences of up to this many tiles are not split
+// Sequences of up to this many tiles are not split: a split costs the second kernel and, before the first tile, the
+// sums over the batch.  Measured (bf16, 32-token tiles; split and whole): 16 heads, 4 tiles 1 sequence 11.0 and 10.3 us,
+// 64 sequences 14.4 and 10.6; 8 tiles 12.6 and 15.0, 15.9 and 15.4, 256 sequences 20.6 and 18.0; 16 tiles 64 sequences
+// 19.2 and 24.0; 128 heads, 1 sequence 2 tiles 13.8 and 13.2, 4 tiles 14.6 and 16.6, 64 sequences 8 tiles 33.2 and 24.7.
+int64_t whole_tiles(int64_t batch, int row_blocks) { return batch * row_blocks >= 64 ? 8 : row_blocks == 1 ? 4 : 2; }
 
 Plan plan_of(const l20_pd_latent_args &a, int cus) {
   Plan n{};
@@ -796,7 +800,7 @@ Plan plan_of(const l20_pd_latent_args &a, int cus) {
   n.row_blocks = (int)((rows + block - 1) / block);
   n.tile = a.cache_dtype == L20_PD_KV_FP8_E4M3 ? 64 : 32;
   const int64_t tiles = std::max<int64_t>(1, ((int64_t)a.max_seq_len + n.tile - 1) / n.tile);
-  n.split = tiles > kWholeTiles;
+  n.split = tiles > whole_tiles(a.batch, n.row_blocks);
   if (!n.split) {
     n.groups = (a.batch + 7) / 8 * 8;
     return n;

@@ -418,7 +418,7 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="block table"):
         la.l20_paged_latent_attention(*args[:2], c["table"].long(), c["lens"], **ok)
     with pytest.raises(RuntimeError, match="workspace is too small"):
-        la.l20_paged_latent_attention(*args, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"), **ok)
+        la.l20_paged_latent_attention(*args, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"), max_seq_len=1000, **ok)
     with pytest.raises(RuntimeError, match="same device"):
         la.l20_paged_latent_attention(*args[:3], c["lens"].cpu(), **ok)
     with pytest.raises(RuntimeError, match="softmax_scale"):
