@@ -3,20 +3,31 @@
 // One cache row a token is key (rank + 64 dims) and value (its first rank dims) of every head:
 //   S^T = K Q^T   [tokens x rows],   O^T = V^T P^T   [dims x rows],   rows = (draft row, head).
 //
-//  latent_partial<T, KT, RANK, RB>   16 RB rows of one sequence and a run of its 64-token tiles.  A tile is
-//    staged once in LDS as T (fp8 codes are converted on the way, exactly) and read twice: as the left operand
-//    of K Q^T in 16-byte pieces, and as that of V^T P^T by transposing reads.  The waves split the products
-//    differently: scores by 16-token blocks (and halves of the rows, RB = 4), values by dims, so that each
-//    byte of the value part is read by one wave (two row halves never meet).  Between the two, P goes through
-//    LDS.  Softmax statistics and accumulators are fp32; P is rounded to T for the product (relative error
-//    2^-9 bf16, 2^-12 fp16, as the output's own rounding), its sum is of the unrounded values.
-//    Chunks of 16 bytes are XOR-swizzled by their row so that both kinds of read use all LDS banks.
+//  latent_partial<T, KT, RANK, RB>   16 RB rows of one sequence and a run of its tiles, eight waves, a workgroup a CU.
+//    A tile (64 tokens of an fp8 cache, 32 of a 16-bit one: 36 KB) is copied to LDS as it is and read twice: as the
+//    left operand of K Q^T in 16-byte pieces, and as that of V^T P^T by transposing reads; fp8 codes become T in
+//    registers, exactly.  The waves split the products differently: scores by blocks of 16 tokens and of 16 rows,
+//    values by dims, so that each byte of the value part is read by one wave.  Between the two, P goes through LDS.
+//    Four tiles are in LDS: n - 1, whose value product is interleaved with the scores of n in one stretch between
+//    barriers, and n + 1 and n + 2 on their way, by asynchronous copies that nothing but the wait for their tile
+//    waits for.  The stream of tiles runs on over the sequences of a run.
+//    Softmax statistics and accumulators are fp32; the maximum that P refers to moves only when a row exceeds it by
+//    2^8, so most tiles rescale nothing.  P is rounded to T for the product (relative error 2^-8 bf16, 2^-11 fp16, as
+//    the output's own rounding), its sum is of the unrounded values.
 //
-//  Work: the 64-token tiles of all sequences in a row, cut into equal runs, one a group of workgroups (one
-//    workgroup for each block of rows).  A sequence inside one run is written out at once; what a run has of a
-//    longer one goes to the workspace (slot 2 g: the sequence began in an earlier run, 2 g + 1: it began here).
+//  Work: the tiles of all sequences in a row, a few more for each sequence's start, cut into equal runs, one a group
+//    of workgroups (one workgroup for each block of rows).  A sequence inside one run is written out at once; what a
+//    run has of a longer one goes to the workspace (slot 2 g: the sequence began in an earlier run, 2 g + 1: here).
 //
-//  latent_merge<T, RANK>   joins those parts.
+//  latent_merge<T, RANK, WIDE>   joins those parts.
+//
+// Bounds: with 16 rows the cache's bytes (a stream of equal sequences reaches 6.1 TB/s of either cache), with 64 rows
+// and more the products and the LDS reads that feed them (128 heads: 870 TFLOP/s over fp8, 700 over bf16).  A call
+// has 17 to 25 us besides: launches, the runs, the first query and tile, the parts' way through memory, the join (4 to
+// 9).  Calls: 128 lognormal contexts of 16 heads, bf16 60 us; 2 x 131072 tokens, fp8 40; 32 x 4096, 128 heads, fp8
+// 65.5; 24 ragged contexts of 28 heads x 4 drafts, fp16 53.
+// Measured and not taken: two workgroups of four waves a CU (their tiles are half as far ahead); 128-token tiles in
+// two buffers; the copies of a tile spread between the steps of the products (128 heads 66.9 -> 68.3).
 
 #include "l20_latent_attention.h"
 
@@ -116,7 +127,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     return row * kPRow + ((c ^ (kTokens == 64 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
   }
 
-  // What a run spends on one sequence more, in tiles (its query, its output, the stream's pause).
+  // What a run spends on one sequence more, in tiles (its query, its output, the stream's pause).  Measured, 128
+  // lognormal contexts of 16 heads and 24 ragged ones of 28 heads x 4 drafts: 0 76 and 67 us, 1 68 and 66, 2 67 and
+  // 62, 3 63 and 60, 4 60 and 60, 6 62, 8 63.
   static constexpr int kSwitch = 4;
   // (a sequence without tokens has one tile, all masked: its rows are written too)
   static __device__ __forceinline__ int tiles_of(int tokens) { return max(1, (tokens + kTokens - 1) / kTokens); }
@@ -679,7 +692,9 @@ template <typename T, int KT, int RANK, int RB> __global__ __launch_bounds__(kTh
 // Outputs of sequences that several runs share, from their parts, which lie as the accumulators did: a lane holds
 // row lane % 16 of a block of 16, dims 4 (lane / 16) .. + 3 of a block of 16.  Bound by a chain of loads (runs,
 // maxima and parts), so a call's rows are on the chip at once: with few runs a sequence a wave takes all runs of one
-// row block and RANK / 8 dims; with many (WIDE) a workgroup takes 16 dims, its waves every eighth run.
+// row block and RANK / 8 dims; with many (WIDE, more than eight runs a sequence) a workgroup takes 16 dims, its waves
+// every eighth run: 2 x 131072 tokens (128 runs a sequence) 5.5 us instead of 44.7, 4 x 64-512 tokens 3.5 instead of
+// 7.4; 32 x 4096 tokens of 128 heads (four runs) 16.6 instead of 8.3.
 template <typename T, int RANK, bool WIDE>
 __global__ __launch_bounds__(kThreads) void latent_merge(DecodeParams p, int block_rows) {
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
