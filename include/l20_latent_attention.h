@@ -34,7 +34,8 @@ extern "C" {
  *   cos_sin_cache  [max_position, 64] cs_dtype: 32 cosines, then 32 sines
  *   norm_weight    [rank] dtype, or NULL: the latent is stored as it is
  *   slot_mapping   [num_tokens] int64: page slot / page_size, row slot % page_size; < 0, or beyond the
- *                  cache: the token is not stored (its outputs are written all the same)
+ *                  cache: the token is not stored (its outputs are written all the same).  The slots of a
+ *                  call differ: one that is named twice holds pieces of both rows
  *   cache          [num_pages, page_size, rank + 64] cache_dtype (e4m3fn, or the model dtype)
  *
  *   latent_out = latent * rsqrt(mean(latent^2) + eps) * weight          (fp32, rounded once to dtype)
@@ -89,7 +90,7 @@ int32_t l20_pd_latent_rope_and_cache(const l20_pd_latent_write_args *args, void 
  *                page_size a multiple of 16 through 4096, tokens of a page contiguous above 16
  *                (stride_page = page_size * stride_token)
  *   block_table  [batch, table_pages] int32; seq_lens [batch] int32, the q_len new tokens included
- *   output       [batch*q_len, num_heads, rank] dtype; lse [batch*q_len, num_heads] fp32 natural log
+ *   output       [batch*q_len, num_heads, rank] dtype, not over the query; lse [batch*q_len, num_heads] fp32 natural log
  *                or NULL
  *
  * Row b*q_len+i sees tokens 0 .. seq_lens[b]-q_len+i:
@@ -136,7 +137,7 @@ int32_t l20_pd_paged_latent(const l20_pd_latent_args *args, void *stream);
 /*
  * Attention of packed prompts over expanded keys and values (128 dims a head, 64 shared rotary dims).
  *
- *   query      [total_q, num_heads, 192] dtype; output [total_q, num_heads, 128] dtype
+ *   query      [total_q, num_heads, 192] dtype; output [total_q, num_heads, 128] dtype, not over the query
  *   key, value [total_k, num_heads, 128] dtype; key_rope [total_k, 64] dtype, shared by the heads
  *   cu_q, cu_k [batch + 1] int32: sequence b has query rows cu_q[b] .. cu_q[b+1] and keys
  *              cu_k[b] .. cu_k[b+1]; offsets are clamped to the tensors

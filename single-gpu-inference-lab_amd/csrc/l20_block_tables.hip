@@ -235,6 +235,8 @@ int32_t check(const l20_pd_block_tables_args *a) {
   if ((a->batch > 0 && (!a->cached_lens || !a->new_lens || !a->block_table || !a->seq_lens)) || !a->free_pages ||
       !a->free_count || !a->free_count_out || !a->cu_lens || (a->num_slots > 0 && (!a->slots || !a->positions)))
     return set_error(L20_PD_EINVAL, "null tensor pointer");
+  if (a->batch > 1 && a->bt_stride_row < a->table_pages)
+    return set_error(L20_PD_EINVAL, "block table rows overlap");
   if (a->batch > 0 && (a->seq_lens == a->cached_lens || a->seq_lens == a->new_lens))
     return set_error(L20_PD_EINVAL, "seq_lens must not be cached_lens or new_lens");
   return L20_PD_OK;

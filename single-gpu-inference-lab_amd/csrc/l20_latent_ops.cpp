@@ -43,6 +43,9 @@ int32_t int32(int64_t x, const char *what) {
   return (int32_t)x;
 }
 
+// The stride of a dimension; of one of size 1, whose stride says nothing, what it would be with `inner` per step.
+int64_t step(const at::Tensor &t, int64_t dim, int64_t inner) { return t.size(dim) > 1 ? t.stride(dim) : inner; }
+
 void *stream_of(const at::Tensor &t) {
   return at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream();
 }
@@ -85,25 +88,25 @@ void latent_rope_and_cache(const std::optional<at::Tensor> &query, const at::Ten
     check_device(q, latent);
     check_device(o, latent);
     a.query = q.data_ptr();
-    a.q_stride_token = q.stride(0);
-    a.q_stride_head = q.stride(1);
+    a.q_stride_token = step(q, 0, 0);
+    a.q_stride_head = step(q, 1, 0);
     a.query_out = o.data_ptr();
-    a.qo_stride_token = o.stride(0);
-    a.qo_stride_head = o.stride(1);
+    a.qo_stride_token = step(o, 0, 0);
+    a.qo_stride_head = step(o, 1, 0);
     a.num_heads = int32(q.size(1), "head count");
   }
   a.latent = latent.data_ptr();
-  a.l_stride_token = latent.stride(0);
+  a.l_stride_token = step(latent, 0, 0);
   a.latent_out = latent_out.data_ptr();
-  a.lo_stride_token = latent_out.stride(0);
+  a.lo_stride_token = step(latent_out, 0, 0);
   a.key = key_rope.data_ptr();
-  a.k_stride_token = key_rope.stride(0);
+  a.k_stride_token = step(key_rope, 0, 0);
   a.key_out = key_rope_out.data_ptr();
-  a.ko_stride_token = key_rope_out.stride(0);
+  a.ko_stride_token = step(key_rope_out, 0, 0);
   a.dtype = dtype_code(latent);
   a.positions = positions.data_ptr<int64_t>();
   a.cos_sin_cache = cos_sin_cache.data_ptr();
-  a.cs_stride_position = cos_sin_cache.stride(0);
+  a.cs_stride_position = step(cos_sin_cache, 0, 0);
   a.max_position = cos_sin_cache.size(0);
   a.cs_dtype = dtype_code(cos_sin_cache);
   a.is_neox = is_neox;
@@ -117,7 +120,7 @@ void latent_rope_and_cache(const std::optional<at::Tensor> &query, const at::Ten
   a.norm_eps = (float)norm_eps;
   a.slot_mapping = slot_mapping.data_ptr<int64_t>();
   a.cache = latent_cache.data_ptr();
-  a.c_stride_page = latent_cache.stride(0);
+  a.c_stride_page = step(latent_cache, 0, latent_cache.size(1) * latent_cache.stride(1));
   a.c_stride_token = latent_cache.stride(1);
   a.num_pages = latent_cache.size(0);
   a.page_size = int32(latent_cache.size(1), "page size");
@@ -167,23 +170,23 @@ at::Tensor paged_latent(const at::Tensor &query, const at::Tensor &latent_cache,
     a.workspace_bytes = (int64_t)workspace->nbytes();
   }
   a.query = query.data_ptr();
-  a.q_stride_row = query.stride(0);
-  a.q_stride_head = query.stride(1);
+  a.q_stride_row = step(query, 0, 0);
+  a.q_stride_head = step(query, 1, 0);
   a.dtype = dtype_code(query);
   a.cache = latent_cache.data_ptr();
-  a.c_stride_page = latent_cache.stride(0);
+  a.c_stride_page = step(latent_cache, 0, latent_cache.size(1) * latent_cache.stride(1));
   a.c_stride_token = latent_cache.stride(1);
   a.num_pages = latent_cache.size(0);
   a.page_size = int32(latent_cache.size(1), "page size");
   a.cache_dtype = cache_code(latent_cache);
   a.cache_scale = (float)cache_scale;
   a.block_table = block_table.data_ptr<int32_t>();
-  a.bt_stride_row = block_table.stride(0);
+  a.bt_stride_row = step(block_table, 0, block_table.size(1));
   a.table_pages = int32(block_table.size(1), "block table width");
   a.seq_lens = seq_lens.data_ptr<int32_t>();
   a.output = output.data_ptr();
-  a.o_stride_row = output.stride(0);
-  a.o_stride_head = output.stride(1);
+  a.o_stride_row = step(output, 0, 0);
+  a.o_stride_head = step(output, 1, 0);
   a.softmax_scale = (float)softmax_scale;
   a.batch = int32(batch, "batch");
   a.q_len = int32(q_len, "q_len");
@@ -235,22 +238,22 @@ at::Tensor latent_prompt(const at::Tensor &query, const at::Tensor &key, const a
     a.workspace_bytes = (int64_t)workspace->nbytes();
   }
   a.query = query.data_ptr();
-  a.q_stride_token = query.stride(0);
-  a.q_stride_head = query.stride(1);
+  a.q_stride_token = step(query, 0, 0);
+  a.q_stride_head = step(query, 1, 0);
   a.key = key.data_ptr();
-  a.k_stride_token = key.stride(0);
-  a.k_stride_head = key.stride(1);
+  a.k_stride_token = step(key, 0, 0);
+  a.k_stride_head = step(key, 1, 0);
   a.key_rope = key_rope.data_ptr();
-  a.kr_stride_token = key_rope.stride(0);
+  a.kr_stride_token = step(key_rope, 0, 0);
   a.value = value.data_ptr();
-  a.v_stride_token = value.stride(0);
-  a.v_stride_head = value.stride(1);
+  a.v_stride_token = step(value, 0, 0);
+  a.v_stride_head = step(value, 1, 0);
   a.dtype = dtype_code(query);
   a.cu_q = cu_seqlens_q.data_ptr<int32_t>();
   a.cu_k = cu_seqlens_k.data_ptr<int32_t>();
   a.output = output.data_ptr();
-  a.o_stride_token = output.stride(0);
-  a.o_stride_head = output.stride(1);
+  a.o_stride_token = step(output, 0, 0);
+  a.o_stride_head = step(output, 1, 0);
   a.softmax_scale = (float)softmax_scale;
   a.causal = causal;
   a.total_q = query.size(0);
@@ -295,7 +298,7 @@ void build_block_tables(const at::Tensor &cached_lens, const at::Tensor &new_len
   a.cached_lens = cached_lens.data_ptr<int32_t>();
   a.new_lens = new_lens.data_ptr<int32_t>();
   a.block_table = block_table.data_ptr<int32_t>();
-  a.bt_stride_row = block_table.stride(0);
+  a.bt_stride_row = step(block_table, 0, block_table.size(1));
   a.table_pages = int32(block_table.size(1), "block table width");
   a.free_pages = free_pages.data_ptr<int32_t>();
   a.pool = int32(free_pages.size(0), "page pool");

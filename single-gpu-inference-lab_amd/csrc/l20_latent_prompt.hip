@@ -529,6 +529,7 @@ int32_t check(const l20_pd_latent_prompt_args *a) {
   if (a->batch == 0 || a->total_q == 0 || a->max_q_len == 0) return L20_PD_OK;
   if (!a->query || !a->output || !a->cu_q || !a->cu_k || (a->total_k > 0 && (!a->key || !a->key_rope || !a->value)))
     return set_error(L20_PD_EINVAL, "null tensor pointer");
+  if (a->output == a->query) return set_error(L20_PD_EINVAL, "output must not be the query");
   for (const int64_t stride : {a->k_stride_token, a->v_stride_token, a->kr_stride_token})
     if (stride < 0 || stride >= (1 << 24)) return set_error(L20_PD_EINVAL, "key and value token strides out of range");
   auto u = [](const void *x) { return (uint64_t)(uintptr_t)x; };
@@ -575,8 +576,10 @@ PromptPlan plan_of(const l20_pd_latent_prompt_args &a, int cus) {
   const int64_t units = (int64_t)a.batch * a.num_heads * n.blocks, slots = 2 * cus;  // two workgroups a CU
   const int64_t queries = std::min((a.total_q + a.batch - 1) / a.batch, max_q), keys = a.total_k / a.batch;
   const int64_t blocks = (int64_t)a.batch * a.num_heads * ((queries + l20la::kPromptRows - 1) / l20la::kPromptRows);
-  const int64_t longest = (keys + max_q - queries) / l20la::kKeys, mean = std::max<int64_t>(keys - queries / 2, 0) / l20la::kKeys;
+  const int64_t longest = (keys + max_q - queries) / l20la::kKeys, mean = std::max(keys - queries / 2, keys / 2) / l20la::kKeys;
   if (keys < kSplitTiles * l20la::kKeys || kSplitRatio * blocks * mean > slots * longest) return n;
+  // (very ragged batches: the join's grid goes by the longest sequence)
+  if (units > 16 * slots || (int64_t)a.batch * a.num_heads > 65535) return n;
   n.groups = (int)((slots + 7) / 8 * 8);
   n.part_rows = (int64_t)2 * n.groups * l20la::kPromptRows;
   n.workspace = n.part_rows * (l20la::kDim + 2) * (int64_t)sizeof(float) + units * (int64_t)sizeof(l20la::i32x2);

@@ -165,6 +165,38 @@ def test_decode_nan_of_a_draft_reaches_only_the_rows_that_see_it(fp8, heads, ran
     check_decode(c, out, lse)
 
 
+def test_decode_one_sequence_one_page_of_any_stride():
+    """The stride of a dimension of size 1 says nothing."""
+    c = make_decode([15], 1, seed=32, spare=0)
+    want, want_lse = run_decode(c)
+    check_decode(c, want, want_lse)
+    c["query"] = c["query"].as_strided((1, 1, 576), (7, 5, 1))
+    c["cache"] = c["cache"].as_strided((1, 16, 576), (1, 576, 1))
+    out, lse = run_decode(c, output=torch.empty(512, dtype=torch.bfloat16, device="cuda").as_strided((1, 1, 512), (3, 1, 1)))
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def test_two_decode_calls_at_once():
+    """Two streams, a workspace each: what they give alone."""
+    import l20_latent_attention as la
+
+    cases = [make_decode([3000, 1, 2000, 700], 16, seed=33), make_decode([900] * 6, 40, q_len=2, fp8=True, seed=34)]
+    want = [run_decode(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs, spaces = [torch.empty_like(w[0]) for w in want], []
+    for c in cases:
+        spaces.append(la.allocate_l20_paged_latent_workspace(c["query"], c["cache"], c["table"].shape[1] * 16, q_len=c["q_len"]))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, s, o, ws in zip(cases, streams, outs, spaces):
+            with torch.cuda.stream(s):
+                la.l20_paged_latent_attention(c["query"], c["cache"], c["table"], c["lens"], softmax_scale=SCALE,
+                                              cache_scale=c["cache_scale"], q_len=c["q_len"], output=o, workspace=ws)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w[0])
+
+
 def test_decode_workspace_is_reused_and_calls_repeat_bitwise():
     import l20_latent_attention as la
 

@@ -159,3 +159,58 @@ def test_write_refusals():
         la.l20_latent_rope_and_cache(None, torch.zeros(8, 513, dtype=torch.bfloat16, device="cuda")[:, 1:], key, *rest)
     with pytest.raises(RuntimeError, match="query_out needs query_rope"):
         la.l20_latent_rope_and_cache(None, lat, key, *rest, query_out=c["query"])
+
+
+def test_one_token_of_any_stride():
+    """The stride of a dimension of size 1 says nothing: a transposed column, here."""
+    import l20_latent_attention as la
+
+    c = make(1, 1, seed=12)
+    c["slots"].fill_(3)
+    want = {k: c[k].clone() for k in ("down", "query", "cache")}
+    la.l20_latent_rope_and_cache(want["query"], want["down"][:, :512], want["down"][:, 512:], c["positions"], c["cs"], True,
+                                 want["cache"], c["slots"])
+    down, query = c["down"].as_strided((1, 576), (1, 1)), c["query"].clone().as_strided((1, 1, 64), (1, 3, 1))
+    la.l20_latent_rope_and_cache(query, down[:, :512], down[:, 512:], c["positions"], c["cs"], True, c["cache"], c["slots"])
+    torch.cuda.synchronize()
+    assert torch.equal(down, want["down"]) and torch.equal(query, want["query"]) and torch.equal(c["cache"], want["cache"])
+
+
+def test_on_another_stream_and_in_a_graph():
+    c = make(40, 6, fp8=True, seed=13)
+    outs = {"query_out": torch.empty(40, 6, 64, dtype=torch.bfloat16, device="cuda"),
+            "latent_out": torch.empty(40, 512, dtype=torch.bfloat16, device="cuda"),
+            "key_rope_out": torch.empty(40, 64, dtype=torch.bfloat16, device="cuda")}
+    call(c, True, True, **outs)
+    want = {k: v.clone() for k, v in {**outs, "cache": c["cache"].view(torch.uint8)}.items()}
+    import l20_latent_attention as la
+
+    def step():
+        la.l20_latent_rope_and_cache(c["query"], c["down"][:, :512], c["down"][:, 512:], c["positions"], c["cs"], True,
+                                     c["cache"], c["slots"], norm_weight=c["weight"], norm_eps=EPS, cache_scale=c["scale"], **outs)
+
+    def wiped():
+        for v in outs.values():
+            v.zero_()
+        c["cache"].view(torch.uint8).flatten(0, 1)[c["slots"].clamp_min(0)] = 9
+
+    def same():
+        torch.cuda.synchronize()
+        live = c["slots"][c["slots"] >= 0]
+        return all(torch.equal(v, want[k]) for k, v in outs.items()) and torch.equal(
+            c["cache"].view(torch.uint8).flatten(0, 1)[live], want["cache"].flatten(0, 1)[live])
+
+    side = torch.cuda.Stream()
+    wiped()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert same()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        wiped()
+        graph.replay()
+        assert same()

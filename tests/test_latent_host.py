@@ -55,7 +55,8 @@ def write_args():
 
 def paged_args():
     a = cabi.L20PdLatentArgs()
-    a.query = a.cache = a.block_table = a.seq_lens = a.output = a.workspace = FAKE
+    a.query = a.cache = a.block_table = a.seq_lens = a.workspace = FAKE
+    a.output = 2 * FAKE
     a.q_stride_row, a.q_stride_head, a.dtype = 16 * 576, 576, cabi.L20_PD_BF16
     a.c_stride_page, a.c_stride_token, a.num_pages, a.page_size = 64 * 576, 576, 100, 64
     a.cache_dtype, a.cache_scale = cabi.L20_PD_KV_FP8_E4M3, 0.5
@@ -68,7 +69,8 @@ def paged_args():
 
 def prompt_args():
     a = cabi.L20PdLatentPromptArgs()
-    a.query = a.key = a.key_rope = a.value = a.cu_q = a.cu_k = a.output = FAKE
+    a.query = a.key = a.key_rope = a.value = a.cu_q = a.cu_k = FAKE
+    a.output = 2 * FAKE
     a.q_stride_token, a.q_stride_head = 8 * 192, 192
     a.k_stride_token = a.v_stride_token = 8 * 256
     a.k_stride_head = a.v_stride_head = 256
@@ -176,6 +178,9 @@ BAD = [
     ("block_tables", dict(free_count=0), "null tensor pointer"),
     ("block_tables", dict(slots=0), "null tensor pointer"),
     ("block_tables", dict(seq_lens=FAKE), "seq_lens must not be"),
+    ("block_tables", dict(bt_stride_row=0), "rows overlap"),
+    ("paged_latent", dict(output=FAKE), "must not be the query"),
+    ("latent_prompt", dict(output=FAKE), "must not be the query"),
 ]
 
 
@@ -214,6 +219,9 @@ def test_workspace_sizes():
     p.total_k = 3 * 5000
     assert lib.l20_pd_latent_prompt_workspace(ctypes.byref(p), 256) == 2 * 512 * 128 * 130 * 4 + 3 * 8 * 2 * 8
     p.num_heads = 1 << 12  # blocks of rows enough to fill the chip
+    assert lib.l20_pd_latent_prompt_workspace(ctypes.byref(p), 256) == 0
+    p = prompt_args()  # one long sequence among many: the join's grid would be mostly empty
+    p.batch, p.num_heads, p.max_q_len, p.total_q, p.total_k = 64, 32, 1 << 17, 1 << 17, 1 << 18
     assert lib.l20_pd_latent_prompt_workspace(ctypes.byref(p), 256) == 0
     assert lib.l20_pd_latent_prompt_workspace(None, 256) == 0 and lib.l20_pd_paged_latent_workspace(None, 256) == 0
 
