@@ -80,9 +80,10 @@ __device__ __forceinline__ i32x2 read_tr8(const char *p) {
 }
 
 // What the 16-byte chunks of row `row` are XORed with in an LDS tile whose rows are multiples of 256 bytes (all
-// banks): sixteen rows differ, so a read of one chunk of each meets all banks, and four consecutive rows differ in
-// pairs of chunks, so a transposing read of 32 bytes of each does.  A permutation of the row's bits: linear under XOR.
-__device__ __forceinline__ int spread_row(int row) { return (row & 7) << 1 | (row >> 3 & 1); }
+// banks): sixteen rows differ, so a read of one chunk of each meets all banks; four consecutive rows differ in fours
+// of chunks and rows eight apart in pairs, so 32 lanes of a transposing read meet all banks too, whether they take 64
+// bytes of each of four rows or 32 of rows 0 .. 3 and 8 .. 11.  A permutation of the row's bits: linear under XOR.
+__device__ __forceinline__ int spread_row(int row) { return (row & 3) << 2 | (row >> 3 & 1) << 1 | (row >> 2 & 1); }
 
 // Reductions by the row swaps of the vector ALU (no LDS round trip): with both operands the same register a
 // swap returns a lane's value and that of the lane 16 (32) away, in one order for both of them.

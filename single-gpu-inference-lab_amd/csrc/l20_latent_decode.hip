@@ -489,9 +489,9 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         const i32x2 w = read_tr8(lat + ks * 32 * kLatRow + (v_at ^ (d << 4)));
         return i32x4{w[0], w[1], 0, 0};
       } else {
-        // (four rows on, the swizzle differs in chunk bit 3)
+        // (four rows on, the swizzle differs by that of row 4)
         const i32x2 lo = read_tr(lat + ks * 32 * kLatRow + (v_at ^ (d << 5)));
-        const i32x2 hi = read_tr(lat + (ks * 32 + 4) * kLatRow + (v_at ^ (d << 5) ^ 128));
+        const i32x2 hi = read_tr(lat + (ks * 32 + 4) * kLatRow + (v_at ^ (d << 5) ^ (spread_row(4) << 4)));
         return i32x4{lo[0], lo[1], hi[0], hi[1]};
       }
     };
