@@ -80,6 +80,9 @@ __device__ __forceinline__ uint32_t scaled(uint32_t a, uint32_t b, uint32_t c) {
   return n >> 32 ? (uint32_t)(n / c) : (uint32_t)n / c;
 }
 
+// The draft of a row (without drafts no division).
+__device__ __forceinline__ int draft_of(const DecodeParams &p, int row) { return p.q_len == 1 ? 0 : row / p.heads; }
+
 // Four fp8 codes (one dword) -> two dwords of T, exact.  (Whole words: extracting elements of these
 // conversions' results one by one is miscompiled by the ROCm 7.2 LLVM.)
 template <typename T> __device__ __forceinline__ i32x2 fp8x4(int w);
@@ -323,7 +326,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     constexpr int kRow = RANK * 2, kLoadsQ = kRows * kRow / 1024 / kWaves, kRopeQ = kRows * kRope * 2 / 1024;
     static_assert(sizeof(s.lat[0]) * 2 >= kRows * kRow && sizeof(s.p) >= kRows * kRope * 2, "the buffers hold the rows");
     auto row_of = [&](int row) {
-      const int r = min(rblk * kRows + row, p.rows - 1), i = r / p.heads;
+      const int r = min(rblk * kRows + row, p.rows - 1), i = draft_of(p, r);
       return reinterpret_cast<const T *>(p.q) + ((int64_t)b * p.q_len + i) * p.q_sr + (r - i * p.heads) * p.q_sh;
     };
     const uint32_t lat = lds_address(s.lat[2]), rope = lds_address(s.p[0]);
@@ -392,7 +395,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     int lim;
     {
       // (rows past the last repeat it: they are not stored)
-      const int r = min(rblk * kRows + 16 * own + n16, p.rows - 1), i = r / p.heads;
+      const int r = min(rblk * kRows + 16 * own + n16, p.rows - 1), i = draft_of(p, r);
       lim = min(len - p.q_len + i, tokens - 1);
       // the order of the dims in the product is free: over an fp8 cache a lane's are 16 in a row of each 64, so
       // that one 16-byte read gives two slices
@@ -669,7 +672,7 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         continue;
       }
       if (row >= p.rows) continue;
-      const int i = row / p.heads, h = row - i * p.heads;
+      const int i = draft_of(p, row), h = row - i * p.heads;
       const int64_t orow = (int64_t)b * p.q_len + i;
       const float inv = l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
       T *dst = reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + 4 * g4;
@@ -774,7 +777,7 @@ __global__ __launch_bounds__(kThreads) void latent_merge(DecodeParams p, int blo
   }
   const int row = 16 * row16 + n16;
   if (row >= p.rows) return;
-  const int i = row / p.heads, h = row - i * p.heads;
+  const int i = draft_of(p, row), h = row - i * p.heads;
   const int64_t orow = (int64_t)b * p.q_len + i;
   const float inv = l > 0.0f ? p.out_scale / l : (l == 0.0f ? 0.0f : l);  // a NaN sum stays NaN
   T *dst = reinterpret_cast<T *>(p.out) + orow * p.o_sr + h * p.o_sh + 4 * g4;
@@ -794,8 +797,7 @@ using l20pd_host::set_error;
 
 int64_t rows_of(const l20_pd_latent_args &a) { return (int64_t)a.q_len * a.num_heads; }
 
-// How a call is cut: blocks of 16 rows a workgroup takes (as many as the sequence has, up to four), tokens of a
-// tile, runs of tiles.
+// How a call is cut: blocks of 16 rows a workgroup takes, tokens of a tile, runs of tiles.
 struct Plan {
   int row_blocks16, row_blocks, tile, groups;
   bool split;
@@ -805,17 +807,29 @@ struct Plan {
 // sums over the batch.  Measured (bf16, 32-token tiles; split and whole): 16 heads, 4 tiles 1 sequence 11.0 and 10.3 us,
 // 64 sequences 14.4 and 10.6; 8 tiles 12.6 and 15.0, 15.9 and 15.4, 256 sequences 20.6 and 18.0; 16 tiles 64 sequences
 // 19.2 and 24.0; 128 heads, 1 sequence 2 tiles 13.8 and 13.2, 4 tiles 14.6 and 16.6, 64 sequences 8 tiles 33.2 and 24.7.
-int64_t whole_tiles(int64_t batch, int row_blocks) { return batch * row_blocks >= 64 ? 8 : row_blocks == 1 ? 4 : 2; }
+int64_t whole_tiles(int64_t batch, int row_blocks16, int row_blocks) {
+  return batch * row_blocks >= 64 ? 8 : row_blocks16 == 1 ? 4 : 2;
+}
+// Blocks of 16 rows a workgroup: as many as the sequence has, up to four, for long work (each tile is read from the
+// cache once for them all), but where the blocks of 16 (32) rows fit the CUs and have few tiles a CU, one (two): a
+// workgroup of 64 rows takes 4.6 us longer from launch to its first result than one of 16.  Measured (bf16; blocks
+// 1, 2 and 4, with their tiles of 16 rows a CU): 128 heads, 8 x 128 tokens (1) 10.4, 14.8 and 16.9 us, 8 x 1024 (8)
+// 23.5, 24.1 and 27.4, 8 x 2048 (16) 32.8, 28.1 and 29.1, 8 x 4096 (32) 50.8, 37.4 and 34.9, 32 x 4096 (128) 160, 97
+// and 73; 64 heads, 128 x 512 (32; 512 blocks of 16 rows) 50.3, 32.0 and 39.8, 128 x 32 (2) 13.2, 9.5 and 12.5.
+constexpr int64_t kFewTiles1 = 8, kFewTiles2 = 32;
 
 Plan plan_of(const l20_pd_latent_args &a, int cus) {
   Plan n{};
   const int64_t rows = rows_of(a);
-  n.row_blocks16 = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int64_t block = 16 * n.row_blocks16;
-  n.row_blocks = (int)((rows + block - 1) / block);
   n.tile = a.cache_dtype == L20_PD_KV_FP8_E4M3 ? 64 : 32;
   const int64_t tiles = std::max<int64_t>(1, ((int64_t)a.max_seq_len + n.tile - 1) / n.tile);
-  n.split = tiles > whole_tiles(a.batch, n.row_blocks);
+  const int64_t units16 = a.batch * ((rows + 15) / 16), units32 = a.batch * ((rows + 31) / 32);
+  n.row_blocks16 = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  if (units16 <= cus && units16 * tiles <= kFewTiles1 * cus) n.row_blocks16 = 1;
+  else if (units32 <= cus && units16 * tiles <= kFewTiles2 * cus) n.row_blocks16 = std::min(n.row_blocks16, 2);
+  const int64_t block = 16 * n.row_blocks16;
+  n.row_blocks = (int)((rows + block - 1) / block);
+  n.split = tiles > whole_tiles(a.batch, n.row_blocks16, n.row_blocks);
   if (!n.split) {
     n.groups = (a.batch + 7) / 8 * 8;
     return n;

@@ -78,16 +78,30 @@ DECODE = [
 @pytest.mark.parametrize("spec", DECODE, ids=[f"{len(s[0])}x{max(s[0])}_h{s[1]}_q{s[2]}_r{s[3]}_p{s[4]}" for s in DECODE])
 @pytest.mark.parametrize("dtype,fp8", [(torch.bfloat16, False), (torch.float16, False), (torch.bfloat16, True),
                                        (torch.float16, True)], ids=["bf16", "fp16", "bf16_e4m3", "fp16_e4m3"])
-def test_decode_against_float64(spec, dtype, fp8):
+@pytest.mark.parametrize("rows", [16, 32, 64], ids=["rows16", "rows32", "rows64"])
+def test_decode_against_float64(spec, dtype, fp8, rows):
+    """The bound on the lengths says how much work there may be, and so how many rows a workgroup takes."""
     lens, heads, q_len, rank, page = spec
     c = make_decode(lens, heads, q_len, rank, dtype, fp8, page, seed=sum(lens) + heads)
-    check_decode(c, *run_decode(c))
+    units = len(lens) * -(-heads * q_len // 16)
+    tiles = {16: 0, 32: 5000, 64: 20000}[rows] // units
+    check_decode(c, *run_decode(c, max_seq_len=max(c["table"].shape[1] * page, tiles * (64 if fp8 else 32))))
 
 
 def test_decode_many_short_sequences_share_runs():
     """More sequences than runs: whole ones, and ones cut at a run's end, of every length about a tile."""
     lens = [(37 * i) % 200 for i in range(600)]
     c = make_decode(lens, 16, rank=256, seed=5)
+    check_decode(c, *run_decode(c))
+    check_decode(c, *run_decode(c, max_seq_len=1000))
+
+
+@pytest.mark.parametrize("heads,q_len,batch", [(64, 1, 300), (16, 2, 270), (30, 3, 90)], ids=["64", "2x16", "3x30"])
+@pytest.mark.parametrize("fp8", [True, False], ids=["e4m3", "model"])
+def test_decode_many_short_sequences_whole(heads, q_len, batch, fp8):
+    """Workgroups of 64 and 32 rows that take a sequence each."""
+    lens = [(13 * i) % 90 for i in range(batch)]
+    c = make_decode(lens, heads, q_len, fp8=fp8, seed=35)
     check_decode(c, *run_decode(c))
 
 
@@ -147,15 +161,16 @@ def test_decode_nan_in_one_sequence_stays_there():
 @pytest.mark.parametrize("fp8", [True, False], ids=["e4m3", "model"])
 @pytest.mark.parametrize("heads", [5, 16, 40])
 @pytest.mark.parametrize("rank", [512, 256])
-def test_decode_nan_of_a_draft_reaches_only_the_rows_that_see_it(fp8, heads, rank):
+@pytest.mark.parametrize("bound", [None, 100000], ids=["few", "long"])
+def test_decode_nan_of_a_draft_reaches_only_the_rows_that_see_it(fp8, heads, rank, bound):
     """The last, and the second last, token of two sequences hold NaN; the rows before them are as without."""
     q_len = 3
     c = make_decode([70, 2, 129, 900, 64], heads, q_len=q_len, rank=rank, fp8=fp8, seed=31, poison=False)
-    clean, clean_lse = run_decode(c)
+    clean, clean_lse = run_decode(c, max_seq_len=bound)
     kept = c["cache"].clone()
     for b, t in ((0, 69), (2, 127), (3, 899), (4, 63)):
         c["cache"][c["table"][b, t // 16].long(), t % 16] = float("nan")
-    out, lse = run_decode(c)
+    out, lse = run_decode(c, max_seq_len=bound)
     c["cache"] = kept
     seen = torch.zeros(5, q_len, dtype=torch.bool, device="cuda")
     seen[[0, 2, 2, 3, 4], [2, 1, 2, 2, 2]] = True

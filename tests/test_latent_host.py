@@ -210,7 +210,9 @@ def test_nothing_to_do_needs_no_pointers():
 def test_workspace_sizes():
     """Two parts a run and row block, each RANK + 2 floats a row, and the runs of a sequence."""
     lib = cabi.load()
-    a = paged_args()  # 2 x 16 rows: one block of 32; 8 x 40 tiles of 64 tokens on 256 CUs
+    a = paged_args()  # 2 x 16 rows, 8 x 40 tiles of 64 tokens on 256 CUs: 128 runs for each of two blocks of 16 rows
+    assert lib.l20_pd_paged_latent_workspace(ctypes.byref(a), 256) == 2 * 128 * 32 * 514 * 4 + 8 * 8
+    a.max_seq_len = 1 << 20  # long work: 256 runs, 32 rows together
     assert lib.l20_pd_paged_latent_workspace(ctypes.byref(a), 256) == 2 * 256 * 32 * 514 * 4 + 8 * 8
     a.max_seq_len = 64  # one tile a sequence: not split
     assert lib.l20_pd_paged_latent_workspace(ctypes.byref(a), 256) == 0
