@@ -507,11 +507,12 @@ namespace {
 using l20pd_host::set_error;
 
 // The keys are split where the longest block of rows takes more than kSplitRatio times what a workgroup's even share
-// of all tiles is (by the mean lengths, which the host knows), and sequences have kSplitTiles tiles or more.  Measured
-// (bf16, whole -> split): 300 queries on 5000 keys, 28 heads 107 -> 52 us, 8 heads 106 -> 33; 4 x 64 on 8064, 16 heads
-// 168 -> 61; 4096 tokens, 8 heads 95 -> 69, 16 heads (ratio 1.9) 109 -> 112, 32 heads (1.0) 181 -> 205; of few tiles
-// 1000 tokens, 16 heads (16 tiles) 26 -> 30, 2048 tokens, 16 heads (32 tiles) 48 -> 48.
-constexpr int kSplitRatio = 2, kSplitTiles = 24;
+// of all tiles is, and kSplitTiles tiles or more (by the mean lengths and the longest prompt, which the host knows).
+// Measured (bf16, whole -> split): 300 queries on 5000 keys, 28 heads 107 -> 52 us, 8 heads 106 -> 33; 4 x 64 on 8064,
+// 16 heads 168 -> 61; 1594 and 531 tokens, 8 heads 39 -> 31; 4 x 200 on 1200, 8 heads (19 tiles) 31 -> 28; 4096 tokens,
+// 8 heads 95 -> 69, 16 heads (ratio 1.9) 109 -> 112, 32 heads (1.0) 181 -> 205; of few tiles 1000 tokens, 16 heads (16)
+// 27 -> 32, 2 x 700, 8 heads (11) 20 -> 27.
+constexpr int kSplitRatio = 2, kSplitTiles = 18;
 
 int32_t check(const l20_pd_latent_prompt_args *a) {
   if (!a) return set_error(L20_PD_EINVAL, "null argument block");
@@ -579,7 +580,7 @@ PromptPlan plan_of(const l20_pd_latent_prompt_args &a, int cus) {
   const int64_t queries = std::min((a.total_q + a.batch - 1) / a.batch, max_q), keys = a.total_k / a.batch;
   const int64_t blocks = (int64_t)a.batch * a.num_heads * ((queries + l20la::kPromptRows - 1) / l20la::kPromptRows);
   const int64_t longest = (keys + max_q - queries) / l20la::kKeys, mean = std::max(keys - queries / 2, keys / 2) / l20la::kKeys;
-  if (keys < kSplitTiles * l20la::kKeys || kSplitRatio * blocks * mean > slots * longest) return n;
+  if (keys < l20la::kKeys || longest < kSplitTiles || kSplitRatio * blocks * mean > slots * longest) return n;
   // (very ragged batches: the join's grid goes by the longest sequence)
   if (units > 16 * slots || (int64_t)a.batch * a.num_heads > 65535) return n;
   n.groups = (int)((slots + 7) / 8 * 8);
