@@ -364,7 +364,9 @@ template <typename T> __global__ __launch_bounds__(64 * kPromptWaves, 2) void la
 
 // ---- the keys split over runs ----
 // What a run spends on one block of rows more, in tiles (its query, its output, the pipeline's start), and the tiles
-// a run has at the least.
+// a run has at the least.  Measured: a switch of 0, 2 and 4 tiles, four ragged prompts of 100 to 2000 tokens, 16 heads
+// 77, 67 and 66 us, 1594 and 531 tokens, 8 heads 36, 30 and 31, one of 3000 among 20 short ones 122, 120 and 125; runs
+// of 4, 8 and 12 tiles and more, 300 queries on 5000 keys, 8 heads 33, 39 and 47.
 constexpr int kPromptSwitch = 2, kRunTiles = 4;
 
 // The tiles and switches of one head of a sequence, and of one block of rows.
