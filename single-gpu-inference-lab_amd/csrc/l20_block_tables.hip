@@ -286,7 +286,8 @@ int32_t l20_pd_block_tables(const l20_pd_block_tables_args *a, void *stream) {
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t lds = (size_t)(4 * (a->batch + 1)) * sizeof(int);  // at most 128 KB
   static l20la::LdsLimit limit;
-  const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20bt::bt_requests), 4 * (L20_PD_MAX_REQUESTS + 1) * (int)sizeof(int));
+  const int most = 4 * (L20_PD_MAX_REQUESTS + 1) * (int)sizeof(int);
+  const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20bt::bt_requests), most);
   if (e != hipSuccess) return set_error(L20_PD_ELAUNCH, hipGetErrorString(e));
   hipLaunchKernelGGL(l20bt::bt_requests, dim3(1), dim3(l20bt::kThreads), lds, s, p);
   int32_t r = launched();

@@ -872,7 +872,8 @@ int32_t check(const l20_pd_latent_args *a) {
   if (!a->query || !a->cache || !a->block_table || !a->seq_lens || !a->output)
     return set_error(L20_PD_EINVAL, "null tensor pointer");
   if (a->output == a->query) return set_error(L20_PD_EINVAL, "output must not be the query");
-  if (a->c_stride_token < 0 || a->c_stride_token >= (1 << 26)) return set_error(L20_PD_EINVAL, "latent cache token stride out of range");
+  if (a->c_stride_token < 0 || a->c_stride_token >= (1 << 26))
+    return set_error(L20_PD_EINVAL, "latent cache token stride out of range");
   auto u = [](const void *x) { return (uint64_t)(uintptr_t)x; };
   if ((u(a->query) | (uint64_t)(2 * a->q_stride_row) | (uint64_t)(2 * a->q_stride_head)) % 16)
     return set_error(L20_PD_EINVAL, "query rows must be 16-byte aligned");

@@ -113,7 +113,8 @@ __device__ f32x2 exact_row(const PromptParams &p, int h, int64_t row, int64_t ks
     const T *k = reinterpret_cast<const T *>(p.k) + j * p.k_st + h * p.k_sh, *kr = reinterpret_cast<const T *>(p.kr) + j * p.kr_st;
     float s = 0.0f;
     for (int c = 0; c < kDim + kRope; c += 8) {
-      const i32x4 kw = *reinterpret_cast<const i32x4 *>(c < kDim ? k + c : kr + (c - kDim)), qw = *reinterpret_cast<const i32x4 *>(q + c);
+      const i32x4 kw = *reinterpret_cast<const i32x4 *>(c < kDim ? k + c : kr + (c - kDim));
+      const i32x4 qw = *reinterpret_cast<const i32x4 *>(q + c);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s = dot2<T>(kw[e], qw[e], s);
     }

@@ -81,11 +81,11 @@ def l20_latent_rope_and_cache(
 ) -> None:
     """Norm (with ``norm_weight``) and RoPE of new tokens, and their rows into the paged cache.
 
-    ``query_rope`` [tokens, heads, 64] (or None), ``latent`` [tokens, rank] and ``key_rope`` [tokens, 64] are
-    views of any row stride; each result goes to its ``_out`` tensor, or in place where none is given.  A
-    ``query_out`` that is the last 64 dims of the absorbed query saves the copy there.  ``slot_mapping`` below 0
-    or beyond the cache: the token is not stored; two tokens of a call must not name one slot.  An fp8 cache stores ``clamp(x / cache_scale)`` of the rounded
-    results."""
+    ``query_rope`` [tokens, heads, 64] (or None), ``latent`` [tokens, rank] and ``key_rope`` [tokens, 64] are views
+    of any row stride; each result goes to its ``_out`` tensor, or in place where none is given. A ``query_out``
+    that is the last 64 dims of the absorbed query saves the copy there. ``slot_mapping`` below 0 or beyond the
+    cache: the token is not stored; two tokens of a call must not name one slot. An fp8 cache stores ``clamp(x /
+    cache_scale)`` of the rounded results."""
     _need_gpu("l20_latent_rope_and_cache", latent)
     # (shapes and strides are checked by the op: a second time here they would take as long as the kernel)
     if latent.dtype not in (torch.float16, torch.bfloat16):
@@ -131,11 +131,11 @@ def l20_paged_latent_attention(
     """Attention of ``query`` [batch * q_len, heads, kv_rank + 64] over a paged latent cache; returns ``output``
     [batch * q_len, heads, kv_rank], to which the model applies its value up-projection.
 
-    Row b * q_len + i sees the first ``seq_lens[b] - q_len + i + 1`` tokens of sequence b; one that sees none
-    gives zeros (``lse``: -inf).  ``output`` must not lie over ``query``.  ``softmax_scale`` is the model's (its head dims before the absorption, not
-    ``kv_rank``, set it).  ``max_seq_len`` bounds the lengths (default: what the block table can name) and sizes
-    grid and workspace; tokens beyond it, the table, or on a page outside the cache are masked.  With ``output``
-    and ``workspace`` given nothing is allocated and the call can be captured in a graph."""
+    Row b * q_len + i sees the first ``seq_lens[b] - q_len + i + 1`` tokens of sequence b; one that sees none gives
+    zeros (``lse``: -inf). ``output`` must not lie over ``query``. ``softmax_scale`` is the model's (its head dims
+    before the absorption, not ``kv_rank``, set it). ``max_seq_len`` bounds the lengths (default: what the block
+    table can name) and sizes grid and workspace; tokens beyond it, the table, or on a page outside the cache are
+    masked. With ``output`` and ``workspace`` given nothing is allocated and the call can be captured in a graph."""
     _need_gpu("l20_paged_latent_attention", query)
     if query.ndim != 3 or query.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("expected an FP16 or BF16 query [batch * q_len, heads, kv_rank + 64]")

@@ -249,7 +249,8 @@ def test_fake_implementations_keep_shapes():
     import l20_latent_attention  # noqa: F401
 
     with FakeTensorMode():
-        q, cache = torch.empty(8, 16, 576, dtype=torch.bfloat16, device="cuda"), torch.empty(9, 16, 576, dtype=torch.bfloat16, device="cuda")
+        q = torch.empty(8, 16, 576, dtype=torch.bfloat16, device="cuda")
+        cache = torch.empty(9, 16, 576, dtype=torch.bfloat16, device="cuda")
         out, i = torch.empty(8, 16, 512, dtype=torch.bfloat16, device="cuda"), torch.empty(8, dtype=torch.int32, device="cuda")
         got = torch.ops.l20_stack.paged_latent_attention_out(q, cache, i.view(8, 1), i, out, None, 1.0, 1.0, 16)
         assert got.shape == out.shape
