@@ -26,6 +26,23 @@ constexpr int kPerThread = L20_PD_MAX_REQUESTS / kThreads;
 // against two: 2048 tokens 7.4 and 8.7 us, 4096 tokens 11.3 and 11.2, 8192 tokens 15.6 and 11.4.
 constexpr int kTokensInline = 4096;
 
+// n / page without a division (a good hundred instructions at 64 bits, some thirty at 32), for n through
+// 2^31 + 4094, the largest length rounded up by the largest page: n / 16 is below 2^27 + 256 and the magic at most
+// 2^36, so their product is below 2^64, and the magic's rounding, below page / 16 <= 2^8, adds less than one step.
+constexpr uint64_t page_magic(uint32_t page) { return (((uint64_t)1 << 36) + page / 16 - 1) / (page / 16); }
+__host__ __device__ constexpr uint32_t div_magic(uint32_t n, uint64_t magic) { return (uint32_t)((uint64_t)(n >> 4) * magic >> 36); }
+// The ends of the first, a middle and the last multiples of every page size.
+constexpr bool divides_right() {
+  for (uint32_t page = 16; page <= 4096; page += 16)
+    for (uint32_t top : {page, (uint32_t)1 << 30, ((uint32_t)1 << 30) + page, (uint32_t)INT32_MAX, (uint32_t)INT32_MAX + page - 1}) {
+      const uint32_t at = top / page * page;
+      for (uint32_t n : {at - 1, at, at + 1, top})
+        if (div_magic(n, page_magic(page)) != n / page) return false;
+    }
+  return true;
+}
+static_assert(divides_right(), "the division by the page size");
+
 struct Params {
   const int32_t *cached, *fresh;
   int32_t *table;
@@ -39,12 +56,11 @@ struct Params {
   int tokens;
   int32_t *cu, *seq_lens;
   int batch, page;
-  uint64_t magic;  // (n / 16) * magic >> 38 = n / page
+  uint64_t magic;  // division by the page size
   int inline_tokens;
 };
 
-// n / page, for n through 2^31 + 4095 (a division takes a good hundred instructions at 64 bits, some thirty at 32).
-__device__ __forceinline__ uint32_t div_page(const Params &p, uint32_t n) { return (uint32_t)((uint64_t)(n >> 4) * p.magic >> 38); }
+__device__ __forceinline__ uint32_t div_page(const Params &p, uint32_t n) { return div_magic(n, p.magic); }
 // The pages of n tokens.
 __device__ __forceinline__ int pages_of(const Params &p, int n) { return (int)div_page(p, (uint32_t)n + (uint32_t)p.page - 1); }
 
@@ -280,8 +296,7 @@ int32_t l20_pd_block_tables(const l20_pd_block_tables_args *a, void *stream) {
   p.seq_lens = a->seq_lens;
   p.batch = a->batch;
   p.page = a->page_size;
-  // (exact: n / 16 is at most 2^27 + 255, the rounding of the magic below page / 16 <= 2^8)
-  p.magic = (((uint64_t)1 << 38) + p.page / 16 - 1) / (uint64_t)(p.page / 16);
+  p.magic = l20bt::page_magic((uint32_t)p.page);
   p.inline_tokens = a->num_slots <= l20bt::kTokensInline;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t lds = (size_t)(4 * (a->batch + 1)) * sizeof(int);  // at most 128 KB

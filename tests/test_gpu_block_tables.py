@@ -184,3 +184,22 @@ def test_refusals():
     bad("must not be cached_lens", a8=d["cached"])
     bad("same device", a4=count.cpu())
     bad("at most 8192", a0=t32([0] * 9000))
+
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 4096])
+@pytest.mark.parametrize("tokens", [40, 5000], ids=["one", "two"])
+def test_lengths_up_to_the_largest(page, tokens):
+    """Cached lengths around 2^30 and up to 2^31 - 1 exceed every row: such requests are not served and take no page,
+    finished ones give back the pages their rows have, and the others are as without them."""
+    large = [2 ** 30 - 2 * page, 2 ** 30 - page, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 5, 2 ** 30 + page, 2 ** 31 - 2 * page, 2 ** 31 - 2, 2 ** 31 - 1]
+    cached, new = [], []
+    for n in large:
+        cached += [n, n, n, 5]
+        new += [1, -1, 0, page]
+    rows = len(cached)
+    free = list(range(4 * rows, 4 * rows + 3 * rows))
+    table = [[4 * b + k for k in range(4)] for b in range(rows)]
+    c = {"cached": cached, "new": new, "table": table, "free": free + [-5] * (4 * rows), "count": len(free), "page": page}
+    assert sum(max(n, 0) for n in new) >= 40
+    want = check(c, tokens)
+    assert [want["seq_lens"][b] for b in (0, 1, 2)] == [large[0], 0, large[0]]
