@@ -41,7 +41,8 @@ extern "C" {
  *   latent_out = latent * rsqrt(mean(latent^2) + eps) * weight          (fp32, rounded once to dtype)
  *   part_out   = x cos + (x_pair sin) sign                              (fp32, rounded once to dtype),
  *                pairs (d, d + 32) with is_neox, (2 i, 2 i + 1) without
- *   cache row  = [latent_out | key_out], in an fp8 cache RNE_e4m3fn(clamp(. / cache_scale, +-448))
+ *   cache row  = [latent_out | key_out], in an fp8 cache RNE_e4m3fn(clamp(. / cache_scale, +-448)),
+ *                NaN for NaN
  */
 typedef struct l20_pd_latent_write_args {
   const void *query;

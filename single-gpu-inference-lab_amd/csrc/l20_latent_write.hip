@@ -85,11 +85,12 @@ template <int CS, int N> __device__ __forceinline__ void load_cs(const void *bas
   }
 }
 
-// Eight values -> eight e4m3fn codes: RNE of clamp(x / scale).
+// Eight values -> eight e4m3fn codes: RNE of clamp(x / scale), NaN for NaN (which fminf and fmaxf drop; these do not).
 __device__ __forceinline__ i32x2 quant8(const float (&x)[8], float scale) {
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fminf(fmaxf(__fdiv_rn(x[i], scale), -kFp8Max), kFp8Max);
+  for (int i = 0; i < 8; ++i)
+    y[i] = __builtin_elementwise_minimum(__builtin_elementwise_maximum(__fdiv_rn(x[i], scale), -kFp8Max), kFp8Max);
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
   int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);

@@ -214,3 +214,28 @@ def test_on_another_stream_and_in_a_graph():
         wiped()
         graph.replay()
         assert same()
+
+
+@pytest.mark.parametrize("norm", [True, False], ids=["norm", "plain"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("fp8", [True, False], ids=["e4m3", "model"])
+def test_values_that_are_not_finite(norm, dtype, fp8):
+    """The cache holds what the outputs hold: a NaN stays one in an fp8 cache too, an infinity becomes its largest value."""
+    c = make(30, 3, dtype=dtype, cs_dtype=torch.float32, fp8=fp8, seed=14)
+    nan, inf = float("nan"), float("inf")
+    for t, col, x in ((1, 5, nan), (2, 7, inf), (3, 9, -inf), (4, 512 + 3, nan), (5, 512 + 40, inf), (6, 0, -nan), (6, 1, inf),
+                      (8, 511, nan), (8, 512 + 63, -inf)):
+        c["down"][t, col] = x
+    outs = {"query_out": torch.empty_like(c["query"]), "latent_out": torch.empty(30, 512, dtype=dtype, device="cuda"),
+            "key_rope_out": torch.empty(30, 64, dtype=dtype, device="cuda")}
+    before = c["cache"].clone()
+    call(c, True, norm, **outs)
+    key = rope(c["down"][:, 512:], c["cs"], c["positions"], True)
+    assert torch.equal(key.isnan(), outs["key_rope_out"].isnan())
+    assert torch.equal(key.nan_to_num(9.0), outs["key_rope_out"].nan_to_num(9.0))
+    rows = outs["latent_out"].isnan()
+    assert bool(rows[1, 5]) and bool(rows[6, 0]) and bool(rows[8, 511]) and bool(rows[1].all()) == norm
+    got, c["cache"] = c["cache"].float(), before
+    want = stored(c, outs["latent_out"], key).float()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(9.0), want.nan_to_num(9.0))
