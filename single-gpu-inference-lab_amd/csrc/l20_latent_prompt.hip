@@ -186,12 +186,14 @@ __device__ __forceinline__ void block_of_rows(const PromptParams &p, char *smem,
       }
       return;
     }
-    // rows past the last key hold that key again: they are masked, and what they hold is as finite as it is
+    // Key rows past the last repeat it: their scores are masked.  Value rows past it are zeros: their weight is 0, and
+    // 0 x inf is NaN.
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 16 * wave + 4 * i + (ln >> 4), c = (ln & 15) ^ spread_row(row), r = min(row, last);
-      load_lds(kt, r * k_row + 16 * c, buf + (16 * wave + 4 * i) * kWideRow);
-      load_lds(vt, r * v_row + 16 * c, buf + kWideBytes + (16 * wave + 4 * i) * kWideRow);
+      const int row = 16 * wave + 4 * i + (ln >> 4), c = (ln & 15) ^ spread_row(row);
+      load_lds(kt, min(row, last) * k_row + 16 * c, buf + (16 * wave + 4 * i) * kWideRow);
+      const char *v = row > last ? reinterpret_cast<const char *>(kZeroRow) : vt + row * v_row;
+      load_lds(v + 16 * c, buf + kWideBytes + (16 * wave + 4 * i) * kWideRow);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {

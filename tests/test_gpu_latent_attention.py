@@ -480,3 +480,23 @@ def test_refusals():
         la.l20_latent_prompt_attention(p["query"], p["key"][:, :1], p["key_rope"], p["value"], p["cu_q"], p["cu_k"], 8)
     with pytest.raises(RuntimeError, match="cu_seqlens"):
         la.l20_latent_prompt_attention(p["query"], p["key"], p["key_rope"], p["value"], p["cu_q"].long(), p["cu_k"], 8)
+
+
+@pytest.mark.parametrize("lens,keys", [([70, 40, 3], [65, 130, 1]), ([260], [4001])], ids=["whole", "split"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_prompt_infinite_value_of_the_last_key(lens, keys, dtype, causal):
+    """Where a sequence ends inside a tile: infinite dims for the rows that see the last key, all else as without."""
+    c = make_prompt(lens, keys, 2, dtype, seed=27)
+    clean, clean_lse = run_prompt(c, causal)
+    value = c["value"].clone()
+    hit = torch.zeros_like(clean)
+    ends = list(zip(c["cu_q"].tolist(), c["cu_q"][1:].tolist(), c["cu_k"][1:].tolist()))
+    for q0, q1, k1 in ends:
+        c["value"][k1 - 1, 1, 9], c["value"][k1 - 1, 0, 127] = float("inf"), -float("inf")
+        first = q1 - 1 if causal else q0  # (the last row alone sees the last key)
+        hit[first:q1, 1, 9], hit[first:q1, 0, 127] = 1, -1
+    out, lse = run_prompt(c, causal)
+    assert torch.equal(out.isinf(), hit != 0) and bool((out.isinf() * out.sign() == hit).all())
+    out[hit != 0] = clean[hit != 0]
+    R.check_prompt(out, lse, c["query"], c["key"], c["key_rope"], value, c["cu_q"], c["cu_k"], SCALE, causal)
