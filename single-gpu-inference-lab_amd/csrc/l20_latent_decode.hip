@@ -364,17 +364,49 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         for (int e = 0; e < 4; ++e) s = dot2<T>(kw[e], qw[e], s);
       }
       const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c_log2, -use));
-      for (int n = 0; n < min(64, last + 1 - t0); ++n) {
-        const int block = __builtin_amdgcn_readlane(id, n);
-        if (block < 0) continue;
-        const uint8_t *src = p.cache + (int64_t)block * p.c_block + (int64_t)((t0 + n) & 15) * p.c_tok + dim * kBytes;
-        float v;
-        if constexpr (KT == 0) v = __builtin_amdgcn_cvt_f32_fp8(*src, 0);
-        else v = (float)*reinterpret_cast<const T *>(src);
-        out += lane_f(w, n) * v;
+      const int keys = min(64, last + 1 - t0);
+      for (int n = 0; n < keys; n += 8) {  // (eight loads in flight: one at a time a token takes a memory's latency)
+        float v[8];
+        int block[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int k = min(n + u, keys - 1);
+          block[u] = __builtin_amdgcn_readlane(id, k);
+          const uint8_t *src = p.cache + (int64_t)max(block[u], 0) * p.c_block + (int64_t)((t0 + k) & 15) * p.c_tok + dim * kBytes;
+          if constexpr (KT == 0) v[u] = __builtin_amdgcn_cvt_f32_fp8(*src, 0);
+          else v[u] = (float)*reinterpret_cast<const T *>(src);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float wn = lane_f(w, min(n + u, 63));
+          if (n + u < keys && block[u] >= 0) out += wn * v[u];  // (uniform)
+        }
       }
     }
     return out;
+  }
+
+  // The last of tokens first .. last whose value has one of the wave's dims not finite, or -1.
+  static __device__ int last_odd(const DecodeParams &p, int b, int first, int last, int wave) {
+    const int lane = lane_id();
+    for (int t1 = last; t1 >= first; t1 -= 64) {
+      const int t = max(t1 - lane, first), id = block_of(p, b, t >> 4);
+      const uint8_t *src =
+          p.cache + (int64_t)max(id, 0) * p.c_block + (int64_t)(t & 15) * p.c_tok + wave * (16 * kDimBlocks) * kBytes;
+      float odd = 0.0f;
+      for (int c = 0; c < 16 * kDimBlocks; c += 8) {
+        if constexpr (KT == 0) {
+          const i32x2 w = *reinterpret_cast<const i32x2 *>(src + c), lo = fp8x4<T>(w[0]), hi = fp8x4<T>(w[1]);
+          odd = dot2<T>(lo[0], 0, dot2<T>(lo[1], 0, dot2<T>(hi[0], 0, dot2<T>(hi[1], 0, odd))));
+        } else {
+          const i32x4 w = *reinterpret_cast<const i32x4 *>(src + 2 * c);
+          odd = dot2<T>(w[0], 0, dot2<T>(w[1], 0, dot2<T>(w[2], 0, dot2<T>(w[3], 0, odd))));
+        }
+      }
+      const uint64_t found = __ballot(id >= 0 && odd != odd);
+      if (found) return max(t1 - __builtin_ctzll(found), first);
+    }
+    return -1;
   }
 
   // A tile of the run (its number) and its LDS buffers.
@@ -627,7 +659,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     if (scores && g4 == 0) s.sum[16 * own + n16][tg] = sum;
     lds_barrier();
     // A token that a draft row does not see enters its value product with a weight of 0, and 0 x NaN is NaN: rows
-    // that are not finite though their sum is are computed again, from the run's tokens that they see alone.
+    // that are not finite though their sum is, and that do not see a token of the run whose value is not finite, are
+    // computed again, from the run's tokens that they see alone.
     if (p.q_len > 1 && hi * kTokens > len - p.q_len + 1) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
@@ -640,8 +673,11 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
           for (int e = 0; e < 4; ++e) odd = __builtin_fmaf(acc[r][d][e], 0.0f, odd);
         uint64_t again = __ballot(odd != odd && l == l);
         again |= again >> 32;
+        if (!again) continue;
+        const int unseen = last_odd(p, b, max(lo * kTokens, len - p.q_len + 1), min(hi * kTokens, tokens) - 1, wave);
         for (uint32_t left = (uint32_t)(again | again >> 16) & 0xffff; left; left &= left - 1) {
           const int n = __builtin_ctz(left), row = min(rblk * kRows + 16 * r + n, p.rows - 1), i = row / p.heads;
+          if (unseen <= len - p.q_len + i) continue;
           const float x = exact_row(p, b, i, row - i * p.heads, lo * kTokens, min(min(hi * kTokens, tokens) - 1, len - p.q_len + i),
                                     wave, lane_f(m_all[r], n));
 #pragma unroll

@@ -500,3 +500,51 @@ def test_prompt_infinite_value_of_the_last_key(lens, keys, dtype, causal):
     assert torch.equal(out.isinf(), hit != 0) and bool((out.isinf() * out.sign() == hit).all())
     out[hit != 0] = clean[hit != 0]
     R.check_prompt(out, lse, c["query"], c["key"], c["key_rope"], value, c["cu_q"], c["cu_k"], SCALE, causal)
+
+
+@pytest.mark.parametrize("lens,keys", [([200, 70], [200, 333]), ([260], [4000])], ids=["whole", "split"])
+def test_prompt_value_that_all_rows_see_changes_its_dim_alone(lens, keys):
+    """No row is computed again for a value that it sees: the other dims are the same bits (and take no longer)."""
+    c = make_prompt(lens, keys, 2, seed=28)
+    clean, clean_lse = run_prompt(c)
+    for k0 in c["cu_k"].tolist()[:-1]:
+        c["value"][k0, 1, 9], c["value"][k0, 0, 64] = float("inf"), float("nan")
+    out, lse = run_prompt(c)
+    assert bool(out[:, 1, 9].isinf().all()) and bool(out[:, 0, 64].isnan().all())
+    out[:, 1, 9], out[:, 0, 64] = clean[:, 1, 9], clean[:, 0, 64]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("bound", [None, 100000], ids=["few", "long"])
+def test_decode_value_that_all_drafts_see_changes_its_dim_alone(bound):
+    """As above, by a token that its score of -inf gives a weight of 0."""
+    q_len, dim = 3, 9
+    c = make_decode([70, 2, 129, 900, 64], 16, q_len=q_len, seed=36, poison=False)
+    c["query"][..., dim] = c["query"][..., dim].abs().clamp_min(0.125)
+    for b, t in ((0, 3), (2, 100), (3, 890), (4, 0)):
+        c["cache"][c["table"][b, t // 16].long(), t % 16, dim] = -30000.0  # weight 0, finite
+    clean, clean_lse = run_decode(c, max_seq_len=bound)
+    for b, t in ((0, 3), (2, 100), (3, 890), (4, 0)):
+        c["cache"][c["table"][b, t // 16].long(), t % 16, dim] = -float("inf")
+    out, lse = run_decode(c, max_seq_len=bound)
+    hit = torch.ones(5, q_len, dtype=torch.bool, device="cuda")
+    hit[1] = False
+    hit = hit.flatten()
+    assert bool(out[hit][..., dim].isnan().all()) and not bool(out[~hit].isnan().any())  # (0 x inf)
+    out[hit, :, dim] = clean[hit, :, dim]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_prompt_infinite_value_seen_beside_a_nan_not_seen(dtype):
+    c = make_prompt([200, 90], [200, 210], 2, dtype, seed=29)
+    clean, clean_lse = run_prompt(c)
+    value = c["value"].clone()
+    c["value"][0, 1, 9], c["value"][100, 1, 30] = float("inf"), float("nan")  # seen by all rows, by rows 100 .. 199
+    c["value"][200, 0, 9], c["value"][200 + 209, 0] = -float("inf"), float("nan")  # by all, by the last row
+    out, lse = run_prompt(c)
+    assert bool((out[:200, 1, 9] == float("inf")).all()) and bool(out[100:200, 1, 30].isnan().all())
+    assert bool((out[200:289, 0, 9] == -float("inf")).all()) and bool(out[289, 0].isnan().all())
+    for rows, h, dims in ((slice(0, 200), 1, 9), (slice(100, 200), 1, 30), (slice(200, 289), 0, 9), (289, 0, slice(None))):
+        out[rows, h, dims] = clean[rows, h, dims]
+    R.check_prompt(out, lse, c["query"], c["key"], c["key_rope"], value, c["cu_q"], c["cu_k"], SCALE)
