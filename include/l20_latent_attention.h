@@ -130,8 +130,9 @@ typedef struct l20_pd_latent_args {
 } l20_pd_latent_args;
 
 int32_t l20_pd_paged_latent_check(const l20_pd_latent_args *args);
-/* Workspace bytes of a call on a device of cu_count compute units (0: the current device's); reads only
- * batch, q_len, num_heads, rank, cache_dtype and max_seq_len.  0 where no workspace is needed. */
+/* Workspace bytes on a device of cu_count compute units (0: the current device's), enough for every call of up
+ * to `batch` sequences and up to `max_seq_len` with this q_len, num_heads, rank and cache_dtype; reads only
+ * those.  0 where none of them needs a workspace. */
 int64_t l20_pd_paged_latent_workspace(const l20_pd_latent_args *args, int32_t cu_count);
 int32_t l20_pd_paged_latent(const l20_pd_latent_args *args, void *stream);
 

@@ -878,6 +878,27 @@ Plan plan_of(const l20_pd_latent_args &a, int cus) {
   return n;
 }
 
+// The workspace of calls of up to a.batch sequences.  It grows with the batch but where a rule of plan_of takes another
+// side (a small batch is split where a large one has whole sequences a workgroup): the batches just below those places
+// are looked at too.
+int64_t workspace_of(const l20_pd_latent_args &a, int cus) {
+  int64_t most = 0;
+  auto with = [&](int64_t batch) {
+    if (batch < 1 || batch > a.batch) return;
+    l20_pd_latent_args b = a;
+    b.batch = (int32_t)batch;
+    most = std::max(most, plan_of(b, cus).workspace);
+  };
+  const int64_t rows = rows_of(a), units16 = (rows + 15) / 16, units32 = (rows + 31) / 32;
+  const int64_t tile = a.cache_dtype == L20_PD_KV_FP8_E4M3 ? 64 : 32;
+  const int64_t tiles = std::max<int64_t>(1, ((int64_t)a.max_seq_len + tile - 1) / tile);
+  with(a.batch);
+  with(std::min<int64_t>(cus, kFewTiles1 * cus / tiles) / units16);
+  with(std::min(cus / units32, kFewTiles2 * cus / tiles / units16));
+  for (const int64_t block : {16, 32, 64}) with(63 / ((rows + block - 1) / block));  // (whole_tiles)
+  return most;
+}
+
 int32_t check(const l20_pd_latent_args *a) {
   if (!a) return set_error(L20_PD_EINVAL, "null argument block");
   if (a->dtype != L20_PD_BF16 && a->dtype != L20_PD_FP16) return set_error(L20_PD_EINVAL, "query must be bf16 or fp16");
@@ -964,7 +985,7 @@ int32_t l20_pd_paged_latent_check(const l20_pd_latent_args *a) {
 int64_t l20_pd_paged_latent_workspace(const l20_pd_latent_args *a, int32_t cu_count) {
   l20pd_host::clear_error();
   if (!a || a->batch < 0 || a->q_len < 1 || a->num_heads < 1 || a->max_seq_len < 0 || rows_of(*a) > 65535) return 0;
-  return plan_of(*a, cu_count > 0 ? cu_count : l20la::device_cus()).workspace;
+  return workspace_of(*a, cu_count > 0 ? cu_count : l20la::device_cus());
 }
 
 int32_t l20_pd_paged_latent(const l20_pd_latent_args *a, void *stream) {

@@ -106,8 +106,9 @@ def allocate_l20_paged_latent_workspace(
     kv_rank: int = 512,
     q_len: int = 1,
 ) -> torch.Tensor:
-    """The workspace of ``l20_paged_latent_attention`` for this query shape and ``max_seq_len`` (uint8; empty
-    where none is needed).  Calls that may overlap each need their own; its contents do not matter."""
+    """The workspace of ``l20_paged_latent_attention`` for queries of up to this many sequences (and these heads and
+    ``q_len``) and bounds up to ``max_seq_len`` (uint8; empty where none is needed).  Calls that may overlap each need
+    their own; its contents do not matter."""
     size = _paged_bytes(query.shape[0] // q_len, q_len, query.shape[1], kv_rank, int(max_seq_len), latent_cache.dtype,
                         gpu_cus(latent_cache.device))
     return torch.empty(size, dtype=torch.uint8, device=latent_cache.device)
@@ -163,8 +164,9 @@ def allocate_l20_latent_prompt_workspace(
     batch: int,
     max_seqlen_q: int,
 ) -> torch.Tensor:
-    """The workspace of ``l20_latent_prompt_attention`` for these shapes (uint8; empty where the keys are not split).
-    Calls that may overlap each need their own; its contents do not matter."""
+    """The workspace of ``l20_latent_prompt_attention`` for exactly these shapes (uint8; empty where the keys are not
+    split: the call then takes an empty one, and does not split).  Calls that may overlap each need their own; its
+    contents do not matter."""
     size = _prompt_bytes(query.shape[0], query.shape[1], key.shape[0], batch, int(max_seqlen_q), gpu_cus(query.device))
     return torch.empty(size, dtype=torch.uint8, device=query.device)
 

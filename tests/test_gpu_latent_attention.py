@@ -548,3 +548,17 @@ def test_prompt_infinite_value_seen_beside_a_nan_not_seen(dtype):
     for rows, h, dims in ((slice(0, 200), 1, 9), (slice(100, 200), 1, 30), (slice(200, 289), 0, 9), (289, 0, slice(None))):
         out[rows, h, dims] = clean[rows, h, dims]
     R.check_prompt(out, lse, c["query"], c["key"], c["key_rope"], value, c["cu_q"], c["cu_k"], SCALE)
+
+
+@pytest.mark.parametrize("batches", [(64, 32, 8, 1), (70, 9)])
+def test_decode_workspace_of_the_largest_batch_is_enough_for_smaller_ones(batches):
+    """Allocated once for a batch that is not split itself; smaller ones are."""
+    import l20_latent_attention as la
+
+    lens = [(29 * i) % 256 + 1 for i in range(batches[0])]
+    ws = None
+    for n in batches:
+        c = make_decode(lens[:n], 16, rank=256, seed=37)
+        if ws is None:
+            ws = la.allocate_l20_paged_latent_workspace(c["query"], c["cache"], 256, kv_rank=256)
+        check_decode(c, *run_decode(c, workspace=ws, max_seq_len=256))

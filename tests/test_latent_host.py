@@ -254,3 +254,23 @@ def test_fake_implementations_keep_shapes():
         out, i = torch.empty(8, 16, 512, dtype=torch.bfloat16, device="cuda"), torch.empty(8, dtype=torch.int32, device="cuda")
         got = torch.ops.l20_stack.paged_latent_attention_out(q, cache, i.view(8, 1), i, out, None, 1.0, 1.0, 16)
         assert got.shape == out.shape
+
+
+@pytest.mark.parametrize("heads,q_len", [(1, 1), (16, 1), (28, 4), (28, 5), (64, 1), (128, 3)])
+@pytest.mark.parametrize("cache", [cabi.L20_PD_KV_FP8_E4M3, cabi.L20_PD_KV_BF16], ids=["e4m3", "model"])
+@pytest.mark.parametrize("cus", [256, 64])
+def test_workspace_of_a_batch_is_enough_for_smaller_ones(heads, q_len, cache, cus):
+    """A step of a serving loop may have fewer sequences, and a shorter bound, than what was allocated for."""
+    lib, a = cabi.load(), paged_args()
+    a.num_heads, a.q_len, a.cache_dtype = heads, q_len, cache
+
+    def size(batch, length):
+        a.batch, a.max_seq_len = batch, length
+        return lib.l20_pd_paged_latent_workspace(ctypes.byref(a), cus)
+
+    for length in (16, 64, 128, 256, 512, 1000, 4096, 131072):
+        sizes = [size(b, length) for b in [*range(1, 280), 500, 1000, 4096]]
+        assert sizes == sorted(sizes)
+    for batch in (1, 2, 8, 32, 64, 200, 1000):
+        sizes = [size(batch, n) for n in [*range(0, 4096, 16), 8192, 65536, 1 << 19]]
+        assert sizes == sorted(sizes)
