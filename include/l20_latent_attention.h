@@ -91,8 +91,8 @@ int32_t l20_pd_latent_rope_and_cache(const l20_pd_latent_write_args *args, void 
  *                page_size a multiple of 16 through 4096, tokens of a page contiguous above 16
  *                (stride_page = page_size * stride_token)
  *   block_table  [batch, table_pages] int32; seq_lens [batch] int32, the q_len new tokens included
- *   output       [batch*q_len, num_heads, rank] dtype, not over the query; lse [batch*q_len, num_heads] fp32 natural log
- *                or NULL
+ *   output       [batch*q_len, num_heads, rank] dtype; lse [batch*q_len, num_heads] fp32 natural log or NULL.  An
+ *                output that shares bytes with the query is refused by the call (interleaved views do not)
  *
  * Row b*q_len+i sees tokens 0 .. seq_lens[b]-q_len+i:
  *   s_t = softmax_scale q . row_t,  out = sum_t softmax(s)_t row_t[0 .. rank)
@@ -139,7 +139,8 @@ int32_t l20_pd_paged_latent(const l20_pd_latent_args *args, void *stream);
 /*
  * Attention of packed prompts over expanded keys and values (128 dims a head, 64 shared rotary dims).
  *
- *   query      [total_q, num_heads, 192] dtype; output [total_q, num_heads, 128] dtype, not over the query
+ *   query      [total_q, num_heads, 192] dtype; output [total_q, num_heads, 128] dtype; an output that
+ *              shares bytes with the query, the keys or the values is refused by the call
  *   key, value [total_k, num_heads, 128] dtype; key_rope [total_k, 64] dtype, shared by the heads
  *   cu_q, cu_k [batch + 1] int32: sequence b has query rows cu_q[b] .. cu_q[b+1] and keys
  *              cu_k[b] .. cu_k[b+1]; offsets are clamped to the tensors

@@ -35,6 +35,7 @@
 #include <type_traits>
 
 #include "l20_latent_common.h"
+#include "l20_overlap.h"
 
 namespace l20la {
 
@@ -992,6 +993,10 @@ int32_t l20_pd_paged_latent(const l20_pd_latent_args *a, void *stream) {
   l20pd_host::clear_error();
   const int32_t rc = check(a);
   if (rc != L20_PD_OK || a->batch == 0) return rc;
+  const int64_t rows = (int64_t)a->batch * a->q_len;
+  if (l20la::overlap({a->output, 2 * a->o_stride_row, 2 * a->o_stride_head, rows, a->num_heads, 2 * a->rank},
+                     {a->query, 2 * a->q_stride_row, 2 * a->q_stride_head, rows, a->num_heads, 2 * (a->rank + a->rope_dim)}))
+    return set_error(L20_PD_EINVAL, "output must not lie over the query");
   const int cus = l20la::device_cus();
   const Plan plan = plan_of(*a, cus);
   if (plan.workspace > 0 && (!a->workspace || a->workspace_bytes < plan.workspace || (uintptr_t)a->workspace % 16))

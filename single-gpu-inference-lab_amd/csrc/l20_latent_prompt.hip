@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "l20_latent_common.h"
+#include "l20_overlap.h"
 
 namespace l20la {
 
@@ -649,6 +650,13 @@ int32_t l20_pd_latent_prompt(const l20_pd_latent_prompt_args *a, void *stream) {
   l20pd_host::clear_error();
   const int32_t rc = check(a);
   if (rc != L20_PD_OK || a->batch == 0 || a->total_q == 0 || a->max_q_len == 0) return rc;
+  const int64_t heads = a->num_heads;
+  const l20la::Lattice out{a->output, 2 * a->o_stride_token, 2 * a->o_stride_head, a->total_q, heads, 2 * a->value_dim};
+  if (l20la::overlap(out, {a->query, 2 * a->q_stride_token, 2 * a->q_stride_head, a->total_q, heads, 2 * (a->head_dim + a->rope_dim)}) ||
+      l20la::overlap(out, {a->key, 2 * a->k_stride_token, 2 * a->k_stride_head, a->total_k, heads, 2 * a->head_dim}) ||
+      l20la::overlap(out, {a->key_rope, 2 * a->kr_stride_token, 0, a->total_k, 1, 2 * a->rope_dim}) ||
+      l20la::overlap(out, {a->value, 2 * a->v_stride_token, 2 * a->v_stride_head, a->total_k, heads, 2 * a->value_dim}))
+    return set_error(L20_PD_EINVAL, "output must not lie over the query, the keys or the values");
   l20la::PromptParams p{};
   p.q = a->query;
   p.q_st = a->q_stride_token;

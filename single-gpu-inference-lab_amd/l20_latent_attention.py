@@ -133,7 +133,7 @@ def l20_paged_latent_attention(
     [batch * q_len, heads, kv_rank], to which the model applies its value up-projection.
 
     Row b * q_len + i sees the first ``seq_lens[b] - q_len + i + 1`` tokens of sequence b; one that sees none gives
-    zeros (``lse``: -inf). ``output`` must not lie over ``query``. ``softmax_scale`` is the model's (its head dims
+    zeros (``lse``: -inf). ``output`` must not share bytes with ``query``. ``softmax_scale`` is the model's (its head dims
     before the absorption, not ``kv_rank``, set it). ``max_seq_len`` bounds the lengths (default: what the block
     table can name) and sizes grid and workspace; tokens beyond it, the table, or on a page outside the cache are
     masked. With ``output`` and ``workspace`` given nothing is allocated and the call can be captured in a graph."""
@@ -193,7 +193,7 @@ def l20_latent_prompt_attention(
     Sequence b has the query rows and the keys of its ``cu_seqlens`` ranges; with ``causal`` query i of n sees
     keys up to i + (keys - n), so that a chunk whose first tokens are cached already passes all keys.  A row that
     sees none gives zeros (``lse``: -inf); rows outside the ranges, or beyond ``max_seqlen_q``, keep what they
-    held.  ``softmax_scale`` defaults to 192^-0.5.  Calls of few rows and many keys split the keys, with a
+    held.  ``output`` must not share bytes with an input.  ``softmax_scale`` defaults to 192^-0.5.  Calls of few rows and many keys split the keys, with a
     ``workspace`` (default: allocated)."""
     _need_gpu("l20_latent_prompt_attention", query)
     if query.dtype not in (torch.float16, torch.bfloat16):

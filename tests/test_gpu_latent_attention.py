@@ -562,3 +562,33 @@ def test_decode_workspace_of_the_largest_batch_is_enough_for_smaller_ones(batche
         if ws is None:
             ws = la.allocate_l20_paged_latent_workspace(c["query"], c["cache"], 256, kv_rank=256)
         check_decode(c, *run_decode(c, workspace=ws, max_seq_len=256))
+
+
+def test_outputs_beside_their_inputs_and_over_them():
+    """Interleaved with the query, row by row or head by head, is fine; any shared byte is refused."""
+    import l20_latent_attention as la
+
+    c = make_decode([300, 40, 7], 6, q_len=2, seed=38)
+    want, want_lse = run_decode(c)
+    rows, heads = c["query"].shape[:2]
+    by_head = torch.zeros(rows, heads, 576 + 512, dtype=torch.bfloat16, device="cuda")
+    by_row = torch.zeros(rows, heads * (576 + 512), dtype=torch.bfloat16, device="cuda")
+    for query, output in ((by_head[..., :576], by_head[..., 576:]),
+                          (by_row[:, :heads * 576].view(rows, heads, 576), by_row[:, heads * 576:].view(rows, heads, 512)),
+                          (by_row[:, heads * 512:].view(rows, heads, 576), by_row[:, :heads * 512].view(rows, heads, 512))):
+        query.copy_(c["query"])
+        out, lse = run_decode({**c, "query": query}, output=output)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(query, c["query"])
+    for output in (c["query"][..., 64:], c["query"][..., :512], c["query"][..., 16:528],
+                   by_head.view(rows, -1)[:, 8:8 + heads * 512].view(rows, heads, 512)):
+        with pytest.raises(RuntimeError, match="output must not"):
+            run_decode({**c, "query": c["query"] if output.shape[2] == 512 and output.stride(1) == 576 else by_head[..., :576]}, output=output)
+    p = make_prompt([90, 30], [90, 30], 3, seed=39)
+    want, _ = run_prompt(p)
+    both = torch.zeros(120, 3, 192 + 128, dtype=torch.bfloat16, device="cuda")
+    both[..., :192] = p["query"]
+    out, _ = run_prompt({**p, "query": both[..., :192]}, output=both[..., 192:])
+    assert torch.equal(out, want) and torch.equal(both[..., :192], p["query"])
+    for output in (p["query"][..., 64:], p["value"], p["key"]):
+        with pytest.raises(RuntimeError, match="output must not"):
+            run_prompt(p, output=output)

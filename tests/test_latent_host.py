@@ -274,3 +274,27 @@ def test_workspace_of_a_batch_is_enough_for_smaller_ones(heads, q_len, cache, cu
     for batch in (1, 2, 8, 32, 64, 200, 1000):
         sizes = [size(batch, n) for n in [*range(0, 4096, 16), 8192, 65536, 1 << 19]]
         assert sizes == sorted(sizes)
+
+
+OVER = [
+    ("paged_latent", dict(output=FAKE + 128, o_stride_row=16 * 576, o_stride_head=576)),  # query[..., 64:]
+    ("paged_latent", dict(output=FAKE + 2 * 512, o_stride_row=16 * 576, o_stride_head=576)),  # the last 64 dims alone
+    ("paged_latent", dict(output=FAKE + 2 * (15 * 16 * 576 + 15 * 576) + 2 * 568)),  # the last row's last dims
+    ("paged_latent", dict(query=FAKE << 8, output=(FAKE << 8) - 2 * (16 * 16 * 512 - 4))),  # the other end
+    ("paged_latent", dict(batch=1, q_len=1, num_heads=1, output=FAKE + 1144, o_stride_row=0, o_stride_head=0)),
+    ("latent_prompt", dict(output=FAKE + 128, o_stride_token=8 * 192, o_stride_head=192)),
+    ("latent_prompt", dict(query=FAKE << 8, value=FAKE << 12, output=FAKE << 12, o_stride_token=8 * 256, o_stride_head=256)),
+    ("latent_prompt", dict(query=FAKE << 8, key=FAKE << 12, output=(FAKE << 12) + 8, o_stride_token=8 * 256, o_stride_head=256)),
+    ("latent_prompt", dict(query=FAKE << 8, key_rope=FAKE << 12, output=(FAKE << 12) + 500 * 128 - 8)),
+]
+
+
+@pytest.mark.parametrize("kind,change", OVER, ids=[f"{k}-{i}" for i, (k, _) in enumerate(OVER)])
+def test_calls_refuse_outputs_over_their_inputs(kind, change):
+    """Bytes shared with an input, whatever the two views' strides: refused before anything is launched."""
+    args = CHECKS[kind]()
+    for name, value in change.items():
+        setattr(args, name, value)
+    lib = cabi.load()
+    rc = getattr(lib, f"l20_pd_{kind}")(ctypes.byref(args), None)
+    assert rc == cabi.L20_PD_EINVAL and "output must not lie over" in cabi.last_error()
