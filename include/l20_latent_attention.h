@@ -43,6 +43,8 @@ extern "C" {
  *                pairs (d, d + 32) with is_neox, (2 i, 2 i + 1) without
  *   cache row  = [latent_out | key_out], in an fp8 cache RNE_e4m3fn(clamp(. / cache_scale, +-448)),
  *                NaN for NaN
+ *
+ * An output that is not its input (address and strides) must share no bytes with the inputs: the call refuses it.
  */
 typedef struct l20_pd_latent_write_args {
   const void *query;

@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "l20_latent_common.h"
+#include "l20_overlap.h"
 
 namespace l20la {
 
@@ -266,6 +267,23 @@ int32_t check(const l20_pd_latent_write_args *a) {
   return L20_PD_OK;
 }
 
+// Whether an output shares bytes with an input other than by being that input.
+bool outputs_overlap(const l20_pd_latent_write_args &a) {
+  const int64_t n = a.num_tokens, heads = a.query ? a.num_heads : 0;
+  const l20la::Lattice in[] = {{a.query, 2 * a.q_stride_token, 2 * a.q_stride_head, n, heads, 2 * a.rope_dim},
+                               {a.latent, 2 * a.l_stride_token, 0, n, 1, 2 * a.rank},
+                               {a.key, 2 * a.k_stride_token, 0, n, 1, 2 * a.rope_dim}};
+  const l20la::Lattice out[] = {{a.query_out, 2 * a.qo_stride_token, 2 * a.qo_stride_head, n, heads, 2 * a.rope_dim},
+                                {a.latent_out, 2 * a.lo_stride_token, 0, n, 1, 2 * a.rank},
+                                {a.key_out, 2 * a.ko_stride_token, 0, n, 1, 2 * a.rope_dim}};
+  for (int o = 0; o < 3; ++o)
+    for (int i = 0; i < 3; ++i) {
+      const bool itself = i == o && in[i].base == out[o].base && in[i].row == out[o].row && in[i].head == out[o].head;
+      if (!itself && l20la::overlap(out[o], in[i])) return true;
+    }
+  return false;
+}
+
 template <typename T, int CT, int CS>
 void launch_rank(const l20la::WriteParams &p, int rank, hipStream_t s) {
   const unsigned tokens = (unsigned)p.tokens;
@@ -297,6 +315,7 @@ int32_t l20_pd_latent_rope_and_cache(const l20_pd_latent_write_args *a, void *st
   l20pd_host::clear_error();
   const int32_t rc = check(a);
   if (rc != L20_PD_OK || a->num_tokens == 0) return rc;
+  if (outputs_overlap(*a)) return set_error(L20_PD_EINVAL, "an output must be its input itself or lie apart from the inputs");
   l20la::WriteParams p{};
   p.q = a->query;
   p.q_st = a->q_stride_token;

@@ -82,7 +82,8 @@ def l20_latent_rope_and_cache(
     """Norm (with ``norm_weight``) and RoPE of new tokens, and their rows into the paged cache.
 
     ``query_rope`` [tokens, heads, 64] (or None), ``latent`` [tokens, rank] and ``key_rope`` [tokens, 64] are views
-    of any row stride; each result goes to its ``_out`` tensor, or in place where none is given. A ``query_out``
+    of any row stride; each result goes to its ``_out`` tensor, or in place where none is given (an ``_out`` tensor that
+    is not its input must share no bytes with the inputs). A ``query_out``
     that is the last 64 dims of the absorbed query saves the copy there. ``slot_mapping`` below 0 or beyond the
     cache: the token is not stored; two tokens of a call must not name one slot. An fp8 cache stores ``clamp(x /
     cache_scale)`` of the rounded results."""

@@ -239,3 +239,26 @@ def test_values_that_are_not_finite(norm, dtype, fp8):
     want = stored(c, outs["latent_out"], key).float()
     assert torch.equal(got.isnan(), want.isnan())
     assert torch.equal(got.nan_to_num(9.0), want.nan_to_num(9.0))
+
+
+def test_write_into_the_gaps_of_the_inputs():
+    """Outputs interleaved with the inputs share nothing with them; ones in another layout of the same memory do."""
+    import l20_latent_attention as la
+
+    def parts():
+        c = make(40, 3, seed=15)
+        wide = torch.zeros(40, 2 * 576, dtype=torch.bfloat16, device="cuda")
+        wide[:, :576] = c["down"]
+        return c, wide
+
+    c, wide = parts()
+    call(c, True, True)
+    d, wide = parts()
+    d["down"] = wide[:, :576]
+    kept = wide[:, :576].clone()
+    call(d, True, True, latent_out=wide[:, 576:1088], key_rope_out=wide[:, 1088:])
+    assert torch.equal(wide[:, 576:], c["down"]) and torch.equal(wide[:, :576], kept) and torch.equal(c["cache"], d["cache"])
+    with pytest.raises(RuntimeError, match="its input itself or lie apart"):
+        call(d, True, False, latent_out=wide.view(-1)[:40 * 512].view(40, 512))
+    with pytest.raises(RuntimeError, match="its input itself or lie apart"):
+        call(d, True, True, key_rope_out=wide[:, 448:512])

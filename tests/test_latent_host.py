@@ -298,3 +298,22 @@ def test_calls_refuse_outputs_over_their_inputs(kind, change):
     lib = cabi.load()
     rc = getattr(lib, f"l20_pd_{kind}")(ctypes.byref(args), None)
     assert rc == cabi.L20_PD_EINVAL and "output must not lie over" in cabi.last_error()
+
+
+APART = dict(query=FAKE << 8, query_out=FAKE << 9, latent=FAKE << 10, latent_out=FAKE << 11, key=FAKE << 12, key_out=FAKE << 13)
+
+
+@pytest.mark.parametrize("change", [
+    dict(latent_out=FAKE << 10),  # another row stride
+    dict(latent_out=(FAKE << 10) + 16, lo_stride_token=576),
+    dict(key=(FAKE << 10) + 1024, key_out=(FAKE << 10) + 1024 - 112, ko_stride_token=576),  # over the latent
+    dict(query_out=(FAKE << 8) + 2 * 16),  # (strides of an absorbed query)
+    dict(query_out=FAKE << 8, qo_stride_token=16 * 192, qo_stride_head=64),
+    dict(query_out=(FAKE << 12) - 2 * 16 * 576),
+], ids=range(6))
+def test_cache_producer_refuses_outputs_over_other_inputs(change):
+    args = write_args()
+    for name, value in {**APART, **change}.items():
+        setattr(args, name, value)
+    rc = cabi.load().l20_pd_latent_rope_and_cache(ctypes.byref(args), None)
+    assert rc == cabi.L20_PD_EINVAL and "its input itself or lie apart" in cabi.last_error()
