@@ -43,7 +43,7 @@ extern "C" {
  * x' = x cos + (x_pair sin) sign on the first rotary_dim dims (each product
  * and the sum rounded to fp32, the result rounded to dtype), pairs
  * (d, d + rotary_dim/2) with is_neox, (2i, 2i+1) without.  fp8 caches store
- * RNE_e4m3fn(clamp(x / scale, +-448)) of the stored model-dtype values, with
+ * RNE_e4m3fn(clamp(x / scale, +-448)) of the stored model-dtype values (-448 for a NaN), with
  * the per-head scale arrays (fp32 [num_kv_heads], device memory) when
  * non-NULL, else the scalar scales.
  */

@@ -21,11 +21,12 @@
 //
 //  latent_merge<T, RANK, WIDE>   joins those parts.
 //
-// Bounds: with 16 rows the cache's bytes (a stream of equal sequences reaches 6.1 TB/s of either cache), with 64 rows
-// and more the products and the LDS reads that feed them (128 heads: 870 TFLOP/s over fp8, 700 over bf16).  A call
-// has 17 to 25 us besides: launches, the runs, the first query and tile, the parts' way through memory, the join (4 to
-// 9).  Calls: 128 lognormal contexts of 16 heads, bf16 60 us; 2 x 131072 tokens, fp8 40; 32 x 4096, 128 heads, fp8
-// 65.5; 24 ragged contexts of 28 heads x 4 drafts, fp16 53.
+// Bounds: with 16 rows the cache's bytes (a stream of equal sequences reaches 6.1 TB/s of either cache).  With 64 rows
+// and more (128 heads: 870 TFLOP/s over fp8, 700 over bf16) no unit is full, matrix units 28 % and LDS 16 % of a call
+// of 32 x 4096 tokens: what is left is the waits of eight waves between the barriers of a tile.  A call has 17 to 25 us
+// besides: launches, the runs, the first query and tile, the parts' way through memory, the join (4 to 9).  Calls: 128
+// lognormal contexts of 16 heads, bf16 60 us; 2 x 131072 tokens, fp8 40; 32 x 4096, 128 heads, fp8 65.5; 24 ragged
+// contexts of 28 heads x 4 drafts, fp16 53.
 // Measured and not taken: two workgroups of four waves a CU (their tiles are half as far ahead); 128-token tiles in
 // two buffers; the copies of a tile spread between the steps of the products (128 heads 66.9 -> 68.3).
 
@@ -131,7 +132,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
     return row * kPRow + ((c ^ (kTokens == 64 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
   }
 
-  // What a run spends on one sequence more, in tiles (its query, its output, the stream's pause).  Measured, 128
+  // What a run spends on one sequence more, in tiles (its query, its output, the stream's pause).  It lies at the
+  // sequence's start, also where several runs share the sequence: then the first of them have fewer tiles.  Measured, 128
   // lognormal contexts of 16 heads and 24 ragged ones of 28 heads x 4 drafts: 0 76 and 67 us, 1 68 and 66, 2 67 and
   // 62, 3 63 and 60, 4 60 and 60, 6 62, 8 63.
   static constexpr int kSwitch = 4;
@@ -266,7 +268,8 @@ template <typename T, int KT, int RANK, int RB> struct Partial {
         if (w < wave) inc += v;
         total += v;
       }
-      // run g is cost floor(g total / runs) .. floor((g + 1) total / runs); none is empty
+      // run g is cost floor(g total / runs) .. floor((g + 1) total / runs); none is empty (of cost: one that ends before
+      // its sequence's first tile has no tile)
       runs = min(p.groups, total);
       if (group >= runs) return;  // the whole workgroup
       first = (int)scaled(group, total, runs);
@@ -734,7 +737,9 @@ template <typename T, int KT, int RANK, int RB> __global__ __launch_bounds__(kTh
 // maxima and parts), so a call's rows are on the chip at once: with few runs a sequence a wave takes all runs of one
 // row block and RANK / 8 dims; with many (WIDE, more than eight runs a sequence) a workgroup takes 16 dims, its waves
 // every eighth run: 2 x 131072 tokens (128 runs a sequence) 5.5 us instead of 44.7, 4 x 64-512 tokens 3.5 instead of
-// 7.4; 32 x 4096 tokens of 128 heads (four runs) 16.6 instead of 8.3.
+// 7.4; 32 x 4096 tokens of 128 heads (four runs) 16.6 instead of 8.3.  The host knows the mean alone: one long sequence
+// among many short ones is joined by one workgroup a row block, and takes what many runs take there (131072 tokens and
+// 31 x 500, 16 heads, fp8: the call 96 us, 2 x 131072 38).
 template <typename T, int RANK, bool WIDE>
 __global__ __launch_bounds__(kThreads) void latent_merge(DecodeParams p, int block_rows) {
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -871,7 +876,10 @@ Plan plan_of(const l20_pd_latent_args &a, int cus) {
     n.groups = (a.batch + 7) / 8 * 8;
     return n;
   }
-  // As many runs as workgroups fit the chip at once, a multiple of 8 (the XCDs), no more than tiles.
+  // As many runs as workgroups fit the chip at once, and no more than tiles, rounded up to a multiple of 8 (the XCDs).
+  // With 1, 2, 4 or 8 blocks of rows they fit; with others the last few workgroups are a round of their own (24 x 4096
+  // tokens, fp8: 28 heads x 4 drafts, 2 blocks, 59 us, x 5, 3 blocks and 264 workgroups, 109; 128 heads x 4, 8 blocks,
+  // 156, x 3, 6 blocks and 288 workgroups, 202).
   const int64_t fit = std::max<int64_t>(1, cus / n.row_blocks);
   n.groups = (int)((std::min<int64_t>(fit, a.batch * tiles) + 7) / 8 * 8);
   n.workspace = 2 * (int64_t)n.groups * n.row_blocks * block * (a.rank + 2) * (int64_t)sizeof(float) +

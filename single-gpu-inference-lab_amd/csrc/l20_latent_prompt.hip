@@ -9,7 +9,7 @@
 //    the registers that S^T came out in: slot (g, j) of a 16-key step is key 4 g + j (j < 4) or 8 + 4 g + j - 4,
 //    which is what two transposing reads of V give.  Statistics and accumulators are fp32, the maximum moves when it
 //    is exceeded by 2^8; P is rounded to T for the product (relative error 2^-8 bf16, 2^-11 fp16, as the output's own
-//    rounding), its sum is of the unrounded values.  Queries stay in registers.
+//    rounding), its sum is of the unrounded values.  Queries stay in registers.  Values past a sequence's last are zeros.
 //  latent_prompt_runs<T>, latent_prompt_merge<T>   the same with the tiles of all blocks of rows cut into equal runs,
 //    one a workgroup, and the parts of blocks that several runs share joined, for calls of few rows and many keys.
 //
