@@ -141,20 +141,24 @@ __device__ f32x2 exact_row(const PromptParams &p, int h, int64_t row, int64_t ks
   return out;
 }
 
-// The last of keys first .. last whose value has a dim that is not finite, or -1.
-template <typename T> __device__ int last_odd(const PromptParams &p, int h, int64_t ks, int first, int last) {
+// The last of keys first .. last whose value has a dim that is not finite (or, `infinite`, that is infinite), or -1.
+template <typename T> __device__ int last_odd(const PromptParams &p, int h, int64_t ks, int first, int last, bool infinite) {
   for (int j1 = last; j1 >= first; j1 -= 64) {
     const int j = j1 - (int)(threadIdx.x & 63);
-    float odd = 0.0f;
+    bool odd = false;
     if (j >= first) {
       const T *v = reinterpret_cast<const T *>(p.v) + (ks + j) * p.v_st + h * p.v_sh;
       for (int c = 0; c < kDim; c += 8) {
         const i32x4 w = *reinterpret_cast<const i32x4 *>(v + c);
+        const T *e = reinterpret_cast<const T *>(&w);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd = dot2<T>(w[e], 0, odd);
+        for (int k = 0; k < 8; ++k) {
+          const float x = fabsf((float)e[k]);
+          odd |= infinite ? x == INFINITY : !(x < INFINITY);
+        }
       }
     }
-    const uint64_t found = __ballot(odd != odd);
+    const uint64_t found = __ballot(odd);
     if (found) return j1 - __builtin_ctzll(found);
   }
   return -1;
@@ -349,16 +353,28 @@ __device__ __forceinline__ void block_of_rows(const PromptParams &p, char *smem,
   // finite though their sum is, and that do not see a key of the wave's tiles whose value is not finite, are computed
   // again, from the keys they see alone: a row of 4000 keys takes its wave 0.5 ms.  (2 x 4096 tokens of 32 heads, 0.38 ms:
   // an infinite value at key 0 of a head, which all rows see, 0.48, and without the second condition 32; a NaN at key
-  // 4000, which the rows below it in its tiles do not see, 16.)
+  // 4000, which the rows below it in its tiles do not see, 16.)  So are, in fp16, rows that have a NaN and may see an
+  // infinite value: P is 0 there from 2^-25 on, and 0 x inf is NaN too.
   float odd = 0.0f;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) odd = __builtin_fmaf(acc[d][e], 0.0f, odd);
-  uint64_t odd_lanes = __ballot(p.causal && i < rows && odd != odd && l == l);
-  if (odd_lanes)  // (the keys of the wave's tiles that its first row does not see)
-    odd_lanes &= __ballot(lim < last_odd<T>(p, h, ks, max(lo * kKeys, wave_lim + 1),
-                                            min(min(hi * kKeys, nk) - 1, wave_end | (kKeys - 1))));
+  uint64_t odd_lanes = __ballot(i < rows && odd != odd && l == l);
+  if (odd_lanes) {
+    const int last = min(min(hi * kKeys, nk) - 1, wave_end | (kKeys - 1));  // of the wave's tiles
+    uint64_t again = __ballot(lim < last_odd<T>(p, h, ks, max(lo * kKeys, wave_lim + 1), last, false));
+    if constexpr (std::is_same_v<T, _Float16>) {
+      bool nan = false;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nan |= acc[d][e] != acc[d][e];
+      const uint64_t nans = __ballot(nan);
+      if (nans && last_odd<T>(p, h, ks, lo * kKeys, last, true) >= 0) again |= nans;
+    }
+    odd_lanes &= again;
+  }
   for (uint32_t left = (uint32_t)(odd_lanes | odd_lanes >> 32); left; left &= left - 1) {
     const int r = __builtin_ctz(left);
     const f32x2 x = exact_row<T>(p, h, qs + q0 + wave * kWaveRows + r, ks, lo * kKeys,

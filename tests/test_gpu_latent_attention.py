@@ -592,3 +592,30 @@ def test_outputs_beside_their_inputs_and_over_them():
     for output in (p["query"][..., 64:], p["value"], p["key"]):
         with pytest.raises(RuntimeError, match="output must not"):
             run_prompt(p, output=output)
+
+
+@pytest.mark.parametrize("lens,keys", [([200, 70], [200, 333]), ([260], [4000])], ids=["whole", "split"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_prompt_infinite_value_of_a_small_weight(lens, keys, dtype, causal):
+    """A weight of about 2^-33 of the largest, which is 0 in fp16: an infinite value is infinite in the sum all the same,
+    a NaN a NaN."""
+    c = make_prompt(lens, keys, 2, dtype, seed=41)
+    c["query"][..., 0] = 8.0
+    c["key"][..., 0] = 0.0
+    firsts = c["cu_k"].tolist()[:-1]
+    for k0 in firsts:
+        c["key"][k0 + 1, :, 0] = -40.0
+    clean, clean_lse = run_prompt(c, causal)
+    value = c["value"].clone()
+    for k0 in firsts:
+        c["value"][k0 + 1, 1, 9], c["value"][k0 + 1, 0, 127], c["value"][k0 + 2, 0, 64] = float("inf"), -float("inf"), float("nan")
+    out, lse = run_prompt(c, causal)
+    for q0, q1, n in zip(c["cu_q"].tolist(), c["cu_q"][1:].tolist(), [k - q for q, k in zip(lens, keys)]):
+        # (the first row of a prompt without cached keys sees key 0 alone, its second keys 0 and 1)
+        inf0, nan0 = (q0 + max(1 - n, 0), q0 + max(2 - n, 0)) if causal else (q0, q0)
+        assert bool((out[inf0:q1, 1, 9] == float("inf")).all()) and bool((out[inf0:q1, 0, 127] == -float("inf")).all())
+        assert bool(out[nan0:q1, 0, 64].isnan().all())
+        for rows, h, dim in ((slice(inf0, q1), 1, 9), (slice(inf0, q1), 0, 127), (slice(nan0, q1), 0, 64)):
+            out[rows, h, dim] = clean[rows, h, dim]
+    R.check_prompt(out, lse, c["query"], c["key"], c["key_rope"], value, c["cu_q"], c["cu_k"], SCALE, causal)
