@@ -28,11 +28,12 @@ HIP_LIB = HERE / "libl20_paged_decode_hip.so"
 OPS_LIB = HERE / "l20_paged_decode_ops.so"
 ARCH = os.environ.get("L20_PD_ARCH", "gfx950")
 OBJECTS = HERE / "_build"
-# The decode kernels, the paged KV-cache producer, latent attention and the block tables, one shared object.
+# The decode kernels, the paged KV-cache producer, latent attention, the block tables and the page pool, and beam
+# search's selection, one shared object.
 HIP_SOURCES = [CSRC / f"{name}.hip" for name in (
     "l20_paged_decode_fp8", "l20_kv_write", "l20_tree_suffix", "l20_latent_decode", "l20_latent_prompt",
-    "l20_latent_write", "l20_block_tables")]
-OPS_SOURCES = [CSRC / "l20_paged_decode_ops.cpp", CSRC / "l20_latent_ops.cpp"]
+    "l20_latent_write", "l20_block_tables", "l20_page_moves", "l20_beam_search")]
+OPS_SOURCES = [CSRC / f"{name}.cpp" for name in ("l20_paged_decode_ops", "l20_latent_ops", "l20_beam_ops")]
 
 # Packed-FP32 VALU forms are kept out of every HIP build.
 HIP_FLAGS = [

@@ -60,6 +60,17 @@ EXPORTED = (
     "l20_pd_latent_prompt",
     "l20_pd_block_tables_check",
     "l20_pd_block_tables",
+    "l20_pd_reorder_tables_check",
+    "l20_pd_reorder_tables_workspace",
+    "l20_pd_reorder_tables",
+    "l20_pd_compact_pages_check",
+    "l20_pd_compact_pages_workspace",
+    "l20_pd_compact_pages",
+    "l20_pd_copy_pages_check",
+    "l20_pd_copy_pages",
+    "l20_pd_beam_step_check",
+    "l20_pd_beam_step_workspace",
+    "l20_pd_beam_step",
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -188,6 +199,51 @@ class L20PdBlockTablesArgs(ctypes.Structure):
     ]
 
 
+class L20PdReorderArgs(ctypes.Structure):
+    """Mirror of ``l20_pd_reorder_args`` (include/l20_block_tables.h)."""
+
+    _fields_ = [
+        ("parents", _vp), ("block_table", _vp), ("bt_stride_row", _i64), ("table_pages", _i32), ("seq_lens", _vp),
+        ("page_shares", _vp), ("pages", _i32), ("free_pages", _vp), ("pool", _i32), ("free_count", _vp),
+        ("src", _vp), ("dst", _vp), ("tokens", _vp), ("room", _i32), ("count", _vp),
+        ("groups", _i32), ("beams", _i32), ("page_size", _i32), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class L20PdCompactArgs(ctypes.Structure):
+    """Mirror of ``l20_pd_compact_args`` (include/l20_block_tables.h)."""
+
+    _fields_ = [
+        ("limit", _i32), ("block_table", _vp), ("bt_stride_row", _i64), ("table_pages", _i32), ("seq_lens", _vp),
+        ("page_shares", _vp), ("pages", _i32), ("free_pages", _vp), ("pool", _i32), ("free_count", _vp),
+        ("src", _vp), ("dst", _vp), ("tokens", _vp), ("room", _i32), ("count", _vp),
+        ("rows", _i32), ("page_size", _i32), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class L20PdCopyArgs(ctypes.Structure):
+    """Mirror of ``l20_pd_copy_args`` (include/l20_block_tables.h); ``caches`` is a host array of device pointers."""
+
+    _fields_ = [
+        ("src", _vp), ("dst", _vp), ("tokens", _vp), ("room", _i32), ("count", _vp), ("caches", _vp),
+        ("num_caches", _i32), ("pages", _i64), ("stride_page", _i64), ("size0", _i64), ("stride0", _i64),
+        ("size1", _i64), ("stride1", _i64), ("size2", _i64), ("stride2", _i64), ("inner", _i64), ("token_level", _i32),
+    ]
+
+
+class L20PdBeamStepArgs(ctypes.Structure):
+    """Mirror of ``l20_pd_beam_step_args`` (include/l20_beam_search.h); ``end_tokens`` is a host array."""
+
+    _fields_ = [
+        ("logits", _vp), ("l_stride_request", _i64), ("l_stride_beam", _i64), ("dtype", _i32),
+        ("scores", _vp), ("s_stride_request", _i64), ("s_stride_beam", _i64),
+        ("requests", _i32), ("beams", _i32), ("vocab", _i32), ("end_tokens", _vp), ("num_end_tokens", _i32),
+        ("tokens", _vp), ("parents", _vp), ("scores_out", _vp),
+        ("ended_tokens", _vp), ("ended_parents", _vp), ("ended_scores", _vp),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -245,17 +301,26 @@ def load(path: Optional[Path] = None) -> ctypes.CDLL:
     lib.l20_pd_tree_suffix_merge.argtypes = [ts_p, _vp]
     lib.l20_pd_tree_suffix_merge.restype = _i32
     for name, struct in (("latent_write_check", L20PdLatentWriteArgs), ("paged_latent_check", L20PdLatentArgs),
-                         ("latent_prompt_check", L20PdLatentPromptArgs), ("block_tables_check", L20PdBlockTablesArgs)):
+                         ("latent_prompt_check", L20PdLatentPromptArgs), ("block_tables_check", L20PdBlockTablesArgs),
+                         ("reorder_tables_check", L20PdReorderArgs), ("compact_pages_check", L20PdCompactArgs),
+                         ("copy_pages_check", L20PdCopyArgs), ("beam_step_check", L20PdBeamStepArgs)):
         getattr(lib, "l20_pd_" + name).argtypes = [ctypes.POINTER(struct)]
         getattr(lib, "l20_pd_" + name).restype = _i32
     for name, struct in (("latent_rope_and_cache", L20PdLatentWriteArgs), ("paged_latent", L20PdLatentArgs),
-                         ("latent_prompt", L20PdLatentPromptArgs), ("block_tables", L20PdBlockTablesArgs)):
+                         ("latent_prompt", L20PdLatentPromptArgs), ("block_tables", L20PdBlockTablesArgs),
+                         ("reorder_tables", L20PdReorderArgs), ("compact_pages", L20PdCompactArgs),
+                         ("copy_pages", L20PdCopyArgs), ("beam_step", L20PdBeamStepArgs)):
         getattr(lib, "l20_pd_" + name).argtypes = [ctypes.POINTER(struct), _vp]
         getattr(lib, "l20_pd_" + name).restype = _i32
     lib.l20_pd_paged_latent_workspace.argtypes = [ctypes.POINTER(L20PdLatentArgs), _i32]
     lib.l20_pd_paged_latent_workspace.restype = _i64
     lib.l20_pd_latent_prompt_workspace.argtypes = [ctypes.POINTER(L20PdLatentPromptArgs), _i32]
     lib.l20_pd_latent_prompt_workspace.restype = _i64
+    for name, struct in (("reorder_tables", L20PdReorderArgs), ("compact_pages", L20PdCompactArgs)):
+        getattr(lib, f"l20_pd_{name}_workspace").argtypes = [ctypes.POINTER(struct)]
+        getattr(lib, f"l20_pd_{name}_workspace").restype = _i64
+    lib.l20_pd_beam_step_workspace.argtypes = [ctypes.POINTER(L20PdBeamStepArgs), _i32]
+    lib.l20_pd_beam_step_workspace.restype = _i64
     if path is None:
         _lib = lib
     return lib

@@ -1,0 +1,276 @@
+"""GPU: beam search's selection against every candidate in float64 and plain Python."""
+
+import math
+
+import pytest
+import torch
+
+import beam_ref as R
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _require_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs an MI355X GPU")
+    import l20_beam_search  # noqa: F401
+
+
+def filled(requests, beams):
+    """Outputs that hold something else."""
+    import l20_beam_search as bs
+
+    out = bs.BeamSearchStep.empty(requests, beams, "cuda")
+    for t in out:
+        t.fill_(-77)
+    return out
+
+
+def inputs(requests, beams, vocab, dtype, seed, scale=2.0):
+    g = torch.Generator().manual_seed(seed)
+    logits = (scale * torch.randn(requests, beams, vocab, generator=g)).to(dtype)
+    return logits, -3 * torch.rand(requests, beams, generator=g)
+
+
+def compare(out, logits, scores, ends):
+    """logits [requests, beams, vocab] and scores on the CPU."""
+    want = R.beam_step(logits, scores, list(ends))
+    assert want[6] > 1e-6, "the inputs leave the order to the last digits"
+    for at, name in enumerate(("tokens", "parents", "scores", "ended_tokens", "ended_parents", "ended_scores")):
+        got = out[at].tolist()
+        if name.endswith("scores"):
+            for r, (mine, theirs) in enumerate(zip(got, want[at])):
+                for x, y in zip(mine, theirs):
+                    assert x == y if math.isinf(y) else abs(x - y) <= R.score_bound(y, logits.shape[2]), (name, r, x, y)
+        else:
+            assert got == want[at], name
+    return want
+
+
+def check(logits, scores, ends=(), **kw):
+    import l20_beam_search as bs
+
+    out = bs.l20_beam_search_step(logits.cuda(), scores.cuda(), end_tokens=list(ends),
+                                  out=filled(*scores.shape), **kw)
+    torch.cuda.synchronize()
+    return compare(out, logits, scores, ends)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 63, 511, 512, 513, 2047, 2048, 2049, 5001, 16385])
+def test_vocabularies(dtype, vocab):
+    logits, scores = inputs(3, 4, vocab, DTYPES[dtype], seed=vocab)
+    check(logits, scores, ends=[vocab // 2, 0] if vocab > 2 else [])
+
+
+@pytest.mark.parametrize("beams", [1, 2, 3, 5, 8, 16, 31, 32])
+@pytest.mark.parametrize("ends", [0, 1, 8])
+def test_beams_and_end_tokens(beams, ends):
+    logits, scores = inputs(3, beams, 1500, torch.bfloat16, seed=10 * beams + ends)
+    tokens = [5 * e + 1 for e in range(ends)]
+    logits[:, :, tokens] += 7  # likely: they lead many rows
+    check(logits, scores, tokens)
+
+
+def test_end_tokens_that_are_none():
+    """Outside the vocabulary, below it, and named twice."""
+    logits, scores = inputs(2, 3, 100, torch.float16, seed=4)
+    logits[:, :, 9] += 8
+    check(logits, scores, [9, 9, 100, -1, 2 ** 31 - 1])
+
+
+@pytest.mark.parametrize("requests,beams", [(1, 1), (1, 32), (70, 1), (40, 5)])
+def test_numbers_of_rows(requests, beams):
+    logits, scores = inputs(requests, beams, 4100, torch.bfloat16, seed=requests + beams)
+    check(logits, scores, [17])
+
+
+def test_rows_without_candidates():
+    """Masked throughout, a NaN, an infinity, dead beams of several kinds: no candidate of theirs, and none of the
+    others lost.  What a dead beam's row holds does not matter."""
+    inf, nan = math.inf, math.nan
+    for dtype in DTYPES.values():
+        logits, scores = inputs(7, 4, 3000, dtype, seed=3)
+        logits[0, 1] = -inf
+        logits[1, 0, 2999] = nan
+        logits[1, 2, 5] = inf
+        logits[1, 3, 1000:] = -inf
+        scores[2] = torch.tensor([-1.0, -inf, inf, nan])
+        logits[2, 1:] = nan
+        scores[3] = -inf
+        logits[4] = -inf
+        logits[4, 2, [10, 2500]] = torch.tensor([1.0, 0.0]).to(dtype)  # two candidates for four beams
+        logits[5] = nan
+        logits[6, 0, :2500] = nan
+        want = check(logits, scores, [2500])
+        assert want[0][3] == [-1] * 4 and want[0][4][0] == 10 and want[0][4][1:] == [-1] * 3 and want[3][4][0] == 2500
+
+
+@pytest.mark.parametrize("vocab", [40, 515, 2500, 6001])
+def test_ties_go_to_the_lower_beam_and_token(vocab):
+    """Equal rows of equal beams (at odd offsets too), equal logits, and whole rows of one value."""
+    logits, scores = inputs(3, 4, vocab, torch.bfloat16, seed=vocab)
+    logits[0, :] = logits[0, :1]
+    scores[0] = scores[0, 0]
+    logits[1] = 0.25
+    scores[1] = -1.0
+    logits[2, :, : vocab // 2] = 3.0
+    scores[2, 1:] -= 1.5
+    want = check(logits, scores, [1])
+    assert want[1][1] == [0, 0, 0, 0] and want[0][1] == [0, 2, 3, 4] and want[3][1] == [1, -1, -1, -1]
+
+
+def test_minus_zero_ties_with_zero():
+    logits = torch.zeros(1, 1, 100)
+    logits[0, 0, ::2] = -0.0
+    assert check(logits, torch.zeros(1, 1), [0])[0] == [[1]]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_far_values(dtype):
+    """The type's lowest value as a mask, large logits of both signs, and scores far from zero."""
+    d = DTYPES[dtype]
+    logits, scores = inputs(3, 3, 2600, d, seed=8)
+    logits[0, :, 100:] = torch.finfo(d).min
+    big = {"bf16": 2.0 ** 120, "fp16": 60000.0, "fp32": 2.0 ** 126}[dtype]
+    logits[1] = -big
+    logits[1, 0, 7], logits[1, 1, 2599], logits[1, 2, 0] = big, big, -big / 2
+    scores[1] = torch.tensor([-1.0, -2.0, -3.0])
+    scores[2] = torch.tensor([-1e30, -1e30, -3e38])
+    import l20_beam_search as bs
+
+    out = bs.l20_beam_search_step(logits[:2].cuda(), scores[:2].cuda(), out=filled(2, 3))
+    compare(out, logits[:2], scores[:2], [])
+    # 1e30 swallows the logits: equal scores, so the lower beam, then its higher logits
+    out = bs.l20_beam_search_step(logits[2:].cuda(), scores[2:].cuda(), out=filled(1, 3))
+    best = sorted(range(2600), key=lambda t: (-float(logits[2, 0, t]), t))[:3]
+    assert out.tokens.tolist() == [best] and out.parents.tolist() == [[0] * 3]
+    assert out.scores.cpu().equal(torch.full((1, 3), -1e30))
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "blocks"])
+def test_orders_that_pass_every_threshold(order):
+    x = torch.arange(9000.0) / 1000
+    x = {"rising": x, "falling": x.flip(0), "blocks": x.view(9, 1000).flip(0).reshape(-1)}[order]
+    logits = torch.stack([x, x * 0.9 + 0.01]).unsqueeze(0).contiguous()
+    check(logits, torch.tensor([[-1.0, -1.3]]), [8999])
+
+
+def test_layouts():
+    """Padded rows, beams outside requests, rows at every alignment, one request's strides that say nothing."""
+    import l20_beam_search as bs
+
+    logits, scores = inputs(3, 4, 2111, torch.bfloat16, seed=20)
+    want = None
+    for kind in range(6):
+        hold = torch.full((40000,), math.nan, dtype=logits.dtype, device="cuda")
+        if kind < 4:
+            view = hold[kind:].as_strided((3, 4, 2111), (4 * 2200, 2200 + (kind % 2) * 3, 1))
+        elif kind == 4:
+            view = hold.as_strided((3, 4, 2111), (2200, 3 * 2200, 1))
+        else:
+            view = hold[1:].as_strided((12, 2111), (2113, 1))
+        view.copy_(logits.view(view.shape))
+        s = torch.full((3, 9), 5.0, device="cuda")[:, ::2][:, :4] if kind % 2 else torch.empty(4, 3, device="cuda").t()
+        s.copy_(scores)
+        out = bs.l20_beam_search_step(view, s, end_tokens=[3], out=filled(3, 4))
+        if want is None:
+            compare(out, logits, scores, [3])
+            want = [t.clone() for t in out]
+        assert all(a.equal(b) for a, b in zip(out, want)), kind
+    x = logits[:1, :1].cuda()
+    out = bs.l20_beam_search_step(x.as_strided((1, 1, 2111), (1, 7, 1)), scores[:1, :1].cuda(), out=filled(1, 1))
+    compare(out, logits[:1, :1], scores[:1, :1], [])
+
+
+def test_scores_in_place_and_smaller_batches_in_one_workspace():
+    import l20_beam_search as bs
+
+    logits, scores = inputs(9, 4, 8000, torch.float16, seed=31)
+    x = logits.cuda()
+    ws = bs.allocate_l20_beam_search_workspace(x, scores.cuda(), end_tokens=[1])
+    for n in (9, 4, 1, 7):
+        s = scores[:n].cuda()
+        out = filled(n, 4)._replace(scores=s)
+        ws.fill_(255)
+        bs.l20_beam_search_step(x[:n], s, end_tokens=[1], out=out, workspace=ws)
+        compare(out, logits[:n], scores[:n], [1])
+
+
+def test_no_requests():
+    import l20_beam_search as bs
+
+    out = bs.l20_beam_search_step(torch.zeros(0, 50, device="cuda"), torch.zeros(0, 4, device="cuda"))
+    assert out.tokens.shape == (0, 4)
+
+
+def test_wide_rows_and_many_rows():
+    """A vocabulary beyond any tokenizer's in few rows, and more rows than the chip holds waves, against torch in 64
+    bits (with the same order of ties: a stable sort of each row)."""
+    import l20_beam_search as bs
+
+    for requests, beams, vocab, dtype in ((1, 2, 3_000_017, torch.float32), (700, 8, 2500, torch.bfloat16)):
+        g = torch.Generator(device="cuda").manual_seed(vocab)
+        x = (2 * torch.randn(requests, beams, vocab, generator=g, device="cuda")).to(dtype)
+        s = -3 * torch.rand(requests, beams, generator=g, device="cuda")
+        out = bs.l20_beam_search_step(x, s)
+        total = torch.log_softmax(x.double(), -1) + s.double()[..., None]
+        best, at = total.flatten(1).sort(dim=-1, descending=True, stable=True)
+        gaps = best[:, :beams] - best[:, 1:beams + 1]
+        other = at[:, :beams] // vocab != at[:, 1:beams + 1] // vocab
+        sure = ~(other & (gaps < 1e-6)).any(-1)  # (a request in thousands may hang on the last digits)
+        assert sure.float().mean() > 0.99
+        assert out.tokens[sure].equal(at[sure, :beams] % vocab) and out.parents[sure].equal((at[sure, :beams] // vocab).int())
+        assert ((out.scores.double() - best[:, :beams]).abs() <= 2.0 ** -24 * best[:, :beams].abs() +
+                2.0 ** -23 * (4 + math.log(vocab))).all()
+
+
+def test_graph_and_another_stream():
+    """A captured step whose scores advance in place: replays equal eager calls on copies, also beside eager work."""
+    import l20_beam_search as bs
+
+    logits, scores = inputs(5, 4, 9001, torch.bfloat16, seed=50)
+    x, s = logits.cuda(), scores.cuda()
+    eager = s.clone()
+    out = filled(5, 4)._replace(scores=s)
+    ws = bs.allocate_l20_beam_search_workspace(x, s, end_tokens=[2])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        bs.l20_beam_search_step(x, s.clone(), end_tokens=[2], workspace=ws)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        bs.l20_beam_search_step(x, s, end_tokens=[2], out=out, workspace=ws)
+    s.copy_(scores)
+    for step in range(4):
+        x.add_(0.5 * torch.randn(x.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(step)).to(x.dtype))
+        want = bs.l20_beam_search_step(x, eager, end_tokens=[2])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(a.equal(b) for a, b in zip(out, want))
+        eager = want.scores.clone()
+
+
+def test_refusals():
+    import l20_beam_search as bs
+
+    x, s = torch.zeros(6, 100, device="cuda"), torch.zeros(2, 3, device="cuda")
+    for bad, message in (((x[:5], s), "logits must be"), ((x.double(), s), "bf16, fp16 or fp32"), ((x, s.double()), "fp32"),
+                         ((x.t().contiguous().t(), s), "contiguous"), ((x, s[0]), "requests, beams"),
+                         ((torch.zeros(66, 9, device="cuda"), torch.zeros(2, 33, device="cuda")), "1 to 32")):
+        with pytest.raises(RuntimeError, match=message):
+            bs.l20_beam_search_step(*bad)
+    with pytest.raises(RuntimeError, match="at most 8 end tokens"):
+        bs.l20_beam_search_step(x, s, end_tokens=list(range(9)))
+    with pytest.raises(RuntimeError, match="workspace is missing"):
+        bs.l20_beam_search_step(x, s, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    out = bs.BeamSearchStep.empty(2, 3, "cuda")
+    with pytest.raises(RuntimeError, match="tokens must be"):
+        bs.l20_beam_search_step(x, s, out=out._replace(tokens=out.parents))
+    with pytest.raises(RuntimeError, match="lie apart"):
+        bs.l20_beam_search_step(x, s, out=out._replace(ended_tokens=out.tokens))
+    with pytest.raises(RuntimeError, match="not lie over an input"):
+        bs.l20_beam_search_step(x, s, out=out._replace(ended_scores=x.view(-1)[:6].view(2, 3)))
