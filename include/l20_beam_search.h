@@ -60,9 +60,8 @@ typedef struct l20_pd_beam_step_args {
 
 int32_t l20_pd_beam_step_check(const l20_pd_beam_step_args *args);
 
-/* Bytes of workspace for these requests, beams, vocab and num_end_tokens (and for any fewer requests) on a
- * device of `cus` compute units (0: the current device's). */
-int64_t l20_pd_beam_step_workspace(const l20_pd_beam_step_args *args, int32_t cus);
+/* Bytes of workspace for these requests, beams, vocab and num_end_tokens (and for any fewer of each). */
+int64_t l20_pd_beam_step_workspace(const l20_pd_beam_step_args *args);
 
 int32_t l20_pd_beam_step(const l20_pd_beam_step_args *args, void *stream);
 

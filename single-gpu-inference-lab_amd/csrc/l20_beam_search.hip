@@ -5,19 +5,21 @@
 // and the best `beams` of a request's candidates, with and without end tokens.  Both parts of a row come from one
 // pass over its logits:
 //
-//  beam_scan   a wave reads a run of a row, 32 logits a lane and step, one step ahead.  It keeps the run's K best
-//    (K = beams + end tokens: enough for `beams` that are no end tokens) as a list sorted over its lanes, value and
-//    token, and the sum of exp(x - m) below the running maximum m.  The K-th best is a threshold: a step whose
-//    maxima do not pass it (nearly every one after the first few: K ln(n / K) values of n do) costs its loads, one
-//    maximum, one exp and one addition a logit.
-//  beam_join   a workgroup a request.  A wave a row joins the runs' lists (their heads are popped in order: runs lie
-//    one behind the other, so the lowest lane of equal heads has the lowest token) and sums; then every candidate
-//    counts those ahead of it in the other rows' lists, by binary search, and takes the place it counts to.
+//  beam_scan   a workgroup of eight waves a run of a row, a wave 32 logits a lane and step, one step ahead.  A wave
+//    keeps the sum of exp(x - m) below the running maximum m, and in LDS what may be among the run's K best (K = beams
+//    + end tokens: enough for `beams` that are no end tokens): values from the K-th of 64 maxima on, each of the
+//    values so far of eight lanes of the workgroup.  Few pass (about K ln(steps) a workgroup); the entries are brought
+//    down to the K best, by counting those before each, at the end and where a wave has too many.  The workgroups are
+//    shared out over the live rows, which each counts for itself.
+//  beam_join   a workgroup a request.  A wave a row joins the runs' lists in the same way, and their sums; then each
+//    candidate's place is counted in every row's list, by binary search.
 //
 // Numerics: exp in fp32 of (x - m) log2 e with log2 e in two parts, eight of them summed in fp32, everything beyond
 // that in 64 bits: candidates of different beams are told apart by lse's last digits, and its error is about 1e-8.
 
 #include "l20_beam_search.h"
+
+#include <float.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -32,21 +34,28 @@ using l20la::i32x4;
 
 constexpr int kVectors = 4;                // vectors of eight logits a lane and step
 constexpr int kStep = 64 * 8 * kVectors;   // logits of a wave's step
+constexpr int kWaves = 4;                  // of a workgroup, which takes a run
 constexpr int kMaxRuns = 64;               // runs a row: a lane of the join each
-constexpr int kWavesPerCu = 16;            // waves that rows are split for
-constexpr int kJoinLds = 48 * 1024;        // of it, lists of the rows that a workgroup joins at once
+constexpr int kRunsPerCu = 3;              // runs that rows are split for
+constexpr int kEntries = 128;              // what a wave's LDS holds of candidates (two a lane)
+constexpr int kCounted = 4096;             // rows whose live ones every wave may count (a word of 64 a lane)
 
 struct Params {
   const void *logits;
   int64_t l_sr, l_sb;
   const float *scores;
   int64_t s_sr, s_sb;
-  int requests, beams, vocab, runs, k;
+  int requests, beams, vocab, k;
+  int runs;         // of every row
+  int share;        // where some rows are dead `spread` is shared out over the others, at most `most` each
+  int most, spread;
   int ends[L20_PD_MAX_END_TOKENS];
   int num_ends;
-  // [rows * runs] and [rows * runs * k]
+  int flat;         // scores lie one behind the other
+  int *row_runs;    // [rows], with `share`
+  // [rows * most] and [rows * most * k]
   double *sum;
-  float *top;
+  double *top;
   float *value;
   int *token;
   int64_t *tokens;
@@ -112,176 +121,454 @@ __device__ __forceinline__ double wave_sum(double x) {
 }
 __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < INFINITY; }
 
-// log2 e to 48 bits: (x - m) log2 e is off by half a step of itself, and not by (x - m) times that of one fp32 constant,
-// which all terms of a sum would share.
+// log2 e in two parts: one fp32 constant is off by 1.3e-8 of itself, which all terms of a sum would share.
 constexpr float kLog2eHi = 1.44269502f, kLog2eLo = 1.92596299e-08f;
-__device__ __forceinline__ float exp_below(float x, float m) {
-  const float d = x - m;
-  return __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2eHi, d * kLog2eLo));
-}
 
-// A run's K best, the best in lane 0; lanes past them -inf.
-struct List {
-  float v;
-  int t;
-  float last;  // the K-th best (wave-uniform)
-  __device__ __forceinline__ void insert(float x, int token, int k) {
-    const int lane = threadIdx.x & 63;
-    const int at = __builtin_popcountll(__ballot(v >= x));  // equal ones came before: lower tokens
-    // wave_shr: the lane below's
-    const float pv = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x138, 0xf, 0xf, false));
-    const int pt = __builtin_amdgcn_update_dpp(0, t, 0x138, 0xf, 0xf, false);
-    v = lane < at ? v : lane == at ? x : pv;
-    t = lane < at ? t : lane == at ? token : pt;
-    if (lane >= k) v = -INFINITY;
-    last = l20la::lane_f(v, k - 1);
+// What a wave's sum is relative to: the sum of exp(x - at), with `at` near the maximum m (64 bits).
+struct Reference {
+  float m = -INFINITY;    // the value that made it
+  float shift = 0.0f;     // m log2 e, rounded: at = shift ln 2 exactly
+  double at = -INFINITY;
+  bool far = false;       // m is so large that its last place times log2 e is no exponent: at = m
+  __device__ __forceinline__ void set(float m_) {
+    m = m_;
+    shift = m * kLog2eHi;
+    far = __builtin_fabsf(m) >= 0x1p20f;  // (infinite too)
+    at = far ? (double)m : (double)shift * 0.69314718055994530942;
+  }
+  // Two roundings of half a step: of the exponent and of the result's last place (v_exp_f32 is good to one step).
+  __device__ __forceinline__ float term(float x) const {
+    if (far) {
+      const float d = m > -INFINITY ? x - m : x;  // (all -inf so far: the terms are 0)
+      return __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2eHi, d * kLog2eLo));
+    }
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2eLo, __builtin_fmaf(x, kLog2eHi, -shift)));
+  }
+  __device__ __forceinline__ float eight(const float (&x)[8]) const {
+    float e[8];
+    if (far) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = m > -INFINITY ? x[j] - m : x[j];
+        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2eHi, d * kLog2eLo));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], kLog2eLo, __builtin_fmaf(x[j], kLog2eHi, -shift)));
+    }
+    return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+  }
+  // The term of x less what rounding may make of it; 0 where it is too small to tell.
+  __device__ __forceinline__ float low(float x) const {
+    const float e = term(x);
+    return e > 1e-30f ? e * 0.999f : 0.0f;
   }
 };
 
-template <typename T> __global__ __launch_bounds__(256) void beam_scan(Params p) {
-  const int lane = threadIdx.x & 63;
-  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int row = unit / p.runs, run = unit - row * p.runs;
-  if (row >= p.requests * p.beams) return;
-  const int request = row / p.beams, beam = row - request * p.beams;
-  if (!finite(p.scores[request * p.s_sr + beam * p.s_sb])) return;  // a dead beam
-  const T *const x0 = reinterpret_cast<const T *>(p.logits) + request * p.l_sr + beam * p.l_sb;
+// A value and its token as one number: value falling and token rising is the number falling.  (Never a NaN; -0 is 0.)
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 key_of(float v, int token) {
+  const unsigned b = __builtin_bit_cast(unsigned, v + 0.0f);
+  return (u64)(b ^ ((unsigned)((int)b >> 31) | 0x80000000u)) << 32 | (unsigned)~token;
+}
+__device__ __forceinline__ float value_of(u64 key) {
+  const unsigned b = (unsigned)(key >> 32);
+  return l20la::word_f(b ^ ((unsigned)((int)~b >> 31) | 0x80000000u));
+}
+__device__ __forceinline__ int token_of(u64 key) { return (int)~(unsigned)key; }
+
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+// How many of the n keys in LDS come before `a` and `b` (a list is followed by a place for one more).
+__device__ __forceinline__ void count_before(u64 *keys, int n, u64 a, u64 b, int &before_a, int &before_b) {
+  if ((threadIdx.x & 63) == 0) keys[n] = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; j += 2) {
+    const u64x2 y = *reinterpret_cast<const u64x2 *>(keys + j);
+    before_a += (y[0] > a) + (y[1] > a);
+    before_b += (y[0] > b) + (y[1] > b);
+  }
+}
+__device__ __forceinline__ void count_before(u64 *keys, int n, u64 a, int &before) {
+  if ((threadIdx.x & 63) == 0) keys[n] = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; j += 2) {
+    const u64x2 y = *reinterpret_cast<const u64x2 *>(keys + j);
+    before += (y[0] > a) + (y[1] > a);
+  }
+}
+
+// The best k of what a wave is shown, in its LDS (kEntries keys and one more): in any order, brought down to the k best
+// where they are too many.
+struct Best {
+  u64 *keys;
+  int k, count = 0;
+  float least = -FLT_MAX;  // what is below is not among the k best (never -inf)
+  u64 bar = 0;             // nor is a key below this
+
+  __device__ Best(u64 *keys_, int k_) : keys(keys_), k(k_) {}
+  // A bound from 64 values of different entries: their k-th (equal ones may be among the best).
+  __device__ __forceinline__ void bound_by(const float *maxima) {
+    const float x = maxima[threadIdx.x & 63];
+    int upto = 0;
+#pragma unroll 4
+    for (int j = 0; j < 64; j += 4) {
+      const f32x4 y = *reinterpret_cast<const f32x4 *>(maxima + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) upto += y[i] >= x;
+    }
+    // The largest that k of them are no less than.  (Another wave may raise one meanwhile: then the bound is too low.)
+    least = fmaxf(least, wave_max(upto >= k ? x : -FLT_MAX));
+  }
+  // The tokens to come are higher than those shown: a value equal to the last of k is not among them any more.
+  __device__ __forceinline__ void pass() {
+    if (!bar) return;
+    least = fmaxf(least, value_of((bar | 0xffffffffu) + 1));  // the next value up
+    bar = 0;
+  }
+  // An entry of each lane of `which`: there is room.
+  __device__ __forceinline__ void put(float x, int token, u64 which) {
+    const int at = count + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(which >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)which, 0));
+    if (which >> (threadIdx.x & 63) & 1) keys[at] = key_of(x, token);
+    count += __builtin_popcountll(which);
+  }
+  __device__ __forceinline__ void show(float x, int token, bool ok) {
+    ok = ok && x >= least && key_of(x, token) >= bar;
+    u64 which = __ballot(ok);
+    if (count + __builtin_popcountll(which) > kEntries) {
+      settle();
+      which = __ballot(ok && key_of(x, token) >= bar);
+    }
+    if (which) put(x, token, which);
+  }
+  // The k best to the front, in order.
+  __device__ __forceinline__ void settle() {
+    const int lane = threadIdx.x & 63;
+    const u64 a = lane < count ? keys[lane] : 0, b = lane + 64 < count ? keys[lane + 64] : 0;
+    int before_a = 0, before_b = 0;
+    count_before(keys, count, a, b, before_a, before_b);
+    if (a && before_a < k) keys[before_a] = a;
+    if (b && before_b < k) keys[before_b] = b;
+    if (count >= k) {
+      count = k;
+      bar = keys[k - 1];
+      least = fmaxf(least, value_of(bar));
+    }
+  }
+};
+
+// The n-th live row, n = unit / runs, and how many runs each has: every workgroup counts for itself, a bit a row in
+// `s_live` [kCounted / 64].  All scores at once: 1024 rows counted 64 by 64 took 6 us.  -1: none.
+__device__ __forceinline__ int live_row(const Params &p, int rows, int unit, u64 *s_live, int &runs, int &run) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int kEach = kCounted / 64 / kWaves;
+  float s[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int r = (wave + i * kWaves) * 64 + lane;
+    s[i] = INFINITY;
+    if (r < rows) s[i] = p.flat ? p.scores[r] : p.scores[r / p.beams * p.s_sr + r % p.beams * p.s_sb];
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const u64 which = __ballot(finite(s[i]));
+    if (lane == 0) s_live[wave + i * kWaves] = which;
+  }
+  l20la::lds_barrier();
+  const u64 mask = s_live[lane];
+  int upto = __builtin_popcountll(mask);
+  if (!__ballot(upto != min(max(rows - lane * 64, 0), 64))) {  // all of them
+    runs = p.runs;
+    const int row = unit / runs;
+    run = unit - row * runs;
+    return row < rows ? row : -1;
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(upto, off);
+    if (lane >= off) upto += y;
+  }
+  const int live = __builtin_amdgcn_readlane(upto, 63);
+  if (live == 0) return -1;
+  runs = min(p.most, max(p.spread / live, 1));
+  const int n = unit / runs;
+  run = unit - n * runs;
+  if (n >= live) return -1;
+  const int chunk = __builtin_ctzll(__ballot(upto > n));
+  const int skip = n - (chunk ? __builtin_amdgcn_readlane(upto, chunk - 1) : 0);
+  const unsigned lo = __builtin_amdgcn_readlane((int)mask, chunk), hi = __builtin_amdgcn_readlane((int)(mask >> 32), chunk);
+  const bool here = ((lane < 32 ? lo >> lane : hi >> (lane - 32)) & 1) &&
+                    (int)__builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0)) == skip;
+  return chunk * 64 + __builtin_ctzll(__ballot(here));
+}
+
+template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_scan(Params p) {
+  __shared__ __attribute__((aligned(16))) float s_maxima[2][64];  // of `kWaves` lanes each: of the first step, and so far
+  __shared__ __attribute__((aligned(16))) u64 s_keys[kWaves][kEntries + 2];
+  __shared__ __attribute__((aligned(16))) float s_vector[kWaves][512];
+  __shared__ double s_sum[kWaves][64];
+  __shared__ double s_ref[kWaves];
+  __shared__ int s_count[kWaves];
+  __shared__ u64 s_live[kCounted / 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = blockIdx.x, rows = p.requests * p.beams;
   const int full = p.vocab / kStep, steps = (p.vocab + kStep - 1) / kStep;
-  const int first = (int)((int64_t)run * steps / p.runs), end = (int)((int64_t)(run + 1) * steps / p.runs);
+  int runs = p.runs, row = unit / runs, run = unit - row * runs, first = 0, end = 0;
+  const T *x0 = nullptr;
   Eight<T> next[kVectors];
   auto load = [&](int step) {
     const int at = step * kStep + lane * 8;
-    if (step < full) {
+    if (step < min(full, end)) {
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) next[i] = load8(x0 + at + i * 512);
-    } else {
+    } else {  // (a wave without a step: all of it -inf)
+      const int limit = step < end ? p.vocab : 0;
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i) next[i] = load8_guarded(x0 + at + i * 512, p.vocab - (at + i * 512));
+      for (int i = 0; i < kVectors; ++i) next[i] = load8_guarded(x0 + at + i * 512, limit - (at + i * 512));
     }
   };
-  List best{-INFINITY, 0, -INFINITY};
-  float m = -INFINITY;
+  auto begin = [&] {
+    const int request = row / p.beams, beam = row - request * p.beams;
+    x0 = reinterpret_cast<const T *>(p.logits) + request * p.l_sr + beam * p.l_sb;
+    first = (int)((u64)(unsigned)run * (unsigned)steps / (unsigned)runs) + wave;
+    end = (int)((u64)(unsigned)(run + 1) * (unsigned)steps / (unsigned)runs);
+    load(first);
+  };
+  if (p.share) {
+    row = live_row(p, rows, unit, s_live, runs, run);
+    if (row < 0) return;
+    if (run == 0 && threadIdx.x == 0) p.row_runs[row] = runs;
+    begin();
+  } else {
+    if (row >= rows) return;
+    const float s = p.scores[row / p.beams * p.s_sr + row % p.beams * p.s_sb];
+    begin();  // (as if the row lived: its loads need not wait for the score)
+    if (!finite(s)) return;
+  }
+  Best best(s_keys[wave], p.k);
+  Reference ref;
+  float highest = -INFINITY;
+  float low = 0.0f;  // the term of best.least, less a margin: a sum of eight terms below it has none that passes
   double sum = 0.0;
-  load(first);
-  for (int step = first; step < end; ++step) {
-    Eight<T> now[kVectors];
+  int again = 0;  // the step whose maxima make the bound anew: 0, 1, 3, 7 ...
+  for (int step = first, n = 0; n == 0 || step < end; step += kWaves, ++n) {
+    float x[kVectors][8];
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) now[i] = next[i];
-    if (step + 1 < end) load(step + 1);
-    float x[kVectors][8], tops[kVectors];
+    for (int i = 0; i < kVectors; ++i) unpack(next[i], x[i]);
+    if (step + kWaves < end) load(step + kWaves);
+    auto highest_of = [&] {
+      float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      unpack(now[i], x[i]);
-      const float a = l20la::max3(x[i][0], x[i][1], x[i][2]), b = l20la::max3(x[i][3], x[i][4], x[i][5]);
-      tops[i] = l20la::max3(a, b, l20la::max3(x[i][6], x[i][7], x[i][7]));
-    }
-    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    if (__ballot(top > best.last)) {
-      const float raised = fmaxf(m, wave_max(top));
-      if (raised > m) {
-        if (m > -INFINITY) sum *= exp((double)m - (double)raised);
-        m = raised;
+      for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) top = l20la::max3(top, x[i][j], x[i][j + 1]);
+      return top;
+    };
+    if (n == again) {
+      // the maxima of this wave's lanes in such steps, `kWaves` together
+      highest = fmaxf(highest, highest_of());
+      static_assert(kWaves == 4, "64 maxima of four lanes");
+      float g = fmaxf(highest, dpp<0xb1>(highest));  // quad_perm: lane ^ 1, lane ^ 2
+      g = fmaxf(g, dpp<0x4e>(g));
+      float *const maxima = s_maxima[n > 0];
+      if (lane % kWaves == 0) {
+        maxima[wave * (64 / kWaves) + lane / kWaves] = g;
+        if (n == 0) s_maxima[1][wave * (64 / kWaves) + lane / kWaves] = g;
       }
+      if (n == 0) {
+        l20la::lds_barrier();
+        ref.set(wave_max(s_maxima[0][lane]));  // the same for all waves
+      }
+      best.bound_by(maxima);
+      low = ref.low(best.least);
+      again = 2 * n + 1;
+    }
+    float part[kVectors];
+    auto terms = [&] {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) part[i] = ref.eight(x[i]);
+      return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    };
+    float most = terms();
+    // (The reference need not be the maximum, but these are too far above it, or the first that are not -inf.)
+    if (__ballot(ref.m > -INFINITY ? most > 0x1p24f : highest_of() > -INFINITY)) {
+      const double before = ref.at;
+      ref.set(fmaxf(ref.m, wave_max(highest_of())));
+      if (sum != 0.0) sum *= exp(before - ref.at);
+      low = ref.low(best.least);
+      most = terms();
+    }
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) sum += (double)part[i];
+    if (__ballot(low > 0.0f ? most >= low : highest_of() >= best.least)) {
+      unsigned many = 0;  // vectors with more than there is room for
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) {
-        if (!__ballot(tops[i] > best.last)) continue;
-        // this vector's best, one after the other
-        float y[8];
+        if (!__ballot(part[i] >= low)) continue;
+        const int token = step * kStep + i * 512 + lane * 8;
+        u64 which[8];
+        int total = best.count;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[i][j];
-        while (true) {
-          float v = y[0];
-          int at = 0;
-#pragma unroll
-          for (int j = 1; j < 8; ++j) {
-            at = y[j] > v ? j : at;
-            v = y[j] > v ? y[j] : v;
-          }
-          if (!__ballot(v > best.last)) break;
-          const float w = wave_max(v > best.last ? v : -INFINITY);
-          const int leader = __builtin_ctzll(__ballot(v == w));
-          const int taken = __builtin_amdgcn_readlane(at, leader);
-          best.insert(w, step * kStep + i * 512 + leader * 8 + taken, p.k);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (lane == leader && j == taken) y[j] = -INFINITY;
+        for (int j = 0; j < 8; ++j) {
+          which[j] = __ballot(x[i][j] >= best.least);
+          total += __builtin_popcountll(which[j]);
         }
+        if (total > kEntries) {
+          many |= 1u << i;
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (which[j]) best.put(x[i][j], token + j, which[j]);
+      }
+      if (many) {
+        // those one after the other, through LDS
+#pragma unroll 1
+        for (int i = 0; many; ++i, many >>= 1) {
+          if (!(many & 1)) continue;
+#pragma unroll
+          for (int u = 0; u < kVectors; ++u) {
+            if (u != i) continue;
+            float *const to = s_vector[wave] + lane * 8;
+            *reinterpret_cast<f32x4 *>(to) = f32x4{x[u][0], x[u][1], x[u][2], x[u][3]};
+            *reinterpret_cast<f32x4 *>(to + 4) = f32x4{x[u][4], x[u][5], x[u][6], x[u][7]};
+          }
+          const int token = step * kStep + i * 512 + lane * 8;
+#pragma unroll 1
+          for (int j = 0; j < 8; ++j) best.show(s_vector[wave][lane * 8 + j], token + j, true);
+        }
+        best.pass();
+        low = ref.low(best.least);
       }
     }
-    const float ref = m > -INFINITY ? m : 0.0f;  // (all -inf so far: the terms are 0)
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      float e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = exp_below(x[i][j], ref);
-      sum += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
-    }
   }
-  sum = wave_sum(sum);
+  s_sum[wave][lane] = sum;
   if (lane == 0) {
-    p.sum[unit] = sum;
-    p.top[unit] = m;
+    s_ref[wave] = ref.at;
+    s_count[wave] = best.count;
   }
-  if (lane < p.k) {
-    p.value[(int64_t)unit * p.k + lane] = best.v;
-    p.token[(int64_t)unit * p.k + lane] = best.t;
+  l20la::lds_barrier();
+  // Every entry's place among those of all waves, which are brought together.
+  const int64_t slot = (int64_t)row * p.most + run;
+  const int counts = lane < kWaves ? s_count[lane] : 0;
+  int all = 0, at = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w == wave) at = all;
+    all += __builtin_amdgcn_readlane(counts, w);
+  }
+  u64 *const s_all = reinterpret_cast<u64 *>(s_vector);  // (kWaves kEntries and one more: as many bytes and more)
+  const u64 a = lane < best.count ? best.keys[lane] : 0, b = lane + 64 < best.count ? best.keys[lane + 64] : 0;
+  if (a) s_all[at + lane] = a;
+  if (b) s_all[at + 64 + lane] = b;
+  l20la::lds_barrier();
+  if (best.count) {
+    int before_a = 0, before_b = 0;
+    if (best.count > 64) count_before(s_all, all, a, b, before_a, before_b);
+    else count_before(s_all, all, a, before_a);
+    if (a && before_a < p.k) p.value[slot * p.k + before_a] = value_of(a), p.token[slot * p.k + before_a] = token_of(a);
+    if (b && before_b < p.k) p.value[slot * p.k + before_b] = value_of(b), p.token[slot * p.k + before_b] = token_of(b);
+  }
+  if (wave == 0) {
+    if (lane >= all && lane < p.k) p.value[slot * p.k + lane] = -INFINITY;
+    // the waves' sums, below the highest reference (mostly all the same; a NaN stays one)
+    double high = s_ref[0];
+    for (int w = 1; w < kWaves; ++w) high = fmax(high, s_ref[w]);
+    double total = 0.0;
+    for (int w = 0; w < kWaves; ++w) {
+      const double r = s_ref[w], part = s_sum[w][lane];
+      total += r == high || part == 0.0 ? part : part * exp(r - high);
+    }
+    total = wave_sum(total);
+    if (lane == 0) {
+      p.sum[slot] = total;
+      p.top[slot] = high;
+    }
   }
 }
 
 __global__ __launch_bounds__(512) void beam_join(Params p) {
   extern __shared__ double s_mem[];
-  const int waves = p.join_waves, threads = waves * 64, k = p.k, beams = p.beams;
-  double *const s_score = s_mem;                                              // [beams * k]
-  unsigned long long *const s_end = (unsigned long long *)(s_score + beams * k);  // [beams]: which are end tokens
-  int *const s_token = (int *)(s_end + beams);                                // [beams * k]
-  int *const s_count = s_token + beams * k;                                   // [beams]
-  int *const s_ended = s_count + beams;                                       // [1]
-  float *const s_value = (float *)(s_ended + 1);                              // [waves][runs * k], then the tokens
+  const int waves = p.join_waves, threads = waves * 64, k = p.k, beams = p.beams, n = beams * k;
+  double *const s_score = s_mem;                                  // [beams * k]
+  u64 *const s_end = (u64 *)(s_score + n);                        // [beams]: which are end tokens
+  u64 *const s_keys = s_end + beams + ((n + beams) & 1);          // [waves][kEntries + 2], 16-byte aligned
+  int *const s_token = (int *)(s_keys + waves * (kEntries + 2));  // [beams * k]
+  int *const s_rank = s_token + n;                                // [beams * k]: those ahead, and 2^16 an end token
+  int *const s_count = s_rank + n;                                // [beams]
+  int *const s_ended = s_count + beams;                           // [1]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int request = blockIdx.x, per_row = p.runs * k;
-  float *const my_value = s_value + wave * per_row;
-  int *const my_token = (int *)(s_value + waves * per_row) + wave * per_row;
+  const int request = blockIdx.x;
   if (threadIdx.x == 0) *s_ended = 0;
+  for (int i = threadIdx.x; i < n; i += threads) s_rank[i] = 0;
   for (int beam = wave; beam < beams; beam += waves) {
+    // every load at once, also where the row turns out dead or its runs fewer
+    const int row = request * beams + beam;
+    const int64_t slot = (int64_t)row * p.most;
     const float c = p.scores[request * p.s_sr + beam * p.s_sb];
+    const int runs = p.share ? p.row_runs[row] : p.runs;
+    double m = lane < p.most ? p.top[slot + lane] : 0.0;
+    double part = lane < p.most ? p.sum[slot + lane] : 0.0;
+    const float *const value = p.value + slot * k;
+    const int *const token = p.token + slot * k;
+    const int at = min(lane, p.most - 1) * k;
+    float v = lane < k ? value[lane] : 0.0f, head = value[at], head1 = value[at + min(1, k - 1)];
+    int t = lane < k ? token[lane] : 0, headt = token[at], headt1 = token[at + min(1, k - 1)];
     int count = 0;
-    unsigned long long ends = 0;
+    u64 ends = 0;
     if (finite(c)) {
-      const int64_t unit = ((int64_t)request * beams + beam) * p.runs;
-      float m = lane < p.runs ? p.top[unit + lane] : -INFINITY;
-      const double part = lane < p.runs ? p.sum[unit + lane] : 0.0;
-      for (int i = lane; i < per_row; i += 64) {
-        my_value[i] = p.value[unit * k + i];
-        my_token[i] = p.token[unit * k + i];
-      }
-      const float top = wave_max(m);
-      // (a NaN stays one: it is in `part`, and a run of -inf alone has the part 0)
-      const double total = wave_sum(m > -INFINITY ? part * exp((double)m - (double)top) : part);
-      const double lse = (double)top + log(total);
-      __builtin_amdgcn_wave_barrier();
-      int at = 0;
-      float head = lane < p.runs ? my_value[lane * k] : -INFINITY, v = -INFINITY;
-      int token = -1;
-      for (int j = 0; j < k; ++j) {
-        const float w = wave_max(head);
-        if (!(w > -INFINITY)) break;
-        const int leader = __builtin_ctzll(__ballot(head == w));
-        const int t = my_token[leader * k + __builtin_amdgcn_readlane(at, leader)];
-        if (lane == j) v = w, token = t;
-        if (lane == leader) {
-          ++at;
-          head = at < k ? my_value[lane * k + at] : -INFINITY;
+      double lse;
+      if (runs == 1) {  // a list in order
+        lse = __shfl(m + log(part), 0);
+        v = lane < k ? v : -INFINITY;
+      } else {
+        m = lane < runs ? m : -(double)INFINITY;
+        part = lane < runs ? part : 0.0;
+        head = lane < runs ? head : -INFINITY;
+        head1 = lane < runs && k > 1 ? head1 : -INFINITY;
+        Best best(s_keys + wave * (kEntries + 2), k);
+        if (runs * k <= kEntries) {  // all of them
+          for (int i = 0; i < runs * k; i += 64) {
+            const int e = min(i + lane, runs * k - 1);
+            best.show(value[e], token[e], i + lane < runs * k);
+          }
+          best.settle();
+        } else {
+          // lists in order: heads first, until no run has one that may be among the best
+          float *const heads = reinterpret_cast<float *>(best.keys);  // (the list is empty)
+          heads[lane] = head;
+          best.bound_by(heads);
+#pragma unroll 1
+          for (int j = 0; j < k; ++j) {
+            const bool ok = head >= best.least && key_of(head, headt) >= best.bar;
+            if (!__ballot(ok)) break;
+            best.show(head, headt, ok);
+            head = ok ? head1 : -INFINITY;
+            headt = headt1;
+            const bool more = ok && j + 2 < k;
+            head1 = more ? value[at + j + 2] : -INFINITY;
+            headt1 = more ? token[at + j + 2] : -1;
+          }
+          best.settle();
         }
+        double top = m;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) top = fmax(top, __shfl_xor(top, off));
+        // (a NaN stays one: it is in `part`, and a run of -inf alone has the part 0)
+        lse = top + log(wave_sum(part == 0.0 ? part : part * exp(m - top)));
+        const u64 key = lane < best.count ? best.keys[lane] : key_of(-INFINITY, -1);
+        v = value_of(key);
+        t = token_of(key);
       }
       const double score = (double)c + ((double)v - lse);
       bool is_end = false;
-      for (int e = 0; e < p.num_ends; ++e) is_end |= token == p.ends[e];
+      for (int e = 0; e < p.num_ends; ++e) is_end |= t == p.ends[e];
       const bool live = lane < k && finite((float)score);
       count = __builtin_popcountll(__ballot(live));  // the first ones: scores fall with the lane
       ends = __ballot(live && is_end);
       if (live) {
         s_score[beam * k + lane] = score;
-        s_token[beam * k + lane] = token;
+        s_token[beam * k + lane] = t;
       }
     }
     if (lane == 0) {
@@ -290,41 +577,41 @@ __global__ __launch_bounds__(512) void beam_join(Params p) {
     }
   }
   __syncthreads();
+  // a thread a candidate and row: those of the row that come before it (lower beams first among equals)
+  for (unsigned i = threadIdx.x; i < (unsigned)(n * beams); i += threads) {
+    const int w = i / (unsigned)n, mine = i - w * n, beam = (unsigned)mine / (unsigned)k, j = mine - beam * k;
+    if (j >= s_count[beam]) continue;
+    const double score = s_score[mine];
+    int lo = 0, hi = s_count[w];
+    if (w == beam) lo = hi = j;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      const double other = s_score[w * k + mid];
+      if (other > score || (other == score && w < beam)) lo = mid + 1;
+      else hi = mid;
+    }
+    const int ahead_ends = __builtin_popcountll(s_end[w] & (((u64)1 << lo) - 1));
+    if (lo) atomicAdd(s_rank + mine, lo + (ahead_ends << 16));  // (whole numbers: no order)
+  }
+  __syncthreads();
   int running = 0;
   for (int w = 0; w < beams; ++w) running += s_count[w] - __builtin_popcountll(s_end[w]);
-  for (int i = threadIdx.x; i < beams * k; i += threads) {
-    const int beam = i / k, j = i - beam * k;
+  for (int i = threadIdx.x; i < n; i += threads) {
+    const int beam = (unsigned)i / (unsigned)k, j = i - beam * k;
     if (j >= s_count[beam]) continue;
-    const double score = s_score[i];
-    const bool is_end = s_end[beam] >> j & 1;
-    int ahead = 0, ahead_ends = 0;
-    for (int w = 0; w < beams; ++w) {
-      int n = j;
-      if (w != beam) {  // those of row w that come before: lower beams first among equals
-        int lo = 0, hi = s_count[w];
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          const double other = s_score[w * k + mid];
-          if (other > score || (other == score && w < beam)) lo = mid + 1;
-          else hi = mid;
-        }
-        n = lo;
-      }
-      ahead += n;
-      ahead_ends += __builtin_popcountll(s_end[w] & (((unsigned long long)1 << n) - 1));
-    }
-    if (is_end) {
+    const int ahead = s_rank[i] & 0xffff, ahead_ends = s_rank[i] >> 16;
+    if (s_end[beam] >> j & 1) {
       if (ahead >= beams) continue;
-      atomicAdd(s_ended, 1);  // (whole numbers)
+      atomicAdd(s_ended, 1);
       const int64_t o = (int64_t)request * beams + ahead_ends;
       p.ended_tokens[o] = s_token[i];
       p.ended_parents[o] = beam;
-      p.ended_scores[o] = (float)score;
+      p.ended_scores[o] = (float)s_score[i];
     } else if (ahead - ahead_ends < beams) {
       const int64_t o = (int64_t)request * beams + (ahead - ahead_ends);
       p.tokens[o] = s_token[i];
       p.parents[o] = beam;
-      p.scores_out[o] = (float)score;
+      p.scores_out[o] = (float)s_score[i];
     }
   }
   __syncthreads();
@@ -365,18 +652,20 @@ int64_t rows_of(const l20_pd_beam_step_args *a) { return (int64_t)a->requests * 
 int steps_of(const l20_pd_beam_step_args *a) { return (int)(((int64_t)a->vocab + l20bs::kStep - 1) / l20bs::kStep); }
 int listed_of(const l20_pd_beam_step_args *a) { return std::min(a->beams + a->num_end_tokens, a->vocab); }
 
-// Runs a row: rows times runs is about what the chip holds, a run is one step at least.
-int runs_of(const l20_pd_beam_step_args *a, int cus) {
-  const int64_t rows = std::max<int64_t>(1, rows_of(a)), waves = (int64_t)cus * l20bs::kWavesPerCu;
-  return (int)std::min<int64_t>(std::min(l20bs::kMaxRuns, steps_of(a)), std::max<int64_t>(1, (waves + rows - 1) / rows));
+// (a run: a step of each wave at least)
+int most_runs(const l20_pd_beam_step_args *a) {
+  return std::min(l20bs::kMaxRuns, (steps_of(a) + l20bs::kWaves - 1) / l20bs::kWaves);
 }
+int spread_of(int cus) { return cus * l20bs::kRunsPerCu; }
 
-// For every number of requests up to this one: rows times runs_of() is below waves + rows.
-int64_t units_bound(const l20_pd_beam_step_args *a, int cus) {
-  const int64_t rows = rows_of(a), most = std::min(l20bs::kMaxRuns, steps_of(a));
-  return std::min(rows * most, rows + (int64_t)cus * l20bs::kWavesPerCu);
+// Workgroups for every number of live rows up to this many: rows times their runs is at most the larger of rows and
+// what they are spread over.
+int64_t units_of(const l20_pd_beam_step_args *a, int cus) {
+  return std::min(rows_of(a) * most_runs(a), std::max<int64_t>(rows_of(a), spread_of(cus)));
 }
-int64_t bytes_of(int64_t units, int k) { return units * (16 + 8 * (int64_t)k); }
+int64_t bytes_of(const l20_pd_beam_step_args *a) {
+  return rows_of(a) * (8 + most_runs(a) * (16 + 8 * (int64_t)listed_of(a)));
+}
 
 int32_t launched() {
   const hipError_t e = hipGetLastError();
@@ -417,9 +706,9 @@ int32_t l20_pd_beam_step_check(const l20_pd_beam_step_args *a) {
   return check(a);
 }
 
-int64_t l20_pd_beam_step_workspace(const l20_pd_beam_step_args *a, int32_t cus) {
+int64_t l20_pd_beam_step_workspace(const l20_pd_beam_step_args *a) {
   if (!a || a->requests < 1 || a->beams < 1 || a->vocab < 1 || a->num_end_tokens < 0) return 0;
-  return bytes_of(units_bound(a, cus > 0 ? cus : l20la::device_cus()), listed_of(a));
+  return bytes_of(a);
 }
 
 int32_t l20_pd_beam_step(const l20_pd_beam_step_args *a, void *stream) {
@@ -427,10 +716,14 @@ int32_t l20_pd_beam_step(const l20_pd_beam_step_args *a, void *stream) {
   int32_t rc = check(a);
   if (rc != L20_PD_OK || a->requests == 0) return rc;
   l20bs::Params p{};
-  p.runs = runs_of(a, l20la::device_cus());
+  const int cus = l20la::device_cus();
   p.k = listed_of(a);
-  const int64_t rows = rows_of(a), units = rows * p.runs;
-  if (!a->workspace || (uintptr_t)a->workspace % 8 || a->workspace_bytes < bytes_of(units, p.k))
+  p.most = most_runs(a);
+  p.spread = spread_of(cus);
+  const int64_t rows = rows_of(a), units = units_of(a, cus);
+  p.runs = std::min(p.most, std::max((int)(p.spread / rows), 1));
+  p.share = p.runs < p.most && rows <= l20bs::kCounted;
+  if (!a->workspace || (uintptr_t)a->workspace % 8 || a->workspace_bytes < bytes_of(a))
     return set_error(L20_PD_EINVAL, "workspace is missing, misaligned or too small");
   rc = overlaps(a);
   if (rc != L20_PD_OK) return rc;
@@ -445,27 +738,28 @@ int32_t l20_pd_beam_step(const l20_pd_beam_step_args *a, void *stream) {
   p.vocab = a->vocab;
   p.num_ends = a->num_end_tokens;
   for (int i = 0; i < p.num_ends; ++i) p.ends[i] = a->end_tokens[i];
+  p.flat = (a->beams == 1 || a->s_stride_beam == 1) && (a->requests == 1 || a->s_stride_request == a->beams);
+  const int64_t slots = rows * p.most;
   p.sum = reinterpret_cast<double *>(a->workspace);
-  p.top = reinterpret_cast<float *>(p.sum + units);
-  p.value = p.top + units;
-  p.token = reinterpret_cast<int *>(p.value + units * p.k);
+  p.top = p.sum + slots;
+  p.value = reinterpret_cast<float *>(p.top + slots);
+  p.token = reinterpret_cast<int *>(p.value + slots * p.k);
+  p.row_runs = p.token + slots * p.k;
   p.tokens = a->tokens;
   p.parents = a->parents;
   p.scores_out = a->scores_out;
   p.ended_tokens = a->ended_tokens;
   p.ended_parents = a->ended_parents;
   p.ended_scores = a->ended_scores;
-  const int per_row = 8 * p.runs * p.k;  // at most 20 KB
-  p.join_waves = std::min({a->beams, 8, std::max(1, l20bs::kJoinLds / per_row)});
+  p.join_waves = std::min(a->beams, 8);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)((units + 3) / 4));
-  if (a->dtype == L20_PD_BF16) hipLaunchKernelGGL(l20bs::beam_scan<__bf16>, grid, dim3(256), 0, s, p);
-  else if (a->dtype == L20_PD_FP16) hipLaunchKernelGGL(l20bs::beam_scan<_Float16>, grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL(l20bs::beam_scan<float>, grid, dim3(256), 0, s, p);
+  const dim3 grid((unsigned)units), block(64 * l20bs::kWaves);
+  if (a->dtype == L20_PD_BF16) hipLaunchKernelGGL(l20bs::beam_scan<__bf16>, grid, block, 0, s, p);
+  else if (a->dtype == L20_PD_FP16) hipLaunchKernelGGL(l20bs::beam_scan<_Float16>, grid, block, 0, s, p);
+  else hipLaunchKernelGGL(l20bs::beam_scan<float>, grid, block, 0, s, p);
   rc = launched();
   if (rc != L20_PD_OK) return rc;
-  // scores and tokens of a request's candidates (at most 15.5 KB with their counts), and the lists: below 64 KB
-  const size_t lds = (size_t)a->beams * (p.k * 12 + 12) + 4 + (size_t)p.join_waves * per_row;
+  const size_t lds = (size_t)a->beams * (p.k * 16 + 12) + 12 + (size_t)p.join_waves * (l20bs::kEntries + 2) * 8;  // at most 29 KB
   hipLaunchKernelGGL(l20bs::beam_join, dim3((unsigned)a->requests), dim3(64 * p.join_waves), lds, s, p);
   return launched();
 }

@@ -15,7 +15,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 import l20_paged_decode  # noqa: F401  (loads the ops library)
-from l20_paged_split_kv import _gpu_facts, gpu_cus
+from l20_paged_split_kv import _gpu_facts
 
 MAX_BEAMS = 32
 MAX_END_TOKENS = 8
@@ -41,19 +41,19 @@ class BeamSearchStep(NamedTuple):
 
 
 @lru_cache(maxsize=4096)
-def _bytes(requests: int, beams: int, vocab: int, ends: int, cus: int) -> int:
+def _bytes(requests: int, beams: int, vocab: int, ends: int) -> int:
     import l20_pd_cabi
 
     a = l20_pd_cabi.L20PdBeamStepArgs()
     a.requests, a.beams, a.vocab, a.num_end_tokens = requests, beams, vocab, ends
-    return int(l20_pd_cabi.load().l20_pd_beam_step_workspace(l20_pd_cabi.ctypes.byref(a), cus))
+    return int(l20_pd_cabi.load().l20_pd_beam_step_workspace(l20_pd_cabi.ctypes.byref(a)))
 
 
 def allocate_l20_beam_search_workspace(logits: torch.Tensor, scores: torch.Tensor, *,
                                        end_tokens: Sequence[int] = ()) -> torch.Tensor:
-    """The workspace of ``l20_beam_search_step`` for these beams, vocabulary and number of end tokens, and up to as
-    many requests (uint8).  Calls that may overlap each need their own; its contents do not matter."""
-    size = _bytes(scores.shape[0], scores.shape[1], logits.shape[-1], len(end_tokens), gpu_cus(logits.device))
+    """The workspace of ``l20_beam_search_step`` for up to these requests, beams, vocabulary and number of end tokens
+    (uint8).  Calls that may overlap each need their own; its contents do not matter."""
+    size = _bytes(scores.shape[0], scores.shape[1], logits.shape[-1], len(end_tokens))
     return torch.empty(size, dtype=torch.uint8, device=logits.device)
 
 

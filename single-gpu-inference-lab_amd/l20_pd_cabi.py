@@ -316,11 +316,10 @@ def load(path: Optional[Path] = None) -> ctypes.CDLL:
     lib.l20_pd_paged_latent_workspace.restype = _i64
     lib.l20_pd_latent_prompt_workspace.argtypes = [ctypes.POINTER(L20PdLatentPromptArgs), _i32]
     lib.l20_pd_latent_prompt_workspace.restype = _i64
-    for name, struct in (("reorder_tables", L20PdReorderArgs), ("compact_pages", L20PdCompactArgs)):
+    for name, struct in (("reorder_tables", L20PdReorderArgs), ("compact_pages", L20PdCompactArgs),
+                         ("beam_step", L20PdBeamStepArgs)):
         getattr(lib, f"l20_pd_{name}_workspace").argtypes = [ctypes.POINTER(struct)]
         getattr(lib, f"l20_pd_{name}_workspace").restype = _i64
-    lib.l20_pd_beam_step_workspace.argtypes = [ctypes.POINTER(L20PdBeamStepArgs), _i32]
-    lib.l20_pd_beam_step_workspace.restype = _i64
     if path is None:
         _lib = lib
     return lib

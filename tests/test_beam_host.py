@@ -215,11 +215,17 @@ def test_workspaces_are_enough_for_smaller_calls():
     lib, a = cabi.load(), beam_args()
     for beams, vocab, ends in ((1, 1, 0), (4, 152064, 1), (32, 50257, 8), (5, 2049, 2), (32, 200, 8)):
         a.beams, a.vocab, a.num_end_tokens = beams, vocab, ends
-        for cus in (256, 64):
-            sizes = []
-            for a.requests in [*range(1, 300), 1000, 4096, 30000]:
-                sizes.append(lib.l20_pd_beam_step_workspace(ctypes.byref(a), cus))
-            assert sizes == sorted(sizes) and sizes[0] > 0
+        sizes = []
+        for a.requests in [*range(1, 300), 1000, 4096, 30000]:
+            sizes.append(lib.l20_pd_beam_step_workspace(ctypes.byref(a)))
+        assert sizes == sorted(sizes) and sizes[0] > 0
+    for name, values in (("vocab", [*range(1, 40), *range(40, 300000, 777)]), ("beams", range(1, 33)), ("num_end_tokens", range(9))):
+        a = beam_args()
+        sizes = []
+        for value in values:
+            setattr(a, name, value)
+            sizes.append(lib.l20_pd_beam_step_workspace(ctypes.byref(a)))
+        assert sizes == sorted(sizes), name
     r = reorder_args()
     sizes = []
     for r.groups in range(1, 50):
@@ -229,8 +235,7 @@ def test_workspaces_are_enough_for_smaller_calls():
     c = compact_args()
     assert lib.l20_pd_compact_pages_workspace(ctypes.byref(c)) == 4 * (500 + 2 * 16)
     for name in ("beam_step", "reorder_tables", "compact_pages"):
-        args = (None, 256) if name == "beam_step" else (None,)
-        assert getattr(lib, f"l20_pd_{name}_workspace")(*args) == 0
+        assert getattr(lib, f"l20_pd_{name}_workspace")(None) == 0
 
 
 def test_functions_refuse_cpu_tensors():

@@ -150,6 +150,27 @@ def test_far_values(dtype):
     assert out.scores.cpu().equal(torch.full((1, 3), -1e30))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("level", [-300.0, 5.0, 300.0, 60000.0])
+def test_rows_that_begin_masked(dtype, level):
+    """Nothing finite, or only the type's lowest value, in the first 40000 tokens; logits far from zero behind them."""
+    d = DTYPES[dtype]
+    if level == 60000.0 and dtype != "fp16":
+        level = 2.0 ** 22
+    logits, scores = inputs(4, 2, 50000, d, seed=77)
+    step = {"bf16": 2.0 ** -7, "fp16": 2.0 ** -10, "fp32": 2.0 ** -23}[dtype] * abs(level)
+    late = level + step * torch.randint(-20, 20, (4, 2, 10000), generator=torch.Generator().manual_seed(1))
+    logits[:, :, 40000:] = late.to(d)
+    logits[0, :, :40000] = -math.inf
+    logits[1, :, :40000] = torch.finfo(d).min
+    logits[2, 0, :49990] = -math.inf
+    logits[2, 1, :49990] = torch.finfo(d).min
+    logits[3, 0] = torch.finfo(d).min
+    logits[3, 0, 45000] = level
+    logits[3, 1, 1:] = -math.inf
+    check(logits, scores, [49999])
+
+
 @pytest.mark.parametrize("order", ["rising", "falling", "blocks"])
 def test_orders_that_pass_every_threshold(order):
     x = torch.arange(9000.0) / 1000
