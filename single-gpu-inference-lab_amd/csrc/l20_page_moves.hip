@@ -2,13 +2,13 @@
 // compaction, and the copies of pages that both ask for.
 //
 //  rp_cells   a wave a group of beams and 64 columns of its rows, a lane a column.  All of a column's cells are in
-//    LDS before any is written, so rows exchange in place.  What the group's holders of a page change is added to
-//    page_shares in one atomic: the sum reaches -1 in the one atomic after which no row anywhere holds the page (a
-//    group only adds holders to pages that it holds), whatever the order.  Freed pages go to a list a wave.
-//  rp_pool    one workgroup.  The freed pages are put into a bitmap, so that they go on the stack by number and not
-//    by the order of atomics; then the rows that need a copy take theirs, by two scans.
-//  cp_clear, cp_mark, cp_scan, cp_remap   pages to move and pages to move to as bitmaps, their ranks by one
-//    workgroup's scan, and the table's cells after them.
+//    LDS before any is written, so rows exchange in place; the changes of page_shares are atomics whose order does
+//    not matter.  Freed pages go to a list a wave.
+//  rp_pool    one workgroup.  Freed pages go on the stack by number, not by the order of atomics, through a bitmap in
+//    LDS; then the rows that need a copy take theirs.
+//  rp_small   both in one launch.
+//  cp_clear, cp_mark, cp_place, cp_remap   pages to move and pages to move to as bitmaps; a page's rank among them,
+//    and so its place, from the bits before it; the table's cells by the ranks.  cp_small: all of it in one launch.
 //  pc_copy    workgroups take (pair, cache, 16 KB) in turn.
 
 #include "l20_block_tables.h"
@@ -26,8 +26,11 @@ using l20la::i32x4;
 constexpr int kThreads = 1024;
 constexpr int kPerThread = L20_PD_MAX_REQUESTS / kThreads;
 constexpr int kCellWaves = 4;
-constexpr int kBitmap = 1 << 19;  // pages of one pass of rp_pool (64 KB of LDS)
-constexpr int kUnits = 8192;      // waves' lists that rp_pool looks at together
+constexpr int kBitmap = 1 << 18;  // pages of one pass of rp_pool (32 KB of LDS)
+constexpr int kUnits = 4096;      // waves' lists that rp_pool looks at together
+constexpr int kSmall = 16;        // waves' worth of cells that one launch does with the pool
+constexpr int kSmallPages = 1 << 16;  // pages and cells (a row: a multiple of 64) of a compaction in one launch
+constexpr int kSmallCells = 1 << 14;
 
 __device__ __forceinline__ int pages_of(int tokens, int page) { return tokens > 0 ? (int)(((int64_t)tokens + page - 1) / page) : 0; }
 
@@ -52,6 +55,13 @@ __device__ __forceinline__ int scan(int x, int *s_wave, int &total) {
   return x;
 }
 
+// The maximum over the wave (of values that are not negative).
+__device__ __forceinline__ int max_of(int x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x = max(x, __shfl_xor(x, off));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
 struct Reorder {
   const int32_t *parents;
   int32_t *table;
@@ -73,26 +83,32 @@ struct Reorder {
   int32_t *source;      // [groups * beams] the page that a row's copy comes from
 };
 
-// What becomes of a row, from its group's parents and lengths (a lane a row).
+// What becomes of a row, from its group's parents and lengths.
 struct Row {
   int parent;  // -1: given up
   int len;     // new
   int copy;    // the column of its own copy, -1: none
 };
-__device__ __forceinline__ Row row_of(int row, int beams, int parent, int parent_len, bool parent_stays, bool first, int page, int width) {
+__device__ __forceinline__ Row row_of(int row, int parent, int parent_len, bool parent_stays, bool first, int page, int width) {
   Row r{parent, parent >= 0 ? max(parent_len, 0) : 0, -1};
   const bool keeps = parent_stays ? parent == row : first;
   if (parent >= 0 && r.len % page != 0 && !keeps && r.len / page < width) r.copy = r.len / page;
   return r;
 }
 
-__global__ __launch_bounds__(64 * kCellWaves) void rp_cells(Reorder p) {
-  extern __shared__ int s_cells[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int group = blockIdx.y, block = blockIdx.x * kCellWaves + wave;
-  if (block >= p.blocks) return;
-  const int beams = p.beams, c = block * 64 + lane;
-  int *const mine = s_cells + wave * beams * 64 + lane;  // this lane's column: [beams], 64 apart
+// One wave's 64 columns of a group; s_cells: [beams][64] of the wave.  `free_page(page, where)` takes the lanes' pages that
+// nobody holds any more, `source(row, page)` the page that a row's copy comes from.
+//
+// A row whose parent row r has n children: n - 1 more rows hold each full page of r, and its last page, where that is not
+// full, one row or none.  So r's page in column c gains n - 1 holders, or loses one (the last page without children),
+// whatever else holds it.  Where all rows hold one page the changes are added up first (a prefix: mostly nothing is
+// left); elsewhere they go to page_shares one by one, gains before losses: the number of holders a group adds up to is
+// then never below both its old and its new one, so the sum reaches -1 in one atomic only, the one after which no row of
+// any group holds the page, whatever the order.
+template <typename F, typename S>
+__device__ __forceinline__ void follow_parents(const Reorder &p, int group, int block, int *s_cells, F free_page, S source) {
+  const int lane = threadIdx.x & 63, beams = p.beams, c = block * 64 + lane;
+  int *const mine = s_cells + lane;  // this lane's column: [beams], 64 apart
   // a lane a row
   const int known = min(lane, beams - 1), at = group * beams + known;
   const int old_len = max(p.lens[at], 0);
@@ -100,159 +116,227 @@ __global__ __launch_bounds__(64 * kCellWaves) void rp_cells(Reorder p) {
   if (parent < 0 || parent >= beams) parent = -1;
   const int from = max(parent, 0);
   const int parent_len = __shfl(old_len, from), grandparent = __shfl(parent, from);  // (by every lane)
-  const bool stays = parent >= 0 && grandparent == parent;
   bool first = true;
+  int children = 0;
   for (int i = 0; i < beams; ++i) {
     const int other = __builtin_amdgcn_readlane(parent, i);
-    if (i < lane && other == parent) first = false;
+    first &= !(i < lane && other == parent);
+    children += other == lane;
   }
-  const Row row = row_of(known, beams, parent, parent_len, stays, first, p.page, p.width);
+  const Row row = row_of(known, parent, parent_len, parent >= 0 && grandparent == parent, first, p.page, p.width);
   const int held = min(pages_of(old_len, p.page), p.width), new_held = min(pages_of(row.len, p.page), p.width);
-  int32_t *const cells = p.table + (int64_t)group * beams * p.t_sr + c;
-  auto has = [&](int i) { return c < __builtin_amdgcn_readlane(held, i); };
-  for (int i = 0; i < beams; ++i) mine[i * 64] = has(i) ? cells[i * p.t_sr] : -1;
-  // whether row i takes its parent's cell (not its own copy's, and none beyond its length), and what that is, else -1
-  auto next = [&](int i, int &v) {
-    const int q = __builtin_amdgcn_readlane(row.parent, i);
-    const bool follows = q >= 0 && c < __builtin_amdgcn_readlane(new_held, i) && c != __builtin_amdgcn_readlane(row.copy, i);
-    v = follows ? mine[q * 64] : -1;
-    return follows;
+  const int partial = old_len % p.page ? old_len / p.page : -1;  // the column of a last page that is not full
+  const int most = max_of(lane < beams ? max(held, new_held) : 0);
+  if (block * 64 >= most) return;  // nothing here
+  int32_t *const cells = p.table + (int64_t)group * beams * p.t_sr + min(c, p.width - 1);
+  // the cells: loads of eight rows at once (of a lane behind the table: its last column)
+  bool same = true;  // all rows hold the page of row 0
+  int page0 = -1;
+  for (int i0 = 0; i0 < beams; i0 += 8) {
+    int v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + i < beams) v[i] = cells[(i0 + i) * p.t_sr];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= beams) break;
+      const bool has = c < __builtin_amdgcn_readlane(held, i0 + i);
+      v[i] = has ? v[i] : -1;
+      mine[(i0 + i) * 64] = v[i];
+      if (i0 + i == 0) page0 = v[i];
+      same &= has && v[i] == page0;
+    }
+  }
+  auto held_page = [&](int v) { return v >= 0 && v < p.pages; };
+  // page_shares
+  auto freed = [&](int v, bool gone) {
+    if (gone) p.shares[v] = 0;
+    free_page(v, __ballot(gone));
   };
-  bool any = false;
+  auto change_of = [&](int r) {
+    const int n = __builtin_amdgcn_readlane(children, r);
+    return c == __builtin_amdgcn_readlane(partial, r) ? min(n, 1) - 1 : n - 1;
+  };
+  int together = 0;
+  bool gains = false, losses = false;
+  for (int r = 0; r < beams; ++r) {
+    const int d = change_of(r);
+    together += d;
+    gains |= __builtin_amdgcn_readlane(children, r) > 1;
+    losses |= __builtin_amdgcn_readlane(children, r) == 0;
+  }
+  if (gains || losses) {
+    same &= held_page(page0);
+    if (__ballot(same && together != 0)) {
+      bool gone = false;
+      if (same && together != 0) gone = atomicAdd(p.shares + page0, together) + together == -1;
+      freed(page0, gone);
+    }
+    if (__ballot(!same)) {
+      if (gains) {
+        for (int r = 0; r < beams; ++r) {
+          if (__builtin_amdgcn_readlane(children, r) <= 1) continue;
+          const int v = mine[r * 64], d = change_of(r);
+          if (!same && d > 0 && held_page(v)) atomicAdd(p.shares + v, d);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // gains before losses
+      }
+      if (losses) {
+        for (int r0 = 0; r0 < beams; r0 += 8) {
+          int v[8], was[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = -1;
+            was[i] = 1;
+            if (r0 + i >= beams || __builtin_amdgcn_readlane(children, min(r0 + i, beams - 1)) != 0) continue;
+            v[i] = same ? -1 : mine[(r0 + i) * 64];
+            if (held_page(v[i])) was[i] = atomicAdd(p.shares + v[i], -1);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (__ballot(was[i] == 0)) freed(v[i], was[i] == 0);
+        }
+      }
+    }
+  }
+  // the table
   for (int i = 0; i < beams; ++i) {
     const int q = __builtin_amdgcn_readlane(row.parent, i), copy = __builtin_amdgcn_readlane(row.copy, i);
-    if (q >= 0 && c == copy) p.source[group * beams + i] = mine[q * 64];
-    int v;
-    any |= next(i, v) != has(i) || v != mine[i * 64];
+    if (q < 0 || (q == i && copy < 0)) continue;  // given up, or as it was
+    const int v = mine[q * 64];
+    if (c == copy) source(group * beams + i, v);
+    else if (c < __builtin_amdgcn_readlane(new_held, i) && !(c < __builtin_amdgcn_readlane(held, i) && v == mine[i * 64]))
+      cells[i * p.t_sr] = v;
   }
-  const int unit = group * p.blocks + block;
-  int listed = 0;
-  if (__ballot(any)) {
-    int32_t *const list = p.list + (int64_t)unit * beams * 64;
-    for (int r = 0; r < beams; ++r) {
-      const int v = mine[r * 64];
-      bool gone = false;
-      if (any && v >= 0 && v < p.pages) {
-        int change = 0;
-        bool seen = false;  // in an earlier row: counted there
-        for (int i = 0; i < beams; ++i) {
-          const bool same = mine[i * 64] == v;
-          int w;
-          next(i, w);
-          seen |= same && i < r;
-          change += (w == v) - same;
-        }
-        if (!seen && change != 0) gone = atomicAdd(p.shares + v, change) + change == -1;
-        if (gone) p.shares[v] = 0;
-      }
-      const unsigned long long which = __ballot(gone);
-      if (gone) list[listed + __builtin_popcountll(which & (((unsigned long long)1 << lane) - 1))] = v;
-      listed += __builtin_popcountll(which);
-    }
-    for (int i = 0; i < beams; ++i) {
-      int v;
-      if (next(i, v) && (!has(i) || v != mine[i * 64])) cells[i * p.t_sr] = v;
-    }
-  }
-  if (lane == 0) p.list_count[unit] = listed;
 }
 
-__global__ __launch_bounds__(kThreads) void rp_pool(Reorder p) {
-  extern __shared__ int s_mem[];
-  __shared__ int s_wave[kThreads / 64];
-  unsigned int *const s_bits = (unsigned int *)s_mem;  // [min(pages, kBitmap) / 32]
-  int *const s_at = s_mem + (min(p.pages, kBitmap) + 31) / 32;  // [kUnits + 1]: list offsets, then the parents
-  int *const s_len = s_at + kUnits + 1;                         // [rows] old lengths
+// LDS of share_out, in ints: the bitmap, list offsets, then lengths, parents and the freed pages that are on top.
+__host__ __device__ constexpr int bitmap_words(int pages) { return ((pages < kBitmap ? pages : kBitmap) + 31) / 32; }
+__host__ __device__ constexpr int pool_ints(int pages, int units, int rows) {
+  return bitmap_words(pages) + (units < kUnits ? units : kUnits) + 1 + 3 * rows;
+}
+
+// The pool, one workgroup: freed pages onto the stack by number, then each row's copy from it.  The pages to take are the
+// last that were freed, or lie where nothing is written: nothing is read back.  `marked`: the freed pages are in the
+// bitmap already, else in lists a wave.
+__device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int *s_wave, bool marked, const int *s_source) {
   const int tid = threadIdx.x, rows = p.groups * p.beams, units = p.groups * p.blocks;
+  unsigned int *const s_bits = (unsigned int *)s_mem;
+  int *const s_at = s_mem + bitmap_words(p.pages), *const s_len = s_at + min(units, kUnits) + 1;
+  int *const s_parent = s_len + rows, *const s_top = s_parent + rows;
   const int count = min(max(*p.count, 0), p.pool);
-  for (int r = tid; r < rows; r += kThreads) s_len[r] = p.lens[r];
-  // freed pages onto the stack, by number
-  int freed = 0;
-  for (int base = 0; base < p.pages; base += kBitmap) {
-    const int n = min(p.pages - base, kBitmap), words = (n + 31) / 32;
-    for (int i = tid; i < words; i += kThreads) s_bits[i] = 0;
-    bool some = false;
-    for (int u0 = 0; u0 < units; u0 += kUnits) {
-      const int here = min(units - u0, kUnits), per = (here + kThreads - 1) / kThreads;
-      int mine = 0;
-      for (int i = 0; i < per; ++i) {
-        const int u = tid * per + i;
-        if (u < here) mine += p.list_count[u0 + u];
-      }
-      int total;
-      int at = scan(mine, s_wave, total) - mine;  // (its barriers: the bitmap is clear, the offsets are read)
-      if (total == 0) continue;
-      some = true;
-      for (int i = 0; i < per; ++i) {
-        const int u = tid * per + i;
-        if (u < here) {
-          s_at[u] = at;
-          at += p.list_count[u0 + u];
-        }
-      }
-      if (tid == 0) s_at[here] = total;
-      __syncthreads();
-      for (int k = tid; k < total; k += kThreads) {
-        int lo = 0, hi = here - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (s_at[mid] <= k) lo = mid;
-          else hi = mid - 1;
-        }
-        const int v = p.list[(int64_t)(u0 + lo) * p.beams * 64 + (k - s_at[lo])] - base;
-        if (v >= 0 && v < n) atomicOr(s_bits + (v >> 5), 1u << (v & 31));
-      }
-    }
-    __syncthreads();
-    if (!some) break;  // (the same lists for every base)
-    const int per = (words + kThreads - 1) / kThreads;
-    int mine = 0;
-    for (int i = 0; i < per; ++i)
-      if (tid * per + i < words) mine += __builtin_popcount(s_bits[tid * per + i]);
-    int total;
-    int64_t at = (int64_t)count + freed + scan(mine, s_wave, total) - mine;
-    for (int i = 0; i < per && tid * per + i < words; ++i)
-      for (unsigned int w = s_bits[tid * per + i]; w; w &= w - 1, ++at)
-        if (at < p.pool) p.stack[at] = base + (tid * per + i) * 32 + __builtin_ctz(w);
-    freed += total;
-    __syncthreads();
+  for (int r = tid; r < rows; r += kThreads) {
+    s_len[r] = p.lens[r];
+    s_parent[r] = p.parents[r];
   }
-  const int have = (int)min((int64_t)count + freed, (int64_t)p.pool);
-  __syncthreads();
-  // rows that need a page, in order
-  int *const s_parent = s_at;
-  for (int r = tid; r < rows; r += kThreads) s_parent[r] = p.parents[r];
-  __syncthreads();
-  const int per = (rows + kThreads - 1) / kThreads;
-  Row row[kPerThread];
-  int wanted = 0;
+  constexpr int kLists = kUnits / kThreads;
+  int lengths[kLists];  // of the first kUnits lists
+#pragma unroll
+  for (int i = 0; i < kLists; ++i) {
+    const int u = tid * kLists + i;
+    lengths[i] = !marked && u < units ? p.list_count[u] : 0;
+  }
+  const int per_row = (rows + kThreads - 1) / kThreads;
+  int from[kPerThread];  // (of rows without a copy: whatever is there)
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int r = tid * per + i;
+    const int r = tid * per_row + i;
+    if (i < per_row && r < rows) from[i] = s_source ? s_source[r] : p.source[r];
+  }
+  // rows that need a page, in order
+  Row row[kPerThread];
+  int wanted = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    const int r = tid * per_row + i;
     row[i] = Row{-1, 0, -1};
-    if (i < per && r < rows) {
+    if (i < per_row && r < rows) {
       const int group = r / p.beams, me = r - group * p.beams;
       const int *const family = s_parent + group * p.beams;
       int parent = family[me];
       if (parent < 0 || parent >= p.beams) parent = -1;
       bool first = true;
       for (int j = 0; j < me; ++j) first &= family[j] != parent;
-      row[i] = row_of(me, p.beams, parent, s_len[group * p.beams + max(parent, 0)], parent >= 0 && family[parent] == parent, first,
-                      p.page, p.width);
+      row[i] = row_of(me, parent, s_len[group * p.beams + max(parent, 0)], parent >= 0 && family[parent] == parent, first, p.page,
+                      p.width);
       wanted += row[i].copy >= 0;
     }
   }
   int total;
-  int64_t k = scan(wanted, s_wave, total) - wanted;
-  int got[kPerThread], served = 0;
+  const int first_wanted = scan(wanted, s_wave, total) - wanted;
+  // freed pages, by number; places from the top are known once all are counted
+  int freed = 0;
+  auto push = [&](int base, int words) {
+    const int per = (words + kThreads - 1) / kThreads;
+    int mine = 0;
+    for (int i = 0; i < per; ++i)
+      if (tid * per + i < words) mine += __builtin_popcount(s_bits[tid * per + i]);
+    int here;
+    int rank = freed + scan(mine, s_wave, here) - mine;
+    const int last = min(freed + here, p.pool - count);  // (`rows` of these: a place each)
+    for (int i = 0; i < per && tid * per + i < words; ++i)
+      for (unsigned int w = s_bits[tid * per + i]; w; w &= w - 1, ++rank) {
+        const int page = base + (tid * per + i) * 32 + __builtin_ctz(w);
+        if (rank >= last) continue;
+        p.stack[count + rank] = page;
+        if (rank >= last - rows) s_top[rank % rows] = page;
+      }
+    freed += here;
+    __syncthreads();
+  };
+  if (marked) {
+    push(0, bitmap_words(p.pages));
+  } else {
+    for (int base = 0; base < p.pages; base += kBitmap) {
+      const int n = min(p.pages - base, kBitmap), words = (n + 31) / 32;
+      for (int i = tid; i < words; i += kThreads) s_bits[i] = 0;
+      bool some = false;
+      for (int u0 = 0; u0 < units; u0 += kUnits) {  // the entries of kUnits lists, spread over the threads
+        const int here = min(units - u0, kUnits);
+        int mine = 0, length[kLists];
+#pragma unroll
+        for (int i = 0; i < kLists; ++i) {
+          const int u = u0 + tid * kLists + i;
+          length[i] = u0 == 0 ? lengths[i] : u < units ? p.list_count[u] : 0;
+          mine += length[i];
+        }
+        int entries;
+        int at = scan(mine, s_wave, entries) - mine;  // (its barriers: the bitmap is clear, the offsets are read)
+        if (entries == 0) continue;
+        some = true;
+#pragma unroll
+        for (int i = 0; i < kLists; ++i) {
+          if (tid * kLists + i < here) s_at[tid * kLists + i] = at;
+          at += length[i];
+        }
+        __syncthreads();
+        for (int k = tid; k < entries; k += kThreads) {
+          int lo = 0, hi = here - 1;
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_at[mid] <= k) lo = mid;
+            else hi = mid - 1;
+          }
+          const int v = p.list[(int64_t)(u0 + lo) * p.beams * 64 + (k - s_at[lo])] - base;
+          if (v >= 0 && v < n) atomicOr(s_bits + (v >> 5), 1u << (v & 31));
+        }
+      }
+      __syncthreads();
+      if (!some) break;  // (the same lists for every base)
+      push(base, words);
+    }
+  }
+  const int have = (int)min((int64_t)count + freed, (int64_t)p.pool), kept = have - count;
+  int got[kPerThread], served = 0, k = first_wanted;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int r = tid * per + i;
+    const int r = tid * per_row + i;
     got[i] = -1;
-    if (i < per && r < rows) {
+    if (i < per_row && r < rows) {
       p.lens[r] = row[i].len;
       if (row[i].copy >= 0) {
-        if (k < have) got[i] = p.stack[have - 1 - k];
+        if (k < have) got[i] = k < kept ? s_top[(kept - 1 - k) % rows] : p.stack[have - 1 - k];
         ++k;
         if (got[i] < 0 || got[i] >= p.pages) got[i] = -1;
         p.table[r * p.t_sr + row[i].copy] = got[i];
@@ -260,13 +344,12 @@ __global__ __launch_bounds__(kThreads) void rp_pool(Reorder p) {
       }
     }
   }
-  int pairs;
-  int at = scan(served, s_wave, pairs) - served;
+  int pairs = total, at = first_wanted;
+  if (__syncthreads_or(served != wanted)) at = scan(served, s_wave, pairs) - served;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int r = tid * per + i;
-    if (i < per && r < rows && got[i] >= 0) {
-      p.src[at] = p.source[r];
+    if (got[i] >= 0) {
+      p.src[at] = from[i];
       p.dst[at] = got[i];
       p.tokens[at] = row[i].len % p.page;
       ++at;
@@ -278,6 +361,53 @@ __global__ __launch_bounds__(kThreads) void rp_pool(Reorder p) {
     p.pairs[1] = total - pairs;
     *p.count = have - min(total, have);
   }
+}
+
+__global__ __launch_bounds__(64 * kCellWaves) void rp_cells(Reorder p) {
+  extern __shared__ int s_mem[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int group = blockIdx.y, block = blockIdx.x * kCellWaves + wave;
+  if (block >= p.blocks) return;
+  const int unit = group * p.blocks + block;
+  int32_t *const list = p.list + (int64_t)unit * p.beams * 64;
+  int listed = 0;
+  follow_parents(
+      p, group, block, s_mem + wave * p.beams * 64,
+      [&](int v, unsigned long long which) {
+        if (which >> lane & 1) list[listed + __builtin_popcountll(which & (((unsigned long long)1 << lane) - 1))] = v;
+        listed += __builtin_popcountll(which);
+      },
+      [&](int row, int v) { p.source[row] = v; });
+  if (lane == 0) p.list_count[unit] = listed;
+}
+
+__global__ __launch_bounds__(kThreads) void rp_pool(Reorder p) {
+  extern __shared__ int s_mem[];
+  __shared__ int s_wave[kThreads / 64];
+  share_out(p, s_mem, s_wave, false, nullptr);
+}
+
+// Both in one launch, for few waves' worth of cells: freed pages go straight into the bitmap.
+__global__ __launch_bounds__(kThreads) void rp_small(Reorder p) {
+  extern __shared__ int s_mem[];
+  __shared__ int s_wave[kThreads / 64];
+  __shared__ int s_source[kSmall * L20_PD_MAX_BEAMS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int units = p.groups * p.blocks, words = bitmap_words(p.pages);
+  int *const s_cells = s_mem + pool_ints(p.pages, units, p.groups * p.beams);
+  for (int i = threadIdx.x; i < words; i += kThreads) s_mem[i] = 0;
+  __syncthreads();
+  for (int unit = wave; unit < units; unit += kThreads / 64) {
+    const int group = unit / p.blocks;
+    follow_parents(
+        p, group, unit - group * p.blocks, s_cells + wave * p.beams * 64,
+        [&](int v, unsigned long long which) {
+          if (which >> lane & 1) atomicOr((unsigned int *)s_mem + (v >> 5), 1u << (v & 31));
+        },
+        [&](int row, int v) { s_source[row] = v; });
+  }
+  __syncthreads();
+  share_out(p, s_mem, s_wave, true, s_source);
 }
 
 struct Compact {
@@ -295,12 +425,76 @@ struct Compact {
   int room;
   int32_t *pairs;
   int rows, page;
-  int words;            // of a bitmap of the pages
-  unsigned int *high;   // pages held at or beyond the limit
-  unsigned int *low;    // free ones below it
-  int32_t *map;         // [pages] where a page of `high` goes
-  int row_blocks;       // of 256 columns, a row
+  int words;           // of a bitmap of the pages
+  unsigned int *high;  // pages held at or beyond the limit
+  unsigned int *low;   // free ones below it
+  int32_t *rank;       // [words] set bits of `high` before a word
+  int row_blocks;      // of 256 columns, a row
 };
+
+// Bits of both bitmaps before word `first`, and of all, by the workgroup: every one counts for itself, 8 bytes a 32 pages.
+template <int THREADS>
+__device__ __forceinline__ void bits_before(const unsigned int *high, const unsigned int *low, int words, int first, int (*s_sum)[THREADS / 64],
+                                            int (&before)[2], int (&all)[2]) {
+  int n[4] = {0, 0, 0, 0};
+  for (int i0 = threadIdx.x; i0 < words; i0 += 8 * THREADS) {  // eight loads of each at once
+    unsigned int h[8], l[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * THREADS;
+      h[u] = i < words ? high[i] : 0;
+      l[u] = i < words ? low[i] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const bool below = i0 + u * THREADS < first;
+      n[0] += below ? __builtin_popcount(h[u]) : 0;
+      n[1] += below ? __builtin_popcount(l[u]) : 0;
+      n[2] += __builtin_popcount(h[u]);
+      n[3] += __builtin_popcount(l[u]);
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) n[k] += __shfl_xor(n[k], off);
+  if ((threadIdx.x & 63) == 0)
+    for (int k = 0; k < 4; ++k) s_sum[k][threadIdx.x >> 6] = n[k];
+  __syncthreads();
+  for (int k = 0; k < 2; ++k) {
+    before[k] = all[k] = 0;
+    for (int w = 0; w < THREADS / 64; ++w) {
+      before[k] += s_sum[k][w];
+      all[k] += s_sum[2 + k][w];
+    }
+  }
+}
+
+// A page to its place, by its rank in its bitmap (a lane a page: neighbours store side by side): src or dst, or, what
+// stays free, the stack (the lowest on top).
+__device__ __forceinline__ void place(const Compact &p, int page, bool high, bool low, int at_high, int at_low, int moves, int all_low) {
+  if (high && at_high < moves) p.src[at_high] = page;
+  if (low) {
+    if (at_low < moves) p.dst[at_low] = page;
+    else if (all_low - 1 - at_low < p.pool) p.stack[all_low - 1 - at_low] = page;
+  }
+}
+// What goes with pair k, and what stands behind the pairs.
+__device__ __forceinline__ void settle_pair(const Compact &p, int k, int moves) {
+  if (k < moves) {
+    const int from = p.src[k], to = p.dst[k];
+    p.shares[to] = p.shares[from];
+    p.shares[from] = 0;
+    p.tokens[k] = p.page;
+  } else {
+    p.src[k] = -1, p.dst[k] = -1, p.tokens[k] = 0;
+  }
+}
+__device__ __forceinline__ void finish(const Compact &p, int moves, int all_high, int all_low) {
+  *p.count = all_low - moves;
+  p.pairs[0] = moves;
+  p.pairs[1] = all_high - moves;
+}
 
 __global__ __launch_bounds__(256) void cp_clear(Compact p) {
   const int i = blockIdx.x * 256 + threadIdx.x;
@@ -322,56 +516,101 @@ __global__ __launch_bounds__(256) void cp_mark(Compact p) {
   }
 }
 
-__global__ __launch_bounds__(kThreads) void cp_scan(Compact p) {
-  __shared__ int s_wave[kThreads / 64];
-  const int tid = threadIdx.x, per = (p.words + kThreads - 1) / kThreads;
-  int highs = 0, lows = 0;
-  for (int i = 0; i < per; ++i)
-    if (tid * per + i < p.words) {
-      highs += __builtin_popcount(p.high[tid * per + i]);
-      lows += __builtin_popcount(p.low[tid * per + i]);
-    }
-  int all_high, all_low;
-  int high = scan(highs, s_wave, all_high) - highs, low = scan(lows, s_wave, all_low) - lows;
-  const int moves = min(min(all_high, all_low), p.room);
-  for (int i = 0; i < per && tid * per + i < p.words; ++i) {
-    const int base = (tid * per + i) * 32;
-    for (unsigned int w = p.high[tid * per + i]; w; w &= w - 1, ++high) {
-      const int v = base + __builtin_ctz(w);
-      if (high < moves) p.src[high] = v;
-      else p.map[v] = v;
-    }
-    for (unsigned int w = p.low[tid * per + i]; w; w &= w - 1, ++low) {
-      const int v = base + __builtin_ctz(w);
-      if (low < moves) p.dst[low] = v;
-      else if (all_low - 1 - low < p.pool) p.stack[all_low - 1 - low] = v;
-    }
-  }
-  __syncthreads();
-  for (int k = tid; k < p.room; k += kThreads) {
-    if (k < moves) {
-      const int from = p.src[k], to = p.dst[k];
-      p.map[from] = to;
-      p.shares[to] = p.shares[from];
-      p.shares[from] = 0;
-      p.tokens[k] = p.page;
-    } else {
-      p.src[k] = -1, p.dst[k] = -1, p.tokens[k] = 0;
-    }
-  }
-  if (tid == 0) {
-    *p.count = all_low - moves;
-    p.pairs[0] = moves;
-    p.pairs[1] = all_high - moves;
-  }
+// A thread a page.
+__global__ __launch_bounds__(kThreads) void cp_place(Compact p) {
+  constexpr int kWaves = kThreads / 64;
+  __shared__ int s_sum[4][kWaves], s_wave[2][kWaves];
+  const int page = blockIdx.x * kThreads + threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int word = page >> 5, bit = page & 31;
+  const unsigned int h = word < p.words ? p.high[word] : 0, l = word < p.words ? p.low[word] : 0;
+  const bool high = h >> bit & 1, low = l >> bit & 1;
+  const unsigned long long highs = __ballot(high), lows = __ballot(low), below = ((unsigned long long)1 << lane) - 1;
+  if (lane == 0) s_wave[0][wave] = __builtin_popcountll(highs), s_wave[1][wave] = __builtin_popcountll(lows);
+  int before[2], all[2];
+  bits_before<kThreads>(p.high, p.low, p.words, blockIdx.x * (kThreads / 32), s_sum, before, all);  // (its barrier)
+  const int moves = min(min(all[0], all[1]), p.room);
+  for (int w = 0; w < wave; ++w) before[0] += s_wave[0][w], before[1] += s_wave[1][w];
+  const int at_high = before[0] + __builtin_popcountll(highs & below), at_low = before[1] + __builtin_popcountll(lows & below);
+  if (bit == 0 && word < p.words) p.rank[word] = at_high;
+  place(p, page, high, low, at_high, at_low, moves, all[1]);
+  if (page == 0) finish(p, moves, all[0], all[1]);
 }
 
-__global__ __launch_bounds__(256) void cp_remap(Compact p) {
-  const int row = (int)(blockIdx.x / p.row_blocks), c = (int)(blockIdx.x % p.row_blocks) * 256 + threadIdx.x;
+// Where the page of a cell goes: its rank among the pages to move says which pair.
+__device__ __forceinline__ void remap(const Compact &p, const unsigned int *high, const int *rank, int row, int c, int moves) {
   if (c >= min(pages_of(p.lens[row], p.page), p.width)) return;
   int32_t *const cell = p.table + row * p.t_sr + c;
   const int v = *cell;
-  if (v >= p.limit && v < p.pages) *cell = p.map[v];
+  if (v < p.limit || v >= p.pages) return;
+  const int k = rank[v >> 5] + __builtin_popcount(high[v >> 5] & ((1u << (v & 31)) - 1));
+  if (k < moves) *cell = p.dst[k];
+}
+
+__global__ __launch_bounds__(256) void cp_remap(Compact p) {
+  const int64_t tables = (int64_t)p.rows * p.row_blocks;
+  const int moves = p.pairs[0];
+  if (blockIdx.x < tables) {
+    remap(p, p.high, p.rank, (int)(blockIdx.x / p.row_blocks), (int)(blockIdx.x % p.row_blocks) * 256 + threadIdx.x, moves);
+  } else {
+    const int64_t k = (blockIdx.x - tables) * 256 + threadIdx.x;
+    if (k < p.room) settle_pair(p, (int)k, moves);
+  }
+}
+
+// All of it in one workgroup, the bitmaps in LDS.
+__global__ __launch_bounds__(kThreads) void cp_small(Compact p) {
+  __shared__ unsigned int s_high[kSmallPages / 32], s_low[kSmallPages / 32];
+  __shared__ int s_rank[kSmallPages / 32], s_rank_low[kSmallPages / 32], s_wave[kThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int count = min(max(*p.count, 0), p.pool);
+  for (int i = tid; i < p.words; i += kThreads) s_high[i] = s_low[i] = 0;
+  __syncthreads();
+  for (int i = tid; i < count; i += kThreads) {
+    const int v = p.stack[i];
+    if (v >= 0 && v < p.limit) atomicOr(s_low + (v >> 5), 1u << (v & 31));
+  }
+  for (int row = wave; row < p.rows; row += kThreads / 64) {
+    const int held = min(pages_of(p.lens[row], p.page), p.width);
+    for (int c = lane; c < held; c += 64) {
+      const int v = p.table[row * p.t_sr + c];
+      if (v >= p.limit && v < p.pages) atomicOr(s_high + (v >> 5), 1u << (v & 31));
+    }
+  }
+  __syncthreads();
+  constexpr int kPer = kSmallPages / 32 / kThreads;
+  int n[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int word = tid * kPer + i;
+    n[0] += word < p.words ? __builtin_popcount(s_high[word]) : 0;
+    n[1] += word < p.words ? __builtin_popcount(s_low[word]) : 0;
+  }
+  int all_high, all_low;
+  int at_high = scan(n[0], s_wave, all_high) - n[0], at_low = scan(n[1], s_wave, all_low) - n[1];
+  const int moves = min(min(all_high, all_low), p.room);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int word = tid * kPer + i;
+    if (word < p.words) {
+      s_rank[word] = at_high;
+      s_rank_low[word] = at_low;
+      at_high += __builtin_popcount(s_high[word]);
+      at_low += __builtin_popcount(s_low[word]);
+    }
+  }
+  __syncthreads();
+  for (int page = tid; page < p.pages; page += kThreads) {
+    const unsigned int h = s_high[page >> 5], l = s_low[page >> 5], bit = 1u << (page & 31);
+    place(p, page, h & bit, l & bit, s_rank[page >> 5] + __builtin_popcount(h & (bit - 1)),
+          s_rank_low[page >> 5] + __builtin_popcount(l & (bit - 1)), moves, all_low);
+  }
+  __syncthreads();
+  for (int k = tid; k < p.room; k += kThreads) settle_pair(p, k, moves);
+  for (int row = wave; row < p.rows; row += kThreads / 64) {
+    const int held = min(pages_of(p.lens[row], p.page), p.width);
+    for (int c = lane; c < held; c += 64) remap(p, s_high, s_rank, row, c, moves);
+  }
+  if (tid == 0) finish(p, moves, all_high, all_low);
 }
 
 constexpr int kCaches = 64;  // caches of a launch
@@ -559,24 +798,29 @@ int32_t l20_pd_reorder_tables(const l20_pd_reorder_args *a, void *stream) {
   p.groups = a->groups;
   p.beams = a->beams;
   p.page = a->page_size;
-  p.blocks = (a->table_pages + 63) / 64;
+  p.blocks = a->groups > 0 ? (a->table_pages + 63) / 64 : 0;
   p.list_count = reinterpret_cast<int32_t *>(a->workspace);
   p.list = p.list_count + (int64_t)p.groups * p.blocks;
   p.source = p.list + (int64_t)p.groups * p.blocks * p.beams * 64;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (p.groups > 0) {
-    const dim3 grid((unsigned)((p.blocks + l20pm::kCellWaves - 1) / l20pm::kCellWaves), (unsigned)p.groups);
-    hipLaunchKernelGGL(l20pm::rp_cells, grid, dim3(64 * l20pm::kCellWaves), (size_t)l20pm::kCellWaves * p.beams * 256, s, p);
-    rc = launched();
-    if (rc != L20_PD_OK) return rc;
+  const int rows = p.groups * p.beams, units = p.groups * p.blocks;
+  const int most = 4 * l20pm::pool_ints(l20pm::kBitmap, l20pm::kUnits, L20_PD_MAX_REQUESTS);
+  const int lds = 4 * l20pm::pool_ints(p.pages, units, rows), cells = l20pm::kThreads / 64 * p.beams * 256;
+  if (units <= l20pm::kSmall && p.pages <= l20pm::kBitmap && lds + cells <= most) {
+    static l20la::LdsLimit limit;
+    const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20pm::rp_small), most);
+    if (e != hipSuccess) return set_error(L20_PD_ELAUNCH, hipGetErrorString(e));
+    hipLaunchKernelGGL(l20pm::rp_small, dim3(1), dim3(l20pm::kThreads), (size_t)(lds + cells), s, p);
+    return launched();
   }
-  const auto pool_lds = [](int64_t pages, int64_t rows) {
-    return (int)(4 * ((std::min<int64_t>(pages, l20pm::kBitmap) + 31) / 32 + l20pm::kUnits + 1 + rows));
-  };
+  const dim3 grid((unsigned)((p.blocks + l20pm::kCellWaves - 1) / l20pm::kCellWaves), (unsigned)p.groups);
+  hipLaunchKernelGGL(l20pm::rp_cells, grid, dim3(64 * l20pm::kCellWaves), (size_t)l20pm::kCellWaves * p.beams * 256, s, p);
+  rc = launched();
+  if (rc != L20_PD_OK) return rc;
   static l20la::LdsLimit limit;
-  const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20pm::rp_pool), pool_lds(l20pm::kBitmap, L20_PD_MAX_REQUESTS));
+  const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20pm::rp_pool), most);
   if (e != hipSuccess) return set_error(L20_PD_ELAUNCH, hipGetErrorString(e));
-  hipLaunchKernelGGL(l20pm::rp_pool, dim3(1), dim3(l20pm::kThreads), (size_t)pool_lds(p.pages, (int64_t)p.groups * p.beams), s, p);
+  hipLaunchKernelGGL(l20pm::rp_pool, dim3(1), dim3(l20pm::kThreads), (size_t)lds, s, p);
   return launched();
 }
 
@@ -586,7 +830,7 @@ int32_t l20_pd_compact_pages_check(const l20_pd_compact_args *a) {
 }
 
 int64_t l20_pd_compact_pages_workspace(const l20_pd_compact_args *a) {
-  return a && a->pages > 0 ? 4 * (2 * words_of(a) + a->pages) : 0;
+  return a && a->pages > 0 ? 12 * words_of(a) : 0;
 }
 
 int32_t l20_pd_compact_pages(const l20_pd_compact_args *a, void *stream) {
@@ -616,14 +860,20 @@ int32_t l20_pd_compact_pages(const l20_pd_compact_args *a, void *stream) {
   p.words = (int)words_of(a);
   p.high = reinterpret_cast<unsigned int *>(a->workspace);
   p.low = p.high + p.words;
-  p.map = reinterpret_cast<int32_t *>(p.low + p.words);
+  p.rank = reinterpret_cast<int32_t *>(p.low + p.words);
   p.row_blocks = std::max(1, (a->table_pages + 255) / 256);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int64_t tables = (int64_t)p.rows * p.row_blocks, stacks = ((int64_t)p.pool + 255) / 256;
-  hipLaunchKernelGGL(l20pm::cp_clear, dim3((unsigned)((p.words + 255) / 256)), dim3(256), 0, s, p);
-  hipLaunchKernelGGL(l20pm::cp_mark, dim3((unsigned)(tables + stacks)), dim3(256), 0, s, p);
-  hipLaunchKernelGGL(l20pm::cp_scan, dim3(1), dim3(l20pm::kThreads), 0, s, p);
-  if (tables > 0) hipLaunchKernelGGL(l20pm::cp_remap, dim3((unsigned)tables), dim3(256), 0, s, p);
+  const int64_t cells = (int64_t)p.rows * ((p.width + 63) / 64 * 64);
+  if (p.pages <= l20pm::kSmallPages && cells <= l20pm::kSmallCells) {
+    hipLaunchKernelGGL(l20pm::cp_small, dim3(1), dim3(l20pm::kThreads), 0, s, p);
+    return launched();
+  }
+  const auto blocks = [](int64_t n) { return (unsigned)((n + 255) / 256); };
+  const unsigned tables = (unsigned)(p.rows * (int64_t)p.row_blocks);
+  hipLaunchKernelGGL(l20pm::cp_clear, dim3(blocks(p.words)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(l20pm::cp_mark, dim3(tables + blocks(p.pool)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(l20pm::cp_place, dim3((unsigned)((p.pages + l20pm::kThreads - 1) / l20pm::kThreads)), dim3(l20pm::kThreads), 0, s, p);
+  if (tables + blocks(p.room) > 0) hipLaunchKernelGGL(l20pm::cp_remap, dim3(tables + blocks(p.room)), dim3(256), 0, s, p);
   return launched();
 }
 

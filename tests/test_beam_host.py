@@ -233,7 +233,7 @@ def test_workspaces_are_enough_for_smaller_calls():
         sizes.append(lib.l20_pd_reorder_tables_workspace(ctypes.byref(r)))
     assert sizes == sorted(sizes)
     c = compact_args()
-    assert lib.l20_pd_compact_pages_workspace(ctypes.byref(c)) == 4 * (500 + 2 * 16)
+    assert lib.l20_pd_compact_pages_workspace(ctypes.byref(c)) == 12 * 16  # two bits and an int a 32 pages
     for name in ("beam_step", "reorder_tables", "compact_pages"):
         assert getattr(lib, f"l20_pd_{name}_workspace")(None) == 0
 

@@ -481,7 +481,7 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="limit must be"):
         bt.l20_compact_pages(9, i.view(8, 1), i, i, i, i[:1], 16)
     with pytest.raises(RuntimeError, match="workspace is missing"):
-        bt.l20_compact_pages(4, i.view(8, 1), i, i, i, i[:1], 16, workspace=i)
+        bt.l20_compact_pages(4, i.view(8, 1), i, i, i, i[:1], 16, workspace=i[:1])
     with pytest.raises(RuntimeError, match="must be \\[pages, page"):
         bt.l20_copy_pages(bt.PageCopies(i, i), [i])
     with pytest.raises(RuntimeError, match="parts overlap"):
