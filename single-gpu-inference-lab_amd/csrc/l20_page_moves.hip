@@ -34,25 +34,41 @@ constexpr int kSmallCells = 1 << 14;
 
 __device__ __forceinline__ int pages_of(int tokens, int page) { return tokens > 0 ? (int)(((int64_t)tokens + page - 1) / page) : 0; }
 
-// Inclusive scan of a value a thread over the workgroup; `total` is the sum.
-__device__ __forceinline__ int scan(int x, int *s_wave, int &total) {
+// Inclusive scan over the wave: within rows of 16 lanes, then the ends of the rows before (no LDS round trips).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15, row_bcast:31
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
+// Inclusive scans of N values a thread over the workgroup; `total` are the sums.  (Two barriers: what was in LDS before is
+// written, and read, by then.)
+template <int N> __device__ __forceinline__ void scan(int (&x)[N], int (*s_wave)[kThreads / 64], int (&total)[N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(x, off);
-    if (lane >= off) x += y;
-  }
+  for (int n = 0; n < N; ++n) x[n] = wave_scan(x[n]);
   __syncthreads();
-  if (lane == 63) s_wave[wave] = x;
-  __syncthreads();
-  total = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    const int v = s_wave[w];
-    x += w < wave ? v : 0;
-    total += v;
+  for (int n = 0; n < N; ++n)
+    if (lane == 63) s_wave[n][wave] = x[n];
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int v = lane < kThreads / 64 ? s_wave[n][lane] : 0, upto = wave_scan(v);
+    total[n] = __builtin_amdgcn_readlane(upto, kThreads / 64 - 1);
+    x[n] += __builtin_amdgcn_readlane(upto, wave) - __builtin_amdgcn_readlane(v, wave);
   }
-  return x;
+}
+__device__ __forceinline__ int scan(int x, int (*s_wave)[kThreads / 64], int &total) {
+  int y[1] = {x}, all[1];
+  scan<1>(y, s_wave, all);
+  total = all[0];
+  return y[0];
 }
 
 // The maximum over the wave (of values that are not negative).
@@ -219,7 +235,8 @@ __host__ __device__ constexpr int pool_ints(int pages, int units, int rows) {
 // The pool, one workgroup: freed pages onto the stack by number, then each row's copy from it.  The pages to take are the
 // last that were freed, or lie where nothing is written: nothing is read back.  `marked`: the freed pages are in the
 // bitmap already, else in lists a wave.
-__device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int *s_wave, bool marked, const int *s_source) {
+__device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_wave)[kThreads / 64], bool marked,
+                                          const int *s_source) {
   const int tid = threadIdx.x, rows = p.groups * p.beams, units = p.groups * p.blocks;
   unsigned int *const s_bits = (unsigned int *)s_mem;
   int *const s_at = s_mem + bitmap_words(p.pages), *const s_len = s_at + min(units, kUnits) + 1;
@@ -263,8 +280,12 @@ __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int *s_w
       wanted += row[i].copy >= 0;
     }
   }
-  int total;
-  const int first_wanted = scan(wanted, s_wave, total) - wanted;
+  int upto[2] = {wanted, 0}, totals[2];
+#pragma unroll
+  for (int i = 0; i < kLists; ++i) upto[1] += lengths[i];
+  const int listed = upto[1];
+  scan<2>(upto, s_wave, totals);
+  const int total = totals[0], first_wanted = upto[0] - wanted;
   // freed pages, by number; places from the top are known once all are counted
   int freed = 0;
   auto push = [&](int base, int words) {
@@ -301,8 +322,9 @@ __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int *s_w
           length[i] = u0 == 0 ? lengths[i] : u < units ? p.list_count[u] : 0;
           mine += length[i];
         }
-        int entries;
-        int at = scan(mine, s_wave, entries) - mine;  // (its barriers: the bitmap is clear, the offsets are read)
+        int entries = totals[1], at = upto[1] - listed;
+        if (base > 0 || u0 > 0) at = scan(mine, s_wave, entries) - mine;
+        else __syncthreads();  // the bitmap is clear; offsets of other lists are read
         if (entries == 0) continue;
         some = true;
 #pragma unroll
@@ -383,14 +405,14 @@ __global__ __launch_bounds__(64 * kCellWaves) void rp_cells(Reorder p) {
 
 __global__ __launch_bounds__(kThreads) void rp_pool(Reorder p) {
   extern __shared__ int s_mem[];
-  __shared__ int s_wave[kThreads / 64];
+  __shared__ int s_wave[2][kThreads / 64];
   share_out(p, s_mem, s_wave, false, nullptr);
 }
 
 // Both in one launch, for few waves' worth of cells: freed pages go straight into the bitmap.
 __global__ __launch_bounds__(kThreads) void rp_small(Reorder p) {
   extern __shared__ int s_mem[];
-  __shared__ int s_wave[kThreads / 64];
+  __shared__ int s_wave[2][kThreads / 64];
   __shared__ int s_source[kSmall * L20_PD_MAX_BEAMS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int units = p.groups * p.blocks, words = bitmap_words(p.pages);
@@ -455,18 +477,16 @@ __device__ __forceinline__ void bits_before(const unsigned int *high, const unsi
     }
   }
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) n[k] += __shfl_xor(n[k], off);
+  for (int k = 0; k < 4; ++k) n[k] = wave_total(n[k]);
   if ((threadIdx.x & 63) == 0)
+#pragma unroll
     for (int k = 0; k < 4; ++k) s_sum[k][threadIdx.x >> 6] = n[k];
   __syncthreads();
+  const int lane = threadIdx.x & 63;
+#pragma unroll
   for (int k = 0; k < 2; ++k) {
-    before[k] = all[k] = 0;
-    for (int w = 0; w < THREADS / 64; ++w) {
-      before[k] += s_sum[k][w];
-      all[k] += s_sum[2 + k][w];
-    }
+    before[k] = wave_total(lane < THREADS / 64 ? s_sum[k][lane] : 0);
+    all[k] = wave_total(lane < THREADS / 64 ? s_sum[2 + k][lane] : 0);
   }
 }
 
@@ -529,7 +549,8 @@ __global__ __launch_bounds__(kThreads) void cp_place(Compact p) {
   int before[2], all[2];
   bits_before<kThreads>(p.high, p.low, p.words, blockIdx.x * (kThreads / 32), s_sum, before, all);  // (its barrier)
   const int moves = min(min(all[0], all[1]), p.room);
-  for (int w = 0; w < wave; ++w) before[0] += s_wave[0][w], before[1] += s_wave[1][w];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) before[k] += wave_total(lane < wave ? s_wave[k][lane] : 0);
   const int at_high = before[0] + __builtin_popcountll(highs & below), at_low = before[1] + __builtin_popcountll(lows & below);
   if (bit == 0 && word < p.words) p.rank[word] = at_high;
   place(p, page, high, low, at_high, at_low, moves, all[1]);
@@ -560,7 +581,7 @@ __global__ __launch_bounds__(256) void cp_remap(Compact p) {
 // All of it in one workgroup, the bitmaps in LDS.
 __global__ __launch_bounds__(kThreads) void cp_small(Compact p) {
   __shared__ unsigned int s_high[kSmallPages / 32], s_low[kSmallPages / 32];
-  __shared__ int s_rank[kSmallPages / 32], s_rank_low[kSmallPages / 32], s_wave[kThreads / 64];
+  __shared__ int s_rank[kSmallPages / 32], s_rank_low[kSmallPages / 32], s_wave[2][kThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int count = min(max(*p.count, 0), p.pool);
   for (int i = tid; i < p.words; i += kThreads) s_high[i] = s_low[i] = 0;
@@ -585,9 +606,10 @@ __global__ __launch_bounds__(kThreads) void cp_small(Compact p) {
     n[0] += word < p.words ? __builtin_popcount(s_high[word]) : 0;
     n[1] += word < p.words ? __builtin_popcount(s_low[word]) : 0;
   }
-  int all_high, all_low;
-  int at_high = scan(n[0], s_wave, all_high) - n[0], at_low = scan(n[1], s_wave, all_low) - n[1];
-  const int moves = min(min(all_high, all_low), p.room);
+  int upto[2] = {n[0], n[1]}, all[2];
+  scan<2>(upto, s_wave, all);
+  const int all_high = all[0], all_low = all[1], moves = min(min(all_high, all_low), p.room);
+  int at_high = upto[0] - n[0], at_low = upto[1] - n[1];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int word = tid * kPer + i;
