@@ -17,6 +17,7 @@
 
 #include "l20_beam_search.h"
 #include "l20_latent_common.h"
+#include "l20_overlap.h"
 
 namespace l20pm {
 
@@ -28,9 +29,13 @@ constexpr int kPerThread = L20_PD_MAX_REQUESTS / kThreads;
 constexpr int kCellWaves = 4;
 constexpr int kBitmap = 1 << 18;  // pages of one pass of rp_pool (32 KB of LDS)
 constexpr int kUnits = 4096;      // waves' lists that rp_pool looks at together
-constexpr int kSmall = 16;        // waves' worth of cells that one launch does with the pool
-constexpr int kSmallPages = 1 << 16;  // pages and cells (a row: a multiple of 64) of a compaction in one launch
-constexpr int kSmallCells = 1 << 14;
+// Waves' worth of cells that one launch does with the pool, one a wave.  Measured against two launches: 8 groups of 4
+// beams, 64 cells 12.3 and 15.6 us, 16 groups 14.3 and 16.0; more than one a wave, 32 groups 19.5 and 15.9.
+constexpr int kSmall = 16;
+// Pages, and waves' worth of cells, of a compaction in one launch.  Measured against four: 64 rows of 64 cells, 8192 pages
+// 13.1 and 17.4 us, 16 of 128, 4096 pages 8.2 and 16.8; beyond, 64 rows of 256, 20000 pages 28.1 and 17.4, 256 rows of 64,
+// 30000 pages 40.6 and 17.7.
+constexpr int kSmallPages = 1 << 13, kSmallWaves = 64;
 
 __device__ __forceinline__ int pages_of(int tokens, int page) { return tokens > 0 ? (int)(((int64_t)tokens + page - 1) / page) : 0; }
 
@@ -598,28 +603,12 @@ __global__ __launch_bounds__(kThreads) void cp_small(Compact p) {
     }
   }
   __syncthreads();
-  constexpr int kPer = kSmallPages / 32 / kThreads;
-  int n[2] = {0, 0};
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int word = tid * kPer + i;
-    n[0] += word < p.words ? __builtin_popcount(s_high[word]) : 0;
-    n[1] += word < p.words ? __builtin_popcount(s_low[word]) : 0;
-  }
-  int upto[2] = {n[0], n[1]}, all[2];
+  static_assert(kSmallPages / 32 <= kThreads, "a word a thread");
+  const int bits[2] = {tid < p.words ? __builtin_popcount(s_high[tid]) : 0, tid < p.words ? __builtin_popcount(s_low[tid]) : 0};
+  int upto[2] = {bits[0], bits[1]}, all[2];
   scan<2>(upto, s_wave, all);
   const int all_high = all[0], all_low = all[1], moves = min(min(all_high, all_low), p.room);
-  int at_high = upto[0] - n[0], at_low = upto[1] - n[1];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int word = tid * kPer + i;
-    if (word < p.words) {
-      s_rank[word] = at_high;
-      s_rank_low[word] = at_low;
-      at_high += __builtin_popcount(s_high[word]);
-      at_low += __builtin_popcount(s_low[word]);
-    }
-  }
+  if (tid < p.words) s_rank[tid] = upto[0] - bits[0], s_rank_low[tid] = upto[1] - bits[1];
   __syncthreads();
   for (int page = tid; page < p.pages; page += kThreads) {
     const unsigned int h = s_high[page >> 5], l = s_low[page >> 5], bit = 1u << (page & 31);
@@ -774,6 +763,28 @@ int32_t launched() {
   return set_error(L20_PD_ELAUNCH, msg);
 }
 
+// Every tensor of these calls is read or written throughout: none may share bytes with another.
+template <typename A> int32_t apart(const A *a, const void *parents, int64_t rows, int64_t workspace_bytes) {
+  using l20la::Lattice;
+  const auto run = [](const void *at, int64_t bytes) { return Lattice(at, 0, 0, bytes > 0 ? 1 : 0, 1, bytes); };
+  const Lattice all[] = {Lattice(a->block_table, a->bt_stride_row * 4, 0, rows, 1, (int64_t)a->table_pages * 4),
+                         run(a->seq_lens, rows * 4),
+                         run(a->page_shares, (int64_t)a->pages * 4),
+                         run(a->free_pages, (int64_t)a->pool * 4),
+                         run(a->free_count, 4),
+                         run(a->src, (int64_t)a->room * 4),
+                         run(a->dst, (int64_t)a->room * 4),
+                         run(a->tokens, (int64_t)a->room * 4),
+                         run(a->count, 8),
+                         run(a->workspace, workspace_bytes),
+                         run(parents, parents ? rows * 4 : 0)};
+  constexpr int n = sizeof(all) / sizeof(all[0]);
+  for (int i = 0; i < n; ++i)
+    for (int j = 0; j < i; ++j)
+      if (l20la::overlap(all[i], all[j])) return set_error(L20_PD_EINVAL, "tensors and workspace must lie apart");
+  return L20_PD_OK;
+}
+
 template <typename V> int32_t launch_copy(const l20pm::Copy &p, bool dense, hipStream_t s) {
   const int64_t jobs = (int64_t)p.room * p.caches * p.segments;
   const unsigned grid = (unsigned)std::min<int64_t>(jobs, 8 * (int64_t)l20la::device_cus());
@@ -801,6 +812,8 @@ int32_t l20_pd_reorder_tables(const l20_pd_reorder_args *a, void *stream) {
   if (rc != L20_PD_OK) return rc;
   if (a->groups > 0 && (!a->workspace || (uintptr_t)a->workspace % 4 || a->workspace_bytes < workspace(a)))
     return set_error(L20_PD_EINVAL, "workspace is missing, misaligned or too small");
+  rc = apart(a, a->parents, (int64_t)a->groups * a->beams, a->groups > 0 ? workspace(a) : 0);
+  if (rc != L20_PD_OK) return rc;
   l20pm::Reorder p{};
   p.parents = a->parents;
   p.table = a->block_table;
@@ -861,6 +874,8 @@ int32_t l20_pd_compact_pages(const l20_pd_compact_args *a, void *stream) {
   if (rc != L20_PD_OK) return rc;
   if (!a->workspace || (uintptr_t)a->workspace % 4 || a->workspace_bytes < l20_pd_compact_pages_workspace(a))
     return set_error(L20_PD_EINVAL, "workspace is missing, misaligned or too small");
+  rc = apart(a, nullptr, a->rows, l20_pd_compact_pages_workspace(a));
+  if (rc != L20_PD_OK) return rc;
   l20pm::Compact p{};
   p.limit = a->limit;
   p.table = a->block_table;
@@ -885,8 +900,7 @@ int32_t l20_pd_compact_pages(const l20_pd_compact_args *a, void *stream) {
   p.rank = reinterpret_cast<int32_t *>(p.low + p.words);
   p.row_blocks = std::max(1, (a->table_pages + 255) / 256);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int64_t cells = (int64_t)p.rows * ((p.width + 63) / 64 * 64);
-  if (p.pages <= l20pm::kSmallPages && cells <= l20pm::kSmallCells) {
+  if (p.pages <= l20pm::kSmallPages && (int64_t)p.rows * ((p.width + 63) / 64) <= l20pm::kSmallWaves) {
     hipLaunchKernelGGL(l20pm::cp_small, dim3(1), dim3(l20pm::kThreads), 0, s, p);
     return launched();
   }

@@ -211,6 +211,23 @@ def test_beam_step_refuses_outputs_over_others(change):
     assert rc == cabi.L20_PD_EINVAL and ("must not lie over" in cabi.last_error() or "must lie apart" in cabi.last_error())
 
 
+@pytest.mark.parametrize("kind", ["reorder_tables", "compact_pages"])
+@pytest.mark.parametrize("change", [
+    dict(seq_lens=FAKE + 4 * (30 * 19 + 29)),  # the table's last cell
+    dict(page_shares=FAKE * 4 - 4),  # ends in the stack
+    dict(dst=FAKE * 6),
+    dict(count=FAKE * 5 - 4),
+    dict(workspace=FAKE * 8 + 156),
+    dict(free_count=FAKE * 2 + 76),
+], ids=range(6))
+def test_page_calls_refuse_tensors_over_others(kind, change):
+    args = CHECKS[kind]()
+    for name, value in change.items():
+        setattr(args, name, value)
+    rc = getattr(cabi.load(), f"l20_pd_{kind}")(ctypes.byref(args), None)
+    assert rc == cabi.L20_PD_EINVAL and "must lie apart" in cabi.last_error()
+
+
 def test_workspaces_are_enough_for_smaller_calls():
     lib, a = cabi.load(), beam_args()
     for beams, vocab, ends in ((1, 1, 0), (4, 152064, 1), (32, 50257, 8), (5, 2049, 2), (32, 200, 8)):
