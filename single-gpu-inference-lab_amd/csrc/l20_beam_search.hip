@@ -114,10 +114,30 @@ __device__ __forceinline__ float wave_max(float x) {
   x = l20la::max_groups(x);
   return l20la::word_f((unsigned int)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
 }
+// The same of doubles, by sum or maximum: rotations within rows of 16, then a lane of each row.  One order: the same bits.
+template <int CTRL> __device__ __forceinline__ double dpp(double x) {
+  const long long b = __builtin_bit_cast(long long, x);
+  const int lo = __builtin_amdgcn_update_dpp((int)b, (int)b, CTRL, 0xf, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp((int)(b >> 32), (int)(b >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (long long)hi << 32 | (unsigned)lo);
+}
+__device__ __forceinline__ double lane_d(double x, int n) {
+  const long long b = __builtin_bit_cast(long long, x);
+  return __builtin_bit_cast(double, (long long)__builtin_amdgcn_readlane((int)(b >> 32), n) << 32 |
+                                        (unsigned)__builtin_amdgcn_readlane((int)b, n));
+}
+template <typename F> __device__ __forceinline__ double wave_fold(double x, F f) {
+  x = f(x, dpp<0x128>(x));
+  x = f(x, dpp<0x124>(x));
+  x = f(x, dpp<0x122>(x));
+  x = f(x, dpp<0x121>(x));
+  return f(f(lane_d(x, 0), lane_d(x, 16)), f(lane_d(x, 32), lane_d(x, 48)));
+}
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
-  return x;
+  return wave_fold(x, [](double a, double b) { return a + b; });
+}
+__device__ __forceinline__ double wave_max(double x) {
+  return wave_fold(x, [](double a, double b) { return fmax(a, b); });
 }
 __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < INFINITY; }
 
@@ -283,11 +303,7 @@ __device__ __forceinline__ int live_row(const Params &p, int rows, int unit, u64
     run = unit - row * runs;
     return row < rows ? row : -1;
   }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(upto, off);
-    if (lane >= off) upto += y;
-  }
+  upto = l20la::wave_scan(upto);
   const int live = __builtin_amdgcn_readlane(upto, 63);
   if (live == 0) return -1;
   runs = min(p.most, max(p.spread / live, 1));
@@ -511,51 +527,45 @@ __global__ __launch_bounds__(512) void beam_join(Params p) {
     double part = lane < p.most ? p.sum[slot + lane] : 0.0;
     const float *const value = p.value + slot * k;
     const int *const token = p.token + slot * k;
-    const int at = min(lane, p.most - 1) * k;
-    float v = lane < k ? value[lane] : 0.0f, head = value[at], head1 = value[at + min(1, k - 1)];
-    int t = lane < k ? token[lane] : 0, headt = token[at], headt1 = token[at + min(1, k - 1)];
+    const int last = p.most * k - 1;
+    float v = value[min(lane, last)], v1 = value[min(lane + 64, last)];
+    int t = token[min(lane, last)], t1 = token[min(lane + 64, last)];
     int count = 0;
     u64 ends = 0;
     if (finite(c)) {
       double lse;
       if (runs == 1) {  // a list in order
-        lse = __shfl(m + log(part), 0);
+        lse = lane_d(m, 0) + log(lane_d(part, 0));
         v = lane < k ? v : -INFINITY;
       } else {
         m = lane < runs ? m : -(double)INFINITY;
         part = lane < runs ? part : 0.0;
-        head = lane < runs ? head : -INFINITY;
-        head1 = lane < runs && k > 1 ? head1 : -INFINITY;
         Best best(s_keys + wave * (kEntries + 2), k);
         if (runs * k <= kEntries) {  // all of them
-          for (int i = 0; i < runs * k; i += 64) {
-            const int e = min(i + lane, runs * k - 1);
-            best.show(value[e], token[e], i + lane < runs * k);
-          }
-          best.settle();
+          best.show(v, t, lane < runs * k);
+          if (runs * k > 64) best.show(v1, t1, lane + 64 < runs * k);
         } else {
           // lists in order: heads first, until no run has one that may be among the best
+          const int at = min(lane, runs - 1) * k;
           float *const heads = reinterpret_cast<float *>(best.keys);  // (the list is empty)
+          float head = lane < runs ? value[at] : -INFINITY;
+          int headt = token[at];
           heads[lane] = head;
           best.bound_by(heads);
 #pragma unroll 1
-          for (int j = 0; j < k; ++j) {
+          for (int j = 1;; ++j) {
             const bool ok = head >= best.least && key_of(head, headt) >= best.bar;
             if (!__ballot(ok)) break;
             best.show(head, headt, ok);
-            head = ok ? head1 : -INFINITY;
-            headt = headt1;
-            const bool more = ok && j + 2 < k;
-            head1 = more ? value[at + j + 2] : -INFINITY;
-            headt1 = more ? token[at + j + 2] : -1;
+            if (j == k) break;
+            head = ok ? value[at + j] : -INFINITY;
+            headt = token[at + j];
           }
-          best.settle();
         }
-        double top = m;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) top = fmax(top, __shfl_xor(top, off));
+        best.settle();
         // (a NaN stays one: it is in `part`, and a run of -inf alone has the part 0)
-        lse = top + log(wave_sum(part == 0.0 ? part : part * exp(m - top)));
+        const double top = wave_max(m);
+        lse = top + log(wave_sum(m == top || part == 0.0 ? part : part * exp(m - top)));
         const u64 key = lane < best.count ? best.keys[lane] : key_of(-INFINITY, -1);
         v = value_of(key);
         t = token_of(key);

@@ -1,5 +1,6 @@
 // Shared by the latent attention kernels (gfx950): element types, the 16x16x32 matrix product, the
-// transposing LDS read and the chunk swizzles of their LDS tiles.
+// transposing LDS read and the chunk swizzles of their LDS tiles; and, with beam search and the page pool, reductions
+// and scans over a wave.
 #ifndef L20_LATENT_COMMON_H_
 #define L20_LATENT_COMMON_H_
 
@@ -107,6 +108,17 @@ __device__ __forceinline__ float max_halves(float x) { return max_swap<32>(x); }
 __device__ __forceinline__ float sum_halves(float x) { return sum_swap<32>(x); }
 __device__ __forceinline__ float max_groups(float x) { return max_swap<32>(max_swap<16>(x)); }  // the four groups of 16
 __device__ __forceinline__ float sum_groups(float x) { return sum_swap<32>(sum_swap<16>(x)); }
+
+// Inclusive scan over the wave: within rows of 16 lanes, then the ends of the rows before (no LDS round trips).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15, row_bcast:31
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
 
 // The lane's number, made anew: where registers are short it is not kept.
 __device__ __forceinline__ int lane_id() {

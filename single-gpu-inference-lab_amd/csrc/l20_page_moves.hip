@@ -23,6 +23,7 @@ namespace l20pm {
 
 using l20la::i32x2;
 using l20la::i32x4;
+using l20la::wave_scan;
 
 constexpr int kThreads = 1024;
 constexpr int kPerThread = L20_PD_MAX_REQUESTS / kThreads;
@@ -39,16 +40,6 @@ constexpr int kSmallPages = 1 << 13, kSmallWaves = 64;
 
 __device__ __forceinline__ int pages_of(int tokens, int page) { return tokens > 0 ? (int)(((int64_t)tokens + page - 1) / page) : 0; }
 
-// Inclusive scan over the wave: within rows of 16 lanes, then the ends of the rows before (no LDS round trips).
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15, row_bcast:31
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-  return x;
-}
 __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
 // Inclusive scans of N values a thread over the workgroup; `total` are the sums.  (Two barriers: what was in LDS before is
