@@ -131,9 +131,9 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
   bool first = true;
   int children = 0;
   for (int i = 0; i < beams; ++i) {
-    const int other = __builtin_amdgcn_readlane(parent, i);
-    first &= !(i < lane && other == parent);
-    children += other == lane;
+    const unsigned long long mine_of = __ballot(parent == i && lane < beams);
+    if (lane == i) children = __builtin_popcountll(mine_of);
+    if (parent == i) first = lane == __builtin_ctzll(mine_of);
   }
   const Row row = row_of(known, parent, parent_len, parent >= 0 && grandparent == parent, first, p.page, p.width);
   const int held = min(pages_of(old_len, p.page), p.width), new_held = min(pages_of(row.len, p.page), p.width);
@@ -165,60 +165,57 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
     if (gone) p.shares[v] = 0;
     free_page(v, __ballot(gone));
   };
-  auto change_of = [&](int r) {
-    const int n = __builtin_amdgcn_readlane(children, r);
-    return c == __builtin_amdgcn_readlane(partial, r) ? min(n, 1) - 1 : n - 1;
-  };
-  int together = 0;
-  bool gains = false, losses = false;
-  for (int r = 0; r < beams; ++r) {
-    const int d = change_of(r);
-    together += d;
-    gains |= __builtin_amdgcn_readlane(children, r) > 1;
-    losses |= __builtin_amdgcn_readlane(children, r) == 0;
-  }
-  if (gains || losses) {
-    same &= held_page(page0);
-    if (__ballot(same && together != 0)) {
-      bool gone = false;
-      if (same && together != 0) gone = atomicAdd(p.shares + page0, together) + together == -1;
-      freed(page0, gone);
-    }
+  const unsigned long long rows = beams < 64 ? ((unsigned long long)1 << beams) - 1 : ~0ull;
+  const unsigned long long gains = __ballot(children > 1) & rows, losses = __ballot(children == 0) & rows;
+  if (gains | losses) {
+    // rows whose last page is this column's count differently: no sum for it (nor where there is no page)
+    unsigned long long ends = 0;
+    for (unsigned long long m = __ballot(partial >= block * 64 && partial < block * 64 + 64) & rows; m; m &= m - 1)
+      ends |= (unsigned long long)1 << (__builtin_amdgcn_readlane(partial, __builtin_ctzll(m)) - block * 64);
+    same &= held_page(page0) && !(ends >> lane & 1);
+    const int together = __builtin_popcountll(__ballot(parent >= 0) & rows) - beams;
+    if (together != 0 && __ballot(same)) freed(page0, same && atomicAdd(p.shares + page0, together) + together == -1);
     if (__ballot(!same)) {
       if (gains) {
-        for (int r = 0; r < beams; ++r) {
-          if (__builtin_amdgcn_readlane(children, r) <= 1) continue;
-          const int v = mine[r * 64], d = change_of(r);
-          if (!same && d > 0 && held_page(v)) atomicAdd(p.shares + v, d);
+        for (unsigned long long m = gains; m; m &= m - 1) {
+          const int r = __builtin_ctzll(m), v = mine[r * 64];
+          if (!same && held_page(v) && c != __builtin_amdgcn_readlane(partial, r))
+            atomicAdd(p.shares + v, __builtin_amdgcn_readlane(children, r) - 1);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // gains before losses
       }
-      if (losses) {
-        for (int r0 = 0; r0 < beams; r0 += 8) {
-          int v[8], was[8];
+      for (unsigned long long m = losses; m;) {  // eight at once
+        int v[8], was[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = -1;
-            was[i] = 1;
-            if (r0 + i >= beams || __builtin_amdgcn_readlane(children, min(r0 + i, beams - 1)) != 0) continue;
-            v[i] = same ? -1 : mine[(r0 + i) * 64];
-            if (held_page(v[i])) was[i] = atomicAdd(p.shares + v[i], -1);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (__ballot(was[i] == 0)) freed(v[i], was[i] == 0);
+        for (int i = 0; i < 8; ++i, m &= m - 1) {
+          v[i] = m && !same ? mine[__builtin_ctzll(m) * 64] : -1;
+          was[i] = 1;
+          if (held_page(v[i])) was[i] = atomicAdd(p.shares + v[i], -1);
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (__ballot(was[i] == 0)) freed(v[i], was[i] == 0);
       }
     }
   }
-  // the table
-  for (int i = 0; i < beams; ++i) {
-    const int q = __builtin_amdgcn_readlane(row.parent, i), copy = __builtin_amdgcn_readlane(row.copy, i);
-    if (q < 0 || (q == i && copy < 0)) continue;  // given up, or as it was
-    const int v = mine[q * 64];
-    if (c == copy) source(group * beams + i, v);
-    else if (c < __builtin_amdgcn_readlane(new_held, i) && !(c < __builtin_amdgcn_readlane(held, i) && v == mine[i * 64]))
-      cells[i * p.t_sr] = v;
+  // the table, eight rows at once
+  for (int i0 = 0; i0 < beams; i0 += 8) {
+    int v[8], old[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= beams) break;
+      v[i] = mine[max(__builtin_amdgcn_readlane(row.parent, i0 + i), 0) * 64];
+      old[i] = mine[(i0 + i) * 64];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= beams) break;
+      const int q = __builtin_amdgcn_readlane(row.parent, i0 + i), copy = __builtin_amdgcn_readlane(row.copy, i0 + i);
+      if (q < 0 || (q == i0 + i && copy < 0)) continue;  // given up, or as it was
+      if (c == copy) source(group * beams + i0 + i, v[i]);
+      else if (c < __builtin_amdgcn_readlane(new_held, i0 + i) && !(c < __builtin_amdgcn_readlane(held, i0 + i) && v[i] == old[i]))
+        cells[(i0 + i) * p.t_sr] = v[i];
+    }
   }
 }
 
