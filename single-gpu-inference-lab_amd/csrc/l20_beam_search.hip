@@ -662,19 +662,23 @@ int64_t rows_of(const l20_pd_beam_step_args *a) { return (int64_t)a->requests * 
 int steps_of(const l20_pd_beam_step_args *a) { return (int)(((int64_t)a->vocab + l20bs::kStep - 1) / l20bs::kStep); }
 int listed_of(const l20_pd_beam_step_args *a) { return std::min(a->beams + a->num_end_tokens, a->vocab); }
 
-// (a run: a step of each wave at least)
-int most_runs(const l20_pd_beam_step_args *a) {
-  return std::min(l20bs::kMaxRuns, (steps_of(a) + l20bs::kWaves - 1) / l20bs::kWaves);
+// The most runs of a row: a step of each wave at least; one where nobody counts the live rows.
+int most_runs(const l20_pd_beam_step_args *a, int64_t rows) {
+  return rows > l20bs::kCounted ? 1 : std::min(l20bs::kMaxRuns, (steps_of(a) + l20bs::kWaves - 1) / l20bs::kWaves);
 }
 int spread_of(int cus) { return cus * l20bs::kRunsPerCu; }
 
 // Workgroups for every number of live rows up to this many: rows times their runs is at most the larger of rows and
 // what they are spread over.
 int64_t units_of(const l20_pd_beam_step_args *a, int cus) {
-  return std::min(rows_of(a) * most_runs(a), std::max<int64_t>(rows_of(a), spread_of(cus)));
+  return std::min(rows_of(a) * most_runs(a, rows_of(a)), std::max<int64_t>(rows_of(a), spread_of(cus)));
 }
+int64_t bytes_for(const l20_pd_beam_step_args *a, int64_t rows) {
+  return rows * (8 + most_runs(a, rows) * (16 + 8 * (int64_t)listed_of(a)));
+}
+// (enough for every smaller number of rows)
 int64_t bytes_of(const l20_pd_beam_step_args *a) {
-  return rows_of(a) * (8 + most_runs(a) * (16 + 8 * (int64_t)listed_of(a)));
+  return std::max(bytes_for(a, rows_of(a)), bytes_for(a, std::min<int64_t>(rows_of(a), l20bs::kCounted)));
 }
 
 int32_t launched() {
@@ -728,7 +732,7 @@ int32_t l20_pd_beam_step(const l20_pd_beam_step_args *a, void *stream) {
   l20bs::Params p{};
   const int cus = l20la::device_cus();
   p.k = listed_of(a);
-  p.most = most_runs(a);
+  p.most = most_runs(a, rows_of(a));
   p.spread = spread_of(cus);
   const int64_t rows = rows_of(a), units = units_of(a, cus);
   p.runs = std::min(p.most, std::max((int)(p.spread / rows), 1));

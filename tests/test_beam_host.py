@@ -156,6 +156,9 @@ BAD = [
     ("copy_pages", dict(stride0=0), "parts overlap"),
     ("copy_pages", dict(size1=4, stride1=1024), "parts overlap"),
     ("copy_pages", dict(stride_page=0), "pages overlap"),
+    ("copy_pages", dict(stride_page=16 * 1024 - 1024), "pages overlap"),
+    ("copy_pages", dict(size0=4, stride0=16 * 1024, size1=16, stride1=1024, token_level=1, stride_page=32 * 1024), "pages overlap"),
+    ("copy_pages", dict(size0=1 << 22), "page too large"),
     ("copy_pages", dict(inner=1 << 41), "page too large"),
     ("copy_pages", dict(dst=0), "null tensor pointer"),
     ("copy_pages", dict(caches=0), "null tensor pointer"),
@@ -170,6 +173,13 @@ def test_refusals(case):
         setattr(args, name, value)
     rc, error = check(kind, args)
     assert rc != 0 and message in error, error
+
+
+def test_pages_may_lie_inside_other_levels():
+    """Heads outside pages: a page is in pieces, and no two share bytes."""
+    args = copy_args()
+    args.size0, args.stride0, args.size1, args.stride1, args.token_level = 4, 50 * 16 * 1024, 16, 1024, 1
+    assert check("copy_pages", args) == (0, "")
 
 
 def test_nothing_to_do_needs_no_pointers():

@@ -248,6 +248,24 @@ def test_wide_rows_and_many_rows():
                 2.0 ** -23 * (4 + math.log(vocab))).all()
 
 
+def test_rows_beyond_32_bits():
+    """Logits whose rows lie further apart than 2^31 elements, and more rows than are counted."""
+    import l20_beam_search as bs
+
+    logits, scores = inputs(2, 2, 5000, torch.bfloat16, seed=60)
+    view = torch.empty(3 * (1 << 31) // 2 + 3 * (1 << 30) + 5000, dtype=torch.bfloat16, device="cuda").as_strided(
+        (2, 2, 5000), (3 * (1 << 30), 3 * (1 << 29), 1))
+    view.copy_(logits)
+    compare(bs.l20_beam_search_step(view, scores.cuda(), out=filled(2, 2)), logits, scores, [])
+    del view
+    g = torch.Generator(device="cuda").manual_seed(61)
+    x = torch.randn(9000, 1, 300, generator=g, device="cuda")
+    s = torch.rand(9000, 1, generator=g, device="cuda")
+    s[::3] = -math.inf
+    out = bs.l20_beam_search_step(x, s, out=filled(9000, 1))
+    assert out.tokens.equal(torch.where(s > -math.inf, x.argmax(-1), -1)) and out.parents.equal((s > -math.inf).int() - 1)
+
+
 def test_graph_and_another_stream():
     """A captured step whose scores advance in place: replays equal eager calls on copies, also beside eager work."""
     import l20_beam_search as bs

@@ -486,5 +486,7 @@ def test_refusals():
         bt.l20_copy_pages(bt.PageCopies(i, i), [i])
     with pytest.raises(RuntimeError, match="parts overlap"):
         bt.l20_copy_pages(bt.PageCopies(i, i), [i.view(8, 1, 1).expand(8, 16, 4)])
+    with pytest.raises(RuntimeError, match="pages overlap"):
+        bt.l20_copy_pages(bt.PageCopies(i, i), [torch.zeros(900, device="cuda").as_strided((5, 16, 8), (64, 8, 1))])
     with pytest.raises(RuntimeError, match="too many strides"):
         bt.l20_copy_pages(bt.PageCopies(i, i), [torch.zeros(3, 16, 5, 6, 7, 8, device="cuda")[:, ::2, ::2, ::2, ::2, ::2]])
