@@ -38,6 +38,8 @@ constexpr int kWaves = 4;                  // of a workgroup, which takes a run
 constexpr int kMaxRuns = 64;               // runs a row: a lane of the join each
 constexpr int kRunsPerCu = 3;              // runs that rows are split for
 constexpr int kEntries = 128;              // what a wave's LDS holds of candidates (two a lane)
+constexpr int kJoinWaves = 16;             // of the joins' workgroups, a beam each
+constexpr int kPrune = 8;                  // beams up to which all candidates are placed
 constexpr int kCounted = 4096;             // rows whose live ones every wave may count (a word of 64 a lane)
 
 struct Params {
@@ -503,7 +505,7 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
   }
 }
 
-__global__ __launch_bounds__(512) void beam_join(Params p) {
+__global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
   extern __shared__ double s_mem[];
   const int waves = p.join_waves, threads = waves * 64, k = p.k, beams = p.beams, n = beams * k;
   double *const s_score = s_mem;                                  // [beams * k]
@@ -512,10 +514,11 @@ __global__ __launch_bounds__(512) void beam_join(Params p) {
   int *const s_token = (int *)(s_keys + waves * (kEntries + 2));  // [beams * k]
   int *const s_rank = s_token + n;                                // [beams * k]: those ahead, and 2^16 an end token
   int *const s_count = s_rank + n;                                // [beams]
-  int *const s_ended = s_count + beams;                           // [1]
+  int *const s_ended = s_count + beams, *const s_kept = s_ended + 1;  // [1] each
+  int *const s_list = s_kept + 1;                                 // [beams * k], with many beams
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int request = blockIdx.x;
-  if (threadIdx.x == 0) *s_ended = 0;
+  if (threadIdx.x == 0) *s_ended = *s_kept = 0;
   for (int i = threadIdx.x; i < n; i += threads) s_rank[i] = 0;
   for (int beam = wave; beam < beams; beam += waves) {
     // every load at once, also where the row turns out dead or its runs fewer
@@ -587,9 +590,30 @@ __global__ __launch_bounds__(512) void beam_join(Params p) {
     }
   }
   __syncthreads();
+  // With many beams first the candidates that may be taken: one row alone has `beams` that are no end tokens from its
+  // last on, so nothing below that is.  (Of wide rows most fall out: the searches below are a row for each candidate.)
+  int survivors = n;
+  if (beams > kPrune) {
+    double bar = -INFINITY;
+    if (k == beams + p.num_ends)
+      for (int w = 0; w < beams; ++w)
+        if (s_count[w] == k) bar = fmax(bar, s_score[w * k + k - 1]);
+    for (int i0 = 0; i0 < n; i0 += threads) {
+      const int i = i0 + threadIdx.x, beam = (unsigned)i / (unsigned)k;
+      const bool keep = i < n && i - beam * k < s_count[beam] && s_score[i] >= bar;
+      const u64 which = __ballot(keep);
+      int at = 0;
+      if (lane == 0 && which) at = atomicAdd(s_kept, __builtin_popcountll(which));  // (their order does not matter)
+      at = __builtin_amdgcn_readfirstlane(at);
+      if (keep) s_list[at + __builtin_amdgcn_mbcnt_hi((unsigned)(which >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)which, 0))] = i;
+    }
+    __syncthreads();
+    survivors = *s_kept;
+  }
   // a thread a candidate and row: those of the row that come before it (lower beams first among equals)
-  for (unsigned i = threadIdx.x; i < (unsigned)(n * beams); i += threads) {
-    const int w = i / (unsigned)n, mine = i - w * n, beam = (unsigned)mine / (unsigned)k, j = mine - beam * k;
+  for (unsigned i = threadIdx.x; i < (unsigned)(survivors * beams); i += threads) {
+    const int w = i / (unsigned)survivors, c = i - w * survivors, mine = beams > kPrune ? s_list[c] : c;
+    const int beam = (unsigned)mine / (unsigned)k, j = mine - beam * k;
     if (j >= s_count[beam]) continue;
     const double score = s_score[mine];
     int lo = 0, hi = s_count[w];
@@ -606,8 +630,8 @@ __global__ __launch_bounds__(512) void beam_join(Params p) {
   __syncthreads();
   int running = 0;
   for (int w = 0; w < beams; ++w) running += s_count[w] - __builtin_popcountll(s_end[w]);
-  for (int i = threadIdx.x; i < n; i += threads) {
-    const int beam = (unsigned)i / (unsigned)k, j = i - beam * k;
+  for (int c = threadIdx.x; c < survivors; c += threads) {
+    const int i = beams > kPrune ? s_list[c] : c, beam = (unsigned)i / (unsigned)k, j = i - beam * k;
     if (j >= s_count[beam]) continue;
     const int ahead = s_rank[i] & 0xffff, ahead_ends = s_rank[i] >> 16;
     if (s_end[beam] >> j & 1) {
@@ -765,7 +789,7 @@ int32_t l20_pd_beam_step(const l20_pd_beam_step_args *a, void *stream) {
   p.ended_tokens = a->ended_tokens;
   p.ended_parents = a->ended_parents;
   p.ended_scores = a->ended_scores;
-  p.join_waves = std::min(a->beams, 8);
+  p.join_waves = std::min(a->beams, l20bs::kJoinWaves);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)units), block(64 * l20bs::kWaves);
   if (a->dtype == L20_PD_BF16) hipLaunchKernelGGL(l20bs::beam_scan<__bf16>, grid, block, 0, s, p);
@@ -773,7 +797,7 @@ int32_t l20_pd_beam_step(const l20_pd_beam_step_args *a, void *stream) {
   else hipLaunchKernelGGL(l20bs::beam_scan<float>, grid, block, 0, s, p);
   rc = launched();
   if (rc != L20_PD_OK) return rc;
-  const size_t lds = (size_t)a->beams * (p.k * 16 + 12) + 12 + (size_t)p.join_waves * (l20bs::kEntries + 2) * 8;  // at most 29 KB
+  const size_t lds = (size_t)a->beams * (p.k * 20 + 12) + 16 + (size_t)p.join_waves * (l20bs::kEntries + 2) * 8;  // at most 43 KB
   hipLaunchKernelGGL(l20bs::beam_join, dim3((unsigned)a->requests), dim3(64 * p.join_waves), lds, s, p);
   return launched();
 }
