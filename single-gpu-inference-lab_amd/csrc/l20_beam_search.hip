@@ -5,17 +5,23 @@
 // and the best `beams` of a request's candidates, with and without end tokens.  Both parts of a row come from one
 // pass over its logits:
 //
-//  beam_scan   a workgroup of eight waves a run of a row, a wave 32 logits a lane and step, one step ahead.  A wave
-//    keeps the sum of exp(x - m) below the running maximum m, and in LDS what may be among the run's K best (K = beams
-//    + end tokens: enough for `beams` that are no end tokens): values from the K-th of 64 maxima on, each of the
-//    values so far of eight lanes of the workgroup.  Few pass (about K ln(steps) a workgroup); the entries are brought
-//    down to the K best, by counting those before each, at the end and where a wave has too many.  The workgroups are
-//    shared out over the live rows, which each counts for itself.
+//  beam_scan   a workgroup of four waves a run of a row, a wave 32 logits a lane and step, one step ahead.  A wave keeps
+//    the sum of exp(x - at) for a reference `at` near the maximum, and in LDS what may be among the run's K best (K =
+//    beams + end tokens: enough for `beams` that are no end tokens): values from the K-th of 64 maxima on, each of four
+//    lanes of the workgroup over steps 1, 2, 4, 8 ...  Few pass, about K a doubling of the steps, and the sums of eight
+//    terms tell where to look.  At the end each entry counts those before it.  The workgroups are shared out over the
+//    live rows, which each counts for itself.
 //  beam_join   a workgroup a request.  A wave a row joins the runs' lists in the same way, and their sums; then each
 //    candidate's place is counted in every row's list, by binary search.
 //
-// Numerics: exp in fp32 of (x - m) log2 e with log2 e in two parts, eight of them summed in fp32, everything beyond
-// that in 64 bits: candidates of different beams are told apart by lse's last digits, and its error is about 1e-8.
+// What bounds them (128 x 8 beams of 152064 bf16 logits, 311 MB, 61 us): the vector units are busy 79 % of the scan's time
+// (280 instructions for 32 logits a lane: conversions, two fused products, exp, sum), which streams 7.8 TB/s between a
+// start and an end of 5 us; 5 us are the join's: loads, exp and log in 64 bits, searches.  Small calls are that
+// latency (1 x 4 beams of 32000: 6.4 + 4.7 us).
+//
+// Numerics: exp in fp32 of (x - at) log2 e with log2 e in two parts, eight of them summed in fp32, everything beyond
+// that in 64 bits: candidates of different beams are told apart by lse's last digits, and its error is about 1e-8.  (With
+// one fp32 constant for log2 e, 2 % faster, all terms would share an error of 1.3e-8 of x - at.)
 
 #include "l20_beam_search.h"
 
@@ -32,6 +38,9 @@ namespace l20bs {
 using l20la::f32x4;
 using l20la::i32x4;
 
+// 128 x 8 beams of 152064 tokens, 64 x 4 of 128256, 16 x 5 of 50257: 62.3, 25.2 and 15.8 us; with 8 waves and two runs a CU
+// 63.4, 26.0 and 17.0 (a workgroup ends with its slowest wave), with four runs a CU 61.8, 26.6 and 15.7, with two vectors
+// and six waves a SIMD 76.4, 32.0 and 20.6 (what is done once a step counts twice).
 constexpr int kVectors = 4;                // vectors of eight logits a lane and step
 constexpr int kStep = 64 * 8 * kVectors;   // logits of a wave's step
 constexpr int kWaves = 4;                  // of a workgroup, which takes a run
@@ -39,7 +48,9 @@ constexpr int kMaxRuns = 64;               // runs a row: a lane of the join eac
 constexpr int kRunsPerCu = 3;              // runs that rows are split for
 constexpr int kEntries = 128;              // what a wave's LDS holds of candidates (two a lane)
 constexpr int kJoinWaves = 16;             // of the joins' workgroups, a beam each
-constexpr int kPrune = 8;                  // beams up to which all candidates are placed
+// Beams up to which all candidates are placed.  Measured, 40000 tokens, with and without a choice before: 4 beams of 64
+// requests 18.1 and 17.3 us, 16 of 32 the same, 32 of 16 45.3 and 58.4.
+constexpr int kPrune = 16;
 constexpr int kCounted = 4096;             // rows whose live ones every wave may count (a word of 64 a lane)
 
 struct Params {
@@ -544,26 +555,19 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
         m = lane < runs ? m : -(double)INFINITY;
         part = lane < runs ? part : 0.0;
         Best best(s_keys + wave * (kEntries + 2), k);
-        if (runs * k <= kEntries) {  // all of them
-          best.show(v, t, lane < runs * k);
-          if (runs * k > 64) best.show(v1, t1, lane + 64 < runs * k);
-        } else {
-          // lists in order: heads first, until no run has one that may be among the best
-          const int at = min(lane, runs - 1) * k;
+        if (runs >= k) {  // the k-th of the lists' heads bounds what there may be among the best
           float *const heads = reinterpret_cast<float *>(best.keys);  // (the list is empty)
-          float head = lane < runs ? value[at] : -INFINITY;
-          int headt = token[at];
-          heads[lane] = head;
+          heads[lane] = lane < runs ? value[lane * k] : -INFINITY;
           best.bound_by(heads);
+        }
+        // 64 entries at once, two such loads ahead
 #pragma unroll 1
-          for (int j = 1;; ++j) {
-            const bool ok = head >= best.least && key_of(head, headt) >= best.bar;
-            if (!__ballot(ok)) break;
-            best.show(head, headt, ok);
-            if (j == k) break;
-            head = ok ? value[at + j] : -INFINITY;
-            headt = token[at + j];
-          }
+        for (int i = 0; i < runs * k; i += 64) {
+          const float x = v;
+          const int y = t, e = min(i + 128 + lane, last);
+          v = v1, t = t1;
+          v1 = value[e], t1 = token[e];
+          best.show(x, y, i + lane < runs * k);
         }
         best.settle();
         // (a NaN stays one: it is in `part`, and a run of -inf alone has the part 0)
