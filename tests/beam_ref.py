@@ -5,19 +5,21 @@ import math
 import torch
 
 
-def candidates(logits, scores):
-    """Every candidate of one request, best first: (score, beam, logit, token).  logits [beams, vocab] and scores [beams]
-    in float64."""
-    found = []
-    for w in range(logits.shape[0]):
-        c, x = float(scores[w]), logits[w]
-        if not math.isfinite(c) or bool(x.isnan().any()) or bool((x == math.inf).any()) or bool((x == -math.inf).all()):
-            continue
-        top = x.max()
-        lse = float(top + (x - top).exp().sum().log())
-        found += [(c + (v - lse), w, v, t) for t, v in enumerate(x.tolist()) if v > -math.inf]
-    found = [f for f in found if math.isfinite(float(torch.tensor(f[0], dtype=torch.float64).float()))]
-    return sorted(found, key=lambda f: (-f[0], f[1], -f[2], f[3]))
+def candidates(logits, scores, most):
+    """The first `most` candidates of one request, best first: (score, beam, logit, token).  logits [beams, vocab] and
+    scores [beams] in float64."""
+    x, vocab = logits, logits.shape[1]
+    bad = ~scores.isfinite() | x.isnan().any(1) | (x == math.inf).any(1) | (x == -math.inf).all(1)
+    x = torch.where(bad[:, None], -math.inf, x)
+    top = x.amax(1, keepdim=True)
+    lse = top + (x - top).exp().sum(1, keepdim=True).log()
+    total = torch.where(bad[:, None], -math.inf, scores[:, None] + (x - lse)).flatten()
+    x = x.flatten()
+    keep = torch.nonzero(total.float().isfinite())[:, 0]  # by beam and token
+    for key in (-x, torch.div(torch.arange(x.numel()), vocab, rounding_mode="floor"), -total):  # least important first
+        keep = keep[torch.sort(key[keep], stable=True).indices]
+    keep = keep[:most].tolist()
+    return [(float(total[i]), i // vocab, float(x[i]), i % vocab) for i in keep]
 
 
 def beam_step(logits, scores, ends):
@@ -26,7 +28,7 @@ def beam_step(logits, scores, ends):
     out, gap = [[] for _ in range(6)], math.inf
     beams = scores.shape[1]
     for r in range(scores.shape[0]):
-        ranked = candidates(logits[r].double(), scores[r].double())
+        ranked = candidates(logits[r].double(), scores[r].double(), beams * (len(ends) + 1) + 1)
         runs = [f for f in ranked if f[3] not in ends][:beams]
         over = [f for f in ranked[:beams] if f[3] in ends]
         seen = 0

@@ -74,6 +74,15 @@ def test_beams_and_end_tokens(beams, ends):
     check(logits, scores, tokens)
 
 
+@pytest.mark.parametrize("beams,vocab,ends", [(32, 40000, 8), (20, 66000, 1), (32, 20, 3), (17, 18, 1), (32, 40, 8), (9, 200000, 0)])
+def test_many_beams_over_long_and_short_vocabularies(beams, vocab, ends):
+    """More entries than a wave's list holds, joined from several runs; fewer tokens than beams."""
+    logits, scores = inputs(2, beams, vocab, torch.bfloat16, seed=7 * beams + vocab)
+    tokens = [(2 * e + 1) % vocab for e in range(ends)]
+    logits[:, ::3, tokens] += 6
+    check(logits, scores, tokens)
+
+
 def test_end_tokens_that_are_none():
     """Outside the vocabulary, below it, and named twice."""
     logits, scores = inputs(2, 3, 100, torch.float16, seed=4)
@@ -291,6 +300,26 @@ def test_graph_and_another_stream():
         torch.cuda.synchronize()
         assert all(a.equal(b) for a, b in zip(out, want))
         eager = want.scores.clone()
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with its workspace and outputs, of different sizes: as alone."""
+    import l20_beam_search as bs
+
+    cases = []
+    for n, (requests, beams, vocab) in enumerate(((40, 4, 30000), (3, 8, 90000))):
+        logits, scores = inputs(requests, beams, vocab, torch.float16, seed=90 + n)
+        x, s = logits.cuda(), scores.cuda()
+        cases.append((x, s, filled(requests, beams), bs.allocate_l20_beam_search_workspace(x, s, end_tokens=[4]),
+                      bs.l20_beam_search_step(x, s, end_tokens=[4]), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x, s, out, ws, _, stream in cases:
+            with torch.cuda.stream(stream):
+                bs.l20_beam_search_step(x, s, end_tokens=[4], out=out, workspace=ws)
+    torch.cuda.synchronize()
+    for _, _, out, _, want, _ in cases:
+        assert all(a.equal(b) for a, b in zip(out, want))
 
 
 def test_refusals():
