@@ -22,7 +22,7 @@ extern "C" {
  *
  *   logits  [requests, beams, vocab] dtype (bf16, fp16 or fp32), rows of any alignment of the element
  *   scores  [requests, beams] fp32, the beams' summed log-probabilities; a beam whose score is not finite
- *           is dead: its logits are not read
+ *           is dead: its logits do not matter
  *   end_tokens  HOST array of num_end_tokens ids
  *
  * The candidate (w, v) of a request has the score  s = scores[w] + (logits[w][v] - log sum_u exp logits[w][u])

@@ -80,7 +80,8 @@ int32_t l20_pd_block_tables(const l20_pd_block_tables_args *args, void *stream);
  * page must be held by one row only, which these calls keep true.  Pages that no row holds any more go on top of
  * the stack first, by rising number (what it cannot hold is dropped); then the copies take theirs from the top,
  * row by row.  A row that finds none, or no page number, keeps -1 in that cell and is counted in count[1].  Cells that no row
- * holds are left as they were; numbers outside 0 .. pages - 1 are held by nobody.  Pairs: room >= groups * beams.
+ * holds are left as they were; numbers outside 0 .. pages - 1 are held by nobody, and children get them as they are, as
+ * a last page too.  Pairs: room >= groups * beams.
  * One or two launches.
  */
 typedef struct l20_pd_reorder_args {

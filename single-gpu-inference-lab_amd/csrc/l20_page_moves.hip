@@ -213,7 +213,8 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
       const int q = __builtin_amdgcn_readlane(row.parent, i0 + i), copy = __builtin_amdgcn_readlane(row.copy, i0 + i);
       if (q < 0 || (q == i0 + i && copy < 0)) continue;  // given up, or as it was
       if (c == copy) source(group * beams + i0 + i, v[i]);
-      else if (c < __builtin_amdgcn_readlane(new_held, i0 + i) && !(c < __builtin_amdgcn_readlane(held, i0 + i) && v[i] == old[i]))
+      if (c == copy && held_page(v[i])) continue;  // (its own page comes from the pool)
+      if (c < __builtin_amdgcn_readlane(new_held, i0 + i) && !(c < __builtin_amdgcn_readlane(held, i0 + i) && v[i] == old[i]))
         cells[(i0 + i) * p.t_sr] = v[i];
     }
   }
@@ -270,6 +271,7 @@ __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_
       for (int j = 0; j < me; ++j) first &= family[j] != parent;
       row[i] = row_of(me, parent, s_len[group * p.beams + max(parent, 0)], parent >= 0 && family[parent] == parent, first, p.page,
                       p.width);
+      if (row[i].copy >= 0 && (from[i] < 0 || from[i] >= p.pages)) row[i].copy = -1;  // the parent has no page there either
       wanted += row[i].copy >= 0;
     }
   }

@@ -73,7 +73,7 @@ def l20_beam_search_step(
     in ``end_tokens`` (at most 8); candidates with an end token are given apart where they are among the first
     ``beams`` of all.  Candidates are ordered by score (in 64 bits), then lower beam, higher logit, lower token.
 
-    A beam whose score is not finite is dead and its logits are not read: a first step has scores 0 and, for all but
+    A beam whose score is not finite is dead and its logits do not matter: a first step has scores 0 and, for all but
     one beam, -inf; a finished request has -inf alone, and gets parents of -1.  Masked tokens (-inf) are never taken,
     and a row with a NaN or +inf, or masked throughout, gives no candidates.  Where there are fewer candidates than
     beams the rest are tokens and parents of -1 with a score of -inf.

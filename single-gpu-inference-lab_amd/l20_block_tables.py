@@ -117,7 +117,7 @@ def l20_reorder_block_tables(
     the first); every other child gets a fresh page, and a pair that says which tokens to copy to it.  Pages that no
     row holds any more go on top of the stack by rising number, before fresh ones are taken, so a search never needs
     more pages than it has given up.  A row that finds none keeps -1 in that cell and is counted in ``count[1]``: its
-    tokens there are masked by the attention and skipped by the producers.
+    tokens there, and its children's, are masked by the attention and skipped by the producers.
 
     Rows that share pages are given up here, and not by ``l20_build_block_tables``, which knows no shares; a page that
     is not full must be held by one row, which both keep true.  With ``copies`` (room for a pair a row) and
@@ -156,10 +156,10 @@ def l20_compact_pages(
 
     The lowest such page moves to the lowest free one, and so on, as long as there is room (in ``copies`` too: by default
     for every cell of the table or page of the pool, whichever are fewer); ``count[1]`` says how many had to stay.
-    ``block_table``, ``page_shares`` and the stack follow: it keeps the pages below ``limit`` that are still free, the lowest on top, and
-    those beyond leave the pool.  The contents are still to be copied (``l20_copy_pages``, whole pages).  A page that
-    neither the stack nor a row of the table holds stays where it is, so every table that shares pages with this one
-    has to be in the call."""
+    ``block_table``, ``page_shares`` and the stack follow: it keeps the pages below ``limit`` that are still free, the
+    lowest on top, and those beyond leave the pool.  The contents are still to be copied (``l20_copy_pages``, whole
+    pages).  A page that neither the stack nor a row of the table holds stays where it is, so every table that shares
+    pages with this one has to be in the call."""
     _need_gpu("l20_compact_pages", block_table)
     if copies is None:
         copies = PageCopies.empty(min(block_table.numel(), page_shares.numel()), block_table.device)

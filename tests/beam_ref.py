@@ -77,7 +77,7 @@ def reorder(parents, table, lens, shares, free, count, page):
             keeper = q if alive[q] == q else alive.index(q)
             own = length // page if length % page and keeper != i and length // page < width else -1
             for c in range(pages_of(length, page, width)):
-                if c == own:
+                if c == own and 0 <= source[c] < pages:
                     wanted.append((row, c, source[c], length % page))
                     continue
                 new_table[row][c] = source[c]

@@ -172,6 +172,27 @@ def test_reorder_when_pages_run_out():
     assert sum(r.count(-1) for r in after["table"]) == 8
 
 
+@pytest.mark.parametrize("groups", [2, 20], ids=["one launch", "two"])
+def test_reorder_children_of_a_row_without_its_last_page(groups):
+    """What found no page has none to copy from either: its children get the same number, masked as it is, and take no
+    page from the pool, whose contents would be another's."""
+    c = pool(groups, 4, 16, longest=40, spare=0, seed=8, lens=[40] * groups, shared=0.0)
+    first = check_reorder(c, [[0, -1, -1, -1]] * groups)
+    first["count"] = 0
+    short = check_reorder(first, [[0, 0, 0, 0]] * groups)
+    assert short["short"] == 3 * groups and not short["pairs"]
+    short["free"], short["count"] = [v for v in range(len(c["shares"])) if not any(v in r[:3] for r in short["table"])], 2 * groups
+    after = check_reorder(short, [[2, 2, 3, 2]] * groups)
+    assert after["short"] == 0 and not after["pairs"]
+    assert all(r[2] == -1 for r in after["table"])
+    back = check_reorder(after, [[-1, -1, -1, -1]] * groups)
+    assert back["count"] == after["count"] + 2 * groups
+    # a number beyond the pool is no page either, and lies in a column where the child held another one
+    c["table"][1][2] = 10 ** 7
+    odd = check_reorder(c, [[1, 1, 1, 3]] + [[0, 1, 2, 3]] * (groups - 1))
+    assert [r[2] for r in odd["table"][:3]] == [10 ** 7] * 3 and not odd["pairs"]
+
+
 def test_reorder_with_bad_numbers():
     """Numbers outside the pool in table, stack and parents, negative lengths, rows longer than the table, a stack too
     small for what comes back: nothing is read or written out of bounds, and the rules hold."""
