@@ -139,6 +139,7 @@ BAD = [
     ("compact_pages", dict(page_size=0), "page size"),
     ("compact_pages", dict(table_pages=0), "must not be empty"),
     ("compact_pages", dict(limit=-1), "limit must be"),
+    ("compact_pages", dict(pages=(1 << 30) + 1), "too large"),
     ("compact_pages", dict(limit=501), "limit must be"),
     ("compact_pages", dict(room=-1), "room must not"),
     ("compact_pages", dict(src=0), "null tensor pointer"),

@@ -349,6 +349,10 @@ def test_compact_large_pool():
     used = len(c["shares"]) - c["count"]
     after, _, left = check_compact(c, used + 5)
     assert left == 0 and after["count"] == 5
+    c = pool(10, 4, 16, longest=2000, spare=700_000, seed=22)  # more than one thread takes a page of
+    used = len(c["shares"]) - c["count"]
+    for limit in (used + 400_000, used, 300):
+        check_compact(c, limit)
 
 
 def test_compact_no_rows_and_graph():
