@@ -82,20 +82,24 @@ struct Params {
 
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // (global loads of any alignment are one load here)
 
-// Eight logits as loaded.
+// Eight logits a lane of a vector of 512, 16 bytes a lane side by side: of fp32 four and, 256 further on, four (1024 rows of
+// 128256 104 us, with all eight in a row 122).
 template <typename T> struct Eight { i32x4 w[sizeof(T) / 2]; };
+template <typename T> constexpr int kSide = 16 / sizeof(T);
+template <typename T> __device__ __forceinline__ constexpr int place_of(int i) { return i / kSide<T> * 64 * kSide<T> + i % kSide<T>; }
 
 template <typename T> __device__ __forceinline__ Eight<T> load8(const T *p) {
   Eight<T> r;
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4_any *>(p) + i);
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    r.w[i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4_any *>(p + place_of<T>(i * kSide<T>)));
   return r;
 }
 // Those at or beyond `n` are -inf and not read.
 template <typename T> __device__ __forceinline__ Eight<T> load8_guarded(const T *p, int n) {
   T e[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : (T)-INFINITY;
+  for (int i = 0; i < 8; ++i) e[i] = place_of<T>(i) < n ? p[place_of<T>(i)] : (T)-INFINITY;
   return __builtin_bit_cast(Eight<T>, e);
 }
 template <typename T> __device__ __forceinline__ void unpack(const Eight<T> &r, float (&x)[8]) {
@@ -295,17 +299,22 @@ struct Best {
 __device__ __forceinline__ int live_row(const Params &p, int rows, int unit, u64 *s_live, int &runs, int &run) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int kEach = kCounted / 64 / kWaves;
-  float s[kEach];
+  if (p.flat) {
+    float s[kEach];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int r = (wave + i * kWaves) * 64 + lane;
-    s[i] = INFINITY;
-    if (r < rows) s[i] = p.flat ? p.scores[r] : p.scores[r / p.beams * p.s_sr + r % p.beams * p.s_sb];
-  }
+    for (int i = 0; i < kEach; ++i) s[i] = p.scores[min((wave + i * kWaves) * 64 + lane, rows - 1)];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const u64 which = __ballot(finite(s[i]));
-    if (lane == 0) s_live[wave + i * kWaves] = which;
+    for (int i = 0; i < kEach; ++i) {
+      const u64 which = __ballot(finite(s[i]) && (wave + i * kWaves) * 64 + lane < rows);
+      if (lane == 0) s_live[wave + i * kWaves] = which;
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kEach; ++i) {
+      const int r = (wave + i * kWaves) * 64 + lane, at = min(r, rows - 1), request = at / p.beams;
+      const u64 which = __ballot(finite(p.scores[request * p.s_sr + (at - request * p.beams) * p.s_sb]) && r < rows);
+      if (lane == 0) s_live[wave + i * kWaves] = which;
+    }
   }
   l20la::lds_barrier();
   const u64 mask = s_live[lane];
@@ -346,7 +355,7 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
   const T *x0 = nullptr;
   Eight<T> next[kVectors];
   auto load = [&](int step) {
-    const int at = step * kStep + lane * 8;
+    const int at = step * kStep + lane * kSide<T>;
     if (step < min(full, end)) {
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) next[i] = load8(x0 + at + i * 512);
@@ -434,7 +443,7 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) {
         if (!__ballot(part[i] >= low)) continue;
-        const int token = step * kStep + i * 512 + lane * 8;
+        const int token = step * kStep + i * 512 + lane * kSide<T>;
         u64 which[8];
         int total = best.count;
 #pragma unroll
@@ -448,7 +457,7 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (which[j]) best.put(x[i][j], token + j, which[j]);
+          if (which[j]) best.put(x[i][j], token + place_of<T>(j), which[j]);
       }
       if (many) {
         // those one after the other, through LDS
@@ -462,9 +471,9 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
             *reinterpret_cast<f32x4 *>(to) = f32x4{x[u][0], x[u][1], x[u][2], x[u][3]};
             *reinterpret_cast<f32x4 *>(to + 4) = f32x4{x[u][4], x[u][5], x[u][6], x[u][7]};
           }
-          const int token = step * kStep + i * 512 + lane * 8;
+          const int token = step * kStep + i * 512 + lane * kSide<T>;
 #pragma unroll 1
-          for (int j = 0; j < 8; ++j) best.show(s_vector[wave][lane * 8 + j], token + j, true);
+          for (int j = 0; j < 8; ++j) best.show(s_vector[wave][lane * 8 + j], token + place_of<T>(j), true);
         }
         best.pass();
         low = ref.low(best.least);
