@@ -10,6 +10,17 @@
 //  cp_clear, cp_mark, cp_place, cp_remap   pages to move and pages to move to as bitmaps; a page's rank among them,
 //    and so its place, from the bits before it; the table's cells by the ranks.  cp_small: all of it in one launch.
 //  pc_copy    workgroups take (pair, cache, 16 KB) in turn.
+//
+// What bounds them: for all but the copies the latency of a few dependent loads, not bytes (kernel times).
+//  rp_cells   64 groups of 4 beams of 4000-8000 tokens (0.4 MB of cells) 6.6 us: lengths and parents, cells, atomics of
+//    page_shares in two waves (gains, losses), cells.  24 groups of 16 beams, a quarter given back, 11.9: up to 16 atomics
+//    a lane, eight in flight.
+//  rp_pool    7-9 us: lists' lengths, their entries, two scans, the stack; one workgroup, since its answer is an order.
+//  rp_small   4 groups of 4 beams 9.7 us, both chains one behind the other (two launches: 15.6 a call against 12.3).
+//  cp_clear, cp_mark, cp_place, cp_remap   256 rows, a pool of 200000 pages 2.1 + 6.6 + 7.1 + 3.7 us: launches, 200000 atomics
+//    on the bitmaps, and counting before placing.  cp_small: 16 rows, 4096 pages 6.0 us.
+//  pc_copy    memory: 512 whole pages of 16 tokens of 56 caches (470 MB read and written) 198 us, 4.75 TB/s (a library copy of
+//    1 GiB 5.12); 12 pages in part of 56 fp8 caches 4.3 us.
 
 #include "l20_block_tables.h"
 
