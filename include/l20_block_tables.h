@@ -114,7 +114,8 @@ int32_t l20_pd_reorder_tables(const l20_pd_reorder_args *args, void *stream);
  * l20_pd_compact_pages: the pool shrinks to the pages below `limit`.  Pages that the table's rows hold at or
  * beyond it move to free pages below it, the lowest to the lowest, as many as there is room for; table, page_shares
  * and stack follow, and the pairs say what to copy (tokens: page_size).  The stack keeps the pages below the limit
- * that are still free, the lowest on top; those beyond it leave the pool.  count[1]: pages that had to stay beyond.
+ * that are still free, the lowest on top; those beyond it leave the pool.  count[1]: pages that had to stay beyond
+ * (the stack gets them back when they are given up).
  * A page that neither the stack nor a row of the table holds stays where it is.
  */
 typedef struct l20_pd_compact_args {

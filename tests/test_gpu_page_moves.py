@@ -297,6 +297,35 @@ def test_reorder_replayed_with_the_block_tables():
     assert width * page > max(c["lens"])
 
 
+def test_two_pools_on_two_streams():
+    """Calls on two pools, of one launch and of two, each on its stream with its workspace: as alone."""
+    import l20_block_tables as bt
+
+    runs = []
+    for groups, beams, spare in ((3, 4, 60), (40, 3, 400)):
+        c = pool(groups, beams, 16, longest=100, spare=spare, seed=groups)
+        steps = [parents_of(groups, beams, 50 + n, released=0.05) for n in range(6)]
+        sent, dev, stream = [t32(p) for p in steps], on_device(c), torch.cuda.Stream()
+        runs.append((c, steps, sent, dev, stream, bt.allocate_l20_reorder_workspace(sent[0], dev["table"]),
+                     [bt.PageCopies.empty(groups * beams, "cuda") for _ in steps]))
+    torch.cuda.synchronize()
+    for n in range(6):
+        for _, _, sent, dev, stream, ws, copies in runs:
+            with torch.cuda.stream(stream):
+                bt.l20_reorder_block_tables(sent[n], dev["table"], dev["lens"], dev["shares"], dev["free"], dev["count"], 16,
+                                            copies=copies[n], workspace=ws)
+    torch.cuda.synchronize()
+    for c, steps, _, dev, _, _, copies in runs:
+        for parents, pairs in zip(steps, copies):
+            want = R.reorder(parents, c["table"], c["lens"], c["shares"], c["free"], c["count"], 16)
+            c.update(zip(("table", "lens", "shares", "free", "count"), want))
+            assert listed(pairs) == (want[5], want[6])
+        held_once(c)
+        for k in ("table", "lens", "shares", "free"):
+            assert dev[k].tolist() == c[k], k
+        assert int(dev["count"]) == c["count"]
+
+
 # --------------------------------------------------------------------------- compaction
 def check_compact(c, limit, room=None):
     import l20_block_tables as bt
