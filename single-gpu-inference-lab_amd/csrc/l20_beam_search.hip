@@ -59,11 +59,12 @@ struct Params {
   const float *scores;
   int64_t s_sr, s_sb;
   int requests, beams, vocab, k;
+  unsigned by_beams, by_runs, by_k;  // for `over`
   int runs;         // of every row
   int share;        // where some rows are dead `spread` is shared out over the others, at most `most` each
   int most, spread;
-  int ends[L20_PD_MAX_END_TOKENS];
-  int num_ends;
+  int ends[L20_PD_MAX_END_TOKENS];  // behind the last: -2, no token
+  int full_lists;   // k is beams and end tokens, not the vocabulary
   int flat;         // scores lie one behind the other
   int *row_runs;    // [rows], with `share`
   // [rows * most] and [rows * most * k]
@@ -97,10 +98,22 @@ template <typename T> __device__ __forceinline__ Eight<T> load8(const T *p) {
 }
 // Those at or beyond `n` are -inf and not read.
 template <typename T> __device__ __forceinline__ Eight<T> load8_guarded(const T *p, int n) {
-  T e[8];
+  typedef T side __attribute__((ext_vector_type(kSide<T>)));
+  Eight<T> r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = place_of<T>(i) < n ? p[place_of<T>(i)] : (T)-INFINITY;
-  return __builtin_bit_cast(Eight<T>, e);
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    const int first = place_of<T>(i * kSide<T>);
+    side e = (side)(T)-INFINITY;
+    if (first + kSide<T> <= n) {
+      e = __builtin_bit_cast(side, __builtin_nontemporal_load(reinterpret_cast<const i32x4_any *>(p + first)));
+    } else if (first < n) {  // the row's end
+#pragma unroll
+      for (int j = 0; j < kSide<T> - 1; ++j)
+        if (first + j < n) e[j] = p[first + j];
+    }
+    r.w[i] = __builtin_bit_cast(i32x4, e);
+  }
+  return r;
 }
 template <typename T> __device__ __forceinline__ void unpack(const Eight<T> &r, float (&x)[8]) {
   if constexpr (std::is_same_v<T, __bf16>) {
@@ -156,6 +169,9 @@ __device__ __forceinline__ double wave_sum(double x) {
 __device__ __forceinline__ double wave_max(double x) {
   return wave_fold(x, [](double a, double b) { return fmax(a, b); });
 }
+// n / d by mul = ceil(2^32 / d), 0 for d = 1: exact while n d is below 2^32, since the product's excess is below n / 2^32.
+__host__ __device__ constexpr unsigned mul_of(unsigned d) { return d == 1 ? 0 : 0xffffffffu / d + 1; }
+__device__ __forceinline__ int over(int n, unsigned mul) { return mul ? (int)__umulhi((unsigned)n, mul) : n; }
 __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < INFINITY; }
 
 // log2 e in two parts: one fp32 constant is off by 1.3e-8 of itself, which all terms of a sum would share.
@@ -295,33 +311,28 @@ struct Best {
 };
 
 // The n-th live row, n = unit / runs, and how many runs each has: every workgroup counts for itself, a bit a row in
-// `s_live` [kCounted / 64].  All scores at once: 1024 rows counted 64 by 64 took 6 us.  -1: none.
-__device__ __forceinline__ int live_row(const Params &p, int rows, int unit, u64 *s_live, int &runs, int &run) {
+// `s_live` [kCounted / 64].  Scores of 1024 rows at once (counted 64 by 64 they took 6 us).  -1: none.
+__device__ __forceinline__ int live_row(const Params &p, int rows, int unit, u64 *s_live, int &runs, unsigned &by_runs, int &run) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  constexpr int kEach = kCounted / 64 / kWaves;
-  if (p.flat) {
-    float s[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) s[i] = p.scores[min((wave + i * kWaves) * 64 + lane, rows - 1)];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const u64 which = __ballot(finite(s[i]) && (wave + i * kWaves) * 64 + lane < rows);
-      if (lane == 0) s_live[wave + i * kWaves] = which;
-    }
-  } else {
 #pragma unroll 1
-    for (int i = 0; i < kEach; ++i) {
-      const int r = (wave + i * kWaves) * 64 + lane, at = min(r, rows - 1), request = at / p.beams;
-      const u64 which = __ballot(finite(p.scores[request * p.s_sr + (at - request * p.beams) * p.s_sb]) && r < rows);
-      if (lane == 0) s_live[wave + i * kWaves] = which;
+  for (int i0 = wave; i0 * 64 < rows; i0 += 4 * kWaves) {
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = min((i0 + i * kWaves) * 64 + lane, rows - 1), request = p.flat ? 0 : over(at, p.by_beams);
+      s[i] = p.scores[p.flat ? at : request * p.s_sr + (at - request * p.beams) * p.s_sb];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u64 which = __ballot(finite(s[i]) && (i0 + i * kWaves) * 64 + lane < rows);
+      if (lane == 0 && (i0 + i * kWaves) * 64 < rows) s_live[i0 + i * kWaves] = which;
     }
   }
   l20la::lds_barrier();
-  const u64 mask = s_live[lane];
+  const u64 mask = lane * 64 < rows ? s_live[lane] : 0;
   int upto = __builtin_popcountll(mask);
   if (!__ballot(upto != min(max(rows - lane * 64, 0), 64))) {  // all of them
-    runs = p.runs;
-    const int row = unit / runs;
+    const int row = over(unit, by_runs);
     run = unit - row * runs;
     return row < rows ? row : -1;
   }
@@ -329,7 +340,8 @@ __device__ __forceinline__ int live_row(const Params &p, int rows, int unit, u64
   const int live = __builtin_amdgcn_readlane(upto, 63);
   if (live == 0) return -1;
   runs = min(p.most, max(p.spread / live, 1));
-  const int n = unit / runs;
+  by_runs = mul_of(runs);
+  const int n = over(unit, by_runs);
   run = unit - n * runs;
   if (n >= live) return -1;
   const int chunk = __builtin_ctzll(__ballot(upto > n));
@@ -351,7 +363,8 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = blockIdx.x, rows = p.requests * p.beams;
   const int full = p.vocab / kStep, steps = (p.vocab + kStep - 1) / kStep;
-  int runs = p.runs, row = unit / runs, run = unit - row * runs, first = 0, end = 0;
+  unsigned by_runs = p.by_runs;
+  int runs = p.runs, row = over(unit, by_runs), run = unit - row * runs, first = 0, end = 0;
   const T *x0 = nullptr;
   Eight<T> next[kVectors];
   auto load = [&](int step) {
@@ -366,20 +379,21 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
     }
   };
   auto begin = [&] {
-    const int request = row / p.beams, beam = row - request * p.beams;
+    const int request = over(row, p.by_beams), beam = row - request * p.beams;
     x0 = reinterpret_cast<const T *>(p.logits) + request * p.l_sr + beam * p.l_sb;
-    first = (int)((u64)(unsigned)run * (unsigned)steps / (unsigned)runs) + wave;
-    end = (int)((u64)(unsigned)(run + 1) * (unsigned)steps / (unsigned)runs);
+    first = over(run * steps, by_runs) + wave;  // (at most 2^6 runs, 2^19 steps)
+    end = over((run + 1) * steps, by_runs);
     load(first);
   };
   if (p.share) {
-    row = live_row(p, rows, unit, s_live, runs, run);
+    row = live_row(p, rows, unit, s_live, runs, by_runs, run);
     if (row < 0) return;
     if (run == 0 && threadIdx.x == 0) p.row_runs[row] = runs;
     begin();
   } else {
     if (row >= rows) return;
-    const float s = p.scores[row / p.beams * p.s_sr + row % p.beams * p.s_sb];
+    const int request = over(row, p.by_beams);
+    const float s = p.scores[request * p.s_sr + (row - request * p.beams) * p.s_sb];
     begin();  // (as if the row lived: its loads need not wait for the score)
     if (!finite(s)) return;
   }
@@ -513,6 +527,7 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
     double high = s_ref[0];
     for (int w = 1; w < kWaves; ++w) high = fmax(high, s_ref[w]);
     double total = 0.0;
+#pragma unroll 1
     for (int w = 0; w < kWaves; ++w) {
       const double r = s_ref[w], part = s_sum[w][lane];
       total += r == high || part == 0.0 ? part : part * exp(r - high);
@@ -539,7 +554,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int request = blockIdx.x;
   if (threadIdx.x == 0) *s_ended = *s_kept = 0;
+#pragma unroll 1
   for (int i = threadIdx.x; i < n; i += threads) s_rank[i] = 0;
+#pragma unroll 1
   for (int beam = wave; beam < beams; beam += waves) {
     // every load at once, also where the row turns out dead or its runs fewer
     const int row = request * beams + beam;
@@ -553,12 +570,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
     const int last = p.most * k - 1;
     float v = value[min(lane, last)], v1 = value[min(lane + 64, last)];
     int t = token[min(lane, last)], t1 = token[min(lane + 64, last)];
+    const float head = value[min(lane * k, last)];
     int count = 0;
     u64 ends = 0;
     if (finite(c)) {
-      double lse;
+      double top, total;
       if (runs == 1) {  // a list in order
-        lse = lane_d(m, 0) + log(lane_d(part, 0));
+        top = lane_d(m, 0);
+        total = lane_d(part, 0);
         v = lane < k ? v : -INFINITY;
       } else {
         m = lane < runs ? m : -(double)INFINITY;
@@ -566,7 +585,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
         Best best(s_keys + wave * (kEntries + 2), k);
         if (runs >= k) {  // the k-th of the lists' heads bounds what there may be among the best
           float *const heads = reinterpret_cast<float *>(best.keys);  // (the list is empty)
-          heads[lane] = lane < runs ? value[lane * k] : -INFINITY;
+          heads[lane] = lane < runs ? head : -INFINITY;
           best.bound_by(heads);
         }
         // 64 entries at once, two such loads ahead
@@ -576,19 +595,20 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
           const int y = t, e = min(i + 128 + lane, last);
           v = v1, t = t1;
           v1 = value[e], t1 = token[e];
-          best.show(x, y, i + lane < runs * k);
+          best.put(x, y, __ballot(i + lane < runs * k && x >= best.least && key_of(x, y) >= best.bar));
+          if (i + 64 >= runs * k || best.count > kEntries - 64) best.settle();
         }
-        best.settle();
         // (a NaN stays one: it is in `part`, and a run of -inf alone has the part 0)
-        const double top = wave_max(m);
-        lse = top + log(wave_sum(m == top || part == 0.0 ? part : part * exp(m - top)));
+        top = wave_max(m);
+        total = wave_sum(m == top || part == 0.0 ? part : part * exp(m - top));
         const u64 key = lane < best.count ? best.keys[lane] : key_of(-INFINITY, -1);
         v = value_of(key);
         t = token_of(key);
       }
-      const double score = (double)c + ((double)v - lse);
+      const double score = (double)c + ((double)v - (top + log(total)));
       bool is_end = false;
-      for (int e = 0; e < p.num_ends; ++e) is_end |= t == p.ends[e];
+#pragma unroll
+      for (int e = 0; e < L20_PD_MAX_END_TOKENS; ++e) is_end |= t == p.ends[e];
       const bool live = lane < k && finite((float)score);
       count = __builtin_popcountll(__ballot(live));  // the first ones: scores fall with the lane
       ends = __ballot(live && is_end);
@@ -607,12 +627,11 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
   // last on, so nothing below that is.  (Of wide rows most fall out: the searches below are a row for each candidate.)
   int survivors = n;
   if (beams > kPrune) {
-    double bar = -INFINITY;
-    if (k == beams + p.num_ends)
-      for (int w = 0; w < beams; ++w)
-        if (s_count[w] == k) bar = fmax(bar, s_score[w * k + k - 1]);
+    const int w = min(lane, beams - 1);
+    const double bar = wave_max(p.full_lists && s_count[w] == k ? s_score[w * k + k - 1] : -(double)INFINITY);
+#pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += threads) {
-      const int i = i0 + threadIdx.x, beam = (unsigned)i / (unsigned)k;
+      const int i = i0 + threadIdx.x, beam = over(i, p.by_k);
       const bool keep = i < n && i - beam * k < s_count[beam] && s_score[i] >= bar;
       const u64 which = __ballot(keep);
       int at = 0;
@@ -626,7 +645,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
   // a thread a candidate and row: those of the row that come before it (lower beams first among equals)
   for (unsigned i = threadIdx.x; i < (unsigned)(survivors * beams); i += threads) {
     const int w = i / (unsigned)survivors, c = i - w * survivors, mine = beams > kPrune ? s_list[c] : c;
-    const int beam = (unsigned)mine / (unsigned)k, j = mine - beam * k;
+    const int beam = over(mine, p.by_k), j = mine - beam * k;
     if (j >= s_count[beam]) continue;
     const double score = s_score[mine];
     int lo = 0, hi = s_count[w];
@@ -641,10 +660,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join(Params p) {
     if (lo) atomicAdd(s_rank + mine, lo + (ahead_ends << 16));  // (whole numbers: no order)
   }
   __syncthreads();
-  int running = 0;
-  for (int w = 0; w < beams; ++w) running += s_count[w] - __builtin_popcountll(s_end[w]);
+  const int running = __builtin_amdgcn_readlane(l20la::wave_scan(lane < beams ? s_count[lane] - __builtin_popcountll(s_end[lane]) : 0), 63);
+#pragma unroll 1
   for (int c = threadIdx.x; c < survivors; c += threads) {
-    const int i = beams > kPrune ? s_list[c] : c, beam = (unsigned)i / (unsigned)k, j = i - beam * k;
+    const int i = beams > kPrune ? s_list[c] : c, beam = over(i, p.by_k), j = i - beam * k;
     if (j >= s_count[beam]) continue;
     const int ahead = s_rank[i] & 0xffff, ahead_ends = s_rank[i] >> 16;
     if (s_end[beam] >> j & 1) {
@@ -787,8 +806,8 @@ int32_t l20_pd_beam_step(const l20_pd_beam_step_args *a, void *stream) {
   p.requests = a->requests;
   p.beams = a->beams;
   p.vocab = a->vocab;
-  p.num_ends = a->num_end_tokens;
-  for (int i = 0; i < p.num_ends; ++i) p.ends[i] = a->end_tokens[i];
+  for (int i = 0; i < L20_PD_MAX_END_TOKENS; ++i) p.ends[i] = i < a->num_end_tokens ? a->end_tokens[i] : -2;
+  p.full_lists = p.k == a->beams + a->num_end_tokens;
   p.flat = (a->beams == 1 || a->s_stride_beam == 1) && (a->requests == 1 || a->s_stride_request == a->beams);
   const int64_t slots = rows * p.most;
   p.sum = reinterpret_cast<double *>(a->workspace);
@@ -802,6 +821,9 @@ int32_t l20_pd_beam_step(const l20_pd_beam_step_args *a, void *stream) {
   p.ended_tokens = a->ended_tokens;
   p.ended_parents = a->ended_parents;
   p.ended_scores = a->ended_scores;
+  p.by_beams = l20bs::mul_of(p.beams);
+  p.by_runs = l20bs::mul_of(p.runs);
+  p.by_k = l20bs::mul_of(p.k);
   p.join_waves = std::min(a->beams, l20bs::kJoinWaves);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)units), block(64 * l20bs::kWaves);

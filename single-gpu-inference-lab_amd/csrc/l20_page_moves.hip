@@ -49,7 +49,21 @@ constexpr int kSmall = 16;
 // 30000 pages 40.6 and 17.7.
 constexpr int kSmallPages = 1 << 13, kSmallWaves = 64;
 
-__device__ __forceinline__ int pages_of(int tokens, int page) { return tokens > 0 ? (int)(((int64_t)tokens + page - 1) / page) : 0; }
+// A page of 16 d tokens, and division by it: of n / 16 below 2^28 by d as a product with ceil(2^(28 + l) / d), 2^l >= d, whose
+// excess is below 2^-l.  (The compiler's divisions are long, and code is what small calls wait for.)
+struct Page {
+  int size;
+  uint32_t mul;
+  int shift;
+  Page(int size_ = 16) : size(size_), shift(28) {
+    const uint64_t d = (uint64_t)size / 16;
+    while (((uint64_t)1 << (shift - 28)) < d) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ int whole(unsigned n) const { return (int)((uint64_t)(n >> 4) * mul >> shift); }
+  __device__ __forceinline__ int part(int n) const { return n - whole(n) * size; }  // (n not negative)
+  __device__ __forceinline__ int held(int tokens) const { return tokens > 0 ? whole((unsigned)tokens + size - 1) : 0; }
+};
 
 __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
@@ -78,11 +92,14 @@ __device__ __forceinline__ int scan(int x, int (*s_wave)[kThreads / 64], int &to
   return y[0];
 }
 
-// The maximum over the wave (of values that are not negative).
+// The maximum over the wave: rotations within rows of 16, then a lane of each.
+template <int CTRL> __device__ __forceinline__ int rotated_max(int x) {
+  return max(x, __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false));
+}
 __device__ __forceinline__ int max_of(int x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x = max(x, __shfl_xor(x, off));
-  return __builtin_amdgcn_readfirstlane(x);
+  x = rotated_max<0x121>(rotated_max<0x122>(rotated_max<0x124>(rotated_max<0x128>(x))));
+  return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+             max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
 }
 
 struct Reorder {
@@ -99,8 +116,11 @@ struct Reorder {
   int32_t *src, *dst, *tokens;
   int room;
   int32_t *pairs;
-  int groups, beams, page;
+  int groups, beams;
+  Page page;
   int blocks;           // of 64 columns
+  unsigned by_beams;    // ceil(2^18 / beams): rows (below 2^13) by beams
+  int ring;             // a power of two, no less than the rows
   int32_t *list_count;  // [groups * blocks]
   int32_t *list;        // [groups * blocks][beams * 64]
   int32_t *source;      // [groups * beams] the page that a row's copy comes from
@@ -112,10 +132,11 @@ struct Row {
   int len;     // new
   int copy;    // the column of its own copy, -1: none
 };
-__device__ __forceinline__ Row row_of(int row, int parent, int parent_len, bool parent_stays, bool first, int page, int width) {
+__device__ __forceinline__ Row row_of(int row, int parent, int parent_len, bool parent_stays, bool first, const Page &page, int width) {
   Row r{parent, parent >= 0 ? max(parent_len, 0) : 0, -1};
   const bool keeps = parent_stays ? parent == row : first;
-  if (parent >= 0 && r.len % page != 0 && !keeps && r.len / page < width) r.copy = r.len / page;
+  const int last = page.whole(r.len);
+  if (parent >= 0 && last * page.size != r.len && !keeps && last < width) r.copy = last;
   return r;
 }
 
@@ -147,21 +168,21 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
     if (parent == i) first = lane == __builtin_ctzll(mine_of);
   }
   const Row row = row_of(known, parent, parent_len, parent >= 0 && grandparent == parent, first, p.page, p.width);
-  const int held = min(pages_of(old_len, p.page), p.width), new_held = min(pages_of(row.len, p.page), p.width);
-  const int partial = old_len % p.page ? old_len / p.page : -1;  // the column of a last page that is not full
+  const int held = min(p.page.held(old_len), p.width), new_held = min(p.page.held(row.len), p.width);
+  const int partial = p.page.part(old_len) ? p.page.whole(old_len) : -1;  // the column of a last page that is not full
   const int most = max_of(lane < beams ? max(held, new_held) : 0);
   if (block * 64 >= most) return;  // nothing here
   int32_t *const cells = p.table + (int64_t)group * beams * p.t_sr + min(c, p.width - 1);
-  // the cells: loads of eight rows at once (of a lane behind the table: its last column)
+  // the cells: loads of four rows at once (of a lane behind the table: its last column)
   bool same = true;  // all rows hold the page of row 0
   int page0 = -1;
-  for (int i0 = 0; i0 < beams; i0 += 8) {
-    int v[8];
+  for (int i0 = 0; i0 < beams; i0 += 4) {
+    int v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
       if (i0 + i < beams) v[i] = cells[(i0 + i) * p.t_sr];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if (i0 + i >= beams) break;
       const bool has = c < __builtin_amdgcn_readlane(held, i0 + i);
       v[i] = has ? v[i] : -1;
@@ -209,17 +230,17 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
       }
     }
   }
-  // the table, eight rows at once
-  for (int i0 = 0; i0 < beams; i0 += 8) {
-    int v[8], old[8];
+  // the table, four rows at once
+  for (int i0 = 0; i0 < beams; i0 += 4) {
+    int v[4], old[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if (i0 + i >= beams) break;
       v[i] = mine[max(__builtin_amdgcn_readlane(row.parent, i0 + i), 0) * 64];
       old[i] = mine[(i0 + i) * 64];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if (i0 + i >= beams) break;
       const int q = __builtin_amdgcn_readlane(row.parent, i0 + i), copy = __builtin_amdgcn_readlane(row.copy, i0 + i);
       if (q < 0 || (q == i0 + i && copy < 0)) continue;  // given up, or as it was
@@ -231,22 +252,25 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
   }
 }
 
-// LDS of share_out, in ints: the bitmap, list offsets, then lengths, parents and the freed pages that are on top.
+// LDS of share_out, in ints: the bitmap, list offsets, then lengths, parents and (`ring`) the freed pages that are on top.
 __host__ __device__ constexpr int bitmap_words(int pages) { return ((pages < kBitmap ? pages : kBitmap) + 31) / 32; }
-__host__ __device__ constexpr int pool_ints(int pages, int units, int rows) {
-  return bitmap_words(pages) + (units < kUnits ? units : kUnits) + 1 + 3 * rows;
+__host__ __device__ constexpr int pool_ints(int pages, int units, int rows, int ring) {
+  return bitmap_words(pages) + (units < kUnits ? units : kUnits) + 1 + 2 * rows + ring;
 }
 
 // The pool, one workgroup: freed pages onto the stack by number, then each row's copy from it.  The pages to take are the
 // last that were freed, or lie where nothing is written: nothing is read back.  `marked`: the freed pages are in the
-// bitmap already, else in lists a wave.
-__device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_wave)[kThreads / 64], bool marked,
+// bitmap already, else in lists a wave.  PER: rows a thread, at most (1 or all that there may be: 256 rows PERFIG).
+template <int PER> __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_wave)[kThreads / 64], bool marked,
                                           const int *s_source) {
   const int tid = threadIdx.x, rows = p.groups * p.beams, units = p.groups * p.blocks;
   unsigned int *const s_bits = (unsigned int *)s_mem;
   int *const s_at = s_mem + bitmap_words(p.pages), *const s_len = s_at + min(units, kUnits) + 1;
   int *const s_parent = s_len + rows, *const s_top = s_parent + rows;
   const int count = min(max(*p.count, 0), p.pool);
+  __shared__ int s_short;  // a row found no page
+  if (tid == 0) s_short = 0;
+#pragma unroll 1
   for (int r = tid; r < rows; r += kThreads) {
     s_len[r] = p.lens[r];
     s_parent[r] = p.parents[r];
@@ -258,27 +282,28 @@ __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_
     const int u = tid * kLists + i;
     lengths[i] = !marked && u < units ? p.list_count[u] : 0;
   }
-  const int per_row = (rows + kThreads - 1) / kThreads;
-  int from[kPerThread];  // (of rows without a copy: whatever is there)
+  const int per_row = PER == 1 ? 1 : (rows + kThreads - 1) / kThreads;
+  int from[PER];  // (of rows without a copy: whatever is there)
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int r = tid * per_row + i;
     if (i < per_row && r < rows) from[i] = s_source ? s_source[r] : p.source[r];
   }
   // rows that need a page, in order
-  Row row[kPerThread];
+  Row row[PER];
   int wanted = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int r = tid * per_row + i;
     row[i] = Row{-1, 0, -1};
     if (i < per_row && r < rows) {
-      const int group = r / p.beams, me = r - group * p.beams;
+      const int group = (int)((unsigned)r * p.by_beams >> 18), me = r - group * p.beams;
       const int *const family = s_parent + group * p.beams;
       int parent = family[me];
       if (parent < 0 || parent >= p.beams) parent = -1;
       bool first = true;
+#pragma unroll 1
       for (int j = 0; j < me; ++j) first &= family[j] != parent;
       row[i] = row_of(me, parent, s_len[group * p.beams + max(parent, 0)], parent >= 0 && family[parent] == parent, first, p.page,
                       p.width);
@@ -297,6 +322,7 @@ __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_
   auto push = [&](int base, int words) {
     const int per = (words + kThreads - 1) / kThreads;
     int mine = 0;
+#pragma unroll 1
     for (int i = 0; i < per; ++i)
       if (tid * per + i < words) mine += __builtin_popcount(s_bits[tid * per + i]);
     int here;
@@ -307,7 +333,7 @@ __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_
         const int page = base + (tid * per + i) * 32 + __builtin_ctz(w);
         if (rank >= last) continue;
         p.stack[count + rank] = page;
-        if (rank >= last - rows) s_top[rank % rows] = page;
+        if (rank >= last - rows) s_top[rank & (p.ring - 1)] = page;
       }
     freed += here;
     __syncthreads();
@@ -356,15 +382,15 @@ __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_
     }
   }
   const int have = (int)min((int64_t)count + freed, (int64_t)p.pool), kept = have - count;
-  int got[kPerThread], served = 0, k = first_wanted;
+  int got[PER], served = 0, k = first_wanted;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int r = tid * per_row + i;
     got[i] = -1;
     if (i < per_row && r < rows) {
       p.lens[r] = row[i].len;
       if (row[i].copy >= 0) {
-        if (k < have) got[i] = k < kept ? s_top[(kept - 1 - k) % rows] : p.stack[have - 1 - k];
+        if (k < have) got[i] = k < kept ? s_top[(kept - 1 - k) & (p.ring - 1)] : p.stack[have - 1 - k];
         ++k;
         if (got[i] < 0 || got[i] >= p.pages) got[i] = -1;
         p.table[r * p.t_sr + row[i].copy] = got[i];
@@ -373,16 +399,19 @@ __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_
     }
   }
   int pairs = total, at = first_wanted;
-  if (__syncthreads_or(served != wanted)) at = scan(served, s_wave, pairs) - served;
+  if (served != wanted) s_short = 1;
+  __syncthreads();
+  if (s_short) at = scan(served, s_wave, pairs) - served;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
+  for (int i = 0; i < PER; ++i) {
     if (got[i] >= 0) {
       p.src[at] = from[i];
       p.dst[at] = got[i];
-      p.tokens[at] = row[i].len % p.page;
+      p.tokens[at] = p.page.part(row[i].len);
       ++at;
     }
   }
+#pragma unroll 1
   for (int i = pairs + tid; i < p.room; i += kThreads) p.src[i] = -1, p.dst[i] = -1, p.tokens[i] = 0;
   if (tid == 0) {
     p.pairs[0] = pairs;
@@ -409,10 +438,10 @@ __global__ __launch_bounds__(64 * kCellWaves) void rp_cells(Reorder p) {
   if (lane == 0) p.list_count[unit] = listed;
 }
 
-__global__ __launch_bounds__(kThreads) void rp_pool(Reorder p) {
+template <int PER> __global__ __launch_bounds__(kThreads) void rp_pool(Reorder p) {
   extern __shared__ int s_mem[];
   __shared__ int s_wave[2][kThreads / 64];
-  share_out(p, s_mem, s_wave, false, nullptr);
+  share_out<PER>(p, s_mem, s_wave, false, nullptr);
 }
 
 // Both in one launch, for few waves' worth of cells: freed pages go straight into the bitmap.
@@ -422,9 +451,11 @@ __global__ __launch_bounds__(kThreads) void rp_small(Reorder p) {
   __shared__ int s_source[kSmall * L20_PD_MAX_BEAMS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int units = p.groups * p.blocks, words = bitmap_words(p.pages);
-  int *const s_cells = s_mem + pool_ints(p.pages, units, p.groups * p.beams);
+  int *const s_cells = s_mem + pool_ints(p.pages, units, p.groups * p.beams, p.ring);
+#pragma unroll 1
   for (int i = threadIdx.x; i < words; i += kThreads) s_mem[i] = 0;
   __syncthreads();
+#pragma unroll 1
   for (int unit = wave; unit < units; unit += kThreads / 64) {
     const int group = unit / p.blocks;
     follow_parents(
@@ -435,7 +466,8 @@ __global__ __launch_bounds__(kThreads) void rp_small(Reorder p) {
         [&](int row, int v) { s_source[row] = v; });
   }
   __syncthreads();
-  share_out(p, s_mem, s_wave, true, s_source);
+  static_assert(kSmall * L20_PD_MAX_BEAMS <= kThreads, "a row a thread");
+  share_out<1>(p, s_mem, s_wave, true, s_source);
 }
 
 struct Compact {
@@ -452,7 +484,8 @@ struct Compact {
   int32_t *src, *dst, *tokens;
   int room;
   int32_t *pairs;
-  int rows, page;
+  int rows;
+  Page page;
   int words;           // of a bitmap of the pages
   unsigned int *high;  // pages held at or beyond the limit
   unsigned int *low;   // free ones below it
@@ -511,7 +544,7 @@ __device__ __forceinline__ void settle_pair(const Compact &p, int k, int moves) 
     const int from = p.src[k], to = p.dst[k];
     p.shares[to] = p.shares[from];
     p.shares[from] = 0;
-    p.tokens[k] = p.page;
+    p.tokens[k] = p.page.size;
   } else {
     p.src[k] = -1, p.dst[k] = -1, p.tokens[k] = 0;
   }
@@ -531,7 +564,7 @@ __global__ __launch_bounds__(256) void cp_mark(Compact p) {
   const int64_t tables = (int64_t)p.rows * p.row_blocks;
   if (blockIdx.x < tables) {
     const int row = (int)(blockIdx.x / p.row_blocks), c = (int)(blockIdx.x % p.row_blocks) * 256 + threadIdx.x;
-    if (c >= min(pages_of(p.lens[row], p.page), p.width)) return;
+    if (c >= min(p.page.held(p.lens[row]), p.width)) return;
     const int v = p.table[row * p.t_sr + c];
     if (v >= p.limit && v < p.pages) atomicOr(p.high + (v >> 5), 1u << (v & 31));
   } else {
@@ -581,7 +614,7 @@ __global__ __launch_bounds__(kThreads) void cp_place(Compact p, int each) {
 
 // Where the page of a cell goes: its rank among the pages to move says which pair.
 __device__ __forceinline__ void remap(const Compact &p, const unsigned int *high, const int *rank, int row, int c, int moves) {
-  if (c >= min(pages_of(p.lens[row], p.page), p.width)) return;
+  if (c >= min(p.page.held(p.lens[row]), p.width)) return;
   int32_t *const cell = p.table + row * p.t_sr + c;
   const int v = *cell;
   if (v < p.limit || v >= p.pages) return;
@@ -613,7 +646,7 @@ __global__ __launch_bounds__(kThreads) void cp_small(Compact p) {
     if (v >= 0 && v < p.limit) atomicOr(s_low + (v >> 5), 1u << (v & 31));
   }
   for (int row = wave; row < p.rows; row += kThreads / 64) {
-    const int held = min(pages_of(p.lens[row], p.page), p.width);
+    const int held = min(p.page.held(p.lens[row]), p.width);
     for (int c = lane; c < held; c += 64) {
       const int v = p.table[row * p.t_sr + c];
       if (v >= p.limit && v < p.pages) atomicOr(s_high + (v >> 5), 1u << (v & 31));
@@ -635,7 +668,7 @@ __global__ __launch_bounds__(kThreads) void cp_small(Compact p) {
   __syncthreads();
   for (int k = tid; k < p.room; k += kThreads) settle_pair(p, k, moves);
   for (int row = wave; row < p.rows; row += kThreads / 64) {
-    const int held = min(pages_of(p.lens[row], p.page), p.width);
+    const int held = min(p.page.held(p.lens[row]), p.width);
     for (int c = lane; c < held; c += 64) remap(p, s_high, s_rank, row, c, moves);
   }
   if (tid == 0) finish(p, moves, all_high, all_low);
@@ -837,6 +870,14 @@ template <typename A> int32_t apart(const A *a, const void *parents, int64_t row
   return L20_PD_OK;
 }
 
+template <int PER> int32_t launch_pool(const l20pm::Reorder &p, int most, int lds, hipStream_t s) {
+  static l20la::LdsLimit limit;
+  const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20pm::rp_pool<PER>), most);
+  if (e != hipSuccess) return set_error(L20_PD_ELAUNCH, hipGetErrorString(e));
+  hipLaunchKernelGGL(l20pm::rp_pool<PER>, dim3(1), dim3(l20pm::kThreads), (size_t)lds, s, p);
+  return launched();
+}
+
 template <typename V> int32_t launch_copy(const l20pm::Copy &p, bool runs, hipStream_t s) {
   const int64_t jobs = (int64_t)p.room * p.caches * p.runs * p.segments;
   const unsigned grid = (unsigned)std::min<int64_t>(jobs, 8 * (int64_t)l20la::device_cus());
@@ -884,15 +925,17 @@ int32_t l20_pd_reorder_tables(const l20_pd_reorder_args *a, void *stream) {
   p.pairs = a->count;
   p.groups = a->groups;
   p.beams = a->beams;
-  p.page = a->page_size;
+  p.page = l20pm::Page(a->page_size);
   p.blocks = a->groups > 0 ? (a->table_pages + 63) / 64 : 0;
   p.list_count = reinterpret_cast<int32_t *>(a->workspace);
   p.list = p.list_count + (int64_t)p.groups * p.blocks;
   p.source = p.list + (int64_t)p.groups * p.blocks * p.beams * 64;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int rows = p.groups * p.beams, units = p.groups * p.blocks;
-  const int most = 4 * l20pm::pool_ints(l20pm::kBitmap, l20pm::kUnits, L20_PD_MAX_REQUESTS);
-  const int lds = 4 * l20pm::pool_ints(p.pages, units, rows), cells = l20pm::kThreads / 64 * p.beams * 256;
+  p.by_beams = ((1u << 18) + p.beams - 1) / p.beams;
+  for (p.ring = 1; p.ring < rows;) p.ring *= 2;
+  const int most = 4 * l20pm::pool_ints(l20pm::kBitmap, l20pm::kUnits, L20_PD_MAX_REQUESTS, L20_PD_MAX_REQUESTS);
+  const int lds = 4 * l20pm::pool_ints(p.pages, units, rows, p.ring), cells = l20pm::kThreads / 64 * p.beams * 256;
   if (units <= l20pm::kSmall && p.pages <= l20pm::kBitmap && lds + cells <= most) {
     static l20la::LdsLimit limit;
     const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20pm::rp_small), most);
@@ -904,11 +947,7 @@ int32_t l20_pd_reorder_tables(const l20_pd_reorder_args *a, void *stream) {
   hipLaunchKernelGGL(l20pm::rp_cells, grid, dim3(64 * l20pm::kCellWaves), (size_t)l20pm::kCellWaves * p.beams * 256, s, p);
   rc = launched();
   if (rc != L20_PD_OK) return rc;
-  static l20la::LdsLimit limit;
-  const hipError_t e = limit.raise(reinterpret_cast<const void *>(&l20pm::rp_pool), most);
-  if (e != hipSuccess) return set_error(L20_PD_ELAUNCH, hipGetErrorString(e));
-  hipLaunchKernelGGL(l20pm::rp_pool, dim3(1), dim3(l20pm::kThreads), (size_t)lds, s, p);
-  return launched();
+  return rows <= l20pm::kThreads ? launch_pool<1>(p, most, lds, s) : launch_pool<l20pm::kPerThread>(p, most, lds, s);
 }
 
 int32_t l20_pd_compact_pages_check(const l20_pd_compact_args *a) {
@@ -945,7 +984,7 @@ int32_t l20_pd_compact_pages(const l20_pd_compact_args *a, void *stream) {
   p.room = a->room;
   p.pairs = a->count;
   p.rows = a->rows;
-  p.page = a->page_size;
+  p.page = l20pm::Page(a->page_size);
   p.words = (int)words_of(a);
   p.high = reinterpret_cast<unsigned int *>(a->workspace);
   p.low = p.high + p.words;
