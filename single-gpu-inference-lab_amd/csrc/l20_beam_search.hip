@@ -17,11 +17,12 @@
 // What bounds them (128 x 8 beams of 152064 bf16 logits, 311 MB, 61 us): the vector units are busy 79 % of the scan's time
 // (280 instructions for 32 logits a lane: conversions, two fused products, exp, sum), which streams 7.8 TB/s between a
 // start and an end of 5 us; 5 us are the join's: loads, exp and log in 64 bits, searches.  Small calls are that
-// latency (1 x 4 beams of 32000: 6.4 + 4.7 us).
+// latency, of loads and of code that is not in the instruction cache yet (1 x 4 beams of 32000: 6.1 + 4.9 us).
 //
 // Numerics: exp in fp32 of (x - at) log2 e with log2 e in two parts, eight of them summed in fp32, everything beyond
-// that in 64 bits: candidates of different beams are told apart by lse's last digits, and its error is about 1e-8.  (With
-// one fp32 constant for log2 e, 2 % faster, all terms would share an error of 1.3e-8 of x - at.)
+// that in 64 bits: candidates of different beams are told apart by lse's last digits, and its error is about 1e-8 (where one
+// token has nearly all of the mass that term's own: up to 1e-7, which shows in a score near 0 only).  (With one fp32 constant
+// for log2 e, 2 % faster, all terms would share an error of 1.3e-8 of x - at.)
 
 #include "l20_beam_search.h"
 
@@ -49,8 +50,8 @@ constexpr int kRunsPerCu = 3;              // runs that rows are split for
 constexpr int kEntries = 128;              // what a wave's LDS holds of candidates (two a lane)
 constexpr int kJoinWaves = 16;             // of the joins' workgroups, a beam each
 // Beams up to which all candidates are placed.  Measured, 40000 tokens, with and without a choice before: 4 beams of 64
-// requests 18.1 and 17.3 us, 16 of 32 the same, 32 of 16 45.3 and 58.4.
-constexpr int kPrune = 16;
+// requests 17.2 and 16.7 us, 8 of 64 the same, 16 of 32 25.2 and 26.1, 32 of 16 40.6 and 54.8.
+constexpr int kPrune = 8;
 constexpr int kCounted = 4096;             // rows whose live ones every wave may count (a word of 64 a lane)
 
 struct Params {

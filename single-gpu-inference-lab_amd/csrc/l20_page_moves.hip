@@ -12,13 +12,14 @@
 //  pc_copy    workgroups take (pair, cache, 16 KB) in turn.
 //
 // What bounds them: for all but the copies the latency of a few dependent loads, not bytes (kernel times).
-//  rp_cells   64 groups of 4 beams of 4000-8000 tokens (0.4 MB of cells) 6.6 us: lengths and parents, cells, atomics of
-//    page_shares in two waves (gains, losses), cells.  24 groups of 16 beams, a quarter given back, 11.9: up to 16 atomics
-//    a lane, eight in flight.
-//  rp_pool    7-9 us: lists' lengths, their entries, two scans, the stack; one workgroup, since its answer is an order.
-//  rp_small   4 groups of 4 beams 9.7 us, both chains one behind the other (two launches: 15.6 a call against 12.3).
-//  cp_clear, cp_mark, cp_place, cp_remap   256 rows, a pool of 200000 pages 2.1 + 6.6 + 7.1 + 3.7 us: launches, 200000 atomics
-//    on the bitmaps, and counting before placing.  cp_small: 16 rows, 4096 pages 6.0 us.
+//  rp_cells   64 groups of 4 beams of 4000-8000 tokens (0.4 MB of cells) 6.0 us: lengths and parents, cells, atomics of
+//    page_shares in two waves (gains, losses), cells.  24 groups of 16 beams, a quarter given back, 11.0: up to 16 atomics
+//    a lane, eight in flight (two, four, 16 at once: 1.7 and 0.6 us more, and 4.5: small calls and single waves wait for code
+//    as much as for data, and 16 are too much of it).
+//  rp_pool    5.3-6.7 us: lists' lengths, their entries, two scans, the stack; one workgroup, since its answer is an order.
+//  rp_small   4 groups of 4 beams 7.4 us, both chains one behind the other.
+//  cp_clear, cp_mark, cp_place, cp_remap   256 rows, a pool of 200000 pages 2.0 + 6.8 + 6.6 + 3.3 us: launches, 200000 atomics
+//    on the bitmaps, and counting before placing.  cp_small: 16 rows, 4096 pages 5.7 us.
 //  pc_copy    memory: 512 whole pages of 16 tokens of 56 caches (470 MB read and written) 198 us, 4.75 TB/s (a library copy of
 //    1 GiB 5.12); 12 pages in part of 56 fp8 caches 4.3 us.
 
@@ -42,7 +43,7 @@ constexpr int kCellWaves = 4;
 constexpr int kBitmap = 1 << 18;  // pages of one pass of rp_pool (32 KB of LDS)
 constexpr int kUnits = 4096;      // waves' lists that rp_pool looks at together
 // Waves' worth of cells that one launch does with the pool, one a wave.  Measured against two launches: 8 groups of 4
-// beams, 64 cells 12.3 and 15.6 us, 16 groups 14.3 and 16.0; more than one a wave, 32 groups 19.5 and 15.9.
+// beams, 64 cells 10.2 and 13.1 us, 16 groups 12.0 and 13.7; more than one a wave, 32 groups 17.3 and 13.9.
 constexpr int kSmall = 16;
 // Pages, and waves' worth of cells, of a compaction in one launch.  Measured against four: 64 rows of 64 cells, 8192 pages
 // 13.1 and 17.4 us, 16 of 128, 4096 pages 8.2 and 16.8; beyond, 64 rows of 256, 20000 pages 28.1 and 17.4, 256 rows of 64,
@@ -140,7 +141,7 @@ __device__ __forceinline__ Row row_of(int row, int parent, int parent_len, bool 
   return r;
 }
 
-// One wave's 64 columns of a group; s_cells: [beams][64] of the wave.  `free_page(page, where)` takes the lanes' pages that
+// One wave's 64 columns of a group; s_cells: [beams][64] of the wave, wave-uniform.  `free_page(page, where)` takes the lanes' pages that
 // nobody holds any more, `source(row, page)` the page that a row's copy comes from.
 //
 // A row whose parent row r has n children: n - 1 more rows hold each full page of r, and its last page, where that is not
@@ -160,37 +161,34 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
   if (parent < 0 || parent >= beams) parent = -1;
   const int from = max(parent, 0);
   const int parent_len = __shfl(old_len, from), grandparent = __shfl(parent, from);  // (by every lane)
-  bool first = true;
-  int children = 0;
-  for (int i = 0; i < beams; ++i) {
-    const unsigned long long mine_of = __ballot(parent == i && lane < beams);
-    if (lane == i) children = __builtin_popcountll(mine_of);
-    if (parent == i) first = lane == __builtin_ctzll(mine_of);
+  // rows of the same parent, and this row's children, by the bits of the parents' numbers
+  const bool alive = parent >= 0 && lane < beams;
+  unsigned long long siblings = __ballot(alive), mine_of = siblings;
+  for (int b = 0; 1 << b < beams; ++b) {
+    const unsigned long long set = __ballot(parent >> b & 1);
+    siblings &= parent >> b & 1 ? set : ~set;
+    mine_of &= lane >> b & 1 ? set : ~set;
   }
+  const bool first = lane == __builtin_ctzll(siblings | (unsigned long long)1 << 63);
+  const int children = lane < beams ? __builtin_popcountll(mine_of) : 0;
   const Row row = row_of(known, parent, parent_len, parent >= 0 && grandparent == parent, first, p.page, p.width);
   const int held = min(p.page.held(old_len), p.width), new_held = min(p.page.held(row.len), p.width);
   const int partial = p.page.part(old_len) ? p.page.whole(old_len) : -1;  // the column of a last page that is not full
   const int most = max_of(lane < beams ? max(held, new_held) : 0);
   if (block * 64 >= most) return;  // nothing here
   int32_t *const cells = p.table + (int64_t)group * beams * p.t_sr + min(c, p.width - 1);
-  // the cells: loads of four rows at once (of a lane behind the table: its last column)
-  bool same = true;  // all rows hold the page of row 0
-  int page0 = -1;
-  for (int i0 = 0; i0 < beams; i0 += 4) {
-    int v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i0 + i < beams) v[i] = cells[(i0 + i) * p.t_sr];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i0 + i >= beams) break;
-      const bool has = c < __builtin_amdgcn_readlane(held, i0 + i);
-      v[i] = has ? v[i] : -1;
-      mine[(i0 + i) * 64] = v[i];
-      if (i0 + i == 0) page0 = v[i];
-      same &= has && v[i] == page0;
-    }
-  }
+  // the cells, all rows' in flight together (of a lane behind the table: its last column; of rows that end before: whatever
+  // lies there)
+#pragma unroll 1
+  for (int i = 0; i < beams; ++i)
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(cells + i * p.t_sr),
+                                     (__attribute__((address_space(3))) void *)(s_cells + i * 64), 4, 0, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  bool same = c < __builtin_amdgcn_readlane(held, 0);  // all rows hold the page of row 0
+  const int page0 = same ? mine[0] : -1;
+#pragma unroll 4
+  for (int i = 1; i < beams; ++i) same &= c < __builtin_amdgcn_readlane(held, i) && mine[i * 64] == page0;
+  const bool settled = same;  // nothing of this column is written
   auto held_page = [&](int v) { return v >= 0 && v < p.pages; };
   // page_shares
   auto freed = [&](int v, bool gone) {
@@ -211,7 +209,7 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
       if (gains) {
         for (unsigned long long m = gains; m; m &= m - 1) {
           const int r = __builtin_ctzll(m), v = mine[r * 64];
-          if (!same && held_page(v) && c != __builtin_amdgcn_readlane(partial, r))
+          if (!same && c < __builtin_amdgcn_readlane(held, r) && held_page(v) && c != __builtin_amdgcn_readlane(partial, r))
             atomicAdd(p.shares + v, __builtin_amdgcn_readlane(children, r) - 1);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // gains before losses
@@ -220,7 +218,8 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
         int v[8], was[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i, m &= m - 1) {
-          v[i] = m && !same ? mine[__builtin_ctzll(m) * 64] : -1;
+          const int r = m ? __builtin_ctzll(m) : 0;
+          v[i] = m && !same && c < __builtin_amdgcn_readlane(held, r) ? mine[r * 64] : -1;
           was[i] = 1;
           if (held_page(v[i])) was[i] = atomicAdd(p.shares + v[i], -1);
         }
@@ -231,14 +230,12 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
     }
   }
   // the table, four rows at once
+  if (!__ballot(!settled || (row.copy >= block * 64 && row.copy < block * 64 + 64))) return;
   for (int i0 = 0; i0 < beams; i0 += 4) {
-    int v[4], old[4];
+    int v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i0 + i >= beams) break;
-      v[i] = mine[max(__builtin_amdgcn_readlane(row.parent, i0 + i), 0) * 64];
-      old[i] = mine[(i0 + i) * 64];
-    }
+    for (int i = 0; i < 4; ++i)
+      if (i0 + i < beams) v[i] = mine[max(__builtin_amdgcn_readlane(row.parent, i0 + i), 0) * 64];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i0 + i >= beams) break;
@@ -246,8 +243,7 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
       if (q < 0 || (q == i0 + i && copy < 0)) continue;  // given up, or as it was
       if (c == copy) source(group * beams + i0 + i, v[i]);
       if (c == copy && held_page(v[i])) continue;  // (its own page comes from the pool)
-      if (c < __builtin_amdgcn_readlane(new_held, i0 + i) && !(c < __builtin_amdgcn_readlane(held, i0 + i) && v[i] == old[i]))
-        cells[(i0 + i) * p.t_sr] = v[i];
+      if (!settled && c < __builtin_amdgcn_readlane(new_held, i0 + i)) cells[(i0 + i) * p.t_sr] = v[i];
     }
   }
 }
@@ -260,13 +256,14 @@ __host__ __device__ constexpr int pool_ints(int pages, int units, int rows, int 
 
 // The pool, one workgroup: freed pages onto the stack by number, then each row's copy from it.  The pages to take are the
 // last that were freed, or lie where nothing is written: nothing is read back.  `marked`: the freed pages are in the
-// bitmap already, else in lists a wave.  PER: rows a thread, at most (1 or all that there may be: 256 rows PERFIG).
+// bitmap already, else in lists a wave.  PER: rows a thread, at most: 1, or all that there may be (256 rows 13.9 and 14.5 us
+// a call).
 template <int PER> __device__ __forceinline__ void share_out(const Reorder &p, int *s_mem, int (*s_wave)[kThreads / 64], bool marked,
                                           const int *s_source) {
   const int tid = threadIdx.x, rows = p.groups * p.beams, units = p.groups * p.blocks;
   unsigned int *const s_bits = (unsigned int *)s_mem;
   int *const s_at = s_mem + bitmap_words(p.pages), *const s_len = s_at + min(units, kUnits) + 1;
-  int *const s_parent = s_len + rows, *const s_top = s_parent + rows;
+  int *const s_parent = s_len + rows, *const s_top = s_parent + rows, *const s_first = s_top;  // (done with by then)
   const int count = min(max(*p.count, 0), p.pool);
   __shared__ int s_short;  // a row found no page
   if (tid == 0) s_short = 0;
@@ -274,6 +271,7 @@ template <int PER> __device__ __forceinline__ void share_out(const Reorder &p, i
   for (int r = tid; r < rows; r += kThreads) {
     s_len[r] = p.lens[r];
     s_parent[r] = p.parents[r];
+    s_first[r] = L20_PD_MAX_BEAMS;
   }
   constexpr int kLists = kUnits / kThreads;
   int lengths[kLists];  // of the first kUnits lists
@@ -293,19 +291,28 @@ template <int PER> __device__ __forceinline__ void share_out(const Reorder &p, i
   Row row[PER];
   int wanted = 0;
   __syncthreads();
+  auto row_at = [&](int r, int &me, int &parent) {  // its group's first row
+    const int base = (int)((unsigned)r * p.by_beams >> 18) * p.beams;
+    me = r - base;
+    parent = s_parent[r];
+    if (parent < 0 || parent >= p.beams) parent = -1;
+    return base;
+  };
+#pragma unroll 1
+  for (int r = tid; r < rows; r += kThreads) {
+    int me, parent;
+    const int base = row_at(r, me, parent);
+    if (parent >= 0) atomicMin(s_first + base + parent, me);
+  }
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int r = tid * per_row + i;
     row[i] = Row{-1, 0, -1};
     if (i < per_row && r < rows) {
-      const int group = (int)((unsigned)r * p.by_beams >> 18), me = r - group * p.beams;
-      const int *const family = s_parent + group * p.beams;
-      int parent = family[me];
-      if (parent < 0 || parent >= p.beams) parent = -1;
-      bool first = true;
-#pragma unroll 1
-      for (int j = 0; j < me; ++j) first &= family[j] != parent;
-      row[i] = row_of(me, parent, s_len[group * p.beams + max(parent, 0)], parent >= 0 && family[parent] == parent, first, p.page,
+      int me, parent;
+      const int base = row_at(r, me, parent), from_row = base + max(parent, 0);
+      row[i] = row_of(me, parent, s_len[from_row], parent >= 0 && s_parent[from_row] == parent, s_first[from_row] == me, p.page,
                       p.width);
       if (row[i].copy >= 0 && (from[i] < 0 || from[i] >= p.pages)) row[i].copy = -1;  // the parent has no page there either
       wanted += row[i].copy >= 0;
