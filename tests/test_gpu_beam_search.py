@@ -65,6 +65,23 @@ def test_vocabularies(dtype, vocab):
     check(logits, scores, ends=[vocab // 2, 0] if vocab > 2 else [])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [3, 5, 255, 257, 259, 260, 261, 508, 517, 770, 1023, 2303, 2305, 2309, 8190, 8451])
+def test_rows_that_end_inside_a_load(dtype, vocab):
+    """The last tokens are the best, and what lies behind each row would take all of it."""
+    import l20_beam_search as bs
+
+    logits, scores = inputs(2, 3, vocab, DTYPES[dtype], seed=vocab + 1)
+    for back in range(1, min(vocab, 4)):
+        logits[:, :, vocab - back] += 13 - back
+    hold = torch.full((2, 3, vocab + 7), math.nan, dtype=DTYPES[dtype], device="cuda")
+    hold[:, :, :vocab] = logits.cuda()
+    out = bs.l20_beam_search_step(hold[:, :, :vocab], scores.cuda(), end_tokens=[vocab - 1], out=filled(2, 3))
+    torch.cuda.synchronize()
+    want = compare(out, logits, scores, [vocab - 1])
+    assert any(vocab - 1 in row for row in want[3])
+
+
 @pytest.mark.parametrize("beams", [1, 2, 3, 5, 8, 16, 31, 32])
 @pytest.mark.parametrize("ends", [0, 1, 8])
 def test_beams_and_end_tokens(beams, ends):
