@@ -102,6 +102,7 @@ __device__ __forceinline__ int max_of(int x) {
   return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
              max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
 }
+__device__ __forceinline__ int min_of(int x) { return ~max_of(~x); }
 
 struct Reorder {
   const int32_t *parents;
@@ -141,8 +142,8 @@ __device__ __forceinline__ Row row_of(int row, int parent, int parent_len, bool 
   return r;
 }
 
-// One wave's 64 columns of a group; s_cells: [beams][64] of the wave, wave-uniform.  `free_page(page, where)` takes the lanes' pages that
-// nobody holds any more, `source(row, page)` the page that a row's copy comes from.
+// One wave's 64 columns of a group; s_cells: [beams][64] of the wave, wave-uniform.  `free_page(page, where)` takes the
+// lanes' pages that nobody holds any more, `source(row, page)` the page that a row's copy comes from.
 //
 // A row whose parent row r has n children: n - 1 more rows hold each full page of r, and its last page, where that is not
 // full, one row or none.  So r's page in column c gains n - 1 holders, or loses one (the last page without children),
@@ -184,10 +185,10 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(cells + i * p.t_sr),
                                      (__attribute__((address_space(3))) void *)(s_cells + i * 64), 4, 0, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  bool same = c < __builtin_amdgcn_readlane(held, 0);  // all rows hold the page of row 0
-  const int page0 = same ? mine[0] : -1;
+  const int page0 = mine[0];
+  bool same = c < min_of(lane < beams ? held : INT32_MAX);  // all rows hold the page of row 0
 #pragma unroll 4
-  for (int i = 1; i < beams; ++i) same &= c < __builtin_amdgcn_readlane(held, i) && mine[i * 64] == page0;
+  for (int i = 1; i < beams; ++i) same &= mine[i * 64] == page0;
   const bool settled = same;  // nothing of this column is written
   auto held_page = [&](int v) { return v >= 0 && v < p.pages; };
   // page_shares
@@ -200,17 +201,28 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
   if (gains | losses) {
     // rows whose last page is this column's count differently: no sum for it (nor where there is no page)
     unsigned long long ends = 0;
-    for (unsigned long long m = __ballot(partial >= block * 64 && partial < block * 64 + 64) & rows; m; m &= m - 1)
-      ends |= (unsigned long long)1 << (__builtin_amdgcn_readlane(partial, __builtin_ctzll(m)) - block * 64);
+    for (unsigned long long m = __ballot(partial >= block * 64 && partial < block * 64 + 64) & rows; m;) {
+      const int column = __builtin_amdgcn_readlane(partial, __builtin_ctzll(m));
+      ends |= (unsigned long long)1 << (column - block * 64);
+      m &= ~__ballot(partial == column);
+    }
     same &= held_page(page0) && !(ends >> lane & 1);
     const int together = __builtin_popcountll(__ballot(parent >= 0) & rows) - beams;
     if (together != 0 && __ballot(same)) freed(page0, same && atomicAdd(p.shares + page0, together) + together == -1);
     if (__ballot(!same)) {
       if (gains) {
-        for (unsigned long long m = gains; m; m &= m - 1) {
-          const int r = __builtin_ctzll(m), v = mine[r * 64];
-          if (!same && c < __builtin_amdgcn_readlane(held, r) && held_page(v) && c != __builtin_amdgcn_readlane(partial, r))
-            atomicAdd(p.shares + v, __builtin_amdgcn_readlane(children, r) - 1);
+        for (unsigned long long m = gains; m;) {  // four at once
+          int v[4], more[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i, m &= m - 1) {
+            const int r = m ? __builtin_ctzll(m) : 0;
+            v[i] = mine[r * 64];
+            more[i] = m && c < __builtin_amdgcn_readlane(held, r) && c != __builtin_amdgcn_readlane(partial, r)
+                          ? __builtin_amdgcn_readlane(children, r) - 1 : 0;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!same && more[i] && held_page(v[i])) atomicAdd(p.shares + v[i], more[i]);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // gains before losses
       }
@@ -219,9 +231,9 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
 #pragma unroll
         for (int i = 0; i < 8; ++i, m &= m - 1) {
           const int r = m ? __builtin_ctzll(m) : 0;
-          v[i] = m && !same && c < __builtin_amdgcn_readlane(held, r) ? mine[r * 64] : -1;
+          v[i] = mine[r * 64];
           was[i] = 1;
-          if (held_page(v[i])) was[i] = atomicAdd(p.shares + v[i], -1);
+          if (m && !same && c < __builtin_amdgcn_readlane(held, r) && held_page(v[i])) was[i] = atomicAdd(p.shares + v[i], -1);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -229,22 +241,22 @@ __device__ __forceinline__ void follow_parents(const Reorder &p, int group, int 
       }
     }
   }
-  // the table, four rows at once
-  if (!__ballot(!settled || (row.copy >= block * 64 && row.copy < block * 64 + 64))) return;
+  // a lane a row: where its copy comes from, and the columns that it is given
+  int upto = alive && !(parent == lane && row.copy < 0) ? new_held : 0;  // (else given up, or as it was)
+  if (lane < beams && row.copy >= block * 64 && row.copy < block * 64 + 64) {
+    const int v = s_cells[from * 64 + row.copy - block * 64];
+    source(group * beams + lane, v);
+    if (held_page(v)) upto = row.copy;  // (its own page comes from the pool)
+  }
+  if (!__ballot(!settled)) return;
+  int32_t *to = cells;
   for (int i0 = 0; i0 < beams; i0 += 4) {
     int v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i0 + i < beams) v[i] = mine[max(__builtin_amdgcn_readlane(row.parent, i0 + i), 0) * 64];
+    for (int i = 0; i < 4; ++i) v[i] = mine[__builtin_amdgcn_readlane(from, i0 + i) * 64];  // (rows behind the last: upto 0)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i0 + i >= beams) break;
-      const int q = __builtin_amdgcn_readlane(row.parent, i0 + i), copy = __builtin_amdgcn_readlane(row.copy, i0 + i);
-      if (q < 0 || (q == i0 + i && copy < 0)) continue;  // given up, or as it was
-      if (c == copy) source(group * beams + i0 + i, v[i]);
-      if (c == copy && held_page(v[i])) continue;  // (its own page comes from the pool)
-      if (!settled && c < __builtin_amdgcn_readlane(new_held, i0 + i)) cells[(i0 + i) * p.t_sr] = v[i];
-    }
+    for (int i = 0; i < 4; ++i, to += p.t_sr)
+      if (!settled && c < __builtin_amdgcn_readlane(upto, i0 + i)) *to = v[i];
   }
 }
 
