@@ -12,12 +12,12 @@
 //  pc_copy    workgroups take (pair, cache, 16 KB) in turn.
 //
 // What bounds them: for all but the copies the latency of a few dependent loads, not bytes (kernel times).
-//  rp_cells   64 groups of 4 beams of 4000-8000 tokens (0.4 MB of cells) 6.0 us: lengths and parents, cells, atomics of
-//    page_shares in two waves (gains, losses), cells.  24 groups of 16 beams, a quarter given back, 11.0: up to 16 atomics
+//  rp_cells   64 groups of 4 beams of 4000-8000 tokens (0.4 MB of cells) 5.8 us: lengths and parents, cells, atomics of
+//    page_shares in two waves (gains, losses), cells.  24 groups of 16 beams, a quarter given back, 8.9: up to 16 atomics
 //    a lane, eight in flight (two, four, 16 at once: 1.7 and 0.6 us more, and 4.5: small calls and single waves wait for code
 //    as much as for data, and 16 are too much of it).
-//  rp_pool    5.3-6.7 us: lists' lengths, their entries, two scans, the stack; one workgroup, since its answer is an order.
-//  rp_small   4 groups of 4 beams 7.4 us, both chains one behind the other.
+//  rp_pool    5.3-7.2 us: lists' lengths, their entries, two scans, the stack; one workgroup, since its answer is an order.
+//  rp_small   4 groups of 4 beams 6.9 us, both chains one behind the other.
 //  cp_clear, cp_mark, cp_place, cp_remap   256 rows, a pool of 200000 pages 2.0 + 6.8 + 6.6 + 3.3 us: launches, 200000 atomics
 //    on the bitmaps, and counting before placing.  cp_small: 16 rows, 4096 pages 5.7 us.
 //  pc_copy    memory: 512 whole pages of 16 tokens of 56 caches (470 MB read and written) 198 us, 4.75 TB/s (a library copy of
@@ -43,7 +43,7 @@ constexpr int kCellWaves = 4;
 constexpr int kBitmap = 1 << 18;  // pages of one pass of rp_pool (32 KB of LDS)
 constexpr int kUnits = 4096;      // waves' lists that rp_pool looks at together
 // Waves' worth of cells that one launch does with the pool, one a wave.  Measured against two launches: 8 groups of 4
-// beams, 64 cells 10.2 and 13.1 us, 16 groups 12.0 and 13.7; more than one a wave, 32 groups 17.3 and 13.9.
+// beams, 64 cells 9.8 and 13.1 us, 16 groups 11.8 and 13.7; more than one a wave, 32 groups 17.3 and 13.0.
 constexpr int kSmall = 16;
 // Pages, and waves' worth of cells, of a compaction in one launch.  Measured against four: 64 rows of 64 cells, 8192 pages
 // 13.1 and 17.4 us, 16 of 128, 4096 pages 8.2 and 16.8; beyond, 64 rows of 256, 20000 pages 28.1 and 17.4, 256 rows of 64,
