@@ -6,7 +6,7 @@
 // pass over its logits:
 //
 //  beam_scan   a workgroup of four waves a run of a row, a wave 32 logits a lane and step, one step ahead.  A wave keeps
-//    the sum of exp(x - at) for a reference `at` near the maximum, and in LDS what may be among the run's K best (K =
+//    the sum of exp(x - m) for a reference m near the maximum, and in LDS what may be among the run's K best (K =
 //    beams + end tokens: enough for `beams` that are no end tokens): values from the K-th of 64 maxima on, each of four
 //    lanes of the workgroup over steps 1, 2, 4, 8 ...  Few pass, about K a doubling of the steps, and the sums of eight
 //    terms tell where to look.  At the end each entry counts those before it.  The workgroups are shared out over the
@@ -19,10 +19,12 @@
 // start and an end of 5 us; 5 us are the join's: loads, exp and log in 64 bits, searches.  Small calls are that
 // latency, of loads and of code that is not in the instruction cache yet (1 x 4 beams of 32000: 6.1 + 4.9 us).
 //
-// Numerics: exp in fp32 of (x - at) log2 e with log2 e in two parts, eight of them summed in fp32, everything beyond
-// that in 64 bits: candidates of different beams are told apart by lse's last digits, and its error is about 1e-8 (where one
-// token has nearly all of the mass that term's own: up to 1e-7, which shows in a score near 0 only).  (With one fp32 constant
-// for log2 e, 2 % faster, all terms would share an error of 1.3e-8 of x - at.)
+// Numerics: d = x - m and exp2 of d log2 e in fp32, with log2 e in two parts and one rounding of their sum; eight terms
+// summed in fp32, everything beyond that in 64 bits: candidates of different beams are told apart by lse's last digits.  No
+// exponent is above 4, so the terms that make up a sum are near 1 and the exponents' rounding small.  lse is off by 2-4e-9 on
+// average where many tokens share the mass, and by up to 1.6e-7 where one has most of it: the roundings of its sum of eight,
+// which show in a score near 0 only.  (Two products of x itself, an instruction less, took 62.1 us for 63.3, but the second
+// rounding loses the low part of log2 e: 4e-8 in all of a row's scores.  References up to 2^24 below the best token: up to 1e-6.)
 
 #include "l20_beam_search.h"
 
@@ -178,39 +180,23 @@ __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < IN
 // log2 e in two parts: one fp32 constant is off by 1.3e-8 of itself, which all terms of a sum would share.
 constexpr float kLog2eHi = 1.44269502f, kLog2eLo = 1.92596299e-08f;
 
-// What a wave's sum is relative to: the sum of exp(x - at), with `at` near the maximum m (64 bits).
+// What a wave's sum is relative to: the sum of exp(x - m), with m near the maximum.
 struct Reference {
-  float m = -INFINITY;    // the value that made it
-  float shift = 0.0f;     // m log2 e, rounded: at = shift ln 2 exactly
-  double at = -INFINITY;
-  bool far = false;       // m is so large that its last place times log2 e is no exponent: at = m
+  float m = -INFINITY;  // the value that made it
+  float from = 0.0f;    // m, or 0 where that is -inf (then all terms are 0)
   __device__ __forceinline__ void set(float m_) {
     m = m_;
-    shift = m * kLog2eHi;
-    far = __builtin_fabsf(m) >= 0x1p20f;  // (infinite too)
-    at = far ? (double)m : (double)shift * 0.69314718055994530942;
+    from = m > -INFINITY ? m : 0.0f;
   }
-  // Two roundings of half a step: of the exponent and of the result's last place (v_exp_f32 is good to one step).
+  // Half a step of the exponent (of d too, in fp32 logits) and one of the result (v_exp_f32 is good to one).
   __device__ __forceinline__ float term(float x) const {
-    if (far) {
-      const float d = m > -INFINITY ? x - m : x;  // (all -inf so far: the terms are 0)
-      return __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2eHi, d * kLog2eLo));
-    }
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2eLo, __builtin_fmaf(x, kLog2eHi, -shift)));
+    const float d = x - from;
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2eHi, d * kLog2eLo));
   }
   __device__ __forceinline__ float eight(const float (&x)[8]) const {
     float e[8];
-    if (far) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float d = m > -INFINITY ? x[j] - m : x[j];
-        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2eHi, d * kLog2eLo));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], kLog2eLo, __builtin_fmaf(x[j], kLog2eHi, -shift)));
-    }
+    for (int j = 0; j < 8; ++j) e[j] = term(x[j]);
     return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
   }
   // The term of x less what rounding may make of it; 0 where it is too small to tell.
@@ -443,11 +429,12 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
       return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
     };
     float most = terms();
-    // (The reference need not be the maximum, but these are too far above it, or the first that are not -inf.)
-    if (__ballot(ref.m > -INFINITY ? most > 0x1p24f : highest_of() > -INFINITY)) {
-      const double before = ref.at;
+    // (The reference need not be the maximum, but these are too far above it, or the first that are not -inf: an exponent up to 4
+    // is off by 2^-23, one of 16 by 2^-21.  Eight terms no higher than the reference add up to 8: equal ones do not move it.)
+    if (__ballot(ref.m > -INFINITY ? most > 0x1p4f : highest_of() > -INFINITY)) {
+      const double before = ref.m;
       ref.set(fmaxf(ref.m, wave_max(highest_of())));
-      if (sum != 0.0) sum *= exp(before - ref.at);
+      if (sum != 0.0) sum *= exp(before - (double)ref.m);
       low = ref.low(best.least);
       most = terms();
     }
@@ -497,7 +484,7 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
   }
   s_sum[wave][lane] = sum;
   if (lane == 0) {
-    s_ref[wave] = ref.at;
+    s_ref[wave] = ref.m;
     s_count[wave] = best.count;
   }
   l20la::lds_barrier();

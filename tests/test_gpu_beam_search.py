@@ -359,3 +359,44 @@ def test_refusals():
         bs.l20_beam_search_step(x, s, out=out._replace(ended_tokens=out.tokens))
     with pytest.raises(RuntimeError, match="not lie over an input"):
         bs.l20_beam_search_step(x, s, out=out._replace(ended_scores=x.view(-1)[:6].view(2, 3)))
+
+
+# --------------------------------------------------------------------------- accuracy of a row's log-sum-exp
+def lse_bound(x):
+    """How far the log-sum-exp of each row of `x` (float64) may be off.  A term is exp2 of an fp32 exponent e relative to a
+    reference that no value exceeds by more than 4 ln 2 (a sum of eight terms up to 2^4), so |e| <= max(4, (top - x) log2 e):
+    half a step of e, and log2 e halves of one for the difference that it is made of (no larger steps), times ln 2; exp2 itself (one step: 2^-23); three additions (2^-24 each).  The
+    rest is in 64 bits.  The terms' errors weigh as the terms do; 1 % for products of them."""
+    top = x.amax(-1, keepdim=True)
+    weight = (x - torch.logsumexp(x, -1, keepdim=True)).exp()
+    e = ((top - x) * math.log2(math.e)).clamp_min(4.0)
+    half = torch.exp2(e.log2().ceil() - 25)  # of the steps of (2^(n-1), 2^n]
+    return 1.01 * (weight * ((1 + math.log2(math.e)) * math.log(2) * half + 2.0 ** -23 + 3 * 2.0 ** -24)).sum(-1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [0.0, 100.0, -100.0])
+@pytest.mark.parametrize("late", [True, False], ids=["best late", "spread"])
+@pytest.mark.parametrize("rows,vocab", [(200, 150000), (800, 30000)], ids=["three runs", "one run"])
+def test_log_sum_exp_to_its_last_digits(dtype, offset, late, rows, vocab):
+    """Each row's best score, moved next to 0, where 32 bits show 1e-10: what is left is the error of lse.  Rows whose best
+    token comes last, 0 to 16 above all before it, and rows without one; far from zero too, where log2 e has to be good to
+    more than 32 bits."""
+    import l20_beam_search as bs
+
+    g = torch.Generator(device="cuda").manual_seed(rows + int(offset))
+    x = offset + 2 * torch.randn(rows, 1, vocab, generator=g, device="cuda")
+    if late:
+        at = torch.randint(vocab - vocab // 8, vocab, (rows, 1, 1), generator=g, device="cuda")
+        gap = 16 * torch.rand(rows, 1, 1, generator=g, device="cuda")
+        x.scatter_(2, at, x.amax(-1, keepdim=True) + gap)
+    x = x.to(DTYPES[dtype])
+    wide = x.double()
+    lse, best = torch.logsumexp(wide, -1), wide.amax(-1)
+    scores = (lse - best).float()
+    out = bs.l20_beam_search_step(x, scores, out=filled(rows, 1))
+    want = scores.double() + (best - lse)
+    off = (out.scores.double() - want).abs()
+    assert out.tokens.equal(wide.argmax(-1)) and (out.parents == 0).all()
+    over = float((off / (2.0 ** -24 * want.abs() + lse_bound(wide))).max())
+    assert over <= 1, f"errors up to {float(off.max()):.2g}, {float(off.mean()):.2g} on average"
