@@ -962,10 +962,12 @@ int32_t l20_pd_reorder_tables(const l20_pd_reorder_args *a, void *stream) {
     hipLaunchKernelGGL(l20pm::rp_small, dim3(1), dim3(l20pm::kThreads), (size_t)(lds + cells), s, p);
     return launched();
   }
-  const dim3 grid((unsigned)((p.blocks + l20pm::kCellWaves - 1) / l20pm::kCellWaves), (unsigned)p.groups);
-  hipLaunchKernelGGL(l20pm::rp_cells, grid, dim3(64 * l20pm::kCellWaves), (size_t)l20pm::kCellWaves * p.beams * 256, s, p);
-  rc = launched();
-  if (rc != L20_PD_OK) return rc;
+  if (units > 0) {  // (without groups the pool's part alone: it says that there is nothing to copy)
+    const dim3 grid((unsigned)((p.blocks + l20pm::kCellWaves - 1) / l20pm::kCellWaves), (unsigned)p.groups);
+    hipLaunchKernelGGL(l20pm::rp_cells, grid, dim3(64 * l20pm::kCellWaves), (size_t)l20pm::kCellWaves * p.beams * 256, s, p);
+    rc = launched();
+    if (rc != L20_PD_OK) return rc;
+  }
   return rows <= l20pm::kThreads ? launch_pool<1>(p, most, lds, s) : launch_pool<l20pm::kPerThread>(p, most, lds, s);
 }
 

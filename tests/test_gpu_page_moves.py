@@ -250,6 +250,22 @@ def test_reorder_row_strides_and_no_groups():
     assert copies.count.tolist() == [0, 0] and int(dev["count"]) == want[4]
 
 
+@pytest.mark.parametrize("pages", [1 << 18, (1 << 18) + 1, 300_000, 600_000])
+def test_reorder_no_groups_of_a_large_pool(pages):
+    """Nothing to do, but the copies still say so; around the number of pages that one launch's bitmap holds."""
+    import l20_block_tables as bt
+
+    empty = torch.zeros(0, 4, dtype=torch.int32, device="cuda")
+    shares, free, count = torch.zeros(pages, dtype=torch.int32, device="cuda"), t32([4, 9, pages - 1]), t32([2])
+    copies = bt.PageCopies.empty(5, "cuda")
+    for t in copies:
+        t.fill_(99)
+    bt.l20_reorder_block_tables(empty, empty, empty[:, 0].contiguous(), shares, free, count, 16, copies=copies)
+    assert copies.src.tolist() == copies.dst.tolist() == [-1] * 5 and copies.tokens.tolist() == [0] * 5
+    assert copies.count.tolist() == [0, 0] and count.tolist() == [2] and free.tolist() == [4, 9, pages - 1]
+    assert int(shares.abs().sum()) == 0
+
+
 def test_reorder_replayed_with_the_block_tables():
     """A captured step -- append a token, follow the parents -- whose state advances in device memory; every replay
     equals the plain rules, with eager work between."""
