@@ -115,9 +115,11 @@ def l20_reorder_block_tables(
 
     Full pages are shared.  A last page that is not full stays with one child (the one in its parent's own row, else
     the first); every other child gets a fresh page, and a pair that says which tokens to copy to it.  Pages that no
-    row holds any more go on top of the stack by rising number, before fresh ones are taken, so a search never needs
-    more pages than it has given up.  A row that finds none keeps -1 in that cell and is counted in ``count[1]``: its
-    tokens there, and its children's, are masked by the attention and skipped by the producers.
+    row holds any more go on top of the stack by rising number, before fresh ones are taken.  A group of one length takes as
+    many pages more than it gives back as it has live rows more than before: to be sure of them the stack has to hold
+    ``beams`` less its live rows for every group, also those that a step gave back which left fewer.  A row that finds none
+    keeps -1 in that cell and is counted in ``count[1]``: its tokens there, and its children's, are masked by the attention
+    and skipped by the producers.
 
     Rows that share pages are given up here, and not by ``l20_build_block_tables``, which knows no shares; a page that
     is not full must be held by one row, which both keep true.  With ``copies`` (room for a pair a row) and

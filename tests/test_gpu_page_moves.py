@@ -172,6 +172,46 @@ def test_reorder_when_pages_run_out():
     assert sum(r.count(-1) for r in after["table"]) == 8
 
 
+@pytest.mark.parametrize("groups", [1, 20], ids=["one launch", "two"])
+def test_reorder_that_forks_again_needs_the_pages_it_gave_up(groups):
+    """A step with fewer running beams gives their pages back; one that has all beams again takes a page for each beam that
+    it gains, and a row without one is counted where others took them meanwhile."""
+    c = pool(groups, 4, 16, longest=20, spare=0, seed=17, lens=[20] * groups, shared=0.0)
+    fewer = check_reorder(c, [[0, 1, -1, -1]] * groups)
+    held_once(fewer)
+    assert fewer["count"] == 4 * groups and not fewer["pairs"] and fewer["short"] == 0
+    for left in (0, 1, 2 * groups - 1, 2 * groups):  # what others left on the stack
+        after = check_reorder(dict(fewer, count=left), [[0, 0, 1, 1]] * groups)
+        assert len(after["pairs"]) == left and after["short"] == 2 * groups - left
+        assert sum(r[1] == -1 for r in after["table"]) == after["short"]
+    # as many running beams as before: what a step takes it has given up
+    same = check_reorder(dict(c, count=0), [[0, 0, 1, 1]] * groups)
+    assert same["short"] == 0 and len(same["pairs"]) == 2 * groups
+
+
+@pytest.mark.parametrize("groups,beams", [(3, 4), (20, 5)], ids=["one launch", "two"])
+def test_reorder_takes_a_page_for_each_beam_that_it_gains(groups, beams):
+    """Beams of one length with a page each that is not full: whatever the parents, a step is short of exactly the pages
+    that it gains live rows and that the stack does not hold."""
+    rng = random.Random(23)
+    c = pool(groups, beams, 16, longest=15, spare=0, seed=beams, lens=[1 + g % 15 for g in range(groups)], shared=0.0)
+    for left in (0, 1, 3, 7):
+        state, live = c, groups * beams
+        for most in (2, beams, 1, beams):
+            parents = []
+            for g in range(groups):
+                alive = [q for q in range(beams) if state["lens"][g * beams + q]]
+                now = rng.randint(1, most)
+                parents.append([rng.choice(alive) if i < now else -1 for i in range(beams)])
+            gained = sum(q >= 0 for row in parents for q in row) - live
+            after = check_reorder(dict(state, count=min(left, state["count"])), parents)
+            assert after["short"] == max(0, gained - min(left, state["count"]))
+            state = check_reorder(state, parents)
+            held_once(state)
+            assert state["short"] == 0
+            live += gained
+
+
 @pytest.mark.parametrize("groups", [2, 20], ids=["one launch", "two"])
 def test_reorder_children_of_a_row_without_its_last_page(groups):
     """What found no page has none to copy from either: its children get the same number, masked as it is, and take no
