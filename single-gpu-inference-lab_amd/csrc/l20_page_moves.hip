@@ -827,18 +827,19 @@ int32_t check(const l20_pd_copy_args *a) {
     return set_error(L20_PD_EINVAL, "cache must not be empty");
   if (a->token_level < -1 || a->token_level > 2) return set_error(L20_PD_EINVAL, "token level must be -1 to 2");
   const int64_t size[3] = {a->size0, a->size1, a->size2}, stride[3] = {a->stride0, a->stride1, a->stride2};
-  constexpr int64_t kFar = (int64_t)1 << 40;
-  int64_t span[4] = {a->inner, a->inner, a->inner, a->inner};  // of a step of the level inside
+  constexpr int64_t kFar = (int64_t)1 << 40;  // no level reaches further: sums and products of these stay within 64 bits
+  const auto far = [](int64_t n, int64_t step) { return n > kMaxCells || (n > 1 && step > kFar / (n - 1)); };
+  int64_t bytes = a->inner, span[4] = {a->inner, a->inner, a->inner, a->inner};  // of a step of the level inside
   for (int i = 2; i >= 0; --i) {
-    if (size[i] > kMaxCells || span[i + 1] > kFar) return set_error(L20_PD_EINVAL, "page too large");
-    if (size[i] > 1 && (stride[i] < span[i + 1] || stride[i] > kFar)) return set_error(L20_PD_EINVAL, "a page's parts overlap");
-    span[i] = size[i] > 1 ? (size[i] - 1) * stride[i] + span[i + 1] : span[i + 1];
+    if (bytes > INT32_MAX || far(size[i], stride[i])) return set_error(L20_PD_EINVAL, "page too large");
+    if (size[i] > 1 && stride[i] < span[i + 1]) return set_error(L20_PD_EINVAL, "a page's parts overlap");
+    span[i] = (size[i] > 1 ? (size[i] - 1) * stride[i] : 0) + span[i + 1];
+    bytes *= size[i];
   }
-  if (a->inner * a->size2 > INT32_MAX || a->inner * a->size2 * a->size1 > INT32_MAX ||
-      a->inner * a->size2 * a->size1 * a->size0 > INT32_MAX)
-    return set_error(L20_PD_EINVAL, "page too large");
+  if (bytes > INT32_MAX) return set_error(L20_PD_EINVAL, "page too large");
   if (a->pages > 1) {  // pages are a level among the others, wherever their stride puts them
-    if (a->stride_page < 1 || a->pages > kMaxCells || a->stride_page > kFar) return set_error(L20_PD_EINVAL, "pages overlap");
+    if (far(a->pages, a->stride_page)) return set_error(L20_PD_EINVAL, "cache too large");
+    if (a->stride_page < 1) return set_error(L20_PD_EINVAL, "pages overlap");
     int64_t inside = a->inner;
     bool placed = false;
     for (int i = 2; i >= -1; --i) {

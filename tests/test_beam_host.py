@@ -176,6 +176,31 @@ def test_refusals(case):
     assert rc != 0 and message in error, error
 
 
+@pytest.mark.parametrize("change,message", [
+    (dict(size0=1, token_level=-1, inner=1 << 34, size2=1 << 30, stride2=1 << 34, pages=1), "page too large"),  # 2^64 bytes: 0
+    (dict(size0=1, token_level=-1, inner=1 << 33, size1=4, stride1=1 << 63 - 2, size2=1 << 29, stride2=1 << 33, pages=1), "page too large"),
+    (dict(size0=1 << 30, stride0=1 << 38, inner=1, token_level=-1, pages=1), "page too large"),
+    (dict(size0=2, stride0=1 << 41, inner=1, token_level=-1, pages=1), "page too large"),
+    (dict(pages=1 << 30, stride_page=1 << 36), "cache too large"),
+    (dict(pages=1 << 31, stride_page=1 << 14), "cache too large"),
+    (dict(pages=2, stride_page=(1 << 63) - 1), "cache too large"),
+], ids=str)
+def test_sizes_whose_products_pass_64_bits_are_refused(change, message):
+    args = copy_args()
+    for name, value in change.items():
+        setattr(args, name, value)
+    rc, error = check("copy_pages", args)
+    assert rc != 0 and message in error, error
+
+
+def test_the_largest_caches_pass():
+    """A page of 2^31 - 16 bytes, and pages that reach a terabyte."""
+    args = copy_args()
+    args.size0, args.inner, args.token_level, args.pages = 1, (1 << 31) - 16, -1, 512
+    args.stride_page = 1 << 31
+    assert check("copy_pages", args) == (0, "")
+
+
 def test_pages_may_lie_inside_other_levels():
     """Heads outside pages: a page is in pieces, and no two share bytes."""
     args = copy_args()
