@@ -400,3 +400,57 @@ def test_log_sum_exp_to_its_last_digits(dtype, offset, late, rows, vocab):
     assert out.tokens.equal(wide.argmax(-1)) and (out.parents == 0).all()
     over = float((off / (2.0 ** -24 * want.abs() + lse_bound(wide))).max())
     assert over <= 1, f"errors up to {float(off.max()):.2g}, {float(off.mean()):.2g} on average"
+
+
+# --------------------------------------------------------------------------- workgroups shared out over the live rows
+LIVE = {"all": lambda r, w: True, "scattered": lambda r, w: (7 * r + 3 * w) % 5 > 1, "one beam a request": lambda r, w: w == r % 3,
+        "one row": lambda r, w: (r, w) == (41, 2), "whole requests": lambda r, w: r % 9 == 4, "the last": lambda r, w: r > 66,
+        "none": lambda r, w: False}
+
+
+@pytest.mark.parametrize("live", LIVE)
+@pytest.mark.parametrize("dtype,flat", [("bf16", True), ("bf16", False), ("fp32", False)], ids=["bf16", "bf16 strided", "fp32 strided"])
+def test_runs_shared_out_over_live_rows(live, dtype, flat):
+    """More rows than there are workgroups for the runs that live ones may get: every number of live rows, so that lists and
+    sums lie further apart than they are filled.  What the workspace holds before does not matter."""
+    import l20_beam_search as bs
+
+    requests, beams, vocab, ends = 69, 4, 30000, [17, 29999]
+    rows, most = requests * beams, min(64, (-(-vocab // 2048) + 3) // 4)
+    spread = 3 * torch.cuda.get_device_properties(0).multi_processor_count
+    assert rows % 64 and max(spread // rows, 1) < most, "the rows are not shared out"
+    logits, scores = inputs(requests, beams, vocab, DTYPES[dtype], seed=len(live))
+    logits[:, ::2, 17] += 9
+    logits[:, 1, 29999] += 10
+    dead = torch.tensor([[not LIVE[live](r, w) for w in range(beams)] for r in range(requests)])
+    scores[dead] = -math.inf
+    scores[::2] = torch.where(dead[::2], math.nan, scores[::2])
+    logits[dead] = math.nan  # (nothing of it matters)
+    s = scores.cuda() if flat else torch.full((beams, 2 * requests), 3.0, device="cuda")[:, ::2].t().copy_(scores)
+    x = logits.cuda()
+    ws = bs.allocate_l20_beam_search_workspace(x, s, end_tokens=ends)
+    out = None
+    for fill in (255, 0, 85):
+        ws.fill_(fill)
+        got = bs.l20_beam_search_step(x, s, end_tokens=ends, out=filled(requests, beams), workspace=ws)
+        torch.cuda.synchronize()
+        assert out is None or all(a.equal(b) for a, b in zip(got, out))
+        out = got
+    if dead.all():
+        assert all((t == v).all() for t, v in zip(out, (-1, -1, -math.inf) * 2))
+    else:
+        compare(out, logits, scores, ends)
+
+
+def test_one_workspace_for_rows_shared_out_and_not():
+    """The same workspace for a batch whose rows are shared out, smaller ones that get all their runs, and dead ones."""
+    import l20_beam_search as bs
+
+    logits, scores = inputs(130, 4, 20000, torch.bfloat16, seed=5)
+    x, full = logits.cuda(), scores.cuda()
+    ws = bs.allocate_l20_beam_search_workspace(x, full, end_tokens=[3])
+    for n, step in ((130, 1), (2, 1), (130, 3), (40, 1), (130, 50)):
+        s = full[:n].clone()
+        s[:, 1:][torch.arange(n) % step > 0] = -math.inf
+        got = bs.l20_beam_search_step(x[:n], s, end_tokens=[3], out=filled(n, 4), workspace=ws)
+        compare(got, logits[:n], s.cpu(), [3])
