@@ -274,6 +274,22 @@ def test_reorder_large():
     check_reorder(c, [[-1, -1], [-1, -1]])
 
 
+@pytest.mark.parametrize("spare", [9000, 300_000], ids=["one bitmap", "two"])
+def test_reorder_more_lists_than_are_looked_at_together(spare):
+    """The most rows, in more column blocks than one pass over the lists of freed pages takes (4096), short and long ones:
+    pages come back, and copies are taken, in both passes."""
+    rng = random.Random(spare)
+    lens = [4780 + g % 16 if g % 97 == 3 or g > 1020 else rng.randint(0, 60) for g in range(1024)]
+    c = pool(1024, 8, 16, longest=4796, spare=spare, seed=14, lens=lens)
+    assert 1024 * -(-len(c["table"][0]) // 64) > 4096 and (len(c["shares"]) > 1 << 18) == (spare > 9000)
+    after = check_reorder(c, parents_of(1024, 8, 14))
+    held_once(after)
+    freed = {v for v in after["free"][:after["count"]]} - {v for v in c["free"][:c["count"]]}
+    rows = [r for r, n in enumerate(c["lens"]) for v in c["table"][r][:R.pages_of(n, 16, 302)] if v in freed]
+    assert min(rows) < 8 * 800 and max(rows) > 8 * 1000  # (lists of a group lie together, 5 a group)
+    held_once(check_reorder(after, [[-1] * 8] * 1024))
+
+
 def test_reorder_row_strides_and_no_groups():
     import l20_block_tables as bt
 
@@ -523,6 +539,27 @@ def test_copy_views():
     check_copy([random_bytes((6, 4, 64, 16), torch.bfloat16, 5).permute(0, 3, 1, 2)], src, dst)
     check_copy([random_bytes((4, 6, 16, 32), torch.float16, 6).permute(1, 2, 0, 3)], src, dst, tokens)  # heads outside pages
     check_copy([random_bytes((6, 32, 40), torch.float16, 7)[:, ::2, :24]], src, dst, tokens)
+
+
+@pytest.mark.parametrize("page,dim", [(64, 128), (64, 576), (256, 128), (64, 132), (80, 130)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.bfloat16, torch.uint8], ids=["e4m3", "bf16", "u8"])
+def test_copy_runs_inside_a_page(page, dim, dtype):
+    """A page of several runs of bytes, each by itself: heads outside tokens, whole and in part (tokens that end inside a
+    load of 16 bytes, and runs longer than what a workgroup takes at once); heads outside the pages; padded heads."""
+    src, dst, tokens = [5, 0, 2, 6], [1, 4, 3, 7], [page, 3, 41, 0]
+    heads = 3
+
+    def held(*shape):
+        return random_bytes(shape, dtype, page + dim)
+
+    for view in (held(8, heads, page, dim).permute(0, 2, 1, 3), held(heads, 8, page, dim).permute(1, 2, 0, 3),
+                 held(8, heads, page + 3, dim)[:, :, :page].permute(0, 2, 1, 3), held(8, heads + 1, page, dim)[:, 1:].permute(0, 2, 1, 3),
+                 held(8, 2, heads, page, dim)[:, 1].permute(0, 2, 1, 3)):
+        assert view.shape[1:] == (page, heads, dim)
+        check_copy([view], src, dst, tokens)
+        check_copy([view], dst, src)
+    caches = [held(8, heads, page, dim).permute(0, 2, 1, 3) for _ in range(3)]
+    check_copy(caches, src, dst, tokens, [2, 0])
 
 
 def test_copy_many_caches_and_mixed_layouts():
