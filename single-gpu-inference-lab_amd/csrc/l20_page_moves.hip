@@ -695,8 +695,9 @@ __global__ __launch_bounds__(kThreads) void cp_small(Compact p) {
 
 constexpr int kCaches = 64;  // caches of a launch
 // Bytes of a run from which on a workgroup takes it by itself.  Measured, 512 pages of 16 caches by runs and by divisions:
-// runs of 2 KB 42.0 and 20.4 us, of 4 KB 59.6 and 47.8.
-constexpr int kRun = 8192;
+// whole pages with runs of 2 KB 42.5 and 21.1 us, 4 KB 63.5 and 48.1, 8 KB 113.9 and 113.7, 16 KB 218 and 218; half of their
+// tokens, 8 KB 66.9 and 60.8, 16 KB 119 and 125, 32 KB 271 and 283.
+constexpr int kRun = 16384;
 
 struct Copy {
   const int32_t *src, *dst, *tokens;
