@@ -36,8 +36,8 @@ extern "C" {
  *   ended_tokens, _parents, _scores the candidates with an end token among the first `beams` of all, in
  *                                   order; -1, -1 and -inf behind them
  *
- * Two launches, nothing allocated, no atomics: equal inputs give equal bits.  The workspace's contents do not
- * matter; calls that may overlap each need their own.
+ * Two launches, nothing allocated.  Atomics are on whole numbers, whose order does not matter: equal inputs give equal
+ * bits.  The workspace's contents do not matter; calls that may overlap each need their own.
  */
 typedef struct l20_pd_beam_step_args {
   const void *logits;

@@ -272,8 +272,8 @@ struct Best {
     if (which >> (threadIdx.x & 63) & 1) keys[at] = key_of(x, token);
     count += __builtin_popcountll(which);
   }
-  __device__ __forceinline__ void show(float x, int token, bool ok) {
-    ok = ok && x >= least && key_of(x, token) >= bar;
+  __device__ __forceinline__ void show(float x, int token) {
+    const bool ok = x >= least && key_of(x, token) >= bar;
     u64 which = __ballot(ok);
     if (count + __builtin_popcountll(which) > kEntries) {
       settle();
@@ -475,7 +475,7 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
           }
           const int token = step * kStep + i * 512 + lane * kSide<T>;
 #pragma unroll 1
-          for (int j = 0; j < 8; ++j) best.show(s_vector[wave][lane * 8 + j], token + place_of<T>(j), true);
+          for (int j = 0; j < 8; ++j) best.show(s_vector[wave][lane * 8 + j], token + place_of<T>(j));
         }
         best.pass();
         low = ref.low(best.least);

@@ -130,12 +130,11 @@ struct Reorder {
 
 // What becomes of a row, from its group's parents and lengths.
 struct Row {
-  int parent;  // -1: given up
-  int len;     // new
-  int copy;    // the column of its own copy, -1: none
+  int len;   // new
+  int copy;  // the column of its own copy, -1: none
 };
 __device__ __forceinline__ Row row_of(int row, int parent, int parent_len, bool parent_stays, bool first, const Page &page, int width) {
-  Row r{parent, parent >= 0 ? max(parent_len, 0) : 0, -1};
+  Row r{parent >= 0 ? max(parent_len, 0) : 0, -1};
   const bool keeps = parent_stays ? parent == row : first;
   const int last = page.whole(r.len);
   if (parent >= 0 && last * page.size != r.len && !keeps && last < width) r.copy = last;
@@ -320,7 +319,7 @@ template <int PER> __device__ __forceinline__ void share_out(const Reorder &p, i
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int r = tid * per_row + i;
-    row[i] = Row{-1, 0, -1};
+    row[i] = Row{0, -1};
     if (i < per_row && r < rows) {
       int me, parent;
       const int base = row_at(r, me, parent), from_row = base + max(parent, 0);
