@@ -14,17 +14,17 @@
 //  beam_join   a workgroup a request.  A wave a row joins the runs' lists in the same way, and their sums; then each
 //    candidate's place is counted in every row's list, by binary search.
 //
-// What bounds them (128 x 8 beams of 152064 bf16 logits, 311 MB, 61 us): the vector units are busy 79 % of the scan's time
-// (280 instructions for 32 logits a lane: conversions, two fused products, exp, sum), which streams 7.8 TB/s between a
-// start and an end of 5 us; 5 us are the join's: loads, exp and log in 64 bits, searches.  Small calls are that
-// latency, of loads and of code that is not in the instruction cache yet (1 x 4 beams of 32000: 6.1 + 4.9 us).
+// What bounds them (128 x 8 beams of 152064 bf16 logits, 311 MB, 61 us): the vector units are busy 84 % of the scan's time
+// (285 instructions for 32 logits a lane: conversions, difference, product, exp, sum), of which a start and an end take 5 us
+// each; 5 us are the join's: loads, exp and log in 64 bits, searches.  Small calls are that
+// latency, of loads and of code that is not in the instruction cache yet (1 x 4 beams of 32000: 6.0 + 4.7 us).
 //
-// Numerics: d = x - m and exp2 of d log2 e in fp32, with log2 e in two parts and one rounding of their sum; eight terms
-// summed in fp32, everything beyond that in 64 bits: candidates of different beams are told apart by lse's last digits.  No
-// exponent is above 4, so the terms that make up a sum are near 1 and the exponents' rounding small.  lse is off by 2-4e-9 on
-// average where many tokens share the mass, and by up to 1.6e-7 where one has most of it: the roundings of its sum of eight,
-// which show in a score near 0 only.  (Two products of x itself, an instruction less, took 62.1 us for 63.3, but the second
-// rounding loses the low part of log2 e: 4e-8 in all of a row's scores.  References up to 2^24 below the best token: up to 1e-6.)
+// Numerics: exp2 of (x - m) log2 e in fp32, eight terms summed in fp32, everything beyond that in 64 bits: candidates of
+// different beams are told apart by lse's last digits.  No exponent is above 4, so the terms that make up a sum are near 1 and
+// their exponents' rounding small.  lse is off by 2e-9 on average where many tokens share the mass, and by up to 1.6e-7 where one
+// has most of it: the roundings of its sum of eight, which show in a score near 0 only.  (log2 e in two parts, added in one
+// rounding: 2-4e-9, but an instruction more a logit, 63.3 us; two fused products of x itself, 62.6 us: the second rounding loses
+// the low part, 4e-8 in all of a row's scores.  References up to 2^24 below the best token: up to 1e-6.)
 
 #include "l20_beam_search.h"
 
@@ -177,8 +177,10 @@ __host__ __device__ constexpr unsigned mul_of(unsigned d) { return d == 1 ? 0 : 
 __device__ __forceinline__ int over(int n, unsigned mul) { return mul ? (int)__umulhi((unsigned)n, mul) : n; }
 __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < INFINITY; }
 
-// log2 e in two parts: one fp32 constant is off by 1.3e-8 of itself, which all terms of a sum would share.
-constexpr float kLog2eHi = 1.44269502f, kLog2eLo = 1.92596299e-08f;
+// log2 e lies between two floats, 5/32 of the way up (to 6e-10): as many of a lane's 32 logits take the upper one, each place
+// always the same.  A term may be off by 7e-8 of its x - m, but a sum of many by next to nothing; with the lower one alone they
+// would share an error of 1.3e-8 of x - m.
+constexpr float kLog2e = 0x1.715476p0f, kLog2eUp = 0x1.715478p0f;
 
 // What a wave's sum is relative to: the sum of exp(x - m), with m near the maximum.
 struct Reference {
@@ -188,15 +190,14 @@ struct Reference {
     m = m_;
     from = m > -INFINITY ? m : 0.0f;
   }
-  // Half a step of the exponent (of d too, in fp32 logits) and one of the result (v_exp_f32 is good to one).
-  __device__ __forceinline__ float term(float x) const {
-    const float d = x - from;
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2eHi, d * kLog2eLo));
-  }
-  __device__ __forceinline__ float eight(const float (&x)[8]) const {
+  // Half a step of the exponent (of x - m too, in fp32 logits) and one of the result (v_exp_f32 is good to one).
+  __device__ __forceinline__ float term(float x, float log2e = kLog2e) const { return __builtin_amdgcn_exp2f((x - from) * log2e); }
+  // Those of a lane's vector i.
+  __device__ __forceinline__ float eight(const float (&x)[8], int i) const {
+    static_assert(kVectors == 4, "5 of 32");
     float e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = term(x[j]);
+    for (int j = 0; j < 8; ++j) e[j] = term(x[j], 7 * (8 * i + j) % 32 < 5 ? kLog2eUp : kLog2e);
     return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
   }
   // The term of x less what rounding may make of it; 0 where it is too small to tell.
@@ -425,7 +426,7 @@ template <typename T> __global__ __launch_bounds__(64 * kWaves, 4) void beam_sca
     float part[kVectors];
     auto terms = [&] {
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i) part[i] = ref.eight(x[i]);
+      for (int i = 0; i < kVectors; ++i) part[i] = ref.eight(x[i], i);
       return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
     };
     float most = terms();

@@ -365,13 +365,16 @@ def test_refusals():
 def lse_bound(x):
     """How far the log-sum-exp of each row of `x` (float64) may be off.  A term is exp2 of an fp32 exponent e relative to a
     reference that no value exceeds by more than 4 ln 2 (a sum of eight terms up to 2^4), so |e| <= max(4, (top - x) log2 e):
-    half a step of e, and log2 e halves of one for the difference that it is made of (no larger steps), times ln 2; exp2 itself (one step: 2^-23); three additions (2^-24 each).  The
-    rest is in 64 bits.  The terms' errors weigh as the terms do; 1 % for products of them."""
+    half a step of e, and log2 e halves of one for the difference that it is made of (no larger steps), times ln 2; the
+    distance of log2 e from the further of the two floats around it, 1e-7, times that difference and ln 2; exp2 itself
+    (one step: 2^-23); three additions (2^-24 each).  The rest is in 64 bits.  The terms' errors weigh as the terms do; 1 %
+    for products of them."""
     top = x.amax(-1, keepdim=True)
     weight = (x - torch.logsumexp(x, -1, keepdim=True)).exp()
     e = ((top - x) * math.log2(math.e)).clamp_min(4.0)
     half = torch.exp2(e.log2().ceil() - 25)  # of the steps of (2^(n-1), 2^n]
-    return 1.01 * (weight * ((1 + math.log2(math.e)) * math.log(2) * half + 2.0 ** -23 + 3 * 2.0 ** -24)).sum(-1)
+    apart = 1e-7 * math.log(2) * (e / math.log2(math.e))
+    return 1.01 * (weight * ((1 + math.log2(math.e)) * math.log(2) * half + apart + 2.0 ** -23 + 3 * 2.0 ** -24)).sum(-1)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
