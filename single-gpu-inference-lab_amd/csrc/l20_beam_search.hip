@@ -41,9 +41,10 @@ namespace l20bs {
 using l20la::f32x4;
 using l20la::i32x4;
 
-// 128 x 8 beams of 152064 tokens, 64 x 4 of 128256, 16 x 5 of 50257: 62.3, 25.2 and 15.8 us; with 8 waves and two runs a CU
-// 63.4, 26.0 and 17.0 (a workgroup ends with its slowest wave), with four runs a CU 61.8, 26.6 and 15.7, with two vectors
-// and six waves a SIMD 76.4, 32.0 and 20.6 (what is done once a step counts twice).
+// 128 x 8 beams of 152064 tokens, 64 x 4 of 128256, 16 x 5 of 50257, a first step of 64 x 8: 61.1, 24.1, 15.3 and 22.3 us;
+// with two runs a CU 60.9, 25.5, 15.9 and 21.4, with four 61.3, 24.9, 15.1 and 22.4, with two vectors and six waves a SIMD
+// 77.0, 30.4, 18.3 and 25.0 (what is done once a step counts twice); eight waves and two runs a CU lost 1-1.2 us (a workgroup
+// ends with its slowest wave).
 constexpr int kVectors = 4;                // vectors of eight logits a lane and step
 constexpr int kStep = 64 * 8 * kVectors;   // logits of a wave's step
 constexpr int kWaves = 4;                  // of a workgroup, which takes a run
