@@ -16,8 +16,8 @@
 //
 // What bounds them (128 x 8 beams of 152064 bf16 logits, 311 MB, 61 us): the vector units are busy 84 % of the scan's time
 // (285 instructions for 32 logits a lane: conversions, difference, product, exp, sum), of which a start and an end take 5 us
-// each; 5 us are the join's: loads, exp and log in 64 bits, searches.  Small calls are that
-// latency, of loads and of code that is not in the instruction cache yet (1 x 4 beams of 32000: 6.0 + 4.7 us).
+// each; 5 us are the join's: loads, exp and log in 64 bits, searches.  Small calls are that latency, of loads and of code that
+// is not in the instruction cache yet (1 x 4 beams of 32000: 5.9 + 4.9 us).
 //
 // Numerics: exp2 of (x - m) log2 e in fp32, eight terms summed in fp32, everything beyond that in 64 bits: candidates of
 // different beams are told apart by lse's last digits.  No exponent is above 4, so the terms that make up a sum are near 1 and
